@@ -64,6 +64,11 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
   }
 }
 
+// First error wins; `err` is the device error word (code, auxiliary value).
+__device__ __forceinline__ void report_error_at(uint32_t* err, uint32_t code, uint32_t info) {
+  if (atomicCAS(&err[0], 0u, code) == 0u) err[1] = info;
+}
+
 // ---- system-scope flags (another GPU reads or writes them over NVLink) -----------
 __device__ __forceinline__ void st_relaxed_sys(unsigned int* p, unsigned int v) {
   asm volatile("st.relaxed.sys.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");

@@ -19,6 +19,7 @@
 
 #include "kvc_common.h"
 #include "kvc_internal.h"
+#include "kvc_spec.h"
 #include "kvcache.h"
 
 namespace kvc {
@@ -261,6 +262,24 @@ int layer_forward_paged(kvc_pool* pool, kvc_plan* plan, const int32_t* d_bt, int
   });
 }
 
+// The layer for the drafted tokens of a tree plan (d.seq of them): rotation and append
+// at the plan's slots in one launch, then the tree attention.
+static int layer_forward_tree(kvc_pool* pool, kvc_tree_plan* plan, const int32_t* d_mask,
+                              int mask_words, const int32_t* d_rope_pos, const int32_t* d_bt,
+                              int bt_rows, int bt_stride, const LayerIO& io, const LayerDims& d,
+                              cudaStream_t s) {
+  return layer_steps(plan->d_layer, io, d, s, [&](const __half* q, const __half* k,
+                                                  const __half* v, __half* qr, __half*,
+                                                  __half* attn) -> int {
+    const int rc = do_append_rope(pool, d.layer, q, 0, qr, d.H, k, 0, v, 0, d_bt, bt_rows,
+                                  bt_stride, plan->dev_rows, plan->dev_slots, d_rope_pos, d.seq,
+                                  d.base, d.neox ? 1 : 0, s);
+    if (rc) return rc;
+    return do_decode_tree(pool, plan, d.layer, qr, d_mask, mask_words, attn, d_bt, bt_stride,
+                          d.scale, s);
+  });
+}
+
 }  // namespace kvc
 
 using namespace kvc;
@@ -371,4 +390,56 @@ extern "C" int kvc_forward_layer_paged(
   if (const int rc_dev = use_device(pool->device)) return rc_dev;
   return layer_forward_paged(pool, const_cast<kvc_plan*>(plan), d_block_tables, bt_stride, io, d,
                              static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int kvc_forward_layer_tree(
+    kvc_pool_t* pool, kvc_tree_plan_t* plan, int layer_idx, const void* d_x_in, void* d_x_out,
+    const void* d_attn_norm_w, const void* d_wq, int wq_type, const void* d_wk, int wk_type,
+    const void* d_wv, int wv_type, const void* d_wo, int wo_type, const void* d_ffn_norm_w,
+    const void* d_wgate, int wgate_type, const void* d_wup, int wup_type, const void* d_wdown,
+    int wdown_type, const int32_t* d_mask, int mask_words, const int32_t* d_rope_positions,
+    const int32_t* d_block_tables, int bt_rows, int bt_stride, int hidden_size,
+    int intermediate_size, float rms_norm_eps, float rope_freq_base, int rope_neox, float scale,
+    void* stream) {
+  if (!pool || !plan) return set_error(KVC_ERR_INVALID_ARG, "pool and plan must not be null.");
+  if (!plan->valid) return set_error(KVC_ERR_INVALID_ARG, "plan has not been built.");
+  const PoolGeom& g = pool->g;
+  if (g.dtype != KVC_DTYPE_F16)
+    return set_error(KVC_ERR_INVALID_ARG, "the layer pipeline needs an fp16 KV pool.");
+  if (layer_idx < 0 || layer_idx >= g.num_layers)
+    return set_error(KVC_ERR_OUT_OF_RANGE, "layer_idx out of range for the KV pool.");
+  LayerDims d;
+  d.layer = layer_idx;
+  d.seq = plan->n_tokens;
+  d.hidden = hidden_size;
+  d.inter = intermediate_size;
+  d.H = plan->num_heads;
+  d.Hkv = g.num_kv_heads;
+  d.D = g.head_dim;
+  d.eps = rms_norm_eps;
+  d.base = rope_freq_base;
+  d.scale = scale;
+  d.neox = rope_neox != 0;
+  const int types[7] = {wq_type, wk_type, wv_type, wo_type, wgate_type, wup_type, wdown_type};
+  const void* w[7] = {d_wq, d_wk, d_wv, d_wo, d_wgate, d_wup, d_wdown};
+  if (const int rc = check_layer(d, types)) return rc;
+  if (d.seq == 0) return KVC_OK;
+  if (!d_x_in || !d_x_out || !d_attn_norm_w || !d_ffn_norm_w || !d_block_tables)
+    return set_error(KVC_ERR_INVALID_ARG, "device buffers must not be null.");
+  if (bt_rows <= plan->max_row)
+    return set_error(KVC_ERR_OUT_OF_RANGE, "a sequence's block-table row is outside the table.");
+  LayerIO io;
+  for (int i = 0; i < 7; ++i) {
+    if (!w[i]) return set_error(KVC_ERR_INVALID_ARG, "weight buffers must not be null.");
+    io.w[i] = w[i];
+    io.type[i] = types[i];
+  }
+  io.x_in = static_cast<const __half*>(d_x_in);
+  io.x_out = static_cast<__half*>(d_x_out);
+  io.attn_norm = static_cast<const __half*>(d_attn_norm_w);
+  io.ffn_norm = static_cast<const __half*>(d_ffn_norm_w);
+  DeviceScope dev(pool->device);
+  if (dev.rc()) return dev.rc();
+  return layer_forward_tree(pool, plan, d_mask, mask_words, d_rope_positions, d_block_tables,
+                            bt_rows, bt_stride, io, d, static_cast<cudaStream_t>(stream));
 }

@@ -54,6 +54,7 @@ _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _c_size = ctypes.c_size_t
 _vp = ctypes.c_void_p
+_i64 = ctypes.c_int64
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
 # forward_layer_cached's 30 arguments (bindings.cpp:562-587 order; rope_neox as int)
@@ -153,7 +154,31 @@ SIGNATURES = {
                                          _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp, _c_int,
                                          _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_float,
                                          _c_float, _c_int, _c_float, _vp]),
+    "kvc_append_rope": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int,
+                                 _vp, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_float, _c_int,
+                                 _vp]),
+    "kvc_tree_plan_create": (_c_int, [ctypes.POINTER(_vp)]),
+    "kvc_tree_plan_destroy": (_c_int, [_vp]),
+    "kvc_plan_tree": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _vp]),
+    "kvc_tree_plan_info": (_c_int, [_vp, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
+                                    ctypes.POINTER(_c_size)]),
+    "kvc_decode_tree": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_int, _c_float,
+                                 _vp]),
+    "kvc_forward_layer_tree": (_c_int, [_vp, _vp, _c_int] + _LAYER_ARGS[:18]
+                               + [_vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_float,
+                                  _c_float, _c_int, _c_float, _vp]),
+    "kvc_commit_tree": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int,
+                                 _vp]),
+    "kvc_beam_create": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(_vp)]),
+    "kvc_beam_destroy": (_c_int, [_vp]),
+    "kvc_beam_select": (_c_int, [_vp, _vp, _c_int, _i64, _vp, _c_int, _c_int, _c_int, _c_int, _vp,
+                                 _vp, _vp, _vp]),
+    "kvc_reorder_beams": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
 }
+
+MAX_TREE_NODES = 256
+MAX_BEAMS = 16
+MAX_BEAM_OUT = 32
 
 XCHG_HANDLE_BYTES = 64
 

@@ -49,6 +49,36 @@ def _dev(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> int:
     return int(t.data_ptr())
 
 
+def _on(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: int) -> int:
+    """_dev, and on CUDA device `device`."""
+    if t.dtype != dtype or t.device.type != "cuda" or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor")
+    if t.device.index != device:
+        raise ValueError(f"{name} is on {t.device}, not on the pool's cuda:{device}")
+    if t.numel() < numel:
+        raise ValueError(f"{name} buffer is smaller than expected dimensions.")
+    return t.data_ptr()
+
+
+def _token_rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, heads: int, dim: int,
+                device: int):
+    """(address, elements between tokens) of (n, heads, dim) rows whose heads are packed."""
+    if t.dtype != dtype or t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{name} must be a {dtype} tensor on cuda:{device}")
+    if tuple(t.shape) != (n, heads, dim):
+        raise ValueError(f"{name} must be ({n}, {heads}, {dim}), got {tuple(t.shape)}")
+    st = t.stride()
+    if (dim > 1 and st[2] != 1) or (heads > 1 and st[1] != dim) or \
+            (n > 1 and st[0] < heads * dim):
+        raise ValueError(f"the heads of a token of {name} must be packed")
+    return t.data_ptr(), (st[0] if n > 1 else heads * dim)
+
+
+def _stream_on(stream, device: int) -> Optional[int]:
+    s = stream if stream is not None else torch.cuda.current_stream(device)
+    return int(s.cuda_stream) or None
+
+
 @dataclass
 class PlanInfo:
     n_queries: int
@@ -103,6 +133,37 @@ class DecodePlan:
     def close(self):
         if self.handle is not None:
             ffi.check(ffi.lib.kvc_plan_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class TreePlan:
+    """Work list of one verification step of drafted tokens (see kvc_plan_tree)."""
+
+    def __init__(self):
+        h = ctypes.c_void_p()
+        ffi.check(ffi.lib.kvc_tree_plan_create(ctypes.byref(h)))
+        self.handle = h
+        self.n_tokens = 0
+        self.num_heads = 0
+        self.max_row = 0
+        self.ctx_lens: Optional[np.ndarray] = None
+        self.node_counts: Optional[np.ndarray] = None
+
+    def info(self) -> PlanInfo:
+        n, ctas, scratch = ctypes.c_int(), ctypes.c_int(), ctypes.c_size_t()
+        ffi.check(ffi.lib.kvc_tree_plan_info(self.handle, ctypes.byref(n), ctypes.byref(ctas),
+                                             ctypes.byref(scratch)))
+        return PlanInfo(n.value, ctas.value, ctas.value, scratch.value)
+
+    def close(self):
+        if self.handle is not None:
+            ffi.check(ffi.lib.kvc_tree_plan_destroy(self.handle))
             self.handle = None
 
     def __del__(self):
@@ -258,6 +319,164 @@ class PagedKVCache:
             weights.hidden, weights.intermediate, float(eps), float(freq_base), int(bool(neox)),
             sc, _sp(stream)))
 
+    # -- drafted tokens and beams ---------------------------------------------------
+    def append_rope(self, layer: int, q: Optional[torch.Tensor], k_new: torch.Tensor,
+                    v_new: torch.Tensor, block_tables: torch.Tensor, positions: torch.Tensor,
+                    rows: Optional[torch.Tensor] = None,
+                    rope_positions: Optional[torch.Tensor] = None,
+                    q_out: Optional[torch.Tensor] = None, freq_base: float = 10000.0,
+                    neox: bool = False, stream=None) -> Optional[torch.Tensor]:
+        """append with the K rows rotated (RoPE) on the way, and q (n, heads, D) rotated
+        into q_out (allocated if not given; returned), in one launch (kvc_append_rope).
+        q, k_new, v_new may be slices of one fused projection (n, heads, D): only the
+        heads of a token must be packed.  positions are cache slots (negative: padding,
+        that token is skipped), rope_positions the angles' positions where they differ."""
+        dev, dt, d = self.device, self.dtype, self.head_dim
+        n = positions.numel()
+        kp, ks = _token_rows(k_new, "k_new", dt, n, self.num_kv_heads, d, dev)
+        vp, vs = _token_rows(v_new, "v_new", dt, n, self.num_kv_heads, d, dev)
+        qp = op = None
+        heads = qs = 0
+        if q is not None:
+            if q.dim() != 3:
+                raise ValueError("q must be (n, heads, head_dim)")
+            heads = q.shape[1]
+            qp, qs = _token_rows(q, "q", dt, n, heads, d, dev)
+            if q_out is None:
+                q_out = torch.empty((n, heads, d), dtype=dt, device=q.device)
+            op = _on(q_out, "q_out", dt, n * heads * d, dev)
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be (rows, pages)")
+        ffi.check(ffi.lib.kvc_append_rope(
+            self.handle, layer, qp, qs, op, heads, kp, ks, vp, vs,
+            _on(block_tables, "block_tables", torch.int32, 0, dev), block_tables.shape[0],
+            block_tables.shape[1],
+            None if rows is None else _on(rows, "rows", torch.int32, n, dev),
+            _on(positions, "positions", torch.int32, n, dev),
+            None if rope_positions is None else _on(rope_positions, "rope_positions", torch.int32,
+                                                    n, dev),
+            n, freq_base, 1 if neox else 0, _stream_on(stream, dev)))
+        return q_out
+
+    def plan_tree(self, ctx_lens: Sequence[int], node_counts: Sequence[int], num_heads: int,
+                  rows: Optional[Sequence[int]] = None, plan: Optional[TreePlan] = None,
+                  stream=None) -> TreePlan:
+        """Plan the attention of node_counts[i] drafted tokens per sequence behind
+        ctx_lens[i] cached positions of block-table row rows[i] (default i)."""
+        p = plan if plan is not None else TreePlan()
+        ctx = np.ascontiguousarray(np.asarray(ctx_lens, dtype=np.int32))
+        cnt = np.ascontiguousarray(np.asarray(node_counts, dtype=np.int32))
+        r = None if rows is None else np.ascontiguousarray(np.asarray(rows, dtype=np.int32))
+        if ctx.shape != cnt.shape or ctx.ndim != 1 or (r is not None and r.shape != ctx.shape):
+            raise ValueError("ctx_lens, node_counts and rows must have one entry per sequence")
+        ffi.check(ffi.lib.kvc_plan_tree(p.handle, self.handle, ffi.np_ptr(r), ffi.np_ptr(ctx),
+                                        ffi.np_ptr(cnt), ctx.size, int(num_heads),
+                                        _stream_on(stream, self.device)))
+        p.n_tokens = int(cnt.sum())
+        p.num_heads = int(num_heads)
+        p.max_row = int(r.max(initial=0)) if r is not None else max(0, ctx.size - 1)
+        p.ctx_lens, p.node_counts = ctx, cnt
+        return p
+
+    def decode_tree(self, plan: TreePlan, layer: int, q: torch.Tensor,
+                    mask: Optional[torch.Tensor], out: torch.Tensor, block_tables: torch.Tensor,
+                    scale: float, stream=None):
+        """Attention of the plan's drafted tokens (kvc_decode_tree): q, out (tokens,
+        heads, D); mask (tokens, words) int32 bit rows (see tree_masks), None for a
+        chain.  Their K/V rows must be appended already (append_rope)."""
+        dev, dt, t = self.device, self.dtype, plan.n_tokens
+        n = t * plan.num_heads * self.head_dim
+        mp, words = self._mask(mask, t)
+        self._table(block_tables, plan)
+        ffi.check(ffi.lib.kvc_decode_tree(
+            self.handle, plan.handle, layer, _on(q, "q", dt, n, dev), mp, words,
+            _on(out, "out", dt, n, dev), block_tables.data_ptr(), block_tables.shape[1], scale,
+            _stream_on(stream, dev)))
+
+    def _mask(self, mask: Optional[torch.Tensor], tokens: int):
+        if mask is None:
+            return None, 0
+        if mask.dim() != 2:
+            raise ValueError("mask must be (tokens, words)")
+        words = mask.shape[1]
+        return _on(mask, "mask", torch.int32, tokens * words, self.device), words
+
+    def _table(self, block_tables: torch.Tensor, plan: TreePlan) -> None:
+        _on(block_tables, "block_tables", torch.int32, 0, self.device)
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be (rows, pages)")
+        if plan.n_tokens and plan.max_row >= block_tables.shape[0]:
+            raise IndexError("a sequence's block-table row is outside the table")
+
+    def forward_layer_tree(self, plan: TreePlan, layer: int, x: torch.Tensor, out: torch.Tensor,
+                           weights: "DeviceLayerWeights", mask: Optional[torch.Tensor],
+                           block_tables: torch.Tensor,
+                           rope_positions: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                           freq_base: float = 10000.0, neox: bool = False,
+                           scale: Optional[float] = None, stream=None):
+        """One transformer layer for the plan's drafted tokens (kvc_forward_layer_tree):
+        x / out (tokens, hidden) fp16; rope_positions (tokens) int32, context + depth of
+        each token (None: its cache slot, right for a chain).  out may be x."""
+        dev, t = self.device, plan.n_tokens
+        n = t * weights.hidden
+        sc = default_scale(self.head_dim) if scale is None else float(scale)
+        if len(weights.w) != 7 or len(weights.types) != 7:
+            raise ValueError("a layer has seven weights: q, k, v, o, gate, up, down")
+        for w in weights.w:
+            if not w.is_cuda or not w.is_contiguous():
+                raise ValueError("weights must be contiguous CUDA tensors")
+        wt = [x for w, ty in zip(weights.w, weights.types) for x in (int(w.data_ptr()), int(ty))]
+        mp, words = self._mask(mask, t)
+        self._table(block_tables, plan)
+        ffi.check(ffi.lib.kvc_forward_layer_tree(
+            self.handle, plan.handle, layer, _on(x, "x", torch.float16, n, dev),
+            _on(out, "out", torch.float16, n, dev),
+            _on(weights.attn_norm, "attn_norm", torch.float16, weights.hidden, dev), *wt[:8],
+            _on(weights.ffn_norm, "ffn_norm", torch.float16, weights.hidden, dev), *wt[8:], mp,
+            words,
+            None if rope_positions is None else _on(rope_positions, "rope_positions", torch.int32,
+                                                    t, dev),
+            block_tables.data_ptr(), block_tables.shape[0], block_tables.shape[1], weights.hidden,
+            weights.intermediate, float(eps), float(freq_base), 1 if neox else 0, sc,
+            _stream_on(stream, dev)))
+
+    def commit_tree(self, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+                    paths: torch.Tensor, path_lens: torch.Tensor,
+                    rows: Optional[torch.Tensor] = None, stream=None):
+        """Move the accepted paths' rows together in every layer (kvc_commit_tree):
+        the row of slot ctx_lens[i] + paths[i, j] goes to slot ctx_lens[i] + j.  All int32
+        CUDA tensors; paths (sequences, longest), ascending; rows default to i."""
+        dev, n = self.device, path_lens.numel()
+        if paths.dim() != 2 or block_tables.dim() != 2:
+            raise ValueError("paths and block_tables must have two dimensions")
+        if paths.shape[0] != n:
+            raise ValueError("paths needs one row per sequence")
+        if rows is None and n > block_tables.shape[0]:
+            raise IndexError("a sequence's block-table row is outside the table")
+        ffi.check(ffi.lib.kvc_commit_tree(
+            self.handle, _on(block_tables, "block_tables", torch.int32, 0, dev),
+            block_tables.shape[0], block_tables.shape[1],
+            None if rows is None else _on(rows, "rows", torch.int32, n, dev),
+            _on(ctx_lens, "ctx_lens", torch.int32, n, dev),
+            _on(paths, "paths", torch.int32, 0, dev), paths.shape[1],
+            _on(path_lens, "path_lens", torch.int32, 0, dev), n, _stream_on(stream, dev)))
+
+    def reorder_beams(self, block_tables: torch.Tensor, parents: torch.Tensor,
+                      ctx_lens: torch.Tensor, stream=None):
+        """Let the beams' cached states follow their parents, in place
+        (kvc_reorder_beams): block_tables (sequences * beams, pages), parents
+        (sequences, beams) and ctx_lens (sequences), int32 CUDA tensors."""
+        dev = self.device
+        if parents.dim() != 2 or block_tables.dim() != 2:
+            raise ValueError("parents and block_tables must have two dimensions")
+        n, beams = parents.shape
+        if block_tables.shape[0] != n * beams:
+            raise ValueError("block_tables needs one row per beam")
+        ffi.check(ffi.lib.kvc_reorder_beams(
+            self.handle, _on(block_tables, "block_tables", torch.int32, 0, dev),
+            block_tables.shape[1], _on(parents, "parents", torch.int32, 0, dev),
+            _on(ctx_lens, "ctx_lens", torch.int32, n, dev), n, beams, _stream_on(stream, dev)))
+
     def gather(self, layer: int, block_tables: torch.Tensor, row: int, start: int, count: int,
                stream=None):
         k = torch.empty((count, self.num_kv_heads, self.head_dim), dtype=self.dtype,
@@ -359,6 +578,34 @@ class BatchDecoder:
 
     def close(self):
         self.plan.close()
+
+
+# -- drafted trees --------------------------------------------------------------------
+def tree_masks(parents: Sequence[int], words: Optional[int] = None) -> np.ndarray:
+    """Mask rows (nodes, words) int32 of one drafted tree for decode_tree: node i sees
+    itself and its ancestors.  parents[i] is the node above i, smaller than i, or -1."""
+    n = len(parents)
+    need = max(1, (n + 31) // 32)
+    words = need if words is None else int(words)
+    if n > ffi.MAX_TREE_NODES or words < need:
+        raise ValueError(f"{n} nodes do not fit {words} mask words or the limit of "
+                         f"{ffi.MAX_TREE_NODES}")
+    m = np.zeros((n, words), dtype=np.uint32)
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError("a node's parent must be drafted before it (or be -1)")
+        if p >= 0:
+            m[i] = m[p]
+        m[i, i // 32] |= np.uint32(1 << (i % 32))
+    return m.view(np.int32)
+
+
+def tree_depths(parents: Sequence[int]) -> np.ndarray:
+    """Depth of each node: 0 for a node right behind the context."""
+    d = np.zeros(len(parents), dtype=np.int32)
+    for i, p in enumerate(parents):
+        d[i] = 0 if p < 0 else d[p] + 1
+    return d
 
 
 # -- layout helpers -------------------------------------------------------------------

@@ -524,6 +524,137 @@ KVC_API int kvc_forward_layer_paged(
     int intermediate_size, float rms_norm_eps, float rope_freq_base, int rope_neox, float scale,
     void* stream);
 
+/* ==== 6. Drafted tokens and beams on the paged pool =========================
+ * No counterpart in the reference (it decodes one token of one sequence at a
+ * time).  A verification step of speculative decoding runs, per layer,
+ * kvc_append_rope (the drafted tokens' rows into the cache slots behind the
+ * context) and kvc_decode_tree (every drafted token attends over the cached
+ * context and its own ancestors), or kvc_forward_layer_tree, which does the whole
+ * layer; kvc_commit_tree then moves the accepted path's rows together in every
+ * layer.  A step of beam search picks its continuations with kvc_beam_select and
+ * lets the cached states follow with kvc_reorder_beams.
+ * All pointers are device memory of the pool's (or handle's) device unless named
+ * h_*; work is enqueued on `stream`, with no host synchronisation; the current
+ * device of the calling thread is left as it was. */
+
+#define KVC_MAX_TREE_NODES 256 /* drafted tokens of one sequence */
+#define KVC_MAX_BEAMS 16
+#define KVC_MAX_BEAM_OUT 32
+
+typedef struct kvc_tree_plan kvc_tree_plan_t;
+typedef struct kvc_beam kvc_beam_t;
+
+/* Rotates n rows and appends them: for token i, K row = RoPE(d_k_new[i]) and V row
+ * = d_v_new[i] at slot d_positions[i] of block-table row d_rows[i] (NULL: row 0),
+ * and, when d_q is given, d_q_out[i] = RoPE(d_q[i]).  The angle of pair j is
+ * p / freq_base^(2j/head_dim), p = d_rope_positions[i] (NULL: d_positions[i]; a
+ * drafted token's depth differs from its slot), reduced in 64 bits and so exact at
+ * any position; the rotation is in 32 bits, rounded once to the pool's type.
+ * Pairs as in kvc_rope.  q_stride / k_stride / v_stride: elements between the
+ * tokens of d_q, d_k_new, d_v_new (0: packed), so they may be slices of one fused
+ * projection; d_q_out is packed and may be d_q when that is packed.  A negative
+ * d_positions[i] marks padding: nothing of token i is read or written.  Two
+ * tokens of one call must not name the same slot.  A row outside [0, bt_rows) or
+ * a slot past the table is reported (KVC_DEVERR_BAD_POSITION) and that token
+ * skipped, a bad page likewise (KVC_DEVERR_BAD_PAGE).  Pointers and strides are
+ * multiples of 16 bytes; head_dim even. */
+KVC_API int kvc_append_rope(kvc_pool_t* pool, int layer, const void* d_q, int q_stride,
+                            void* d_q_out, int num_heads, const void* d_k_new, int k_stride,
+                            const void* d_v_new, int v_stride, const int32_t* d_block_tables,
+                            int bt_rows, int bt_stride, const int32_t* d_rows,
+                            const int32_t* d_positions, const int32_t* d_rope_positions, int n,
+                            float freq_base, int neox, void* stream);
+
+/* The work list of one verification step, used by all its layers.  Sequence i has
+ * h_ctx_lens[i] cached positions and h_node_counts[i] drafted tokens (0 to
+ * KVC_MAX_TREE_NODES) whose K/V rows are in slots [ctx, ctx + nodes) of
+ * block-table row h_rows[i] (NULL: row i); its tokens follow those of sequence
+ * i - 1 in q, mask and out.  Built on the host and uploaded on `stream`. */
+KVC_API int kvc_tree_plan_create(kvc_tree_plan_t** out);
+KVC_API int kvc_tree_plan_destroy(kvc_tree_plan_t* plan);
+KVC_API int kvc_plan_tree(kvc_tree_plan_t* plan, const kvc_pool_t* pool, const int32_t* h_rows,
+                          const int32_t* h_ctx_lens, const int32_t* h_node_counts, int n_seqs,
+                          int num_heads, void* stream);
+/* Of the last build: tokens, CTAs of the attention kernel, bytes of split partials. */
+KVC_API int kvc_tree_plan_info(const kvc_tree_plan_t* plan, int* n_tokens, int* n_ctas,
+                               size_t* scratch_bytes);
+
+/* Attention of the drafted tokens for one layer.  d_q, d_out: (tokens, num_heads,
+ * head_dim) in the pool's type.  Token t of a sequence attends over its positions
+ * [0, ctx) and over the sequence's drafted tokens j whose bit is set in its mask
+ * row: bit j % 32 of d_mask[t * mask_words + j / 32].  Bits at or past the
+ * sequence's node count are ignored, and so are nodes past mask_words * 32.
+ * d_mask NULL: a chain, token t sees drafted tokens 0 .. t.  A token that sees
+ * nothing gets a zero row.  Scores, softmax statistics and sums are in fp32; 16-bit
+ * pools round the probabilities to the pool's type for the tensor cores.  The
+ * split partials live in the plan: calls sharing a plan must be ordered on one
+ * stream, and a captured call stays valid until its plan is built again. */
+KVC_API int kvc_decode_tree(kvc_pool_t* pool, const kvc_tree_plan_t* plan, int layer,
+                            const void* d_q, const int32_t* d_mask, int mask_words, void* d_out,
+                            const int32_t* d_block_tables, int bt_stride, float scale,
+                            void* stream);
+
+/* One transformer layer for the drafted tokens of a tree plan: kvc_forward_layer_paged
+ * with the rows appended by kvc_append_rope at the plan's slots, rotated at
+ * d_rope_positions (one per token; NULL: the slots), and the attention of
+ * kvc_decode_tree.  d_x_in / d_x_out: (tokens, hidden_size) fp16.  The activations
+ * live in a workspace of the plan. */
+KVC_API int kvc_forward_layer_tree(
+    kvc_pool_t* pool, kvc_tree_plan_t* plan, int layer_idx, const void* d_x_in, void* d_x_out,
+    const void* d_attn_norm_w, const void* d_wq, int wq_type, const void* d_wk, int wk_type,
+    const void* d_wv, int wv_type, const void* d_wo, int wo_type, const void* d_ffn_norm_w,
+    const void* d_wgate, int wgate_type, const void* d_wup, int wup_type, const void* d_wdown,
+    int wdown_type, const int32_t* d_mask, int mask_words, const int32_t* d_rope_positions,
+    const int32_t* d_block_tables, int bt_rows, int bt_stride, int hidden_size,
+    int intermediate_size, float rms_norm_eps, float rope_freq_base, int rope_neox, float scale,
+    void* stream);
+
+/* Keeps the accepted path of each sequence: in every layer, the K/V row of slot
+ * d_ctx_lens[i] + d_paths[i * path_stride + j] moves to slot d_ctx_lens[i] + j for
+ * j < d_path_lens[i], in block-table row d_rows[i] (NULL: row i).  Paths are
+ * strictly ascending node numbers (an ancestor is drafted before its children), at
+ * most path_stride long; a length of 0 keeps the sequence as it is.  Rows behind
+ * the path stay as they were.  A path that does not ascend or leaves the table is
+ * reported (KVC_DEVERR_BAD_POSITION) and its sequence left alone. */
+KVC_API int kvc_commit_tree(kvc_pool_t* pool, const int32_t* d_block_tables, int bt_rows,
+                            int bt_stride, const int32_t* d_rows, const int32_t* d_ctx_lens,
+                            const int32_t* d_paths, int path_stride, const int32_t* d_path_lens,
+                            int n_seqs, void* stream);
+
+/* Workspace for beam selections of up to max_seqs sequences, max_beams beams,
+ * max_vocab tokens and max_out results each, on `device`. */
+KVC_API int kvc_beam_create(int max_seqs, int max_beams, int max_vocab, int max_out, int device,
+                            kvc_beam_t** out);
+KVC_API int kvc_beam_destroy(kvc_beam_t* beam);
+
+/* The n_out best continuations of each sequence, best first: candidate (b, t) has
+ * the score d_scores_in[seq, b] + log softmax(logits of row seq * n_beams + b)[t].
+ * d_logits: rows of `vocab` values in `dtype` (KVC_DTYPE_*), row_stride elements
+ * apart (0: vocab).  d_tokens, d_parents (beam numbers within the sequence) and
+ * d_scores_out: (n_seqs, n_out).  Equal scores go to the lower beam, then the
+ * lower token.  A logit that is not finite takes no part in the softmax and scores
+ * -inf, and so does every token of a beam whose score is not finite (a beam that
+ * is not in use yet).  n_beams * vocab must be at least n_out.  Calls sharing a handle must be ordered
+ * on one stream. */
+KVC_API int kvc_beam_select(kvc_beam_t* beam, const void* d_logits, int dtype, int64_t row_stride,
+                            const float* d_scores_in, int n_seqs, int n_beams, int vocab,
+                            int n_out, int32_t* d_tokens, int32_t* d_parents,
+                            float* d_scores_out, void* stream);
+
+/* Lets the cached states of beams follow their parents, in place and in every
+ * layer.  Beam b of sequence s owns block-table row s * n_beams + b; all beams of a
+ * sequence have d_ctx_lens[s] cached positions.  Row b's entries of full pages
+ * become those of row d_parents[s, b]; the positions of the last, partly filled
+ * page are copied into the page that row b names there, which must be a page of
+ * its own (the other rows' differ).  Entries behind that stay as they were.  So each
+ * beam needs one page of its own per page of positions, and no page is ever copied
+ * once it is full.  A parent, context or page out of range, or a partly filled page
+ * that two beams name, is reported (KVC_DEVERR_BAD_POSITION / _BAD_PAGE) and the
+ * sequence left alone. */
+KVC_API int kvc_reorder_beams(kvc_pool_t* pool, int32_t* d_block_tables, int bt_stride,
+                              const int32_t* d_parents, const int32_t* d_ctx_lens, int n_seqs,
+                              int n_beams, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
