@@ -6,6 +6,7 @@
 // its mask row names.  The (node, q-head) pairs of one KV head are the rows of one
 // tile, so a K/V byte is read once for all drafted tokens and the whole head group.
 //
+//   tree_mma_kernel     tcgen05 tensor cores: 16-bit pools, head dims 32 ... 256
 //   tree_simt_kernel    CUDA cores: fp32 pools and head dims without a tensor tile
 //   tree_merge_kernel   joins the pieces of rows whose positions were split over CTAs
 #include <cuda_runtime.h>
@@ -13,9 +14,11 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kvc_device.cuh"
 #include "kvc_spec.h"
+#include "kvc_tcgen05.cuh"
 #include "kvcache.h"
 
 namespace kvc {
@@ -40,6 +43,511 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
   const int w = j >> 5;
   return w < a.mask_words &&
          ((a.mask[static_cast<size_t>(tok0 + node) * a.mask_words + w] >> (j & 31)) & 1u);
+}
+
+// =====================================================================================
+// Tensor-core kernel.  One CTA per SM; each takes its share of the plan's position tiles.
+//
+// A tile of kTilePos positions of K and of V arrives by bulk copies, slab by slab, in the
+// pool's own layout: 8-position x 16-byte core matrices, which is the unswizzled
+// operand layout of tcgen05.mma, k-major for K (S = Q K^T) and mn-major for V (O = P V),
+// so nothing is rearranged.  S, P and O live in tensor memory; P takes the place of its S.
+//
+// Two streams share the tensor cores, each with a softmax warpgroup whose thread r owns
+// row r (tensor memory lane r), so that one stream's softmax runs under the other's
+// products.  With more than 128 rows the streams are the two halves of the rows and each
+// tile serves both; with fewer they are the even and the odd tiles of the same rows,
+// joined when the piece ends.  (Head dims above 128 fill tensor memory with one stream.)
+//
+// O is rescaled only when a row's max has grown by more than 2^8 since the last time: the
+// probabilities then stay below 2^8 and a tile normally touches O with the MMA alone.
+//
+// Warps: 0 brings K/V tiles into a ring of stages, 1 (one thread) issues the MMAs,
+// 4 ... 11 are the two softmax warpgroups.  Every wait is bounded; a wait that gives up
+// raises the CTA's abort flag, all roles then run through their loops without waiting,
+// copying or issuing, and the kernel returns.
+// =====================================================================================
+constexpr int kTmemCols = 512;
+constexpr float kRescaleAt = 8.0f;   // log2
+
+template <int D>
+struct TreeShape {
+  static constexpr int kStreams = D <= 128 ? 2 : 1;
+  static constexpr int kPos = D <= 128 ? 128 : 64;               // positions of a tile
+  static constexpr int kThreads = 128 + 128 * kStreams;
+  static constexpr int kStageBytes = kPos * D * 2;
+  static constexpr int kQBytes = 128 * D * 2;
+  static constexpr int kHeadBytes = 3072;                        // barriers, exchange
+  static constexpr int kFit = (232448 - kHeadBytes - kStreams * kQBytes) / kStageBytes;
+  static constexpr int kStages = kFit > 12 ? 12 : kFit;
+  static constexpr int kSmem = kHeadBytes + kStreams * kQBytes + kStages * kStageBytes;
+};
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t h) {
+  constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (h & e) == e;
+}
+
+// Mask word k (drafted tokens 32 k ... 32 k + 31) of a row; below 0: cached positions.
+__device__ __forceinline__ uint32_t mask_word(const TreeArgs& a, const TreeSeg& sg, int node, int k) {
+  if (k < 0) return 0xffffffffu;
+  const int left = sg.nodes - 32 * k;
+  if (left <= 0) return 0u;
+  uint32_t w;
+  if (a.mask) {
+    w = k < a.mask_words ? a.mask[static_cast<size_t>(sg.tok0 + node) * a.mask_words + k] : 0u;
+  } else {
+    const int upto = node - 32 * k;  // a chain
+    w = upto < 0 ? 0u : (upto >= 31 ? 0xffffffffu : (2u << upto) - 1u);
+  }
+  return left < 32 ? w & ((1u << left) - 1u) : w;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(const TreeArgs a) {
+  using S = TreeShape<D>;
+  constexpr int U = D / 8, KP = S::kPos;
+  constexpr uint32_t kSlabBytes = kSlab * D * 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+  volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(smem + 512);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + 516);
+  volatile int* s_dirty = reinterpret_cast<volatile int*>(smem + 520);   // [2]
+  float2* s_ml = reinterpret_cast<float2*>(smem + 1024);                 // [2][128]
+  uint8_t* q_mem = smem + S::kHeadBytes;
+  uint8_t* stage_mem = q_mem + S::kStreams * S::kQBytes;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](int st) { return bar0 + 8u * st; };
+  auto empty = [&](int st) { return bar0 + 8u * (12 + st); };
+  auto s_ready = [&](int x) { return bar0 + 8u * (24 + x); };
+  auto p_ready = [&](int x) { return bar0 + 8u * (26 + x); };
+  auto q_ready = [&](int x) { return bar0 + 8u * (28 + x); };
+  auto o_ready = [&](int x) { return bar0 + 8u * (30 + x); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int st = 0; st < S::kStages; ++st) {
+      mbar_init(full(st), 1);
+      mbar_init(empty(st), 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(s_ready(x), 1);
+      mbar_init(p_ready(x), 128);
+      mbar_init(q_ready(x), 128);
+      mbar_init(o_ready(x), 1);
+    }
+    fence_mbar_init();
+    *s_abort = 0;
+    s_dirty[0] = s_dirty[1] = -1;
+  }
+  if (warp == 1) tmem_alloc(smem_u32(s_tmem), kTmemCols);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  // false: some wait of this CTA gave up
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+#pragma unroll 1
+      for (int i = 0; i < 64; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+      if (*s_abort) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        report_error_at(a.p.err, KVC_DEVERR_WAIT_LIMIT, blockIdx.x);
+        *s_abort = 1;
+        return false;
+      }
+    }
+  };
+  const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
+
+  if (warp == 0) {
+    // ---- K/V tiles into the ring, in the order the MMAs take them -----------------------
+    const uint64_t policy = l2_policy_evict_first();
+    uint32_t n = 0;  // tiles issued
+    bool ok = true;
+    for (int si = seg0; si < seg1 && ok; ++si) {
+      const TreeSeg sg = a.segs[si];
+      const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
+      const int ahead = S::kStreams == 2 && sg.rows <= 128 ? 2 : 1;  // K runs this far ahead
+      for (int step = 0; step < tiles + ahead && ok; ++step) {
+        // step: V of tile step - ahead, then K of tile step
+        for (int kv = 1; kv >= 0 && ok; --kv) {
+          const int t = kv ? step - ahead : step;
+          if (t < 0 || t >= tiles) continue;
+          const int p0 = (sg.tile0 + t) * KP + lane * kSlab;
+          const int slabs = min(KP / kSlab, (end - (sg.tile0 + t) * KP + kSlab - 1) / kSlab);
+          const uint8_t* src = nullptr;
+          if (lane < slabs) {
+            const int page = tree_page(a.p, sg.bt_row, p0);
+            src = (kv ? a.p.v : a.p.k) +
+                  (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) * a.p.page_head_bytes +
+                  static_cast<size_t>(p0 % a.p.page_size / kSlab) * kSlabBytes;
+          }
+          const int st = n % S::kStages;
+          if (n >= S::kStages) ok = wait(empty(st), (n / S::kStages - 1) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(full(st), slabs * kSlabBytes);
+          __syncwarp();
+          if (lane < slabs)
+            bulk_g2s(smem_u32(stage_mem) + st * S::kStageBytes + lane * kSlabBytes, src, kSlabBytes,
+                     full(st), policy);
+          ++n;
+        }
+      }
+    }
+    if (!ok) {  // copies in flight land before the CTA's memory goes
+      for (uint32_t i = n > S::kStages ? n - S::kStages : 0; i < n; ++i)
+        mbar_wait_bounded(full(i % S::kStages), (i / S::kStages) & 1);
+    }
+  } else if (warp == 1) {
+    // ---- MMAs, one thread -----------------------------------------------------------------
+    if (lane == 0) {
+      constexpr uint32_t kDescS = mma_desc<T>(128, KP, false);
+      constexpr uint32_t kDescO = mma_desc<T>(128, D, true);
+      uint32_t n = 0;                       // ring tiles consumed
+      uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
+      bool ok = true;
+      auto scores = [&](int x, int st) {    // S_x = Q_x K^T
+        const uint64_t qd = operand_desc(smem_u32(q_mem) + x * S::kQBytes, 128, U * 128);
+        const uint64_t kd = operand_desc(smem_u32(stage_mem) + st * S::kStageBytes, 128, U * 128);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)    // 16 dims: two core matrices on
+          mma_ss(tmem + x * 128, qd + 16 * k, kd + 16 * k, kDescS, k > 0);
+        mma_commit(s_ready(x));
+      };
+      auto sums = [&](int x, int st, int slabs, bool accumulate) {   // O_x += P_x V
+        const uint64_t vd = operand_desc(smem_u32(stage_mem) + st * S::kStageBytes, U * 128, 128);
+        for (int k = 0; k < slabs; ++k)
+          mma_ts(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
+                 accumulate || k > 0);
+      };
+      for (int si = seg0; si < seg1 && ok; ++si) {
+        const TreeSeg sg = a.segs[si];
+        const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
+        const bool two = sg.rows > 128;
+        const int ahead = S::kStreams == 2 && !two ? 2 : 1;
+        auto take = [&]() -> int {          // the next tile of the ring
+          const int st = n % S::kStages;
+          ok = ok && wait(full(st), (n / S::kStages) & 1);
+          ++n;
+          return st;
+        };
+        auto slabs_of = [&](int t) {
+          return min(KP / kSlab, (end - (sg.tile0 + t) * KP + kSlab - 1) / kSlab);
+        };
+        if (two) {
+          ok = ok && wait(q_ready(0), nq[0]++ & 1) && wait(q_ready(1), nq[1]++ & 1);
+          int kst = take();
+          if (!ok) break;
+          scores(0, kst);
+          scores(1, kst);
+          mma_commit(empty(kst));
+          for (int t = 0; t < tiles && ok; ++t) {
+            const int vst = take();
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              ok = ok && wait(p_ready(x), np[x]++ & 1);
+              if (!ok) break;
+              tmem_fence_after();
+              sums(x, vst, slabs_of(t), t > 0);
+              if (x == 1) mma_commit(empty(vst));
+              if (t + 1 == tiles) mma_commit(o_ready(x));
+              if (t + 1 < tiles) {
+                if (x == 0) kst = take();
+                if (!ok) break;
+                scores(x, kst);
+                if (x == 1) mma_commit(empty(kst));
+              }
+            }
+          }
+        } else {
+          for (int x = 0; x < ahead && x < tiles && ok; ++x) {
+            ok = ok && wait(q_ready(x), nq[x]++ & 1);
+            const int kst = take();
+            if (!ok) break;
+            scores(x, kst);
+            mma_commit(empty(kst));
+          }
+          for (int t = 0; t < tiles && ok; ++t) {
+            const int x = ahead == 2 ? t & 1 : 0;
+            const int vst = take();
+            ok = ok && wait(p_ready(x), np[x]++ & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            sums(x, vst, slabs_of(t), t >= ahead);
+            mma_commit(empty(vst));
+            if (t + ahead < tiles) {
+              const int kst = take();
+              if (!ok) break;
+              scores(x, kst);
+              mma_commit(empty(kst));
+            } else {
+              mma_commit(o_ready(x));
+            }
+          }
+        }
+      }
+      if (!ok) {  // MMAs in flight end before tensor memory is freed
+        mbar_init(bar0 + 8u * 40, 1);
+        fence_mbar_init();
+        mma_commit(bar0 + 8u * 40);
+        mbar_wait_bounded(bar0 + 8u * 40, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---- softmax: thread r of stream x owns row r ---------------------------------------------
+    const int x = (warp - 4) >> 2, w4 = warp & 3, r = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
+    const uint32_t t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * 128;
+    const float sc = fabsf(a.scale_log2);
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale turns q
+    uint32_t ns = 0, no[2] = {0, 0}, nv = 0;
+    bool ok = true;
+    for (int si = seg0; si < seg1; ++si) {
+      const TreeSeg sg = a.segs[si];
+      const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
+      const bool two = sg.rows > 128;
+      const int ahead = S::kStreams == 2 && !two ? 2 : 1;
+      const bool joint = ahead == 2;
+      const int row = (two ? x * 128 : 0) + r;
+      const bool live_row = row < sg.rows;
+      const bool live = (two ? x * 128 : 0) + w4 * 32 < sg.rows;   // some row of the warp
+      const int grow = sg.row0 + min(row, sg.rows - 1);
+      const int node = grow / a.group, head = sg.kvh * a.group + grow - node * a.group;
+      const size_t io_row = (static_cast<size_t>(sg.tok0 + node) * a.num_heads + head) * D;
+      const uint32_t seg_tiles0 = nv;   // ring index of the segment's first tile
+      nv += 2 * tiles;
+      const bool mine = !joint || x < tiles;   // the stream has tiles of this piece
+      if (mine) {
+        // Q, k-major core matrices; a piece's scores are done before the next piece's Q comes
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + io_row);
+        uint8_t* dst = q_mem + x * S::kQBytes + (r >> 3) * U * 128 + (r & 7) * 16;
+#pragma unroll 8
+        for (int u = 0; u < U; ++u) {
+          uint4 v = live_row ? src[u] : make_uint4(0, 0, 0, 0);
+          v.x ^= flip;
+          v.y ^= flip;
+          v.z ^= flip;
+          v.w ^= flip;
+          *reinterpret_cast<uint4*>(dst + u * 128) = v;
+        }
+        fence_proxy_async();
+        mbar_arrive(q_ready(x));
+      }
+      float m = kNegBig, l = 0.f;     // max in log2 units
+      for (int t = joint ? x : 0; t < tiles; t += ahead) {
+        ok = ok && wait(s_ready(x), ns & 1);
+        ++ns;
+        tmem_fence_after();
+        const int p0 = (sg.tile0 + t) * KP;
+        const bool edge = p0 + KP > sg.ctx;
+        if (live) {
+          uint32_t s[KP];
+#pragma unroll
+          for (int c = 0; c < KP; c += 32) tmem_ld32(t_s + c, s + c);
+          uint32_t vis[KP / 32];
+          if (edge) {
+#pragma unroll
+            for (int w = 0; w < KP / 32; ++w) {
+              const int j0 = p0 + 32 * w - sg.ctx;
+              const int k = j0 >> 5;
+              vis[w] = __funnelshift_r(mask_word(a, sg, node, k), mask_word(a, sg, node, k + 1), j0 & 31);
+            }
+          }
+          tmem_wait_ld();
+          tmem_loaded<KP>(s);
+          float mx = -INFINITY;
+          if (edge) {
+#pragma unroll
+            for (int c = 0; c < KP; ++c)
+              mx = fmaxf(mx, (vis[c >> 5] >> (c & 31)) & 1u ? __uint_as_float(s[c]) : -INFINITY);
+          } else {
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < KP; c += 4)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], __uint_as_float(s[c + i]));
+            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          }
+          const float mt = mx == -INFINITY ? kNegBig : mx * sc;
+          const bool first = t < ahead;
+          const bool grew = mt > m + kRescaleAt;
+          if (__any_sync(0xffffffffu, grew)) {
+            const float m2 = grew ? mt : m;
+            const float f = fast_exp2(m - m2);
+            m = m2;
+            l *= f;
+            if (!first) {  // the sums of earlier tiles are complete: the scores came after them
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(t_o + c, o);
+                tmem_wait_ld();
+                tmem_loaded<16>(o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st16(t_o + c, o);
+              }
+            }
+          }
+          float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < KP; c += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float p0f = fast_exp2(fmaf(__uint_as_float(s[c + i]), sc, -m));
+              float p1f = fast_exp2(fmaf(__uint_as_float(s[c + i + 1]), sc, -m));
+              if (edge) {
+                if (!((vis[c >> 5] >> i) & 1u)) p0f = 0.f;
+                if (!((vis[c >> 5] >> (i + 1)) & 1u)) p1f = 0.f;
+              }
+              l4[i & 3] += p0f;
+              l4[(i & 3) + 1] += p1f;
+              pk[i / 2] = Mma<T>::pack(p0f, p1f);
+            }
+            tmem_st16(t_s + c / 2, pk);
+          }
+          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          tmem_wait_st();
+        }
+        if (edge) {
+          // V of the drafted tokens: what is not finite would spread through zero weights
+          // to rows that do not see it, so it leaves the tile here (and comes back at the
+          // end, to the rows that do); positions past the end hold anything, and go to zero.
+          // ring order of the piece: `ahead` K tiles, then V t, K t + ahead, ...
+          const uint32_t vi = seg_tiles0 + min(ahead, tiles) + t + min(t, max(tiles - ahead, 0));
+          const int st = vi % S::kStages;
+          ok = ok && wait(full(st), (vi / S::kStages) & 1);
+          uint8_t* vt = stage_mem + st * S::kStageBytes;
+          const int from = max(0, sg.ctx - p0), to = min(KP, (end - p0 + kSlab - 1) / kSlab * kSlab);
+          bool dirty = false;
+          for (int i = from * U + r; i < to * U; i += 128) {
+            const int pt = i / U, u = i - pt * U;
+            uint4* cell = reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            bool bad = p0 + pt >= end;
+            if (!bad) {
+              v = *cell;
+              uint32_t* e = &v.x;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (not_finite<T>(e[k] & 0xffffu)) e[k] &= 0xffff0000u, bad = dirty = true;
+                if (not_finite<T>(e[k] >> 16)) e[k] &= 0x0000ffffu, bad = dirty = true;
+              }
+            }
+            if (dirty) {
+              s_dirty[si & 1] = si;
+              __threadfence_block();
+            }
+            if (bad) *cell = v;
+          }
+          __threadfence_block();
+          fence_proxy_async();
+        }
+        tmem_fence_before();
+        mbar_arrive(p_ready(x));
+      }
+      // ---- the piece's rows leave tensor memory -----------------------------------------------
+      if (joint) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          if (y < tiles) {
+            ok = ok && wait(o_ready(y), no[y] & 1);
+            ++no[y];
+          }
+        s_ml[x * 128 + r] = make_float2(m, l);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      } else {
+        ok = ok && wait(o_ready(x), no[x] & 1);
+        ++no[0];
+        if (two) ++no[1];
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      tmem_fence_after();
+      if (live && ok) {
+        float w0 = 1.f, w1 = 0.f, mm = m, ll = l;
+        if (joint) {
+          const float2 e0 = s_ml[r], e1 = s_ml[128 + r];
+          mm = fmaxf(e0.x, e1.x);
+          w0 = fast_exp2(e0.x - mm);
+          w1 = fast_exp2(e1.x - mm);
+          ll = e0.y * w0 + e1.y * w1;
+        }
+        const bool dirty = s_dirty[si & 1] == si;
+        const int c0 = joint ? x * (D / 2) : 0, c1 = joint ? c0 + D / 2 : D;
+        const uint32_t o0 = tmem + lanes + 256 + (joint ? 0 : x * 128);
+        const float inv = ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);
+        if (live_row && sg.part >= 0 && (!joint || x == 0))
+          a.part_ml[sg.part + row] = make_float2(mm, ll);
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 16) {
+          uint32_t o[16];
+          float f[16];
+          tmem_ld16(o0 + c, o);
+          if (joint && tiles > 1) {
+            uint32_t q[16];
+            tmem_ld16(o0 + 128 + c, q);
+            tmem_wait_ld();
+            tmem_loaded<16>(o);
+            tmem_loaded<16>(q);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              f[i] = __uint_as_float(o[i]) * w0 + __uint_as_float(q[i]) * w1;
+          } else {
+            tmem_wait_ld();
+            tmem_loaded<16>(o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]);
+          }
+          if (live_row) {
+          if (dirty) {  // rare: add what was taken out of V, for the nodes this row sees
+            const int t0 = max(sg.tile0 * KP, sg.ctx), t1 = min(sg.tile1 * KP, end);
+            for (int pos = t0; pos < t1; ++pos) {
+              const int j = pos - sg.ctx;
+              if (!((mask_word(a, sg, node, j >> 5) >> (j & 31)) & 1u)) continue;
+              const int page = tree_page(a.p, sg.bt_row, pos);
+              const uint8_t* vrow = a.p.v + (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) *
+                                                a.p.page_head_bytes;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const T e = reinterpret_cast<const T*>(
+                    vrow + unit_offset(kLayoutCore, pos % a.p.page_size, (c + i) / 8, U) * 16)[(c + i) % 8];
+                const float v = to_f32<T>(e);
+                if (!isfinite(v)) f[i] += v;
+              }
+            }
+          }
+          if (sg.part >= 0) {
+            float4* po = reinterpret_cast<float4*>(a.part_o + static_cast<size_t>(sg.part + row) * D + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) po[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+          } else {
+            uint32_t pk[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pk[i] = Mma<T>::pack(f[2 * i] * inv, f[2 * i + 1] * inv);
+            uint4* po = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + io_row + c);
+            po[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            po[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+          }
+          }
+          __syncwarp();
+        }
+      }
+      tmem_fence_before();
+      if (joint) asm volatile("bar.sync 1, 256;" ::: "memory");  // both streams' sums are read
+      tmem_fence_after();
+    }
+  }
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
 // =====================================================================================
@@ -254,10 +762,39 @@ cudaError_t run_simt(const TreeArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+template <typename T, int D>
+cudaError_t run_mma(const TreeArgs& a, cudaStream_t s) {
+  using S = TreeShape<D>;
+  const cudaError_t e = allow_smem<tree_mma_kernel<T, D>>(S::kSmem);
+  if (e != cudaSuccess) return e;
+  tree_mma_kernel<T, D><<<a.n_ctas, S::kThreads, S::kSmem, s>>>(a);
+  return cudaGetLastError();
+}
+
 template <typename T>
-cudaError_t run_tree(const TreeArgs& a, const TreeTile&, cudaStream_t s) {
+cudaError_t run_mma_any(const TreeArgs& a, cudaStream_t s) {
+  switch (a.head_dim) {
+    case 32: return run_mma<T, 32>(a, s);
+    case 64: return run_mma<T, 64>(a, s);
+    case 96: return run_mma<T, 96>(a, s);
+    case 128: return run_mma<T, 128>(a, s);
+    case 160: return run_mma<T, 160>(a, s);
+    case 192: return run_mma<T, 192>(a, s);
+    case 256: return run_mma<T, 256>(a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+template <>
+cudaError_t run_mma_any<float>(const TreeArgs&, cudaStream_t) {
+  return cudaErrorInvalidValue;
+}
+
+template <typename T>
+cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
   cudaError_t e;
-  if (a.head_dim <= 64)
+  if (t.tensor)
+    e = run_mma_any<T>(a, s);
+  else if (a.head_dim <= 64)
     e = run_simt<T, 2>(a, s);
   else if (a.head_dim <= 128)
     e = run_simt<T, 4>(a, s);
@@ -272,7 +809,11 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile&, cudaStream_t s) {
 
 }  // namespace
 
-TreeTile tree_tile(const PoolGeom&) { return TreeTile{kSimtPos, kSimtRows, 2, false}; }
+TreeTile tree_tile(const PoolGeom& g) {
+  if (decode_uses_mma(g.dtype, g.head_dim, g.page_size) && g.layout == kLayoutCore)
+    return g.head_dim <= 128 ? TreeTile{128, 256, 1, true} : TreeTile{64, 128, 1, true};
+  return TreeTile{kSimtPos, kSimtRows, 2, false};
+}
 
 cudaError_t launch_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
   if (a.n_ctas <= 0) return cudaSuccess;
