@@ -206,99 +206,122 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         mbar_wait_bounded(full(i % S::kStages), (i / S::kStages) & 1);
     }
   } else if (warp == 1) {
-    // ---- MMAs, one thread -----------------------------------------------------------------
-    if (lane == 0) {
-      constexpr uint32_t kDescS = mma_desc<T>(128, KP, false);
-      constexpr uint32_t kDescO = mma_desc<T>(128, D, true);
-      uint32_t n = 0;                       // ring tiles consumed
-      uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
-      bool ok = true;
-      auto scores = [&](int x, int st) {    // S_x = Q_x K^T
-        const uint64_t qd = operand_desc(smem_u32(q_mem) + x * S::kQBytes, 128, U * 128);
-        const uint64_t kd = operand_desc(smem_u32(stage_mem) + st * S::kStageBytes, 128, U * 128);
+    // ---- MMAs: the warp waits together, one lane issues.  Everything an MMA takes is
+    // the same in all lanes (broadcast where the compiler could not tell), so it sits in
+    // uniform registers: with operands in ordinary ones an issue took over 100 cycles,
+    // twice as long as the MMA itself.
+    constexpr uint32_t kDescS = mma_desc<T>(128, KP, false);
+    constexpr uint32_t kDescO = mma_desc<T>(128, D, true);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t q_desc = operand_desc(smem_u32(q_mem), 128, U * 128);
+    const uint64_t k_desc = operand_desc(smem_u32(stage_mem), 128, U * 128);
+    const uint64_t v_desc = operand_desc(smem_u32(stage_mem), U * 128, 128);
+    const bool leader = elect_one();
+    uint32_t n = 0;                       // ring tiles consumed
+    uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
+    bool ok = true;
+    auto wait_all = [&](uint32_t bar, uint32_t parity) {
+      ok = __all_sync(0xffffffffu, ok && wait(bar, parity));
+    };
+    auto take = [&]() -> int {            // the next tile of the ring
+      const int st = n % S::kStages;
+      wait_all(full(st), (n / S::kStages) & 1);
+      ++n;
+      return st;
+    };
+    auto commit = [&](uint32_t bar) {
+      if (leader) mma_commit(bar);
+    };
+    auto scores = [&](int x, int st) {    // S_x = Q_x K^T
+      const uint64_t qd = q_desc + x * (S::kQBytes / 16), kd = k_desc + st * (S::kStageBytes / 16);
+      if (leader) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)    // 16 dims: two core matrices on
-          mma_ss(tmem + x * 128, qd + 16 * k, kd + 16 * k, kDescS, k > 0);
+        for (int k = 0; k < D / 16; ++k)  // 16 dims: two core matrices on
+          mma_ss(tm + x * 128, qd + 16 * k, kd + 16 * k, kDescS, k > 0);
         mma_commit(s_ready(x));
-      };
-      auto sums = [&](int x, int st, int slabs, bool accumulate) {   // O_x += P_x V
-        const uint64_t vd = operand_desc(smem_u32(stage_mem) + st * S::kStageBytes, U * 128, 128);
-        for (int k = 0; k < slabs; ++k)
-          mma_ts(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
-                 accumulate || k > 0);
-      };
-      for (int si = seg0; si < seg1 && ok; ++si) {
-        const TreeSeg sg = a.segs[si];
-        const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
-        const bool two = sg.rows > 128;
-        const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-        auto take = [&]() -> int {          // the next tile of the ring
-          const int st = n % S::kStages;
-          ok = ok && wait(full(st), (n / S::kStages) & 1);
-          ++n;
-          return st;
-        };
-        auto slabs_of = [&](int t) {
-          return min(KP / kSlab, (end - (sg.tile0 + t) * KP + kSlab - 1) / kSlab);
-        };
-        if (two) {
-          ok = ok && wait(q_ready(0), nq[0]++ & 1) && wait(q_ready(1), nq[1]++ & 1);
-          int kst = take();
-          if (!ok) break;
-          scores(0, kst);
-          scores(1, kst);
-          mma_commit(empty(kst));
-          for (int t = 0; t < tiles && ok; ++t) {
-            const int vst = take();
+      }
+    };
+    auto sums = [&](int x, int st, int slabs, bool accumulate) {   // O_x += P_x V
+      const uint64_t vd = v_desc + st * (S::kStageBytes / 16);
+      if (leader) {
+        if (slabs == KP / kSlab) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              ok = ok && wait(p_ready(x), np[x]++ & 1);
-              if (!ok) break;
-              tmem_fence_after();
-              sums(x, vst, slabs_of(t), t > 0);
-              if (x == 1) mma_commit(empty(vst));
-              if (t + 1 == tiles) mma_commit(o_ready(x));
-              if (t + 1 < tiles) {
-                if (x == 0) kst = take();
-                if (!ok) break;
-                scores(x, kst);
-                if (x == 1) mma_commit(empty(kst));
-              }
-            }
-          }
+          for (int k = 0; k < KP / kSlab; ++k)
+            mma_ts(tm + 256 + x * 128, tm + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
+                   accumulate || k > 0);
         } else {
-          for (int x = 0; x < ahead && x < tiles && ok; ++x) {
-            ok = ok && wait(q_ready(x), nq[x]++ & 1);
-            const int kst = take();
-            if (!ok) break;
-            scores(x, kst);
-            mma_commit(empty(kst));
-          }
-          for (int t = 0; t < tiles && ok; ++t) {
-            const int x = ahead == 2 ? t & 1 : 0;
-            const int vst = take();
-            ok = ok && wait(p_ready(x), np[x]++ & 1);
+#pragma unroll 1
+          for (int k = 0; k < slabs; ++k)
+            mma_ts(tm + 256 + x * 128, tm + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
+                   accumulate || k > 0);
+        }
+      }
+    };
+    for (int si = seg0; si < seg1 && ok; ++si) {
+      const TreeSeg sg = a.segs[si];
+      const int tiles = __shfl_sync(0xffffffffu, sg.tile1 - sg.tile0, 0);
+      const int left = __shfl_sync(0xffffffffu, sg.ctx + sg.nodes - sg.tile0 * KP, 0);
+      const bool two = __shfl_sync(0xffffffffu, sg.rows, 0) > 128;
+      const int ahead = S::kStreams == 2 && !two ? 2 : 1;
+      auto slabs_of = [&](int t) { return min(KP / kSlab, (left - t * KP + kSlab - 1) / kSlab); };
+      if (two) {
+        wait_all(q_ready(0), nq[0]++ & 1);
+        wait_all(q_ready(1), nq[1]++ & 1);
+        int kst = take();
+        if (!ok) break;
+        scores(0, kst);
+        scores(1, kst);
+        commit(empty(kst));
+        for (int t = 0; t < tiles && ok; ++t) {
+          const int vst = take();
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            wait_all(p_ready(x), np[x]++ & 1);
             if (!ok) break;
             tmem_fence_after();
-            sums(x, vst, slabs_of(t), t >= ahead);
-            mma_commit(empty(vst));
-            if (t + ahead < tiles) {
-              const int kst = take();
+            sums(x, vst, slabs_of(t), t > 0);
+            if (x == 1) commit(empty(vst));
+            if (t + 1 == tiles) commit(o_ready(x));
+            if (t + 1 < tiles) {
+              if (x == 0) kst = take();
               if (!ok) break;
               scores(x, kst);
-              mma_commit(empty(kst));
-            } else {
-              mma_commit(o_ready(x));
+              if (x == 1) commit(empty(kst));
             }
           }
         }
+      } else {
+        for (int x = 0; x < ahead && x < tiles && ok; ++x) {
+          wait_all(q_ready(x), nq[x]++ & 1);
+          const int kst = take();
+          if (!ok) break;
+          scores(x, kst);
+          commit(empty(kst));
+        }
+        for (int t = 0; t < tiles && ok; ++t) {
+          const int x = ahead == 2 ? t & 1 : 0;
+          const int vst = take();
+          wait_all(p_ready(x), np[x]++ & 1);
+          if (!ok) break;
+          tmem_fence_after();
+          sums(x, vst, slabs_of(t), t >= ahead);
+          commit(empty(vst));
+          if (t + ahead < tiles) {
+            const int kst = take();
+            if (!ok) break;
+            scores(x, kst);
+            commit(empty(kst));
+          } else {
+            commit(o_ready(x));
+          }
+        }
       }
-      if (!ok) {  // MMAs in flight end before tensor memory is freed
-        mbar_init(bar0 + 8u * 40, 1);
-        fence_mbar_init();
-        mma_commit(bar0 + 8u * 40);
-        mbar_wait_bounded(bar0 + 8u * 40, 0);
-      }
+    }
+    if (!ok && leader) {  // MMAs in flight end before tensor memory is freed
+      mbar_init(bar0 + 8u * 40, 1);
+      fence_mbar_init();
+      mma_commit(bar0 + 8u * 40);
+      mbar_wait_bounded(bar0 + 8u * 40, 0);
     }
     __syncwarp();
   } else if (warp >= 4) {
@@ -342,6 +365,83 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         mbar_arrive(q_ready(x));
       }
       float m = kNegBig, l = 0.f;     // max in log2 units
+      // One tile of the stream: scores to probabilities, in place, and the running max and
+      // sum.  Edge tiles hold positions that some rows do not see.
+      auto softmax = [&](auto edge_tag, int t, int p0) {
+        constexpr bool kEdge = decltype(edge_tag)::value;
+        // The scores are read from tensor memory twice, 32 columns at a time with the next
+        // 32 on their way: a whole row in registers would spill.
+        uint32_t s[2][32];
+        tmem_ld32(t_s, s[0]);
+        uint32_t vis[KP / 32];
+        if constexpr (kEdge) {
+#pragma unroll
+          for (int w = 0; w < KP / 32; ++w) {
+            const int j0 = p0 + 32 * w - sg.ctx;
+            const int k = j0 >> 5;
+            vis[w] = __funnelshift_r(mask_word(a, sg, node, k), mask_word(a, sg, node, k + 1), j0 & 31);
+          }
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int w = 0; w < KP / 32; ++w) {
+          uint32_t* now = s[w & 1];
+          tmem_wait_ld();
+          tmem_loaded<32>(now);
+          // (behind the last columns come the first again, for the second reading)
+          tmem_ld32(t_s + (w + 1 < KP / 32 ? 32 * (w + 1) : 0), s[(w + 1) & 1]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (!kEdge || ((vis[w] >> i) & 1u)) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(now[i]));
+          }
+        }
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float mt = mx == -INFINITY ? kNegBig : mx * sc;
+        const bool grew = mt > m + kRescaleAt;
+        if (__any_sync(0xffffffffu, grew)) {
+          const float m2 = grew ? mt : m;
+          const float f = fast_exp2(m - m2);
+          m = m2;
+          l *= f;
+          if (t >= ahead) {  // the sums of earlier tiles are complete: the scores came after them
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c, o);
+              tmem_wait_ld();
+              tmem_loaded<16>(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(t_o + c, o);
+            }
+          }
+        }
+        const float2 sc2 = make_float2(sc, sc), m2 = make_float2(-m, -m);
+        float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int w = 0; w < KP / 32; ++w) {
+          const uint32_t* now = s[w & 1];
+          tmem_wait_ld();
+          tmem_loaded<32>(s[w & 1]);
+          if (w + 1 < KP / 32) tmem_ld32(t_s + 32 * (w + 1), s[(w + 1) & 1]);
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 e = fma2(make_float2(__uint_as_float(now[i]), __uint_as_float(now[i + 1])), sc2, m2);
+            e.x = fast_exp2(e.x);
+            e.y = fast_exp2(e.y);
+            if constexpr (kEdge) {
+              if (!((vis[w] >> i) & 1u)) e.x = 0.f;
+              if (!((vis[w] >> (i + 1)) & 1u)) e.y = 0.f;
+            }
+            l2[(i >> 1) & 1] = add2(l2[(i >> 1) & 1], e);
+            pk[i / 2] = Mma<T>::pack(e.x, e.y);
+          }
+          tmem_st16(t_s + 16 * w, pk);
+        }
+        l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+        tmem_wait_st();
+      };
       for (int t = joint ? x : 0; t < tiles; t += ahead) {
         ok = ok && wait(s_ready(x), ns & 1);
         ++ns;
@@ -349,74 +449,10 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const int p0 = (sg.tile0 + t) * KP;
         const bool edge = p0 + KP > sg.ctx;
         if (live) {
-          uint32_t s[KP];
-#pragma unroll
-          for (int c = 0; c < KP; c += 32) tmem_ld32(t_s + c, s + c);
-          uint32_t vis[KP / 32];
-          if (edge) {
-#pragma unroll
-            for (int w = 0; w < KP / 32; ++w) {
-              const int j0 = p0 + 32 * w - sg.ctx;
-              const int k = j0 >> 5;
-              vis[w] = __funnelshift_r(mask_word(a, sg, node, k), mask_word(a, sg, node, k + 1), j0 & 31);
-            }
-          }
-          tmem_wait_ld();
-          tmem_loaded<KP>(s);
-          float mx = -INFINITY;
-          if (edge) {
-#pragma unroll
-            for (int c = 0; c < KP; ++c)
-              mx = fmaxf(mx, (vis[c >> 5] >> (c & 31)) & 1u ? __uint_as_float(s[c]) : -INFINITY);
-          } else {
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < KP; c += 4)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], __uint_as_float(s[c + i]));
-            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          }
-          const float mt = mx == -INFINITY ? kNegBig : mx * sc;
-          const bool first = t < ahead;
-          const bool grew = mt > m + kRescaleAt;
-          if (__any_sync(0xffffffffu, grew)) {
-            const float m2 = grew ? mt : m;
-            const float f = fast_exp2(m - m2);
-            m = m2;
-            l *= f;
-            if (!first) {  // the sums of earlier tiles are complete: the scores came after them
-#pragma unroll 1
-              for (int c = 0; c < D; c += 16) {
-                uint32_t o[16];
-                tmem_ld16(t_o + c, o);
-                tmem_wait_ld();
-                tmem_loaded<16>(o);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st16(t_o + c, o);
-              }
-            }
-          }
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < KP; c += 32) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float p0f = fast_exp2(fmaf(__uint_as_float(s[c + i]), sc, -m));
-              float p1f = fast_exp2(fmaf(__uint_as_float(s[c + i + 1]), sc, -m));
-              if (edge) {
-                if (!((vis[c >> 5] >> i) & 1u)) p0f = 0.f;
-                if (!((vis[c >> 5] >> (i + 1)) & 1u)) p1f = 0.f;
-              }
-              l4[i & 3] += p0f;
-              l4[(i & 3) + 1] += p1f;
-              pk[i / 2] = Mma<T>::pack(p0f, p1f);
-            }
-            tmem_st16(t_s + c / 2, pk);
-          }
-          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-          tmem_wait_st();
+          if (edge)
+            softmax(std::true_type(), t, p0);
+          else
+            softmax(std::false_type(), t, p0);
         }
         if (edge) {
           // V of the drafted tokens: what is not finite would spread through zero weights
