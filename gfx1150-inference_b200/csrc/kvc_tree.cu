@@ -62,8 +62,9 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 // O is rescaled only when a row's max has grown by more than 2^8 since the last time: the
 // probabilities then stay below 2^8 and a tile normally touches O with the MMA alone.
 //
-// Warps: 0 brings K/V tiles into a ring of stages, 1 (one thread) issues the MMAs,
-// 4 ... 11 are the two softmax warpgroups.  Every wait is bounded; a wait that gives up
+// Warps: 0 brings K/V tiles into a ring of stages, 1 issues the MMAs, 2 and 3 load each
+// piece's Q and look through V tiles with drafted tokens, 4 ... 11 are the two softmax
+// warpgroups.  Every wait is bounded; a wait that gives up
 // raises the CTA's abort flag, all roles then run through their loops without waiting,
 // copying or issuing, and the kernel returns.
 // =====================================================================================
@@ -122,8 +123,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
   auto empty = [&](int st) { return bar0 + 8u * (12 + st); };
   auto s_ready = [&](int x) { return bar0 + 8u * (24 + x); };
   auto p_ready = [&](int x) { return bar0 + 8u * (26 + x); };
-  auto q_ready = [&](int x) { return bar0 + 8u * (28 + x); };
-  auto o_ready = [&](int x) { return bar0 + 8u * (30 + x); };
+  auto o_ready = [&](int x) { return bar0 + 8u * (28 + x); };
+  const uint32_t q_ready = bar0 + 8u * 30, q_free = bar0 + 8u * 31;
+  // (two of each: K may run two edge tiles ahead of the helpers, and they of the sums)
+  auto edge_go = [&](uint32_t i) { return bar0 + 8u * (32 + (i & 1)); };
+  auto edge_done = [&](uint32_t i) { return bar0 + 8u * (34 + (i & 1)); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -134,8 +138,13 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_ready(x), 1);
       mbar_init(p_ready(x), 128);
-      mbar_init(q_ready(x), 128);
       mbar_init(o_ready(x), 1);
+    }
+    mbar_init(q_ready, 64);
+    mbar_init(q_free, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(edge_go(i), 1);
+      mbar_init(edge_done(i), 64);
     }
     fence_mbar_init();
     *s_abort = 0;
@@ -218,7 +227,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     const uint64_t v_desc = operand_desc(smem_u32(stage_mem), U * 128, 128);
     const bool leader = elect_one();
     uint32_t n = 0;                       // ring tiles consumed
-    uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
+    uint32_t np[2] = {0, 0}, nq = 0, ng = 0, ne = 0;
     bool ok = true;
     auto wait_all = [&](uint32_t bar, uint32_t parity) {
       ok = __all_sync(0xffffffffu, ok && wait(bar, parity));
@@ -263,17 +272,36 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const int left = __shfl_sync(0xffffffffu, sg.ctx + sg.nodes - sg.tile0 * KP, 0);
       const bool two = __shfl_sync(0xffffffffu, sg.rows, 0) > 128;
       const int ahead = S::kStreams == 2 && !two ? 2 : 1;
+      const int edge0 = __shfl_sync(0xffffffffu, sg.ctx - sg.tile0 * KP, 0);
       auto slabs_of = [&](int t) { return min(KP / kSlab, (left - t * KP + kSlab - 1) / kSlab); };
+      auto is_edge = [&](int t) { return (t + 1) * KP > edge0; };
+      // K of tile t is here: when the tile holds drafted positions the helper warps may
+      // take its V on, which the sums then wait for
+      auto take_k = [&](int t) {
+        const int st = take();
+        if (is_edge(t)) {
+          if (ok && leader) mbar_arrive(edge_go(ng));
+          ++ng;
+        }
+        return st;
+      };
+      auto edge_wait = [&](int t) {
+        if (is_edge(t)) {
+          wait_all(edge_done(ne), (ne >> 1) & 1);
+          ++ne;
+        }
+      };
+      wait_all(q_ready, nq++ & 1);
       if (two) {
-        wait_all(q_ready(0), nq[0]++ & 1);
-        wait_all(q_ready(1), nq[1]++ & 1);
-        int kst = take();
+        int kst = take_k(0);
         if (!ok) break;
         scores(0, kst);
         scores(1, kst);
         commit(empty(kst));
+        if (tiles == 1) commit(q_free);
         for (int t = 0; t < tiles && ok; ++t) {
           const int vst = take();
+          edge_wait(t);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             wait_all(p_ready(x), np[x]++ & 1);
@@ -283,34 +311,37 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
             if (x == 1) commit(empty(vst));
             if (t + 1 == tiles) commit(o_ready(x));
             if (t + 1 < tiles) {
-              if (x == 0) kst = take();
+              if (x == 0) kst = take_k(t + 1);
               if (!ok) break;
               scores(x, kst);
               if (x == 1) commit(empty(kst));
+              if (x == 1 && t + 2 == tiles) commit(q_free);
             }
           }
         }
       } else {
         for (int x = 0; x < ahead && x < tiles && ok; ++x) {
-          wait_all(q_ready(x), nq[x]++ & 1);
-          const int kst = take();
+          const int kst = take_k(x);
           if (!ok) break;
           scores(x, kst);
           commit(empty(kst));
+          if (x + 1 == tiles) commit(q_free);
         }
         for (int t = 0; t < tiles && ok; ++t) {
           const int x = ahead == 2 ? t & 1 : 0;
           const int vst = take();
+          edge_wait(t);
           wait_all(p_ready(x), np[x]++ & 1);
           if (!ok) break;
           tmem_fence_after();
           sums(x, vst, slabs_of(t), t >= ahead);
           commit(empty(vst));
           if (t + ahead < tiles) {
-            const int kst = take();
+            const int kst = take_k(t + ahead);
             if (!ok) break;
             scores(x, kst);
             commit(empty(kst));
+            if (t + ahead + 1 == tiles) commit(q_free);
           } else {
             commit(o_ready(x));
           }
@@ -324,14 +355,94 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       mbar_wait_bounded(bar0 + 8u * 40, 0);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    // ---- helpers: each piece's Q, and the V tiles that hold drafted positions -------------
+    const int h = threadIdx.x - 64;
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale turns q
+    uint32_t ring = 0, nf = 0, ng = 0;
+    bool ok = true;
+    for (int si = seg0; si < seg1; ++si) {
+      const TreeSeg sg = a.segs[si];
+      const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
+      const bool two = sg.rows > 128;
+      const int ahead = S::kStreams == 2 && !two ? 2 : 1;
+      if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
+      // Q in k-major core matrices: a warp's load covers 8 rows x 64 bytes.  Streams that
+      // share their rows get a copy each.
+      if (ok) {
+        const int rr = lane >> 2, uu = lane & 3;
+        const int n_rows = two ? 256 : 128;
+        for (int g0 = (warp - 2) * 8; g0 < n_rows; g0 += 16) {
+          const int row = g0 + rr, grow = sg.row0 + row, node = grow / a.group;
+          const uint4* src = reinterpret_cast<const uint4*>(
+              reinterpret_cast<const T*>(a.q) +
+              (static_cast<size_t>(sg.tok0 + node) * a.num_heads + sg.kvh * a.group + grow -
+               node * a.group) * D);
+          uint8_t* dst = q_mem + (row >> 7) * S::kQBytes + ((row & 127) >> 3) * U * 128 + rr * 16;
+          uint4 v[U / 4];
+#pragma unroll
+          for (int i = 0; i < U / 4; ++i)
+            v[i] = row < sg.rows ? src[4 * i + uu] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < U / 4; ++i) {
+            v[i].x ^= flip;
+            v[i].y ^= flip;
+            v[i].z ^= flip;
+            v[i].w ^= flip;
+            *reinterpret_cast<uint4*>(dst + (4 * i + uu) * 128) = v[i];
+            if (S::kStreams == 2 && !two)
+              *reinterpret_cast<uint4*>(dst + S::kQBytes + (4 * i + uu) * 128) = v[i];
+          }
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive(q_ready);
+      // V of drafted tokens: what is not finite would spread through zero weights to rows
+      // that do not see it, so it leaves the tile here (and comes back at the end, to the
+      // rows that do); positions past the end hold anything, and go to zero.
+      for (int t = max(0, sg.ctx / KP - sg.tile0); t < tiles; ++t) {
+        const int p0 = (sg.tile0 + t) * KP;
+        ok = ok && wait(edge_go(ng), (ng >> 1) & 1);
+        // ring order of the piece: `ahead` K tiles, then V t, K t + ahead, ...
+        const uint32_t vi = ring + t + min(ahead + t, tiles);
+        const int st = vi % S::kStages;
+        ok = ok && wait(full(st), (vi / S::kStages) & 1);
+        if (ok) {
+          uint8_t* vt = stage_mem + st * S::kStageBytes;
+          const int from = max(0, sg.ctx - p0), to = min(KP, (end - p0 + kSlab - 1) / kSlab * kSlab);
+          bool dirty = false;
+          for (int i = from * U + h; i < to * U; i += 64) {
+            const int pt = i / U, u = i - pt * U;
+            uint4* cell = reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            bool bad = p0 + pt >= end;
+            if (!bad) {
+              v = *cell;
+              uint32_t* e = &v.x;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (not_finite<T>(e[k] & 0xffffu)) e[k] &= 0xffff0000u, bad = dirty = true;
+                if (not_finite<T>(e[k] >> 16)) e[k] &= 0x0000ffffu, bad = dirty = true;
+              }
+            }
+            if (bad) *cell = v;
+          }
+          if (dirty) s_dirty[si & 1] = si;
+        }
+        __threadfence_block();
+        fence_proxy_async();
+        mbar_arrive(edge_done(ng));
+        ++ng;
+      }
+      ring += 2 * tiles;
+    }
+  } else {
     // ---- softmax: thread r of stream x owns row r ---------------------------------------------
     const int x = (warp - 4) >> 2, w4 = warp & 3, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * 128;
     const float sc = fabsf(a.scale_log2);
-    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale turns q
-    uint32_t ns = 0, no[2] = {0, 0}, nv = 0;
+    uint32_t ns = 0, no[2] = {0, 0};
     bool ok = true;
     for (int si = seg0; si < seg1; ++si) {
       const TreeSeg sg = a.segs[si];
@@ -345,43 +456,15 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const int grow = sg.row0 + min(row, sg.rows - 1);
       const int node = grow / a.group, head = sg.kvh * a.group + grow - node * a.group;
       const size_t io_row = (static_cast<size_t>(sg.tok0 + node) * a.num_heads + head) * D;
-      const uint32_t seg_tiles0 = nv;   // ring index of the segment's first tile
-      nv += 2 * tiles;
-      const bool mine = !joint || x < tiles;   // the stream has tiles of this piece
-      if (mine) {
-        // Q, k-major core matrices; a piece's scores are done before the next piece's Q comes
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + io_row);
-        uint8_t* dst = q_mem + x * S::kQBytes + (r >> 3) * U * 128 + (r & 7) * 16;
-#pragma unroll 8
-        for (int u = 0; u < U; ++u) {
-          uint4 v = live_row ? src[u] : make_uint4(0, 0, 0, 0);
-          v.x ^= flip;
-          v.y ^= flip;
-          v.z ^= flip;
-          v.w ^= flip;
-          *reinterpret_cast<uint4*>(dst + u * 128) = v;
-        }
-        fence_proxy_async();
-        mbar_arrive(q_ready(x));
-      }
       float m = kNegBig, l = 0.f;     // max in log2 units
       // One tile of the stream: scores to probabilities, in place, and the running max and
       // sum.  Edge tiles hold positions that some rows do not see.
-      auto softmax = [&](auto edge_tag, int t, int p0) {
+      auto softmax = [&](auto edge_tag, int t, const uint32_t* vis) {
         constexpr bool kEdge = decltype(edge_tag)::value;
         // The scores are read from tensor memory twice, 32 columns at a time with the next
         // 32 on their way: a whole row in registers would spill.
         uint32_t s[2][32];
         tmem_ld32(t_s, s[0]);
-        uint32_t vis[KP / 32];
-        if constexpr (kEdge) {
-#pragma unroll
-          for (int w = 0; w < KP / 32; ++w) {
-            const int j0 = p0 + 32 * w - sg.ctx;
-            const int k = j0 >> 5;
-            vis[w] = __funnelshift_r(mask_word(a, sg, node, k), mask_word(a, sg, node, k + 1), j0 & 31);
-          }
-        }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int w = 0; w < KP / 32; ++w) {
@@ -443,50 +526,25 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         tmem_wait_st();
       };
       for (int t = joint ? x : 0; t < tiles; t += ahead) {
+        const int p0 = (sg.tile0 + t) * KP;
+        const bool edge = p0 + KP > sg.ctx;
+        uint32_t vis[KP / 32];   // of an edge tile: the positions that the row sees
+        if (edge && live) {
+#pragma unroll
+          for (int w = 0; w < KP / 32; ++w) {
+            const int j0 = p0 + 32 * w - sg.ctx;
+            const int k = j0 >> 5;
+            vis[w] = __funnelshift_r(mask_word(a, sg, node, k), mask_word(a, sg, node, k + 1), j0 & 31);
+          }
+        }
         ok = ok && wait(s_ready(x), ns & 1);
         ++ns;
         tmem_fence_after();
-        const int p0 = (sg.tile0 + t) * KP;
-        const bool edge = p0 + KP > sg.ctx;
         if (live) {
           if (edge)
-            softmax(std::true_type(), t, p0);
+            softmax(std::true_type(), t, vis);
           else
-            softmax(std::false_type(), t, p0);
-        }
-        if (edge) {
-          // V of the drafted tokens: what is not finite would spread through zero weights
-          // to rows that do not see it, so it leaves the tile here (and comes back at the
-          // end, to the rows that do); positions past the end hold anything, and go to zero.
-          // ring order of the piece: `ahead` K tiles, then V t, K t + ahead, ...
-          const uint32_t vi = seg_tiles0 + min(ahead, tiles) + t + min(t, max(tiles - ahead, 0));
-          const int st = vi % S::kStages;
-          ok = ok && wait(full(st), (vi / S::kStages) & 1);
-          uint8_t* vt = stage_mem + st * S::kStageBytes;
-          const int from = max(0, sg.ctx - p0), to = min(KP, (end - p0 + kSlab - 1) / kSlab * kSlab);
-          bool dirty = false;
-          for (int i = from * U + r; i < to * U; i += 128) {
-            const int pt = i / U, u = i - pt * U;
-            uint4* cell = reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            bool bad = p0 + pt >= end;
-            if (!bad) {
-              v = *cell;
-              uint32_t* e = &v.x;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if (not_finite<T>(e[k] & 0xffffu)) e[k] &= 0xffff0000u, bad = dirty = true;
-                if (not_finite<T>(e[k] >> 16)) e[k] &= 0x0000ffffu, bad = dirty = true;
-              }
-            }
-            if (dirty) {
-              s_dirty[si & 1] = si;
-              __threadfence_block();
-            }
-            if (bad) *cell = v;
-          }
-          __threadfence_block();
-          fence_proxy_async();
+            softmax(std::false_type(), t, vis);
         }
         tmem_fence_before();
         mbar_arrive(p_ready(x));
@@ -562,9 +620,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
             }
           }
           if (sg.part >= 0) {
-            float4* po = reinterpret_cast<float4*>(a.part_o + static_cast<size_t>(sg.part + row) * D + c);
+            float4* po = reinterpret_cast<float4*>(a.part_o + static_cast<size_t>(sg.part) * D) +
+                         (c / 4) * sg.rows + row;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) po[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+            for (int i = 0; i < 4; ++i)
+              po[i * sg.rows] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
           } else {
             uint32_t pk[8];
 #pragma unroll
@@ -709,10 +769,12 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
       const int r = warp * 4 + i;
       if (r >= sg.rows) continue;
       if (sg.part >= 0) {
-        float* po = a.part_o + static_cast<size_t>(sg.part + r) * D;
+        float* po = a.part_o + static_cast<size_t>(sg.part) * D;
 #pragma unroll
-        for (int d = 0; d < DPL; ++d)
-          if (lane + 32 * d < D) po[lane + 32 * d] = acc[i][d];
+        for (int d = 0; d < DPL; ++d) {
+          const int c = lane + 32 * d;
+          if (c < D) po[(c / 4 * sg.rows + r) * 4 + c % 4] = acc[i][d];
+        }
         if (lane == 0) a.part_ml[sg.part + r] = make_float2(m[i], l[i]);
       } else {
         const int row = sg.row0 + r, node = row / a.group;
@@ -729,45 +791,58 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
 }
 
 // =====================================================================================
-// Join of split rows: out = sum_k O_k 2^(m_k - m*) / sum_k l_k 2^(m_k - m*).  A thread
-// owns four dims of one row; the pieces of a row are added in position order, so the
-// result does not depend on which CTA finished first.
+// Join of split rows: out = sum_k O_k 2^(m_k - m*) / sum_k l_k 2^(m_k - m*).  A piece's
+// partials are stored four dims of all its rows after one another, so that the threads
+// of a warp, which own a row each, write and read them side by side.  A thread joins 16
+// bytes of output of one row; the pieces are added in position order, so the result does
+// not depend on which CTA finished first.
 // =====================================================================================
 constexpr int kMergeThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
+  constexpr int N = 16 / sizeof(T), F = N / 4;
   const TreeMerge mg = a.merges[blockIdx.x];
-  const int D = a.head_dim, C = D / 4;
+  const int D = a.head_dim;
   const int x = blockIdx.y * kMergeThreads + threadIdx.x;
-  const int r = x / C, c = x - r * C;
-  if (r >= mg.rows) return;
+  const int c = x / mg.rows, r = x - c * mg.rows;   // 16 bytes c of row r
+  if (c * N >= D) return;
   const float2* ml = a.part_ml + mg.part + r;
   float mx = kNegBig;
   for (int k = 0; k < mg.n_parts; ++k) mx = fmaxf(mx, ml[static_cast<size_t>(k) * mg.rows].x);
   float sum = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 o[F];
+#pragma unroll
+  for (int i = 0; i < F; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k = 0; k < mg.n_parts; ++k) {
     const size_t at = static_cast<size_t>(k) * mg.rows;
     const float2 e = ml[at];
     const float w = fast_exp2(e.x - mx);
-    const float4 p = *reinterpret_cast<const float4*>(
-        a.part_o + (static_cast<size_t>(mg.part + r) + at) * D + 4 * c);
+    const float4* p = reinterpret_cast<const float4*>(a.part_o + (mg.part + at) * D) + c * F * mg.rows + r;
     sum += e.y * w;
-    o.x += p.x * w;
-    o.y += p.y * w;
-    o.z += p.z * w;
-    o.w += p.w * w;
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const float4 v = p[i * mg.rows];
+      o[i].x += v.x * w;
+      o[i].y += v.y * w;
+      o[i].z += v.z * w;
+      o[i].w += v.w * w;
+    }
   }
   const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
   const int row = mg.row0 + r, node = row / a.group;
   const int head = mg.kvh * a.group + row - node * a.group;
+  T v[N];
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    v[4 * i] = from_f32<T>(o[i].x * inv);
+    v[4 * i + 1] = from_f32<T>(o[i].y * inv);
+    v[4 * i + 2] = from_f32<T>(o[i].z * inv);
+    v[4 * i + 3] = from_f32<T>(o[i].w * inv);
+  }
   T* out = reinterpret_cast<T*>(a.out) +
-           (static_cast<size_t>(mg.tok0 + node) * a.num_heads + head) * D + 4 * c;
-  out[0] = from_f32<T>(o.x * inv);
-  out[1] = from_f32<T>(o.y * inv);
-  out[2] = from_f32<T>(o.z * inv);
-  out[3] = from_f32<T>(o.w * inv);
+           (static_cast<size_t>(mg.tok0 + node) * a.num_heads + head) * D + c * N;
+  *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);
 }
 
 // Dynamic shared memory opt-in, once per kernel, device and size.
@@ -837,7 +912,7 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
   else
     e = run_simt<T, 8>(a, s);
   if (e != cudaSuccess || a.n_merges == 0) return e;
-  const int per = a.max_merge_rows * (a.head_dim / 4);
+  const int per = a.max_merge_rows * (a.head_dim * static_cast<int>(sizeof(T)) / 16);
   tree_merge_kernel<T><<<dim3(a.n_merges, (per + kMergeThreads - 1) / kMergeThreads), kMergeThreads,
                          0, s>>>(a);
   return cudaGetLastError();
