@@ -112,6 +112,7 @@ struct TreeArgs {
 struct TreeTile {
   int positions, rows;
   int ctas_per_sm;
+  int piece_cost;                // start and end of a piece of work, in tiles
   bool tensor;                   // tcgen05 kernel
 };
 TreeTile tree_tile(const PoolGeom& g);

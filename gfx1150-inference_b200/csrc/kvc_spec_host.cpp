@@ -179,9 +179,8 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
 namespace {
 
 // The work list: every (sequence, KV head, row block) is a run of position tiles;
-// the runs are laid end to end and cut into n_ctas equal shares, one per CTA, so
-// every CTA streams the same number of tiles.  A run that falls into several
-// shares is joined from its pieces' partials.
+// the runs are laid end to end and cut into shares of equal cost, one per CTA.  A run
+// that falls into several shares is joined from its pieces' partials.
 int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
                const int32_t* h_ctx, const int32_t* h_nodes, int n_seqs, int num_heads,
                cudaStream_t s) {
@@ -194,7 +193,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   p->valid = false;
   const TreeTile tile = tree_tile(g);
   const int group = num_heads / g.num_kv_heads;
-  int64_t tokens = 0, tiles = 0, max_end = 0;
+  int64_t tokens = 0, tiles = 0, runs = 0, max_end = 0;
   int max_row = 0, max_nodes = 0;
   std::vector<int32_t> rows, slots;
   for (int i = 0; i < n_seqs; ++i) {
@@ -214,6 +213,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     max_row = std::max(max_row, row);
     max_nodes = std::max(max_nodes, h_nodes[i]);
     const int64_t blocks = (static_cast<int64_t>(h_nodes[i]) * group + tile.rows - 1) / tile.rows;
+    runs += blocks * g.num_kv_heads;
     tiles += blocks * g.num_kv_heads * ((end + tile.positions - 1) / tile.positions);
   }
   if (tokens * num_heads > (1ll << 30) || tiles > (1ll << 30))
@@ -225,8 +225,15 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   std::vector<int> cta_segs(1, 0);
   size_t part_rows = 0;
   int max_merge_rows = 0;
-  int64_t at = 0, cta = 0;  // tiles laid out so far; the CTA whose share they are in
-  auto share_end = [&](int64_t c) { return (c + 1) * tiles / ctas; };
+  // A piece costs its tiles and tile.piece_cost for its start and end.  CTA c's share ends
+  // where the cost laid out so far reaches (c + 1) / ctas of the total (the cuts' own
+  // pieces included); a cut that would leave less than piece_cost on either side moves
+  // to the end of the run.
+  const int64_t total_cost = tiles + (runs + ctas) * tile.piece_cost;
+  int64_t cost = 0, cta = 0;
+  auto share_end = [&](int64_t c) {
+    return c + 1 >= ctas ? INT64_MAX : (c + 1) * total_cost / ctas;
+  };
   int tok0 = 0;
   for (int i = 0; i < n_seqs; ++i) {
     const int n_rows = h_nodes[i] * group;
@@ -236,7 +243,15 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
         const int nr = std::min(tile.rows, n_rows - r0);
         const size_t first = segs.size();
         for (int t = 0; t < run;) {
-          const int take = static_cast<int>(std::min<int64_t>(run - t, share_end(cta) - at));
+          const int64_t room = share_end(cta) - cost - tile.piece_cost;
+          if (room < std::max(1, tile.piece_cost) && room < run - t &&
+              cta_segs.back() < static_cast<int>(segs.size())) {
+            cta_segs.push_back(static_cast<int>(segs.size()));  // this share is full
+            ++cta;
+            continue;
+          }
+          int take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(run - t, room)));
+          if (run - t - take < tile.piece_cost) take = run - t;
           TreeSeg sg = {};
           sg.bt_row = h_rows ? h_rows[i] : i;
           sg.ctx = h_ctx[i];
@@ -250,8 +265,8 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
           sg.part = -1;
           segs.push_back(sg);
           t += take;
-          at += take;
-          while (cta < ctas && at >= share_end(cta)) {
+          cost += take + tile.piece_cost;
+          if (cost >= share_end(cta)) {
             cta_segs.push_back(static_cast<int>(segs.size()));
             ++cta;
           }
@@ -276,6 +291,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     }
     tok0 += h_nodes[i];
   }
+  if (cta_segs.back() < static_cast<int>(segs.size())) cta_segs.push_back(static_cast<int>(segs.size()));
   p->n_seqs = n_seqs;
   p->n_tokens = static_cast<int>(tokens);
   p->num_heads = num_heads;
@@ -283,7 +299,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   p->max_end = static_cast<int>(max_end);
   p->max_row = max_row;
   p->tile = tile;
-  p->n_ctas = static_cast<int>(ctas);
+  p->n_ctas = static_cast<int>(cta_segs.size()) - 1;
   p->n_merges = static_cast<int>(merges.size());
   p->max_merge_rows = max_merge_rows;
   p->part_rows = part_rows;

@@ -70,6 +70,7 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 // =====================================================================================
 constexpr int kTmemCols = 512;
 constexpr float kRescaleAt = 8.0f;   // log2
+constexpr int kPieceCost = 2;        // a piece's start and end, in tiles
 
 template <int D>
 struct TreeShape {
@@ -151,10 +152,14 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     s_dirty[0] = s_dirty[1] = -1;
   }
   if (warp == 1) tmem_alloc(smem_u32(s_tmem), kTmemCols);
+  // (the plan's records are no kernel's output: they may be read before the wait)
+  const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = *s_tmem;
+  launch_dependents();
+  wait_prerequisites();
 
   // false: some wait of this CTA gave up
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -172,8 +177,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       }
     }
   };
-  const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
 
+  // Registers move from the data and MMA warps to the softmax warpgroups: 128 x 104 +
+  // 256 x 200 is what 384 threads were launched with (168 each).
+  if (warp < 4) {
+  if constexpr (S::kStreams == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 0) {
     // ---- K/V tiles into the ring, in the order the MMAs take them -----------------------
     const uint64_t policy = l2_policy_evict_first();
@@ -355,7 +363,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       mbar_wait_bounded(bar0 + 8u * 40, 0);
     }
     __syncwarp();
-  } else if (warp < 4) {
+  } else {
     // ---- helpers: each piece's Q, and the V tiles that hold drafted positions -------------
     const int h = threadIdx.x - 64;
     const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale turns q
@@ -366,35 +374,44 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
       const bool two = sg.rows > 128;
       const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-      if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
-      // Q in k-major core matrices: a warp's load covers 8 rows x 64 bytes.  Streams that
-      // share their rows get a copy each.
-      if (ok) {
-        const int rr = lane >> 2, uu = lane & 3;
-        const int n_rows = two ? 256 : 128;
-        for (int g0 = (warp - 2) * 8; g0 < n_rows; g0 += 16) {
-          const int row = g0 + rr, grow = sg.row0 + row, node = grow / a.group;
+      // Q in k-major core matrices: a warp's load covers 8 rows x 64 bytes, and kQLoads rows
+      // of loads are in flight, the first of them before the last piece's scores are done.
+      // Streams that share their rows get a copy each.
+      constexpr int kQLoads = 2;
+      const int rr = lane >> 2, uu = lane & 3;
+      const int n_rows = two ? 256 : 128;
+      for (int g0 = (warp - 2) * 8 * kQLoads; g0 < n_rows; g0 += 16 * kQLoads) {
+        uint4 v[kQLoads][U / 4];
+#pragma unroll
+        for (int g = 0; g < kQLoads; ++g) {
+          const int row = g0 + 8 * g + rr, grow = sg.row0 + row, node = grow / a.group;
           const uint4* src = reinterpret_cast<const uint4*>(
               reinterpret_cast<const T*>(a.q) +
               (static_cast<size_t>(sg.tok0 + node) * a.num_heads + sg.kvh * a.group + grow -
                node * a.group) * D);
-          uint8_t* dst = q_mem + (row >> 7) * S::kQBytes + ((row & 127) >> 3) * U * 128 + rr * 16;
-          uint4 v[U / 4];
 #pragma unroll
           for (int i = 0; i < U / 4; ++i)
-            v[i] = row < sg.rows ? src[4 * i + uu] : make_uint4(0, 0, 0, 0);
+            v[g][i] = row < sg.rows ? src[4 * i + uu] : make_uint4(0, 0, 0, 0);
+        }
+        if (si > seg0 && g0 < 16 * kQLoads) ok = ok && wait(q_free, nf & 1);
+        if (!ok) break;
+#pragma unroll
+        for (int g = 0; g < kQLoads; ++g) {
+          const int row = g0 + 8 * g + rr;
+          uint8_t* dst = q_mem + (row >> 7) * S::kQBytes + ((row & 127) >> 3) * U * 128 + rr * 16;
 #pragma unroll
           for (int i = 0; i < U / 4; ++i) {
-            v[i].x ^= flip;
-            v[i].y ^= flip;
-            v[i].z ^= flip;
-            v[i].w ^= flip;
-            *reinterpret_cast<uint4*>(dst + (4 * i + uu) * 128) = v[i];
+            v[g][i].x ^= flip;
+            v[g][i].y ^= flip;
+            v[g][i].z ^= flip;
+            v[g][i].w ^= flip;
+            *reinterpret_cast<uint4*>(dst + (4 * i + uu) * 128) = v[g][i];
             if (S::kStreams == 2 && !two)
-              *reinterpret_cast<uint4*>(dst + S::kQBytes + (4 * i + uu) * 128) = v[i];
+              *reinterpret_cast<uint4*>(dst + S::kQBytes + (4 * i + uu) * 128) = v[g][i];
           }
         }
       }
+      if (si > seg0) ++nf;
       fence_proxy_async();
       mbar_arrive(q_ready);
       // V of drafted tokens: what is not finite would spread through zero weights to rows
@@ -436,7 +453,9 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       }
       ring += 2 * tiles;
     }
+  }
   } else {
+    if constexpr (S::kStreams == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---- softmax: thread r of stream x owns row r ---------------------------------------------
     const int x = (warp - 4) >> 2, w4 = warp & 3, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
@@ -461,67 +480,88 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       // sum.  Edge tiles hold positions that some rows do not see.
       auto softmax = [&](auto edge_tag, int t, const uint32_t* vis) {
         constexpr bool kEdge = decltype(edge_tag)::value;
-        // The scores are read from tensor memory twice, 32 columns at a time with the next
-        // 32 on their way: a whole row in registers would spill.
-        uint32_t s[2][32];
-        tmem_ld32(t_s, s[0]);
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // One pass with the max as it was: the probabilities wait in registers, and only
+        // when a row's max turns out to have grown too far is the pass made again.  The
+        // first tile has no such max: it looks for one.
+        uint32_t pk[KP / 2];
+        float mt;
+        float2 l2[2];
+        auto pass = [&]() {
+          uint32_t s[2][16];
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          const float2 sc2 = make_float2(sc, sc), m2 = make_float2(-m, -m);
+          l2[0] = l2[1] = make_float2(0.f, 0.f);
+          tmem_ld16(t_s, s[0]);
 #pragma unroll
-        for (int w = 0; w < KP / 32; ++w) {
-          uint32_t* now = s[w & 1];
-          tmem_wait_ld();
-          tmem_loaded<32>(now);
-          // (behind the last columns come the first again, for the second reading)
-          tmem_ld32(t_s + (w + 1 < KP / 32 ? 32 * (w + 1) : 0), s[(w + 1) & 1]);
+          for (int w = 0; w < KP / 16; ++w) {
+            const uint32_t* now = s[w & 1];
+            tmem_wait_ld();
+            tmem_loaded<16>(s[w & 1]);
+            if (w + 1 < KP / 16) tmem_ld16(t_s + 16 * (w + 1), s[(w + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (!kEdge || ((vis[w] >> i) & 1u)) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(now[i]));
+            for (int i = 0; i < 16; i += 2) {
+              const float a0 = __uint_as_float(now[i]), a1 = __uint_as_float(now[i + 1]);
+              float2 e = fma2(make_float2(a0, a1), sc2, m2);
+              e.x = fast_exp2(e.x);
+              e.y = fast_exp2(e.y);
+              if constexpr (kEdge) {
+                const uint32_t bits = vis[w >> 1] >> ((w & 1) * 16 + i);
+                if (bits & 1u)
+                  m4[i & 3] = fmaxf(m4[i & 3], a0);
+                else
+                  e.x = 0.f;
+                if (bits & 2u)
+                  m4[(i & 3) + 1] = fmaxf(m4[(i & 3) + 1], a1);
+                else
+                  e.y = 0.f;
+              } else {
+                m4[i & 3] = fmaxf(m4[i & 3], a0);
+                m4[(i & 3) + 1] = fmaxf(m4[(i & 3) + 1], a1);
+              }
+              l2[(i >> 1) & 1] = add2(l2[(i >> 1) & 1], e);
+              pk[w * 8 + i / 2] = Mma<T>::pack(e.x, e.y);
+            }
           }
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          mt = mx == -INFINITY ? kNegBig : mx * sc;
+        };
+        if (t < ahead) {
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int w = 0; w < KP / 32; ++w) {
+            uint32_t s[32];
+            tmem_ld32(t_s + 32 * w, s);
+            tmem_wait_ld();
+            tmem_loaded<32>(s);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!kEdge || ((vis[w] >> i) & 1u)) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[i]));
+          }
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          m = mx == -INFINITY ? kNegBig : mx * sc;
         }
-        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        const float mt = mx == -INFINITY ? kNegBig : mx * sc;
-        const bool grew = mt > m + kRescaleAt;
-        if (__any_sync(0xffffffffu, grew)) {
+        for (;;) {
+          pass();
+          const bool grew = mt > m + kRescaleAt;
+          if (!__any_sync(0xffffffffu, grew)) break;
           const float m2 = grew ? mt : m;
           const float f = fast_exp2(m - m2);
           m = m2;
           l *= f;
-          if (t >= ahead) {  // the sums of earlier tiles are complete: the scores came after them
+          // the sums of earlier tiles are complete: the scores came after them
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(t_o + c, o);
-              tmem_wait_ld();
-              tmem_loaded<16>(o);
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(t_o + c, o);
+            tmem_wait_ld();
+            tmem_loaded<16>(o);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st16(t_o + c, o);
-            }
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(t_o + c, o);
           }
         }
-        const float2 sc2 = make_float2(sc, sc), m2 = make_float2(-m, -m);
-        float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int w = 0; w < KP / 32; ++w) {
-          const uint32_t* now = s[w & 1];
-          tmem_wait_ld();
-          tmem_loaded<32>(s[w & 1]);
-          if (w + 1 < KP / 32) tmem_ld32(t_s + 32 * (w + 1), s[(w + 1) & 1]);
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float2 e = fma2(make_float2(__uint_as_float(now[i]), __uint_as_float(now[i + 1])), sc2, m2);
-            e.x = fast_exp2(e.x);
-            e.y = fast_exp2(e.y);
-            if constexpr (kEdge) {
-              if (!((vis[w] >> i) & 1u)) e.x = 0.f;
-              if (!((vis[w] >> (i + 1)) & 1u)) e.y = 0.f;
-            }
-            l2[(i >> 1) & 1] = add2(l2[(i >> 1) & 1], e);
-            pk[i / 2] = Mma<T>::pack(e.x, e.y);
-          }
-          tmem_st16(t_s + 16 * w, pk);
-        }
+        for (int w = 0; w < KP / 32; ++w) tmem_st16(t_s + 16 * w, pk + 16 * w);
         l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
         tmem_wait_st();
       };
@@ -576,65 +616,75 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
           ll = e0.y * w0 + e1.y * w1;
         }
         const bool dirty = s_dirty[si & 1] == si;
+        // rare: what was taken out of V comes back, for the nodes that this row sees
+        auto restore = [&](int c, float* f) {
+          const int t0 = max(sg.tile0 * KP, sg.ctx), t1 = min(sg.tile1 * KP, end);
+          for (int pos = t0; pos < t1; ++pos) {
+            const int j = pos - sg.ctx;
+            if (!((mask_word(a, sg, node, j >> 5) >> (j & 31)) & 1u)) continue;
+            const int page = tree_page(a.p, sg.bt_row, pos);
+            const uint8_t* vrow = a.p.v + (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) *
+                                              a.p.page_head_bytes;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const T e = reinterpret_cast<const T*>(
+                  vrow + unit_offset(kLayoutCore, pos % a.p.page_size, (c + i) / 8, U) * 16)[(c + i) % 8];
+              const float v = to_f32<T>(e);
+              if (!isfinite(v)) f[i] += v;
+            }
+          }
+        };
         const int c0 = joint ? x * (D / 2) : 0, c1 = joint ? c0 + D / 2 : D;
         const uint32_t o0 = tmem + lanes + 256 + (joint ? 0 : x * 128);
         const float inv = ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);
         if (live_row && sg.part >= 0 && (!joint || x == 0))
           a.part_ml[sg.part + row] = make_float2(mm, ll);
-#pragma unroll 1
-        for (int c = c0; c < c1; c += 16) {
-          uint32_t o[16];
-          float f[16];
+        const bool add = joint && tiles > 1;
+        auto load = [&](int c, uint32_t* o, uint32_t* q) {
           tmem_ld16(o0 + c, o);
-          if (joint && tiles > 1) {
-            uint32_t q[16];
-            tmem_ld16(o0 + 128 + c, q);
-            tmem_wait_ld();
-            tmem_loaded<16>(o);
-            tmem_loaded<16>(q);
+          if (add) tmem_ld16(o0 + 128 + c, q);
+        };
+        auto store = [&](int c, const uint32_t* o, const uint32_t* q) {
+          float f[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              f[i] = __uint_as_float(o[i]) * w0 + __uint_as_float(q[i]) * w1;
-          } else {
-            tmem_wait_ld();
-            tmem_loaded<16>(o);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]);
-          }
+          for (int i = 0; i < 16; ++i)
+            f[i] = add ? __uint_as_float(o[i]) * w0 + __uint_as_float(q[i]) * w1 : __uint_as_float(o[i]);
           if (live_row) {
-          if (dirty) {  // rare: add what was taken out of V, for the nodes this row sees
-            const int t0 = max(sg.tile0 * KP, sg.ctx), t1 = min(sg.tile1 * KP, end);
-            for (int pos = t0; pos < t1; ++pos) {
-              const int j = pos - sg.ctx;
-              if (!((mask_word(a, sg, node, j >> 5) >> (j & 31)) & 1u)) continue;
-              const int page = tree_page(a.p, sg.bt_row, pos);
-              const uint8_t* vrow = a.p.v + (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) *
-                                                a.p.page_head_bytes;
+            if (dirty) restore(c, f);
+            if (sg.part >= 0) {
+              float4* po = reinterpret_cast<float4*>(a.part_o + static_cast<size_t>(sg.part) * D) +
+                           (c / 4) * sg.rows + row;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const T e = reinterpret_cast<const T*>(
-                    vrow + unit_offset(kLayoutCore, pos % a.p.page_size, (c + i) / 8, U) * 16)[(c + i) % 8];
-                const float v = to_f32<T>(e);
-                if (!isfinite(v)) f[i] += v;
-              }
+              for (int i = 0; i < 4; ++i)
+                po[i * sg.rows] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+            } else {
+              uint32_t pk[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) pk[i] = Mma<T>::pack(f[2 * i] * inv, f[2 * i + 1] * inv);
+              uint4* po = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + io_row + c);
+              po[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              po[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
             }
           }
-          if (sg.part >= 0) {
-            float4* po = reinterpret_cast<float4*>(a.part_o + static_cast<size_t>(sg.part) * D) +
-                         (c / 4) * sg.rows + row;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              po[i * sg.rows] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-          } else {
-            uint32_t pk[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pk[i] = Mma<T>::pack(f[2 * i] * inv, f[2 * i + 1] * inv);
-            uint4* po = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + io_row + c);
-            po[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            po[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-          }
-          }
           __syncwarp();
+        };
+        // 16 columns at a time, the next ones on their way
+        uint32_t oa[16], qa[16], ob[16], qb[16];
+        load(c0, oa, qa);
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 32) {
+          tmem_wait_ld();
+          tmem_loaded<16>(oa);
+          tmem_loaded<16>(qa);
+          if (c + 16 < c1) load(c + 16, ob, qb);
+          store(c, oa, qa);
+          if (c + 16 < c1) {
+            tmem_wait_ld();
+            tmem_loaded<16>(ob);
+            tmem_loaded<16>(qb);
+            if (c + 32 < c1) load(c + 32, oa, qa);
+            store(c + 16, ob, qb);
+          }
         }
       }
       tmem_fence_before();
@@ -663,6 +713,8 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int N = 16 / sizeof(T);
   const int U = a.p.row_units;
+  launch_dependents();
+  wait_prerequisites();
 
   for (int si = a.cta_segs[blockIdx.x]; si < a.cta_segs[blockIdx.x + 1]; ++si) {
     const TreeSeg sg = a.segs[si];
@@ -804,6 +856,8 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   constexpr int N = 16 / sizeof(T), F = N / 4;
   const TreeMerge mg = a.merges[blockIdx.x];
   const int D = a.head_dim;
+  launch_dependents();
+  wait_prerequisites();
   const int x = blockIdx.y * kMergeThreads + threadIdx.x;
   const int c = x / mg.rows, r = x - c * mg.rows;   // 16 bytes c of row r
   if (c * N >= D) return;
@@ -863,14 +917,45 @@ cudaError_t allow_smem(size_t smem) {
   return e;
 }
 
+// A launch that may begin before the one ahead of it has ended: every kernel here reads
+// and writes what others do only behind wait_prerequisites().  The merge asks for the
+// attention kernels' shared-memory split, so that an SM passes from one to the other
+// without a change of it.
+template <typename A>
+cudaError_t launch_early(void (*kernel)(A), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                         const A& args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+template <auto Kernel>
+cudaError_t prefer_shared() {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire))) return e;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                           cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+  return e;
+}
+
 template <typename T, int DPL>
 cudaError_t run_simt(const TreeArgs& a, cudaStream_t s) {
   const size_t smem = sizeof(float) * (static_cast<size_t>(kSimtRows + kSimtPos) * (a.head_dim + 4) +
                                        static_cast<size_t>(kSimtPos) * a.head_dim);
   const cudaError_t e = allow_smem<tree_simt_kernel<T, DPL>>(smem);
   if (e != cudaSuccess) return e;
-  tree_simt_kernel<T, DPL><<<a.n_ctas, kSimtThreads, smem, s>>>(a);
-  return cudaGetLastError();
+  return launch_early(tree_simt_kernel<T, DPL>, dim3(a.n_ctas), kSimtThreads, smem, s, a);
 }
 
 template <typename T, int D>
@@ -878,8 +963,7 @@ cudaError_t run_mma(const TreeArgs& a, cudaStream_t s) {
   using S = TreeShape<D>;
   const cudaError_t e = allow_smem<tree_mma_kernel<T, D>>(S::kSmem);
   if (e != cudaSuccess) return e;
-  tree_mma_kernel<T, D><<<a.n_ctas, S::kThreads, S::kSmem, s>>>(a);
-  return cudaGetLastError();
+  return launch_early(tree_mma_kernel<T, D>, dim3(a.n_ctas), S::kThreads, S::kSmem, s, a);
 }
 
 template <typename T>
@@ -912,18 +996,20 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
   else
     e = run_simt<T, 8>(a, s);
   if (e != cudaSuccess || a.n_merges == 0) return e;
+  if ((e = prefer_shared<tree_merge_kernel<T>>()) != cudaSuccess) return e;
   const int per = a.max_merge_rows * (a.head_dim * static_cast<int>(sizeof(T)) / 16);
-  tree_merge_kernel<T><<<dim3(a.n_merges, (per + kMergeThreads - 1) / kMergeThreads), kMergeThreads,
-                         0, s>>>(a);
-  return cudaGetLastError();
+  return launch_early(tree_merge_kernel<T>,
+                      dim3(a.n_merges, (per + kMergeThreads - 1) / kMergeThreads), kMergeThreads, 0,
+                      s, a);
 }
 
 }  // namespace
 
 TreeTile tree_tile(const PoolGeom& g) {
   if (decode_uses_mma(g.dtype, g.head_dim, g.page_size) && g.layout == kLayoutCore)
-    return g.head_dim <= 128 ? TreeTile{128, 256, 1, true} : TreeTile{64, 128, 1, true};
-  return TreeTile{kSimtPos, kSimtRows, 2, false};
+    return g.head_dim <= 128 ? TreeTile{128, 256, 1, kPieceCost, true}
+                             : TreeTile{64, 128, 1, kPieceCost, true};
+  return TreeTile{kSimtPos, kSimtRows, 2, 0, false};
 }
 
 cudaError_t launch_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
