@@ -113,6 +113,16 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t
       : "memory");
 }
 
+// Asynchronous copy of 16 bytes to shared memory, of which `bytes` (16 or 0) are read and
+// the rest is zero; the thread's copies have landed after copy_async_wait().
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 // ---- tensor-core fragments (mma.sync m16n8k16, fp32 accumulate) -----------------
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
                                         uint32_t& r3) {

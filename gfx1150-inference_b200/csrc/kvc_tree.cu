@@ -62,8 +62,8 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 // O is rescaled only when a row's max has grown by more than 2^8 since the last time: the
 // probabilities then stay below 2^8 and a tile normally touches O with the MMA alone.
 //
-// Warps: 0 brings K/V tiles into a ring of stages, 1 issues the MMAs, 2 and 3 load each
-// piece's Q and look through V tiles with drafted tokens, 4 ... 11 are the two softmax
+// Warps: 0 and 2 bring K/V tiles into a ring of stages, 1 issues the MMAs, 3 loads each
+// piece's Q and looks through V tiles with drafted tokens, 4 ... 11 are the two softmax
 // warpgroups.  Every wait is bounded; a wait that gives up
 // raises the CTA's abort flag, all roles then run through their loops without waiting,
 // copying or issuing, and the kernel returns.
@@ -141,11 +141,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       mbar_init(p_ready(x), 128);
       mbar_init(o_ready(x), 1);
     }
-    mbar_init(q_ready, 64);
+    mbar_init(q_ready, 32);
     mbar_init(q_free, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(edge_go(i), 1);
-      mbar_init(edge_done(i), 64);
+      mbar_init(edge_done(i), 32);
     }
     fence_mbar_init();
     *s_abort = 0;
@@ -178,49 +178,78 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     }
   };
 
-  // Registers move from the data and MMA warps to the softmax warpgroups: 128 x 104 +
-  // 256 x 200 is what 384 threads were launched with (168 each).
+  // Registers move from the other warps to the softmax warpgroups: 128 x 104 + 256 x 200
+  // is what 384 threads were launched with (168 each).
   if (warp < 4) {
   if constexpr (S::kStreams == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == 0) {
-    // ---- K/V tiles into the ring, in the order the MMAs take them -----------------------
+  if (warp == 0 || warp == 2) {
+    // ---- K/V tiles into the ring, in the order the MMAs take them: one warp issues the
+    // even entries, the other the odd ones (a tile of 16-position pages is eight copies,
+    // and issuing them takes a warp a quarter of the time that memory needs for them).
+    // A lane keeps the place of one slab: 32 slabs of page-table entries at a time, the
+    // next 32 on their way.
+    constexpr int kTileSlabs = KP / kSlab, kWinTiles = 32 / kTileSlabs;
     const uint64_t policy = l2_policy_evict_first();
-    uint32_t n = 0;  // tiles issued
+    const int spp = a.p.page_size / kSlab;             // slabs of a page: neighbours are copied
+    const int run = spp % 8 == 0 ? 8 : spp % 4 == 0 ? 4 : spp % 2 == 0 ? 2 : 1;   // together
+    const uint32_t parity = warp >> 1;
+    uint32_t n = 0;  // ring entries so far
     bool ok = true;
     for (int si = seg0; si < seg1 && ok; ++si) {
       const TreeSeg sg = a.segs[si];
       const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
+      const int last_slab = (end - 1) / kSlab;
+      const int32_t* table = a.p.block_tables + static_cast<size_t>(sg.bt_row) * a.p.bt_stride;
+      auto entry_of = [&](int win) -> int {            // page-table entry of a window's slab
+        const int slab = (sg.tile0 + win * kWinTiles) * kTileSlabs + lane;
+        const int col = slab / spp;
+        return slab <= last_slab && col < a.p.bt_stride ? table[col] : -1;
+      };
+      int win = 0, now = entry_of(0), next = entry_of(1);
       const int ahead = S::kStreams == 2 && sg.rows <= 128 ? 2 : 1;  // K runs this far ahead
       for (int step = 0; step < tiles + ahead && ok; ++step) {
         // step: V of tile step - ahead, then K of tile step
         for (int kv = 1; kv >= 0 && ok; --kv) {
           const int t = kv ? step - ahead : step;
           if (t < 0 || t >= tiles) continue;
-          const int p0 = (sg.tile0 + t) * KP + lane * kSlab;
-          const int slabs = min(KP / kSlab, (end - (sg.tile0 + t) * KP + kSlab - 1) / kSlab);
-          const uint8_t* src = nullptr;
-          if (lane < slabs) {
-            const int page = tree_page(a.p, sg.bt_row, p0);
-            src = (kv ? a.p.v : a.p.k) +
-                  (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) * a.p.page_head_bytes +
-                  static_cast<size_t>(p0 % a.p.page_size / kSlab) * kSlabBytes;
+          if ((n & 1) == parity) {
+            const int w = t / kWinTiles;
+            if (w != win) {
+              now = w == win + 1 ? next : entry_of(w);
+              next = entry_of(w + 1);
+              win = w;
+            }
+            const int slabs = min(kTileSlabs, last_slab + 1 - (sg.tile0 + t) * kTileSlabs);
+            int page = __shfl_sync(0xffffffffu, now, t % kWinTiles * kTileSlabs + (lane & (kTileSlabs - 1)));
+            const bool mine = lane < slabs && lane % run == 0;
+            const uint8_t* src = nullptr;
+            if (mine) {
+              if (page < 0 || page >= a.p.num_pages) {   // reported, and page 0 read instead
+                report_error_at(a.p.err, KVC_DEVERR_BAD_PAGE, static_cast<uint32_t>(page));
+                page = 0;
+              }
+              const int slab = (sg.tile0 + t) * kTileSlabs + lane;
+              src = (kv ? a.p.v : a.p.k) +
+                    (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) * a.p.page_head_bytes +
+                    slab % spp * kSlabBytes;
+            }
+            const int st = n % S::kStages;
+            if (n >= S::kStages) ok = wait(empty(st), (n / S::kStages - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(full(st), slabs * kSlabBytes);
+            __syncwarp();
+            if (mine)
+              bulk_g2s(smem_u32(stage_mem) + st * S::kStageBytes + lane * kSlabBytes, src,
+                       min(run, slabs - lane) * kSlabBytes, full(st), policy);
           }
-          const int st = n % S::kStages;
-          if (n >= S::kStages) ok = wait(empty(st), (n / S::kStages - 1) & 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(full(st), slabs * kSlabBytes);
-          __syncwarp();
-          if (lane < slabs)
-            bulk_g2s(smem_u32(stage_mem) + st * S::kStageBytes + lane * kSlabBytes, src, kSlabBytes,
-                     full(st), policy);
           ++n;
         }
       }
     }
     if (!ok) {  // copies in flight land before the CTA's memory goes
-      for (uint32_t i = n > S::kStages ? n - S::kStages : 0; i < n; ++i)
-        mbar_wait_bounded(full(i % S::kStages), (i / S::kStages) & 1);
+      for (uint32_t i = n > 2 * S::kStages ? n - 2 * S::kStages : 0; i < n; ++i)
+        if ((i & 1) == parity) mbar_wait_bounded(full(i % S::kStages), (i / S::kStages) & 1);
     }
   } else if (warp == 1) {
     // ---- MMAs: the warp waits together, one lane issues.  Everything an MMA takes is
@@ -364,9 +393,8 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     }
     __syncwarp();
   } else {
-    // ---- helpers: each piece's Q, and the V tiles that hold drafted positions -------------
-    const int h = threadIdx.x - 64;
-    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale turns q
+    // ---- helper: each piece's Q, and the V tiles that hold drafted positions --------------
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
     uint32_t ring = 0, nf = 0, ng = 0;
     bool ok = true;
     for (int si = seg0; si < seg1; ++si) {
@@ -374,44 +402,34 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
       const bool two = sg.rows > 128;
       const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-      // Q in k-major core matrices: a warp's load covers 8 rows x 64 bytes, and kQLoads rows
-      // of loads are in flight, the first of them before the last piece's scores are done.
-      // Streams that share their rows get a copy each.
-      constexpr int kQLoads = 2;
-      const int rr = lane >> 2, uu = lane & 3;
-      const int n_rows = two ? 256 : 128;
-      for (int g0 = (warp - 2) * 8 * kQLoads; g0 < n_rows; g0 += 16 * kQLoads) {
-        uint4 v[kQLoads][U / 4];
-#pragma unroll
-        for (int g = 0; g < kQLoads; ++g) {
-          const int row = g0 + 8 * g + rr, grow = sg.row0 + row, node = grow / a.group;
-          const uint4* src = reinterpret_cast<const uint4*>(
-              reinterpret_cast<const T*>(a.q) +
-              (static_cast<size_t>(sg.tok0 + node) * a.num_heads + sg.kvh * a.group + grow -
-               node * a.group) * D);
-#pragma unroll
-          for (int i = 0; i < U / 4; ++i)
-            v[g][i] = row < sg.rows ? src[4 * i + uu] : make_uint4(0, 0, 0, 0);
-        }
-        if (si > seg0 && g0 < 16 * kQLoads) ok = ok && wait(q_free, nf & 1);
-        if (!ok) break;
-#pragma unroll
-        for (int g = 0; g < kQLoads; ++g) {
-          const int row = g0 + 8 * g + rr;
-          uint8_t* dst = q_mem + (row >> 7) * S::kQBytes + ((row & 127) >> 3) * U * 128 + rr * 16;
+      // Q in k-major core matrices, all its copies in flight together: a warp's copy covers
+      // 8 rows x 64 bytes, rows past the block are zero.  Streams that share their rows get
+      // a copy each.
+      if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
+      if (ok) {
+        const int rr = lane >> 2, uu = lane & 3;
+        const int n_rows = two ? 256 : 128;
+        for (int g0 = 0; g0 < n_rows; g0 += 8) {
+          const int row = g0 + rr, grow = sg.row0 + min(row, sg.rows - 1), node = grow / a.group;
+          const T* src = reinterpret_cast<const T*>(a.q) +
+                         (static_cast<size_t>(sg.tok0 + node) * a.num_heads + sg.kvh * a.group +
+                          grow - node * a.group) * D;
+          const uint32_t dst = smem_u32(q_mem) + (row >> 7) * S::kQBytes +
+                               ((row & 127) >> 3) * U * 128 + rr * 16;
+          const uint32_t bytes = row < sg.rows ? 16 : 0;
 #pragma unroll
           for (int i = 0; i < U / 4; ++i) {
-            v[g][i].x ^= flip;
-            v[g][i].y ^= flip;
-            v[g][i].z ^= flip;
-            v[g][i].w ^= flip;
-            *reinterpret_cast<uint4*>(dst + (4 * i + uu) * 128) = v[g][i];
+            copy16_async(dst + (4 * i + uu) * 128, src + (4 * i + uu) * 8, bytes);
             if (S::kStreams == 2 && !two)
-              *reinterpret_cast<uint4*>(dst + S::kQBytes + (4 * i + uu) * 128) = v[g][i];
+              copy16_async(dst + S::kQBytes + (4 * i + uu) * 128, src + (4 * i + uu) * 8, bytes);
           }
         }
+        copy_async_wait();
+        if (flip) {   // a negative scale turns q
+          for (int i = lane; i < S::kStreams * S::kQBytes / 4; i += 32)
+            reinterpret_cast<uint32_t*>(q_mem)[i] ^= flip;
+        }
       }
-      if (si > seg0) ++nf;
       fence_proxy_async();
       mbar_arrive(q_ready);
       // V of drafted tokens: what is not finite would spread through zero weights to rows
@@ -428,7 +446,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
           uint8_t* vt = stage_mem + st * S::kStageBytes;
           const int from = max(0, sg.ctx - p0), to = min(KP, (end - p0 + kSlab - 1) / kSlab * kSlab);
           bool dirty = false;
-          for (int i = from * U + h; i < to * U; i += 64) {
+          for (int i = from * U + lane; i < to * U; i += 32) {
             const int pt = i / U, u = i - pt * U;
             uint4* cell = reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
             uint4 v = make_uint4(0, 0, 0, 0);
