@@ -482,17 +482,13 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     uint32_t ns = 0, no[2] = {0, 0};
     bool ok = true;
     for (int si = seg0; si < seg1; ++si) {
-      const TreeSeg sg = a.segs[si];
-      const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
-      const bool two = sg.rows > 128;
+      const TreeSeg* seg = a.segs + si;   // (read again where it is needed again: no spills)
+      const int tiles = seg->tile1 - seg->tile0, p00 = seg->tile0 * KP, ctx = seg->ctx;
+      const bool two = seg->rows > 128;
       const int ahead = S::kStreams == 2 && !two ? 2 : 1;
       const bool joint = ahead == 2;
       const int row = (two ? x * 128 : 0) + r;
-      const bool live_row = row < sg.rows;
-      const bool live = (two ? x * 128 : 0) + w4 * 32 < sg.rows;   // some row of the warp
-      const int grow = sg.row0 + min(row, sg.rows - 1);
-      const int node = grow / a.group, head = sg.kvh * a.group + grow - node * a.group;
-      const size_t io_row = (static_cast<size_t>(sg.tok0 + node) * a.num_heads + head) * D;
+      const bool live = (two ? x * 128 : 0) + w4 * 32 < seg->rows;   // some row of the warp
       float m = kNegBig, l = 0.f;     // max in log2 units
       // One tile of the stream: scores to probabilities, in place, and the running max and
       // sum.  Edge tiles hold positions that some rows do not see.
@@ -584,13 +580,15 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         tmem_wait_st();
       };
       for (int t = joint ? x : 0; t < tiles; t += ahead) {
-        const int p0 = (sg.tile0 + t) * KP;
-        const bool edge = p0 + KP > sg.ctx;
+        const int p0 = p00 + t * KP;
+        const bool edge = p0 + KP > ctx;
         uint32_t vis[KP / 32];   // of an edge tile: the positions that the row sees
         if (edge && live) {
+          const TreeSeg sg = *seg;
+          const int node = (sg.row0 + min(row, sg.rows - 1)) / a.group;
 #pragma unroll
           for (int w = 0; w < KP / 32; ++w) {
-            const int j0 = p0 + 32 * w - sg.ctx;
+            const int j0 = p0 + 32 * w - ctx;
             const int k = j0 >> 5;
             vis[w] = __funnelshift_r(mask_word(a, sg, node, k), mask_word(a, sg, node, k + 1), j0 & 31);
           }
@@ -625,6 +623,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       ok = __all_sync(0xffffffffu, ok);
       tmem_fence_after();
       if (live && ok) {
+        const TreeSeg sg = *seg;
+        const bool live_row = row < sg.rows;
+        const int grow = sg.row0 + min(row, sg.rows - 1);
+        const int node = grow / a.group, head = sg.kvh * a.group + grow - node * a.group;
+        const size_t io_row = (static_cast<size_t>(sg.tok0 + node) * a.num_heads + head) * D;
         float w0 = 1.f, w1 = 0.f, mm = m, ll = l;
         if (joint) {
           const float2 e0 = s_ml[r], e1 = s_ml[128 + r];
@@ -636,7 +639,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const bool dirty = s_dirty[si & 1] == si;
         // rare: what was taken out of V comes back, for the nodes that this row sees
         auto restore = [&](int c, float* f) {
-          const int t0 = max(sg.tile0 * KP, sg.ctx), t1 = min(sg.tile1 * KP, end);
+          const int t0 = max(sg.tile0 * KP, sg.ctx), t1 = min(sg.tile1 * KP, sg.ctx + sg.nodes);
           for (int pos = t0; pos < t1; ++pos) {
             const int j = pos - sg.ctx;
             if (!((mask_word(a, sg, node, j >> 5) >> (j & 31)) & 1u)) continue;
