@@ -23,9 +23,9 @@ namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kChunkWarps = 8;
-constexpr int kPerLane = 16;                                // logits a lane holds
-constexpr int kWarpSpan = 32 * kPerLane;
-constexpr int kChunk = kChunkWarps * kWarpSpan;             // logits of one CTA
+constexpr int kPerLane = 16;                                // logits a lane holds at a time
+constexpr int kBatch = 32 * kPerLane;                       // logits a warp takes at a time
+constexpr int kMinChunk = kChunkWarps * kBatch;             // logits of one CTA, at least
 
 // Bits of a finite float or -inf that order like the value.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -62,107 +62,171 @@ __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
   return key;
 }
 
-// A chunk: every lane holds kPerLane logits.  The n_out-th largest of the 32 lanes'
-// best is a bound that at least n_out logits of the warp reach, and only lanes whose
-// best reaches it hold any: few logits are sorted.
+// 16 logits of a lane, as fp32; what is not finite, and what lies past the row, is -inf.
+// Which lane holds which token never depends on the row's address, so equal rows have
+// equal sums.  A row that starts off a 16-byte boundary is read in aligned pairs of
+// vectors and shifted into place; vectors that reach past the row go element by element.
+template <typename T>
+struct Batch {
+  static constexpr int N = 16 / sizeof(T), V = kPerLane / N;
+  union Vec {
+    uint32_t w[8];
+    uint4 q[2];
+    T raw[2 * N];
+    __device__ Vec() {}
+  };
+  Vec v[V];
+
+  __device__ __forceinline__ void load(const T* x, int lead, int vocab, int t0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int t = t0 + i * 32 * N;
+      if (lead == 0 && t + N <= vocab) {
+        v[i].q[0] = __ldcs(reinterpret_cast<const uint4*>(x + t));
+      } else if (t >= lead && t - lead + 2 * N <= vocab) {
+        v[i].q[0] = *reinterpret_cast<const uint4*>(x + t - lead);
+        v[i].q[1] = *reinterpret_cast<const uint4*>(x + t - lead + N);
+        const int bytes = lead * static_cast<int>(sizeof(T));
+        if (bytes & 8) {
+#pragma unroll
+          for (int k = 0; k < 6; ++k) v[i].w[k] = v[i].w[k + 2];
+        }
+        if (bytes & 4) {
+#pragma unroll
+          for (int k = 0; k < 5; ++k) v[i].w[k] = v[i].w[k + 1];
+        }
+        if (bytes & 2) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[i].w[k] = __funnelshift_r(v[i].w[k], v[i].w[k + 1], 16);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i].raw[e] = t + e < vocab ? x[t + e] : from_f32<T>(-INFINITY);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float* f, bool dead) const {
+    float odd = 0.f;   // NaN as soon as one is not finite
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      f[i] = to_f32<T>(v[i / N].raw[i % N]);
+      odd = fmaf(f[i], 0.f, odd);
+    }
+    if (dead || odd != 0.f) {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i)
+        if (dead || !isfinite(f[i])) f[i] = -INFINITY;
+    }
+  }
+};
+
+// exp(x - m), x at most m; the difference is taken first, so that nothing is lost or
+// overflows where both are large.
+__device__ __forceinline__ float exp_diff(float x, float m) {
+  return m == -INFINITY ? 0.f : fast_exp2((x - m) * kLog2e);
+}
+
+// One CTA takes `batches` x kMinChunk logits of a row, each warp a run of its own.  A lane
+// keeps a running max and sum.  The warp's best are a sorted list; a logit joins only if it
+// beats the list's n_out-th (an equal one comes later in the row and loses), which soon
+// almost none does: they wait in shared memory and go in 32 at a time.  The first batch has
+// no such bound and takes the n_out-th largest of the lanes' best, which at least n_out
+// logits reach, all of them in n_out lanes.
 template <typename T>
 __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const BeamArgs a) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  launch_dependents();
   __shared__ uint64_t s_pend[kChunkWarps][64];
   __shared__ uint64_t s_list[kChunkWarps][32];
   __shared__ float2 s_ml[kChunkWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.y;
-  const int first = blockIdx.x * kChunk + warp * kWarpSpan;
+  const int first = (blockIdx.x * kChunkWarps + warp) * a.batches * kBatch;
   const T* x = reinterpret_cast<const T*>(a.logits + static_cast<size_t>(row) * a.row_bytes);
-  constexpr int N = 16 / sizeof(T);
-  // Which lane holds which token never depends on the row's address, so equal rows have
-  // equal sums.  A row that starts off a 16-byte boundary is read in aligned pairs of
-  // vectors and shifted into place; vectors that reach past the row go element by element.
+  using B = Batch<T>;
+  constexpr int N = B::N;
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
-  float v[kPerLane];
+  wait_prerequisites();
+  const bool dead = !isfinite(a.cum[row]);   // a beam that is not in use
+  float m = -INFINITY, sum = 0.f;
+  uint64_t list = 0, bound = 0;              // bound: key of the list's n_out-th
+  float bound_f = -INFINITY;
+  int pending = 0;
+  auto flush = [&](int count) {
+    list = merge32(list, sort32(lane < count ? s_pend[warp][lane] : 0, lane), lane);
+    bound = __shfl_sync(kAll, list, a.n_out - 1);
+    bound_f = bound ? from_ordered(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
+  };
+  B now, next;
+  now.load(x, lead, a.vocab, first + lane * N);
+  for (int b = 0; b < a.batches; ++b) {
+    const int t0 = first + b * kBatch + lane * N;
+    if (t0 - lane * N >= a.vocab) break;
+    if (b + 1 < a.batches) next.load(x, lead, a.vocab, t0 + kBatch);
+    float f[kPerLane];
+    now.get(f, dead);
+    float top = f[0];
 #pragma unroll
-  for (int i = 0; i < kPerLane / N; ++i) {
-    const int t0 = first + (i * 32 + lane) * N;
-    union {
-      uint32_t w[8];
-      uint4 q[2];
-      T raw[2 * N];
-    };
-    if (lead == 0 && t0 + N <= a.vocab) {
-      q[0] = __ldcs(reinterpret_cast<const uint4*>(x + t0));
-    } else if (t0 >= lead && t0 - lead + 2 * N <= a.vocab) {
-      q[0] = *reinterpret_cast<const uint4*>(x + t0 - lead);
-      q[1] = *reinterpret_cast<const uint4*>(x + t0 - lead + N);
-      const int bytes = lead * static_cast<int>(sizeof(T));
-      if (bytes & 8) {
+    for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, f[i]);
+    const float mm = fmaxf(m, top), ref = mm == -INFINITY ? 0.f : mm;
+    float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
-      }
-      if (bytes & 4) {
-#pragma unroll
-        for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
-      }
-      if (bytes & 2) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) raw[e] = t0 + e < a.vocab ? x[t0 + e] : from_f32<T>(0.f);
+    for (int i = 0; i < kPerLane; i += 2) {
+      const float2 d = mul2(add2(make_float2(f[i], f[i + 1]), make_float2(-ref, -ref)),
+                            make_float2(kLog2e, kLog2e));
+      part = add2(part, make_float2(fast_exp2(d.x), fast_exp2(d.y)));
     }
+    sum = sum * exp_diff(m, mm) + (part.x + part.y);
+    m = mm;
+    if (b == 0) {
+      uint64_t best = 0;
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[i * N + e] = to_f32<T>(raw[e]);
-  }
-  // a beam that is not in use: its candidates all score -inf
-  const bool dead = !isfinite(a.cum[row]);
-  uint64_t best = 0;
-  float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int t = first + ((i / N) * 32 + lane) * N + i % N;
-    if (dead || !isfinite(v[i])) v[i] = -INFINITY;
-    if (t < a.vocab) {
-      mx = fmaxf(mx, v[i]);
-      const uint64_t key = make_key(v[i], t);
-      best = key > best ? key : best;
+      for (int i = 0; i < kPerLane; ++i) {
+        const int t = t0 + (i / N) * 32 * N + i % N;
+        const uint64_t key = t < a.vocab ? make_key(f[i], t) : 0;
+        best = key > best ? key : best;
+      }
+      const uint64_t reach = __shfl_sync(kAll, sort32(best, lane), a.n_out - 1);
+      bound = reach ? reach - 1 : 0;         // the list is empty: those that reach it join
     }
-  }
+    const bool open = bound == 0;            // fewer than n_out so far: all join
+    if (b == 0 || __any_sync(kAll, open || top > bound_f)) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int t = first + ((i / N) * 32 + lane) * N + i % N;
-    if (t < a.vocab && v[i] != -INFINITY) sum += fast_exp2((v[i] - mx) * kLog2e);
+      for (int i = 0; i < kPerLane; ++i) {
+        const int t = t0 + (i / N) * 32 * N + i % N;
+        const bool in = t < a.vocab && (b == 0 || open ? make_key(f[i], t) > bound : f[i] > bound_f);
+        const unsigned hits = __ballot_sync(kAll, in);
+        if (hits == 0) continue;
+        if (in) s_pend[warp][pending + __popc(hits & ((1u << lane) - 1u))] = make_key(f[i], t);
+        pending += __popc(hits);
+        __syncwarp();
+        if (pending >= 32) {
+          list = merge32(list, sort32(s_pend[warp][lane], lane), lane);
+          pending -= 32;
+          const uint64_t rest = s_pend[warp][32 + lane];
+          __syncwarp();
+          s_pend[warp][lane] = rest;
+          __syncwarp();
+        }
+      }
+      if (pending > 0 && (b == 0 || pending >= 16)) {
+        flush(pending);
+        pending = 0;
+        __syncwarp();
+      } else {
+        bound = __shfl_sync(kAll, list, a.n_out - 1);
+        bound_f = bound ? from_ordered(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
+      }
+    }
+    now = next;
   }
+  if (pending > 0) flush(pending);
+  float wm = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(kAll, wm, o));
+  sum *= exp_diff(m, wm);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-  if (lane == 0) s_ml[warp] = make_float2(mx, sum);
-
-  const uint64_t bound = __shfl_sync(kAll, sort32(best, lane), a.n_out - 1);
-  uint64_t list = 0;
-  int pending = 0;
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int t = first + ((i / N) * 32 + lane) * N + i % N;
-    const uint64_t key = t < a.vocab ? make_key(v[i], t) : 0;
-    const bool in = key != 0 && key >= bound;
-    const unsigned hits = __ballot_sync(kAll, in);
-    if (hits == 0) continue;
-    if (in) s_pend[warp][pending + __popc(hits & ((1u << lane) - 1u))] = key;
-    pending += __popc(hits);
-    __syncwarp();
-    if (pending >= 32) {
-      list = merge32(list, sort32(s_pend[warp][lane], lane), lane);
-      pending -= 32;
-      const uint64_t rest = s_pend[warp][32 + lane];
-      __syncwarp();
-      s_pend[warp][lane] = rest;
-      __syncwarp();
-    }
-  }
-  if (pending > 0) list = merge32(list, sort32(lane < pending ? s_pend[warp][lane] : 0, lane), lane);
+  if (lane == 0) s_ml[warp] = make_float2(wm, sum);
   s_list[warp][lane] = list;
   __syncthreads();
 #pragma unroll
@@ -177,13 +241,13 @@ __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const Beam
     const size_t slot = static_cast<size_t>(row) * a.n_chunks + blockIdx.x;
     if (lane < a.n_out) a.cand[slot * a.n_out + lane] = list;
     float2 ml = lane < kChunkWarps ? s_ml[lane] : make_float2(-INFINITY, 0.f);
-    float m = ml.x;
+    float top = ml.x;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-    float l = ml.y > 0.f ? ml.y * fast_exp2((ml.x - m) * kLog2e) : 0.f;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+    float l = ml.y * exp_diff(ml.x, top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(kAll, l, o);
-    if (lane == 0) a.ml[slot] = make_float2(m, l);
+    if (lane == 0) a.ml[slot] = make_float2(top, l);
   }
 }
 
@@ -213,15 +277,22 @@ __device__ __forceinline__ Scored merge32(Scored x, const Scored& y, int lane) {
 // then the beams' lists are joined pairwise.  Scores are held in 64 bits so that
 // candidates of different beams that lie close together keep their order.
 __global__ void __launch_bounds__(32 * kMaxBeams) beam_merge_kernel(const BeamArgs a) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  launch_dependents();
+  wait_prerequisites();
   __shared__ Scored s_list[kMaxBeams][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seq = blockIdx.x, row = seq * a.beams + warp;
   const size_t slot0 = static_cast<size_t>(row) * a.n_chunks;
   uint64_t list = 0;
   float m = -INFINITY;
-  for (int c = 0; c < a.n_chunks; ++c)
-    list = merge32(list, lane < a.n_out ? a.cand[(slot0 + c) * a.n_out + lane] : 0, lane);
+  for (int c0 = 0; c0 < a.n_chunks; c0 += 4) {   // four lists on their way at a time
+    uint64_t l4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      l4[i] = c0 + i < a.n_chunks && lane < a.n_out ? a.cand[(slot0 + c0 + i) * a.n_out + lane] : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) list = merge32(list, l4[i], lane);
+  }
   for (int c = lane; c < a.n_chunks; c += 32) m = fmaxf(m, a.ml[slot0 + c].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
@@ -263,28 +334,41 @@ __global__ void __launch_bounds__(32 * kMaxBeams) beam_merge_kernel(const BeamAr
 
 }  // namespace
 
-int beam_chunks(int vocab, int) { return (vocab + kChunk - 1) / kChunk; }
+int beam_chunks(int vocab) { return (vocab + kMinChunk - 1) / kMinChunk; }
 
-cudaError_t launch_beam_select(const BeamArgs& a, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.n_chunks), static_cast<unsigned>(a.n * a.beams));
-  switch (a.dtype) {
-    case KVC_DTYPE_F16: beam_chunk_kernel<__half><<<grid, 32 * kChunkWarps, 0, s>>>(a); break;
-    case KVC_DTYPE_BF16: beam_chunk_kernel<__nv_bfloat16><<<grid, 32 * kChunkWarps, 0, s>>>(a); break;
-    case KVC_DTYPE_F32: beam_chunk_kernel<float><<<grid, 32 * kChunkWarps, 0, s>>>(a); break;
-    default: return cudaErrorInvalidValue;
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+namespace {
+// A launch that may begin before the one ahead of it has ended.
+template <typename K>
+cudaError_t launch_early(K kernel, dim3 grid, int threads, cudaStream_t s, const BeamArgs& a) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.n));
-  cfg.blockDim = dim3(static_cast<unsigned>(32 * a.beams));
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, beam_merge_kernel, a);
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+}  // namespace
+
+cudaError_t launch_beam_select(BeamArgs a, cudaStream_t s) {
+  // Longer runs spread a warp's sorting over more logits; shorter ones fill the GPU.
+  const int rows = a.n * a.beams, most = beam_chunks(a.vocab);
+  a.batches = 8;
+  while (a.batches > 1 && static_cast<int64_t>(rows) * most / a.batches < 4 * 148) a.batches /= 2;
+  a.n_chunks = (most + a.batches - 1) / a.batches;
+  const dim3 grid(static_cast<unsigned>(a.n_chunks), static_cast<unsigned>(rows));
+  cudaError_t e;
+  switch (a.dtype) {
+    case KVC_DTYPE_F16: e = launch_early(beam_chunk_kernel<__half>, grid, 32 * kChunkWarps, s, a); break;
+    case KVC_DTYPE_BF16: e = launch_early(beam_chunk_kernel<__nv_bfloat16>, grid, 32 * kChunkWarps, s, a); break;
+    case KVC_DTYPE_F32: e = launch_early(beam_chunk_kernel<float>, grid, 32 * kChunkWarps, s, a); break;
+    default: return cudaErrorInvalidValue;
+  }
+  if (e != cudaSuccess) return e;
+  return launch_early(beam_merge_kernel, dim3(static_cast<unsigned>(a.n)), 32 * a.beams, s, a);
 }
 
 }  // namespace kvc

@@ -129,12 +129,12 @@ struct BeamArgs {
   int32_t* parents;
   float* scores;
   // workspace: per (row, chunk) the max, the sum and the n_out best candidates
-  int n_chunks;
+  int n_chunks, batches;         // set by the launcher: chunks of a row, batches of a warp
   float2* ml;
   uint64_t* cand;
 };
-int beam_chunks(int vocab, int dtype);
-cudaError_t launch_beam_select(const BeamArgs& a, cudaStream_t s);
+int beam_chunks(int vocab);   // at most
+cudaError_t launch_beam_select(BeamArgs a, cudaStream_t s);
 
 cudaError_t launch_append_rope(const AppendRopeArgs& a, cudaStream_t s);
 cudaError_t launch_commit(const CommitArgs& a, cudaStream_t s);

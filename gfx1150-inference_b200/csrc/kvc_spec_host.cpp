@@ -494,7 +494,7 @@ extern "C" int kvc_beam_create(int max_seqs, int max_beams, int max_vocab, int m
     if (max_vocab >= (1 << 27) || static_cast<int64_t>(max_seqs) * max_beams > 65535)
       return set_error(KVC_ERR_INVALID_ARG, "the vocabulary or the batch is too large.");
     const int64_t slots = static_cast<int64_t>(max_seqs) * max_beams *
-                          beam_chunks(max_vocab, KVC_DTYPE_F32);
+                          beam_chunks(max_vocab);
     if (slots > (1ll << 30) / max_out)
       return set_error(KVC_ERR_INVALID_ARG, "the beam workspace would be too large.");
     DeviceScope dev(device);
@@ -562,7 +562,6 @@ extern "C" int kvc_beam_select(kvc_beam_t* beam, const void* d_logits, int dtype
     a.tokens = d_tokens;
     a.parents = d_parents;
     a.scores = d_scores_out;
-    a.n_chunks = beam_chunks(vocab, dtype);
     a.ml = static_cast<float2*>(beam->ws.ptr);
     a.cand = reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(beam->ws.ptr) + beam->ml_bytes);
     const cudaError_t e = launch_beam_select(a, static_cast<cudaStream_t>(stream));
