@@ -126,12 +126,12 @@ __device__ __forceinline__ float exp_diff(float x, float m) {
   return m == -INFINITY ? 0.f : fast_exp2((x - m) * kLog2e);
 }
 
-// One CTA takes `batches` x kMinChunk logits of a row, each warp a run of its own.  A lane
-// keeps a running max and sum.  The warp's best are a sorted list; a logit joins only if it
-// beats the list's n_out-th (an equal one comes later in the row and loses), which soon
-// almost none does: they wait in shared memory and go in 32 at a time.  The first batch has
-// no such bound and takes the n_out-th largest of the lanes' best, which at least n_out
-// logits reach, all of them in n_out lanes.
+// One CTA takes `batches` x kMinChunk logits of a row, each warp a run of its own, in one
+// pass over memory that keeps a running max and sum per lane and nothing else.  The n_out-th
+// largest of the 256 lanes' best then bounds the chunk's n_out best from below, and only the
+// n_out lanes whose best reaches it can hold any of them: these lanes read their logits once
+// more (from L2) for the few that do.  (Keeping candidates during the pass cost four times
+// the instructions: nearly every batch of a run holds one that looks good so far.)
 template <typename T>
 __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const BeamArgs a) {
   launch_dependents();
@@ -145,58 +145,96 @@ __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const Beam
   using B = Batch<T>;
   constexpr int N = B::N;
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+  // batches of this warp that reach into the row; token of a lane's logit i of batch b
+  const int batches = min(a.batches, (a.vocab - first + kBatch - 1) / kBatch);
+  auto token = [&](int b, int i) { return first + b * kBatch + lane * N + (i / N) * 32 * N + i % N; };
   wait_prerequisites();
   const bool dead = !isfinite(a.cum[row]);   // a beam that is not in use
   float m = -INFINITY, sum = 0.f;
-  uint64_t list = 0, bound = 0;              // bound: key of the list's n_out-th
-  float bound_f = -INFINITY;
-  int pending = 0;
-  auto flush = [&](int count) {
-    list = merge32(list, sort32(lane < count ? s_pend[warp][lane] : 0, lane), lane);
-    bound = __shfl_sync(kAll, list, a.n_out - 1);
-    bound_f = bound ? from_ordered(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
-  };
-  B now, next;
-  now.load(x, lead, a.vocab, first + lane * N);
-  for (int b = 0; b < a.batches; ++b) {
-    const int t0 = first + b * kBatch + lane * N;
-    if (t0 - lane * N >= a.vocab) break;
-    if (b + 1 < a.batches) next.load(x, lead, a.vocab, t0 + kBatch);
-    float f[kPerLane];
-    now.get(f, dead);
-    float top = f[0];
+  int at = 0;                                // the batch of the lane's best
+  {
+    B now, next;
+    if (batches > 0) now.load(x, lead, a.vocab, token(0, 0));
+    for (int b = 0; b < batches; ++b) {
+      if (b + 1 < batches) next.load(x, lead, a.vocab, token(b + 1, 0));
+      float f[kPerLane];
+      now.get(f, dead);
+      float top = f[0];
 #pragma unroll
-    for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, f[i]);
-    const float mm = fmaxf(m, top), ref = mm == -INFINITY ? 0.f : mm;
-    float2 part = make_float2(0.f, 0.f);
+      for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, f[i]);
+      if (top > m) at = b;
+      const float mm = fmaxf(m, top), ref = mm == -INFINITY ? 0.f : mm;
+      float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kPerLane; i += 2) {
-      const float2 d = mul2(add2(make_float2(f[i], f[i + 1]), make_float2(-ref, -ref)),
-                            make_float2(kLog2e, kLog2e));
-      part = add2(part, make_float2(fast_exp2(d.x), fast_exp2(d.y)));
-    }
-    sum = sum * exp_diff(m, mm) + (part.x + part.y);
-    m = mm;
-    if (b == 0) {
-      uint64_t best = 0;
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        const int t = t0 + (i / N) * 32 * N + i % N;
-        const uint64_t key = t < a.vocab ? make_key(f[i], t) : 0;
-        best = key > best ? key : best;
+      for (int i = 0; i < kPerLane; i += 2) {
+        const float2 d = mul2(add2(make_float2(f[i], f[i + 1]), make_float2(-ref, -ref)),
+                              make_float2(kLog2e, kLog2e));
+        part = add2(part, make_float2(fast_exp2(d.x), fast_exp2(d.y)));
       }
-      const uint64_t reach = __shfl_sync(kAll, sort32(best, lane), a.n_out - 1);
-      bound = reach ? reach - 1 : 0;         // the list is empty: those that reach it join
+      sum = sum * exp_diff(m, mm) + (part.x + part.y);
+      m = mm;
+      now = next;
     }
-    const bool open = bound == 0;            // fewer than n_out so far: all join
-    if (b == 0 || __any_sync(kAll, open || top > bound_f)) {
+  }
+  float wm = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(kAll, wm, o));
+  sum *= exp_diff(m, wm);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+  if (lane == 0) s_ml[warp] = make_float2(wm, sum);
+
+  // the lane's best: the first logit of its batch that has the lane's max
+  uint64_t best = 0;
+  if (batches > 0) {
+    B again;
+    again.load(x, lead, a.vocab, token(at, 0));
+    float f[kPerLane];
+    again.get(f, dead);
+#pragma unroll
+    for (int i = kPerLane - 1; i >= 0; --i)
+      if (f[i] == m && token(at, i) < a.vocab) best = make_key(m, token(at, i));
+  }
+  // joins the warps' descending lists; the result is warp 0's
+  auto join = [&](uint64_t list) {
+    s_list[warp][lane] = list;
+    __syncthreads();
+#pragma unroll
+    for (int half = kChunkWarps / 2; half > 0; half >>= 1) {
+      if (warp < half) {
+        list = merge32(list, s_list[warp + half][lane], lane);
+        s_list[warp][lane] = list;
+      }
+      __syncthreads();
+    }
+    return list;
+  };
+  join(sort32(best, lane));
+  const uint64_t bound = s_list[0][a.n_out - 1];
+  const float bound_f = bound ? from_ordered(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
+  __syncthreads();
+  const bool holds = best != 0 && best >= bound;
+  uint64_t list = 0;
+  if (__any_sync(kAll, holds)) {
+    int pending = 0;
+    for (int b = 0; b < batches; ++b) {
+      float f[kPerLane], top = -INFINITY;
+      if (holds) {
+        B again;
+        again.load(x, lead, a.vocab, token(b, 0));
+        again.get(f, dead);
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) top = fmaxf(top, f[i]);
+      }
+      if (!__any_sync(kAll, holds && top >= bound_f)) continue;
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) {
-        const int t = t0 + (i / N) * 32 * N + i % N;
-        const bool in = t < a.vocab && (b == 0 || open ? make_key(f[i], t) > bound : f[i] > bound_f);
+        const int t = token(b, i);
+        const uint64_t key = holds && t < a.vocab && f[i] >= bound_f ? make_key(f[i], t) : 0;
+        const bool in = key != 0 && key >= bound;
         const unsigned hits = __ballot_sync(kAll, in);
         if (hits == 0) continue;
-        if (in) s_pend[warp][pending + __popc(hits & ((1u << lane) - 1u))] = make_key(f[i], t);
+        if (in) s_pend[warp][pending + __popc(hits & ((1u << lane) - 1u))] = key;
         pending += __popc(hits);
         __syncwarp();
         if (pending >= 32) {
@@ -208,35 +246,11 @@ __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const Beam
           __syncwarp();
         }
       }
-      if (pending > 0 && (b == 0 || pending >= 16)) {
-        flush(pending);
-        pending = 0;
-        __syncwarp();
-      } else {
-        bound = __shfl_sync(kAll, list, a.n_out - 1);
-        bound_f = bound ? from_ordered(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
-      }
     }
-    now = next;
+    if (pending > 0)
+      list = merge32(list, sort32(lane < pending ? s_pend[warp][lane] : 0, lane), lane);
   }
-  if (pending > 0) flush(pending);
-  float wm = m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(kAll, wm, o));
-  sum *= exp_diff(m, wm);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-  if (lane == 0) s_ml[warp] = make_float2(wm, sum);
-  s_list[warp][lane] = list;
-  __syncthreads();
-#pragma unroll
-  for (int half = kChunkWarps / 2; half > 0; half >>= 1) {
-    if (warp < half) {
-      list = merge32(list, s_list[warp + half][lane], lane);
-      s_list[warp][lane] = list;
-    }
-    __syncthreads();
-  }
+  list = join(list);
   if (warp == 0) {
     const size_t slot = static_cast<size_t>(row) * a.n_chunks + blockIdx.x;
     if (lane < a.n_out) a.cand[slot * a.n_out + lane] = list;
