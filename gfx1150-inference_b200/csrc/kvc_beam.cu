@@ -25,6 +25,7 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int kChunkWarps = 8;
 constexpr int kPerLane = 16;                                // logits a lane holds at a time
 constexpr int kBatch = 32 * kPerLane;                       // logits a warp takes at a time
+constexpr int kMaxBatches = 8;                              // that a warp takes
 constexpr int kMinChunk = kChunkWarps * kBatch;             // logits of one CTA, at least
 
 // Bits of a finite float or -inf that order like the value.
@@ -62,6 +63,21 @@ __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
   return key;
 }
 
+template <typename T>
+struct Pair {
+  using type = float2;
+};
+template <>
+struct Pair<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ __half2 zero() { return __float2half2_rn(0.f); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ __nv_bfloat162 zero() { return __float2bfloat162_rn(0.f); }
+};
+
 // 16 logits of a lane, as fp32; what is not finite, and what lies past the row, is -inf.
 // Which lane holds which token never depends on the row's address, so equal rows have
 // equal sums.  A row that starts off a 16-byte boundary is read in aligned pairs of
@@ -77,46 +93,71 @@ struct Batch {
   };
   Vec v[V];
 
-  __device__ __forceinline__ void load(const T* x, int lead, int vocab, int t0) {
+  static __device__ __forceinline__ void load_vec(Vec& v, const T* x, int lead, int vocab, int t) {
+    if (lead == 0 && t + N <= vocab) {
+      v.q[0] = *reinterpret_cast<const uint4*>(x + t);
+    } else if (t >= lead && t - lead + 2 * N <= vocab) {
+      v.q[0] = *reinterpret_cast<const uint4*>(x + t - lead);
+      v.q[1] = *reinterpret_cast<const uint4*>(x + t - lead + N);
+      const int bytes = lead * static_cast<int>(sizeof(T));
+      if (bytes & 8) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int t = t0 + i * 32 * N;
-      if (lead == 0 && t + N <= vocab) {
-        v[i].q[0] = __ldcs(reinterpret_cast<const uint4*>(x + t));
-      } else if (t >= lead && t - lead + 2 * N <= vocab) {
-        v[i].q[0] = *reinterpret_cast<const uint4*>(x + t - lead);
-        v[i].q[1] = *reinterpret_cast<const uint4*>(x + t - lead + N);
-        const int bytes = lead * static_cast<int>(sizeof(T));
-        if (bytes & 8) {
-#pragma unroll
-          for (int k = 0; k < 6; ++k) v[i].w[k] = v[i].w[k + 2];
-        }
-        if (bytes & 4) {
-#pragma unroll
-          for (int k = 0; k < 5; ++k) v[i].w[k] = v[i].w[k + 1];
-        }
-        if (bytes & 2) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[i].w[k] = __funnelshift_r(v[i].w[k], v[i].w[k + 1], 16);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[i].raw[e] = t + e < vocab ? x[t + e] : from_f32<T>(-INFINITY);
+        for (int k = 0; k < 6; ++k) v.w[k] = v.w[k + 2];
       }
+      if (bytes & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) v.w[k] = v.w[k + 1];
+      }
+      if (bytes & 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v.w[k] = __funnelshift_r(v.w[k], v.w[k + 1], 16);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v.raw[e] = t + e < vocab ? x[t + e] : from_f32<T>(-INFINITY);
     }
   }
-  __device__ __forceinline__ void get(float* f, bool dead) const {
-    float odd = 0.f;   // NaN as soon as one is not finite
+  __device__ __forceinline__ void load(const T* x, int lead, int vocab, int t0) {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      f[i] = to_f32<T>(v[i / N].raw[i % N]);
-      odd = fmaf(f[i], 0.f, odd);
+    for (int i = 0; i < V; ++i) load_vec(v[i], x, lead, vocab, t0 + i * 32 * N);
+  }
+  // the logits in fp32; returns their max
+  __device__ __forceinline__ float get(float* f, bool dead) const {
+    float top, odd;    // odd: NaN as soon as one is not finite
+    if constexpr (sizeof(T) == 2) {
+      using T2 = typename Pair<T>::type;
+      T2 t2 = pair(0), z = Pair<T>::zero(), o2 = z;
+#pragma unroll
+      for (int k = 0; k < kPerLane / 2; ++k) {
+        t2 = __hmax2(t2, pair(k));
+        o2 = __hfma2(pair(k), z, o2);
+      }
+      top = fmaxf(to_f32<T>(t2.x), to_f32<T>(t2.y));
+      odd = to_f32<T>(o2.x) + to_f32<T>(o2.y);
+    } else {
+      top = to_f32<T>(v[0].raw[0]);
+      odd = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const float e = to_f32<T>(v[i / N].raw[i % N]);
+        top = fmaxf(top, e);
+        odd = fmaf(e, 0.f, odd);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) f[i] = to_f32<T>(v[i / N].raw[i % N]);
     if (dead || odd != 0.f) {
+      top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i)
+      for (int i = 0; i < kPerLane; ++i) {
         if (dead || !isfinite(f[i])) f[i] = -INFINITY;
+        top = fmaxf(top, f[i]);
+      }
     }
+    return top;
+  }
+  __device__ __forceinline__ typename Pair<T>::type pair(int k) const {
+    return reinterpret_cast<const typename Pair<T>::type&>(v[2 * k / N].w[2 * k % N / 2]);
   }
 };
 
@@ -135,9 +176,11 @@ __device__ __forceinline__ float exp_diff(float x, float m) {
 template <typename T>
 __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const BeamArgs a) {
   launch_dependents();
-  __shared__ uint64_t s_pend[kChunkWarps][64];
+  // at most n_out lanes hold candidates, and each holds at most its logits
+  __shared__ uint64_t s_keys[kMaxBeamOut * kPerLane * kMaxBatches];
   __shared__ uint64_t s_list[kChunkWarps][32];
   __shared__ float2 s_ml[kChunkWarps];
+  __shared__ int s_holder[32 * kChunkWarps], s_holders, s_keys_n;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.y;
   const int first = (blockIdx.x * kChunkWarps + warp) * a.batches * kBatch;
@@ -158,10 +201,7 @@ __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const Beam
     for (int b = 0; b < batches; ++b) {
       if (b + 1 < batches) next.load(x, lead, a.vocab, token(b + 1, 0));
       float f[kPerLane];
-      now.get(f, dead);
-      float top = f[0];
-#pragma unroll
-      for (int i = 1; i < kPerLane; ++i) top = fmaxf(top, f[i]);
+      const float top = now.get(f, dead);
       if (top > m) at = b;
       const float mm = fmaxf(m, top), ref = mm == -INFINITY ? 0.f : mm;
       float2 part = make_float2(0.f, 0.f);
@@ -212,45 +252,36 @@ __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const Beam
   join(sort32(best, lane));
   const uint64_t bound = s_list[0][a.n_out - 1];
   const float bound_f = bound ? from_ordered(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
+  if (threadIdx.x == 0) s_holders = s_keys_n = 0;
   __syncthreads();
-  const bool holds = best != 0 && best >= bound;
-  uint64_t list = 0;
-  if (__any_sync(kAll, holds)) {
-    int pending = 0;
-    for (int b = 0; b < batches; ++b) {
-      float f[kPerLane], top = -INFINITY;
-      if (holds) {
-        B again;
-        again.load(x, lead, a.vocab, token(b, 0));
-        again.get(f, dead);
+  if (best != 0 && best >= bound) s_holder[atomicAdd(&s_holders, 1)] = threadIdx.x;
+  __syncthreads();
+  // the holders' vectors, spread over the CTA (their order, and the order in which hits are
+  // put down, do not matter: keys are all different and get sorted)
+  const int per = a.batches * B::V, holders = s_holders;
+  for (int j = threadIdx.x; j < holders * per; j += 32 * kChunkWarps) {
+    const int who = s_holder[j / per], q = j % per;
+    const int t0 = (blockIdx.x * kChunkWarps + (who >> 5)) * a.batches * kBatch + (who & 31) * N +
+                   (q / B::V) * kBatch + (q % B::V) * 32 * N;
+    if (t0 >= a.vocab) continue;
+    typename B::Vec v;
+    B::load_vec(v, x, lead, a.vocab, t0);
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) top = fmaxf(top, f[i]);
-      }
-      if (!__any_sync(kAll, holds && top >= bound_f)) continue;
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        const int t = token(b, i);
-        const uint64_t key = holds && t < a.vocab && f[i] >= bound_f ? make_key(f[i], t) : 0;
-        const bool in = key != 0 && key >= bound;
-        const unsigned hits = __ballot_sync(kAll, in);
-        if (hits == 0) continue;
-        if (in) s_pend[warp][pending + __popc(hits & ((1u << lane) - 1u))] = key;
-        pending += __popc(hits);
-        __syncwarp();
-        if (pending >= 32) {
-          list = merge32(list, sort32(s_pend[warp][lane], lane), lane);
-          pending -= 32;
-          const uint64_t rest = s_pend[warp][32 + lane];
-          __syncwarp();
-          s_pend[warp][lane] = rest;
-          __syncwarp();
-        }
+    for (int e = 0; e < N; ++e) {
+      float f = to_f32<T>(v.raw[e]);
+      if (dead || !isfinite(f)) f = -INFINITY;
+      if (t0 + e < a.vocab && f >= bound_f) {
+        const uint64_t key = make_key(f, t0 + e);
+        if (key >= bound) s_keys[atomicAdd(&s_keys_n, 1)] = key;
       }
     }
-    if (pending > 0)
-      list = merge32(list, sort32(lane < pending ? s_pend[warp][lane] : 0, lane), lane);
   }
-  list = join(list);
+  __syncthreads();
+  uint64_t list = 0;
+  const int n_keys = s_keys_n;
+  for (int k = warp * 32; k < n_keys; k += 32 * kChunkWarps)
+    list = merge32(list, sort32(k + lane < n_keys ? s_keys[k + lane] : 0, lane), lane);
+  if (n_keys > 32) list = join(list);
   if (warp == 0) {
     const size_t slot = static_cast<size_t>(row) * a.n_chunks + blockIdx.x;
     if (lane < a.n_out) a.cand[slot * a.n_out + lane] = list;
@@ -370,7 +401,7 @@ cudaError_t launch_early(K kernel, dim3 grid, int threads, cudaStream_t s, const
 cudaError_t launch_beam_select(BeamArgs a, cudaStream_t s) {
   // Longer runs spread a warp's sorting over more logits; shorter ones fill the GPU.
   const int rows = a.n * a.beams, most = beam_chunks(a.vocab);
-  a.batches = 8;
+  a.batches = kMaxBatches;
   while (a.batches > 1 && static_cast<int64_t>(rows) * most / a.batches < 4 * 148) a.batches /= 2;
   a.n_chunks = (most + a.batches - 1) / a.batches;
   const dim3 grid(static_cast<unsigned>(a.n_chunks), static_cast<unsigned>(rows));
