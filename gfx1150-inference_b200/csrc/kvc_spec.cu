@@ -57,186 +57,239 @@ __device__ __forceinline__ void rotate(T& x0, T& x1, float2 cs) {
 }
 
 // =====================================================================================
-// Rotate + append.  One CTA per token: its head_dim / 2 angles are computed once and
-// serve all its heads.  The angle p * inv_freq is taken in turns, p * (inv_freq / 2 pi)
-// in 64 bits with the whole turns removed, so a far position loses nothing; the rest
-// goes through sincospif in 32 bits.  A thread then rotates two 16-byte units whose
-// pairs they hold (units 2i, 2i + 1, or i and i + half the row for NeoX) of one head.
+// Rotate + append.  kPer threads take a token: its head_dim / 2 angles are computed once and
+// serve all its heads.  The angle p * inv_freq is taken in turns, p * (inv_freq / 2 pi) in
+// 64 bits with the whole turns removed, so a far position loses nothing; the rest goes
+// through sincospif in 32 bits.  A thread owns two 16-byte units that hold each other's
+// pairs (units 2i, 2i + 1, or i and i + half the row for NeoX), keeps their angles in
+// registers and goes through the heads of q, K and V, kAppendBatch of them on their way;
+// the first are asked for before the angles are computed.
 // =====================================================================================
 constexpr int kAppendThreads = 256;
+constexpr int kAppendBatch = 3;
 
-template <typename T, bool kNeox>
+template <typename T, bool kNeox, int kPer>
 __global__ void __launch_bounds__(kAppendThreads) append_rope_kernel(const AppendRopeArgs a) {
-  __shared__ float2 cs[kMaxRopePairs];
-  __shared__ int s_page;
-  const int tok = blockIdx.x;
-  const int pos = a.positions[tok];
-  if (pos < 0) return;  // padding
-  const int half = a.head_dim / 2;
-  for (int i = threadIdx.x; i < half; i += kAppendThreads) {
-    double turn = static_cast<double>(a.rope_positions[tok]) * a.turns[i];
-    turn -= rint(turn);
-    sincospif(2.0f * static_cast<float>(turn), &cs[i].y, &cs[i].x);
-  }
-  if (threadIdx.x == 0) s_page = page_of(a.p, a.rows ? a.rows[tok] : 0, pos);
-  __syncthreads();
-  const int page = s_page;
-  if (page < 0) return;
-  const int t = pos % a.p.page_size;
+  constexpr int kTok = kAppendThreads / kPer;
+  __shared__ float2 cs[kTok * kMaxRopePairs];
+  __shared__ int s_page[kTok], s_slot[kTok];
+  launch_dependents();
+  const int tok0 = blockIdx.x * kTok, half = a.head_dim / 2;
+  const int toks = min(kTok, a.n - tok0);
   const int U = a.p.row_units, Hkv = a.p.num_kv_heads;
   constexpr int N = Unit<T>::N;
+  const int pairs = U / 2;                     // unit pairs of a head
+  const int heads = a.num_heads + 2 * Hkv;     // q, K and V heads
+  const bool whole = U % 2 == 0;               // units pair up
+  const int tok = threadIdx.x / kPer, me = threadIdx.x % kPer;
+  const int at_once = whole ? kPer / pairs : 1;
+  const int row0 = whole ? me / pairs : 0, i = whole ? me - row0 * pairs : 0;
+  const int u0 = kNeox ? i : 2 * i, du = kNeox ? pairs : 1;
+  const bool works = whole && tok < toks && row0 < at_once;
+  const size_t t = tok0 + tok;
+  const size_t row_bytes = static_cast<size_t>(U) * 16;
+  wait_prerequisites();
 
-  if (U % 2 == 0) {
-    const int pairs = U / 2;  // unit pairs of a head
-    const int total = (a.num_heads + 2 * Hkv) * pairs;
-    for (int x = threadIdx.x; x < total; x += kAppendThreads) {
-      const int head = x / pairs, i = x - head * pairs;
-      const int u0 = kNeox ? i : 2 * i, u1 = kNeox ? i + pairs : 2 * i + 1;
-      const uint8_t* src;
-      if (head < a.num_heads)
-        src = a.q + tok * a.q_stride + static_cast<size_t>(head) * U * 16;
-      else if (head < a.num_heads + Hkv)
-        src = a.k_new + tok * a.k_stride + static_cast<size_t>(head - a.num_heads) * U * 16;
-      else
-        src = a.v_new + tok * a.v_stride + static_cast<size_t>(head - a.num_heads - Hkv) * U * 16;
-      Unit<T> x0, x1;
-      x0.raw = *reinterpret_cast<const uint4*>(src + u0 * 16);
-      x1.raw = *reinterpret_cast<const uint4*>(src + u1 * 16);
-      if (head < a.num_heads + Hkv) {
-        if (kNeox) {
+  struct Item {
+    Unit<T> x0, x1;
+  };
+  const uint8_t* q_src = a.q + t * a.q_stride + u0 * 16;
+  const uint8_t* k_src = a.k_new + t * a.k_stride + u0 * 16;
+  const uint8_t* v_src = a.v_new + t * a.v_stride + u0 * 16;
+  auto load = [&](int head, Item& it) {
+    const uint8_t* src = head < a.num_heads         ? q_src + head * row_bytes
+                         : head < a.num_heads + Hkv ? k_src + (head - a.num_heads) * row_bytes
+                                                    : v_src + (head - a.num_heads - Hkv) * row_bytes;
+    it.x0.raw = *reinterpret_cast<const uint4*>(src);
+    it.x1.raw = *reinterpret_cast<const uint4*>(src + du * 16);
+  };
+  Item items[kAppendBatch];
 #pragma unroll
-          for (int e = 0; e < N; ++e) rotate(x0.v[e], x1.v[e], cs[u0 * N + e]);
-        } else {
+  for (int k = 0; k < kAppendBatch; ++k)
+    if (works && row0 + k * at_once < heads) load(row0 + k * at_once, items[k]);
+
+  for (int x = threadIdx.x; x < toks * half; x += kAppendThreads) {
+    const int tk = kTok == 1 ? 0 : x / half, j = x - tk * half;
+    double turn = static_cast<double>(a.rope_positions[tok0 + tk]) * a.turns[j];
+    turn -= rint(turn);
+    // (by pair of a unit pair, then unit pair: neighbouring threads read neighbouring angles)
+    float2& out = cs[tk * half + (whole ? j % N * pairs + j / N : j)];
+    sincospif(2.0f * static_cast<float>(turn), &out.y, &out.x);
+  }
+  if (threadIdx.x < toks) {
+    const int pos = a.positions[tok0 + threadIdx.x];
+    s_page[threadIdx.x] = pos < 0 ? -1 : page_of(a.p, a.rows ? a.rows[tok0 + threadIdx.x] : 0, pos);
+    s_slot[threadIdx.x] = pos < 0 ? 0 : pos % a.p.page_size;
+  }
+  __syncthreads();
+  if (works) {
+    const int page = s_page[tok];
+    if (page < 0) return;                      // padding, or reported
+    float2 c[N];
 #pragma unroll
-          for (int e = 0; e < N; e += 2) {
-            rotate(x0.v[e], x0.v[e + 1], cs[(u0 * N + e) / 2]);
-            rotate(x1.v[e], x1.v[e + 1], cs[(u1 * N + e) / 2]);
+    for (int k = 0; k < N; ++k) c[k] = cs[tok * half + k * pairs + i];
+    uint8_t* q_dst = a.q_out + t * a.num_heads * row_bytes + u0 * 16;
+    const size_t place = unit_at(a.p, page, 0, s_slot[tok], u0);
+    const int dp = du * (a.p.layout == kLayoutCore ? 128 : 16);
+    for (int h0 = row0; h0 < heads; h0 += kAppendBatch * at_once) {
+#pragma unroll
+      for (int k = 0; k < kAppendBatch; ++k) {
+        const int head = h0 + k * at_once;
+        if (head >= heads) break;
+        Item& it = items[k];
+        if (head < a.num_heads + Hkv) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            if (kNeox)
+              rotate(it.x0.v[e], it.x1.v[e], c[e]);
+            else if (e < N / 2)
+              rotate(it.x0.v[2 * e], it.x0.v[2 * e + 1], c[e]);
+            else
+              rotate(it.x1.v[2 * e - N], it.x1.v[2 * e - N + 1], c[e]);
           }
         }
+        if (head < a.num_heads) {
+          uint8_t* d = q_dst + head * row_bytes;
+          *reinterpret_cast<uint4*>(d) = it.x0.raw;
+          *reinterpret_cast<uint4*>(d + du * 16) = it.x1.raw;
+        } else {
+          const bool is_k = head < a.num_heads + Hkv;
+          uint8_t* d = (is_k ? a.p.k : a.p.v) + place +
+                       (head - a.num_heads - (is_k ? 0 : Hkv)) * a.p.page_head_bytes;
+          *reinterpret_cast<uint4*>(d) = it.x0.raw;
+          *reinterpret_cast<uint4*>(d + dp) = it.x1.raw;
+        }
       }
-      if (head < a.num_heads) {
-        uint8_t* dst = a.q_out + (static_cast<size_t>(tok) * a.num_heads + head) * U * 16;
-        *reinterpret_cast<uint4*>(dst + u0 * 16) = x0.raw;
-        *reinterpret_cast<uint4*>(dst + u1 * 16) = x1.raw;
-      } else {
-        const bool is_k = head < a.num_heads + Hkv;
-        const int h = head - a.num_heads - (is_k ? 0 : Hkv);
-        uint8_t* dst = is_k ? a.p.k : a.p.v;
-        *reinterpret_cast<uint4*>(dst + unit_at(a.p, page, h, t, u0)) = x0.raw;
-        *reinterpret_cast<uint4*>(dst + unit_at(a.p, page, h, t, u1)) = x1.raw;
-      }
+      const int next = h0 + kAppendBatch * at_once;
+#pragma unroll
+      for (int k = 0; k < kAppendBatch; ++k)
+        if (next + k * at_once < heads) load(next + k * at_once, items[k]);
     }
     return;
   }
+  if (whole) return;
   // An odd number of units per row (head_dim 8, 24, 40 ... of 16-bit types): element pairs.
-  const int total = (a.num_heads + 2 * Hkv) * half;
-  for (int x = threadIdx.x; x < total; x += kAppendThreads) {
-    const int head = x / half, i = x - head * half;
-    const int i0 = kNeox ? i : 2 * i, i1 = kNeox ? i + half : 2 * i + 1;
+  for (int x = threadIdx.x; x < toks * heads * half; x += kAppendThreads) {
+    const int tk = x / (heads * half), r = x - tk * heads * half;
+    const int head = r / half, j = r - head * half;
+    const int page = s_page[tk];
+    if (page < 0) continue;
+    const size_t row = tok0 + tk;
+    const int i0 = kNeox ? j : 2 * j, i1 = kNeox ? j + half : 2 * j + 1;
     const bool is_q = head < a.num_heads, is_k = !is_q && head < a.num_heads + Hkv;
     const int h = head - (is_q ? 0 : is_k ? a.num_heads : a.num_heads + Hkv);
-    const T* src = reinterpret_cast<const T*>(is_q   ? a.q + tok * a.q_stride
-                                              : is_k ? a.k_new + tok * a.k_stride
-                                                     : a.v_new + tok * a.v_stride) +
+    const T* src = reinterpret_cast<const T*>(is_q   ? a.q + row * a.q_stride
+                                              : is_k ? a.k_new + row * a.k_stride
+                                                     : a.v_new + row * a.v_stride) +
                    static_cast<size_t>(h) * a.head_dim;
     T x0 = src[i0], x1 = src[i1];
-    if (is_q || is_k) rotate(x0, x1, cs[i]);
+    if (is_q || is_k) rotate(x0, x1, cs[tk * half + j]);
     if (is_q) {
-      T* dst = reinterpret_cast<T*>(a.q_out) +
-               (static_cast<size_t>(tok) * a.num_heads + h) * a.head_dim;
+      T* dst = reinterpret_cast<T*>(a.q_out) + (row * a.num_heads + h) * a.head_dim;
       dst[i0] = x0;
       dst[i1] = x1;
     } else {
       uint8_t* dst = is_k ? a.p.k : a.p.v;
-      reinterpret_cast<T*>(dst + unit_at(a.p, page, h, t, i0 / N))[i0 % N] = x0;
-      reinterpret_cast<T*>(dst + unit_at(a.p, page, h, t, i1 / N))[i1 % N] = x1;
+      reinterpret_cast<T*>(dst + unit_at(a.p, page, h, s_slot[tk], i0 / N))[i0 % N] = x0;
+      reinterpret_cast<T*>(dst + unit_at(a.p, page, h, s_slot[tk], i1 / N))[i1 % N] = x1;
     }
   }
 }
 
 // =====================================================================================
-// Commit of an accepted path.  A thread owns one 16-byte unit column of one (layer, K
-// or V, head) and moves it for the whole path: it reads up to kCommitBatch sources,
-// then writes them, so no thread reads what another writes.  Ascending paths keep the
-// batches apart: a later source lies behind every slot written before it.
+// Commit of an accepted path.  A CTA moves one layer's K and V of one sequence.  Eight threads
+// take eight steps of the path in one 16-byte column (a unit of one head), whose new places
+// lie side by side in the pool's 8-position blocks; longer paths go eight steps at a time.
+// All of a batch is read before any of it is written, and ascending paths keep the batches
+// apart: a later source lies behind every slot written before it.
+// The rows come in 16-byte pieces 128 bytes apart, and memory is read 64 bytes at a time:
+// the sources alone cost four times their bytes, which is what bounds this.
 // =====================================================================================
 constexpr int kCommitThreads = 256;
-constexpr int kCommitBatch = 8;
+constexpr int kCommitSteps = 8;     // of a path at a time
+constexpr int kCommitCols = 8;      // columns of a thread in flight
 
 __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs a) {
-  __shared__ int s_src[kMaxTreeNodes], s_dst[kMaxTreeNodes];   // pages
+  __shared__ int s_page[2][kMaxTreeNodes], s_t[2][kMaxTreeNodes];   // [source, target]
   __shared__ int s_bad;
+  launch_dependents();
+  if (threadIdx.x == 0) s_bad = 0;
+  wait_prerequisites();
   const int seq = blockIdx.y;
-  const int len = a.path_lens[seq];
-  if (len <= 0) return;
-  if (threadIdx.x == 0) s_bad = len > a.path_stride;
-  __syncthreads();
-  const int ctx = a.ctx[seq];
+  const int len = a.path_lens[seq], ctx = a.ctx[seq];
   const int row = a.rows ? a.rows[seq] : seq;
   const int32_t* path = a.paths + static_cast<size_t>(seq) * a.path_stride;
+  if (len <= 0) return;
+  __syncthreads();
   for (int j = threadIdx.x; j < min(len, a.path_stride); j += kCommitThreads) {
     const int node = path[j];
-    bool ok = node >= j && node < kMaxTreeNodes && (j == 0 || path[j - 1] < node) && ctx >= 0;
-    if (!ok) report_error_at(a.p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(node));
-    int sp = -1, dp = -1;
-    if (ok) {
-      sp = page_of(a.p, row, ctx + node);
-      dp = page_of(a.p, row, ctx + j);
-      ok = sp >= 0 && dp >= 0;
-    }
-    if (!ok) {
+    const bool ok = node >= j && node < kMaxTreeNodes && (j == 0 || path[j - 1] < node) && ctx >= 0 &&
+                    len <= a.path_stride;
+    const int sp = ok ? page_of(a.p, row, ctx + node) : -1, dp = ok ? page_of(a.p, row, ctx + j) : -1;
+    if (sp < 0 || dp < 0) {
+      report_error_at(a.p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(node));
       s_bad = 1;
-    } else {
-      s_src[j] = sp;
-      s_dst[j] = dp;
     }
+    s_page[0][j] = sp;
+    s_page[1][j] = node == j ? -1 : dp;   // a row that stays is not touched
+    s_t[0][j] = (ctx + node) % a.p.page_size;
+    s_t[1][j] = (ctx + j) % a.p.page_size;
+  }
+  if (len > a.path_stride && threadIdx.x == 0) {
+    report_error_at(a.p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(len));
+    s_bad = 1;
   }
   __syncthreads();
-  if (s_bad) {
-    if (threadIdx.x == 0) report_error_at(a.p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(len));
-    return;
-  }
-  const int U = a.p.row_units, Hkv = a.p.num_kv_heads, ps = a.p.page_size;
-  const int total = a.n_layers * 2 * Hkv * U;
-  const int x = blockIdx.x * kCommitThreads + threadIdx.x;
-  if (x >= total) return;
-  const int u = x % U;
-  int r = x / U;
-  const int h = r % Hkv;
-  r /= Hkv;
-  uint8_t* base = ((r & 1) ? a.p.v : a.p.k) + static_cast<size_t>(r >> 1) * a.layer_bytes;
-  for (int j0 = 0; j0 < len; j0 += kCommitBatch) {
-    uint4 v[kCommitBatch];
+  if (s_bad) return;
+  const int U = a.p.row_units, half = a.p.num_kv_heads * U, cols = 2 * half;
+  const size_t layer = blockIdx.x * a.layer_bytes;
+  auto cell = [&](int c, int page, int t) {
+    const int d = c < half ? c : c - half;
+    return reinterpret_cast<uint4*>((c < half ? a.p.k : a.p.v) + layer + unit_at(a.p, page, d / U, t, d % U));
+  };
+  const int step = threadIdx.x % kCommitSteps, col0 = threadIdx.x / kCommitSteps;
+  constexpr int kColsAtOnce = kCommitThreads / kCommitSteps;
+  for (int j0 = 0; j0 < len; j0 += kCommitSteps) {
+    const int j = j0 + step;
+    const bool moves = j < len && s_page[1][j] >= 0;
+    const int rounds = (cols + kColsAtOnce - 1) / kColsAtOnce;
+    for (int c0 = 0; c0 < rounds; c0 += kCommitCols) {
+      uint4 v[kCommitCols];
 #pragma unroll
-    for (int b = 0; b < kCommitBatch; ++b) {
-      const int j = j0 + b;
-      if (j < len && path[j] != j)
-        v[b] = *reinterpret_cast<const uint4*>(base + unit_at(a.p, s_src[j], h, (ctx + path[j]) % ps, u));
-    }
+      for (int k = 0; k < kCommitCols; ++k) {
+        const int c = col0 + (c0 + k) * kColsAtOnce;
+        if (moves && c < cols)
+          v[k] = *cell(c, s_page[0][j], s_t[0][j]);
+      }
+      __syncwarp();   // a column's steps are threads of one warp: all read, then all write
 #pragma unroll
-    for (int b = 0; b < kCommitBatch; ++b) {
-      const int j = j0 + b;
-      if (j < len && path[j] != j)
-        *reinterpret_cast<uint4*>(base + unit_at(a.p, s_dst[j], h, (ctx + j) % ps, u)) = v[b];
+      for (int k = 0; k < kCommitCols; ++k) {
+        const int c = col0 + (c0 + k) * kColsAtOnce;
+        if (moves && c < cols) *cell(c, s_page[1][j], s_t[1][j]) = v[k];
+      }
     }
   }
 }
 
 // =====================================================================================
-// Beam reorder.  blockIdx.x 0 permutes the sequence's page-table columns, the other
-// CTAs the rows of its open pages.  A thread owns one column (one 16-byte unit of one
-// position, head, layer and K or V) for all beams: it reads every moved beam's new
-// value, then writes, so the permutation happens in place without a second buffer.
+// Beam reorder.  blockIdx.x 0 permutes the sequence's page-table columns, every other CTA one
+// head of one layer's K or V in the open pages.  A thread owns one 16-byte unit of a page
+// for all beams: it reads every moved beam's new value, then writes, so the permutation
+// happens in place without a second buffer.  The units in front of `tail` positions are
+// taken in the order of memory; of the last 8-position block only some rows are.
 // =====================================================================================
 constexpr int kReorderThreads = 128;
 
+template <int kBeams>
 __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderArgs a) {
   __shared__ int s_parent[kMaxBeams], s_page[kMaxBeams], s_bad;
+  launch_dependents();
+  if (threadIdx.x == 0) s_bad = 0;
+  wait_prerequisites();
   const int seq = blockIdx.y, B = a.beams, ps = a.p.page_size;
   const int ctx = a.ctx[seq];
   const int full = ctx / ps, tail = ctx - full * ps;
   int32_t* table = a.tables + static_cast<size_t>(seq) * B * a.p.bt_stride;
-  if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
   if (threadIdx.x < B) {
     const int b = threadIdx.x;
@@ -269,57 +322,59 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderA
   if (s_bad) return;
   if (blockIdx.x == 0) {
     for (int c = threadIdx.x; c < full; c += kReorderThreads) {
-      int32_t v[kMaxBeams];
+      int32_t v[kBeams];
 #pragma unroll
-      for (int b = 0; b < kMaxBeams; ++b)
+      for (int b = 0; b < kBeams; ++b)
         if (b < B && s_parent[b] != b) v[b] = table[static_cast<size_t>(s_parent[b]) * a.p.bt_stride + c];
 #pragma unroll
-      for (int b = 0; b < kMaxBeams; ++b)
+      for (int b = 0; b < kBeams; ++b)
         if (b < B && s_parent[b] != b) table[static_cast<size_t>(b) * a.p.bt_stride + c] = v[b];
     }
     return;
   }
-  const int U = a.p.row_units, Hkv = a.p.num_kv_heads;
-  const int per = tail * U;                     // units of one head's open rows
-  const size_t total = static_cast<size_t>(a.n_layers) * 2 * Hkv * per;
-  const size_t step = static_cast<size_t>(gridDim.x - 1) * kReorderThreads;
-  for (size_t x = static_cast<size_t>(blockIdx.x - 1) * kReorderThreads + threadIdx.x; x < total;
-       x += step) {
-    size_t r = x / per;
-    const int tu = static_cast<int>(x - r * per);
-    const int h = static_cast<int>(r % Hkv);
-    r /= Hkv;
-    uint8_t* base = ((r & 1) ? a.p.v : a.p.k) + (r >> 1) * a.layer_bytes;
-    // neighbouring threads take neighbouring 16-byte units of the page's layout
-    int t, u;
-    if (a.p.layout == kLayoutCore) {
-      const int blk = tu / (8 * U), in = tu - blk * 8 * U;
-      const int rows = min(8, tail - blk * 8);  // rows of the last block may be fewer
-      u = in / rows;
-      t = blk * 8 + in - u * rows;
-    } else {
-      t = tu / U;
-      u = tu - t * U;
-    }
-    uint4 v[kMaxBeams];
+  const int r = blockIdx.x - 1, h = r % a.p.num_kv_heads, lk = r / a.p.num_kv_heads;
+  uint8_t* base = ((lk & 1) ? a.p.v : a.p.k) + static_cast<size_t>(lk >> 1) * a.layer_bytes +
+                  static_cast<size_t>(h) * a.p.page_head_bytes;
+  const size_t page_bytes = a.p.page_head_bytes * a.p.num_kv_heads;
+  const int U = a.p.row_units;
+  const bool core = a.p.layout == kLayoutCore;
+  const int whole = core ? tail / 8 * 8 * U : tail * U;        // units of whole blocks
+  const int units = core ? (tail + 7) / 8 * 8 * U : whole, rows = tail & 7;
+  for (int x = threadIdx.x; x < units; x += kReorderThreads) {
+    if (x >= whole && (x & 7) >= rows) continue;
+    uint4 v[kBeams];
 #pragma unroll
-    for (int b = 0; b < kMaxBeams; ++b)
+    for (int b = 0; b < kBeams; ++b)
       if (b < B && s_parent[b] != b)
-        v[b] = *reinterpret_cast<const uint4*>(base + unit_at(a.p, s_page[s_parent[b]], h, t, u));
+        v[b] = *reinterpret_cast<const uint4*>(base + s_page[s_parent[b]] * page_bytes + x * 16);
 #pragma unroll
-    for (int b = 0; b < kMaxBeams; ++b)
-      if (b < B && s_parent[b] != b)
-        *reinterpret_cast<uint4*>(base + unit_at(a.p, s_page[b], h, t, u)) = v[b];
+    for (int b = 0; b < kBeams; ++b)
+      if (b < B && s_parent[b] != b) *reinterpret_cast<uint4*>(base + s_page[b] * page_bytes + x * 16) = v[b];
   }
 }
 
-template <typename T>
+// A launch that may begin before the one ahead of it has ended: every kernel here touches
+// what others do only behind wait_prerequisites().
+template <typename A>
+cudaError_t launch_early(void (*kernel)(A), dim3 grid, int threads, cudaStream_t s, const A& args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+// Many tokens: 64 threads each, four in a CTA; few tokens: a CTA each.
+template <typename T, bool kNeox>
 cudaError_t run_append_rope(const AppendRopeArgs& a, cudaStream_t s) {
-  if (a.neox)
-    append_rope_kernel<T, true><<<a.n, kAppendThreads, 0, s>>>(a);
-  else
-    append_rope_kernel<T, false><<<a.n, kAppendThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  if (a.n >= 4 * 148)
+    return launch_early(append_rope_kernel<T, kNeox, 64>, dim3((a.n + 3) / 4), kAppendThreads, s, a);
+  return launch_early(append_rope_kernel<T, kNeox, kAppendThreads>, dim3(a.n), kAppendThreads, s, a);
 }
 
 }  // namespace
@@ -327,29 +382,24 @@ cudaError_t run_append_rope(const AppendRopeArgs& a, cudaStream_t s) {
 cudaError_t launch_append_rope(const AppendRopeArgs& a, cudaStream_t s) {
   if (a.n <= 0) return cudaSuccess;
   switch (a.dtype) {
-    case KVC_DTYPE_F16: return run_append_rope<__half>(a, s);
-    case KVC_DTYPE_BF16: return run_append_rope<__nv_bfloat16>(a, s);
-    case KVC_DTYPE_F32: return run_append_rope<float>(a, s);
+    case KVC_DTYPE_F16: return a.neox ? run_append_rope<__half, true>(a, s) : run_append_rope<__half, false>(a, s);
+    case KVC_DTYPE_BF16: 
+      return a.neox ? run_append_rope<__nv_bfloat16, true>(a, s) : run_append_rope<__nv_bfloat16, false>(a, s);
+    case KVC_DTYPE_F32: return a.neox ? run_append_rope<float, true>(a, s) : run_append_rope<float, false>(a, s);
     default: return cudaErrorInvalidValue;
   }
 }
 
 cudaError_t launch_commit(const CommitArgs& a, cudaStream_t s) {
-  const int64_t total = static_cast<int64_t>(a.n_layers) * 2 * a.p.num_kv_heads * a.p.row_units;
-  if (total > (1ll << 30) || a.n > 65535) return cudaErrorInvalidValue;
-  const unsigned gx = static_cast<unsigned>((total + kCommitThreads - 1) / kCommitThreads);
-  commit_kernel<<<dim3(gx, static_cast<unsigned>(a.n)), kCommitThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  return launch_early(commit_kernel, dim3(static_cast<unsigned>(a.n_layers), static_cast<unsigned>(a.n)),
+                      kCommitThreads, s, a);
 }
 
 cudaError_t launch_reorder(const ReorderArgs& a, cudaStream_t s) {
-  if (a.n > 65535) return cudaErrorInvalidValue;
-  const size_t most = static_cast<size_t>(a.n_layers) * 2 * a.p.num_kv_heads * a.p.page_size *
-                      a.p.row_units;
-  const size_t gx = std::min<size_t>((most + kReorderThreads - 1) / kReorderThreads, 4096);
-  reorder_kernel<<<dim3(static_cast<unsigned>(gx) + 1, static_cast<unsigned>(a.n)),
-                   kReorderThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  const dim3 grid(static_cast<unsigned>(2 * a.n_layers * a.p.num_kv_heads + 1), static_cast<unsigned>(a.n));
+  if (a.beams <= 4) return launch_early(reorder_kernel<4>, grid, kReorderThreads, s, a);
+  if (a.beams <= 8) return launch_early(reorder_kernel<8>, grid, kReorderThreads, s, a);
+  return launch_early(reorder_kernel<16>, grid, kReorderThreads, s, a);
 }
 
 }  // namespace kvc

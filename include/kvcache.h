@@ -553,7 +553,7 @@ typedef struct kvc_beam kvc_beam_t;
  * Pairs as in kvc_rope.  q_stride / k_stride / v_stride: elements between the
  * tokens of d_q, d_k_new, d_v_new (0: packed), so they may be slices of one fused
  * projection; d_q_out is packed and may be d_q when that is packed.  A negative
- * d_positions[i] marks padding: nothing of token i is read or written.  Two
+ * d_positions[i] marks padding: nothing is written for token i.  Two
  * tokens of one call must not name the same slot.  A row outside [0, bt_rows) or
  * a slot past the table is reported (KVC_DEVERR_BAD_POSITION) and that token
  * skipped, a bad page likewise (KVC_DEVERR_BAD_PAGE).  Pointers and strides are
