@@ -46,7 +46,7 @@ class BeamSelector:
         vocab = logits.shape[1]
         if logits.shape[0] != n * beams:
             raise ValueError("logits needs one row per beam")
-        if logits.device.type != "cuda" or logits.device.index != dev:
+        if logits.get_device() != dev:
             raise ValueError(f"logits must be on cuda:{dev}")
         st = logits.stride()
         if (vocab > 1 and st[1] != 1) or (n * beams > 1 and st[0] < vocab):

@@ -156,7 +156,10 @@ class DeviceScope {
  public:
   explicit DeviceScope(int device) {
     if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
-    rc_ = prev_ == device ? 0 : use_device(device);
+    if (prev_ == device)
+      prev_ = -1;   // nothing to put back
+    else
+      rc_ = use_device(device);
   }
   ~DeviceScope() {
     if (prev_ >= 0) cudaSetDevice(prev_);

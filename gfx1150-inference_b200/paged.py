@@ -49,34 +49,36 @@ def _dev(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> int:
     return int(t.data_ptr())
 
 
+# The operators below run in a few microseconds: their checks look at a tensor as seldom
+# as they can, and put a message together only when one fails.
 def _on(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: int) -> int:
-    """_dev, and on CUDA device `device`."""
-    if t.dtype != dtype or t.device.type != "cuda" or not t.is_contiguous():
+    """Address of a contiguous tensor of `dtype` on CUDA device `device`, `numel` or larger."""
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        if t.is_cuda and t.get_device() != device:
+            raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
         raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor")
-    if t.device.index != device:
-        raise ValueError(f"{name} is on {t.device}, not on the pool's cuda:{device}")
-    if t.numel() < numel:
+    if numel and t.numel() < numel:
         raise ValueError(f"{name} buffer is smaller than expected dimensions.")
     return t.data_ptr()
 
 
-def _token_rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, heads: int, dim: int,
-                device: int):
+def _token_rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device: int):
     """(address, elements between tokens) of (n, heads, dim) rows whose heads are packed."""
-    if t.dtype != dtype or t.device.type != "cuda" or t.device.index != device:
+    if t.dtype is not dtype or t.get_device() != device:
         raise ValueError(f"{name} must be a {dtype} tensor on cuda:{device}")
-    if tuple(t.shape) != (n, heads, dim):
-        raise ValueError(f"{name} must be ({n}, {heads}, {dim}), got {tuple(t.shape)}")
-    st = t.stride()
-    if (dim > 1 and st[2] != 1) or (heads > 1 and st[1] != dim) or \
-            (n > 1 and st[0] < heads * dim):
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    n, heads, dim = shape
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and dim > 1) or (s1 != dim and heads > 1) or (s0 < heads * dim and n > 1):
         raise ValueError(f"the heads of a token of {name} must be packed")
-    return t.data_ptr(), (st[0] if n > 1 else heads * dim)
+    return t.data_ptr(), (s0 if n > 1 else heads * dim)
 
 
 def _stream_on(stream, device: int) -> Optional[int]:
-    s = stream if stream is not None else torch.cuda.current_stream(device)
-    return int(s.cuda_stream) or None
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device) or None
+    return int(stream.cuda_stream) or None
 
 
 @dataclass
@@ -333,15 +335,16 @@ class PagedKVCache:
         that token is skipped), rope_positions the angles' positions where they differ."""
         dev, dt, d = self.device, self.dtype, self.head_dim
         n = positions.numel()
-        kp, ks = _token_rows(k_new, "k_new", dt, n, self.num_kv_heads, d, dev)
-        vp, vs = _token_rows(v_new, "v_new", dt, n, self.num_kv_heads, d, dev)
+        rows_shape = (n, self.num_kv_heads, d)
+        kp, ks = _token_rows(k_new, "k_new", dt, rows_shape, dev)
+        vp, vs = _token_rows(v_new, "v_new", dt, rows_shape, dev)
         qp = op = None
         heads = qs = 0
         if q is not None:
             if q.dim() != 3:
                 raise ValueError("q must be (n, heads, head_dim)")
             heads = q.shape[1]
-            qp, qs = _token_rows(q, "q", dt, n, heads, d, dev)
+            qp, qs = _token_rows(q, "q", dt, (n, heads, d), dev)
             if q_out is None:
                 q_out = torch.empty((n, heads, d), dtype=dt, device=q.device)
             op = _on(q_out, "q_out", dt, n * heads * d, dev)
