@@ -22,6 +22,10 @@ function's signature (the reference's own ``sample_next_token``), fed each
 sequence's logits on the host and a ``numpy`` generator seeded ``seed + i`` for
 prompt i, exactly like the sequential loop.  A sequence that has stopped (EOS)
 keeps riding along in the batch; its extra tokens are discarded.
+
+Two loops have no counterpart in the reference: ``generate_speculative_ids`` verifies
+a tree of drafted tokens per step and yields greedy decoding's tokens in fewer
+steps, and ``generate_beam_ids`` is beam search.
 """
 
 from __future__ import annotations
@@ -282,6 +286,201 @@ class BatchGenerator:
         total = float(sum(len(o) for o in outs))
         return outs, {"batch_size": float(b), "total_tokens_generated": total,
                       "total_time_s": t, "tokens_per_sec": total / max(t, 1e-9)}
+
+    def _check_prompts(self, batch_prompt_ids, rows: int, max_new_tokens: int) -> List[List[int]]:
+        prompts = [[int(t) for t in p] for p in batch_prompt_ids]
+        if len(prompts) * rows > self.max_batch:
+            raise ValueError(f"{len(prompts)} prompts of {rows} rows exceed the generator's "
+                             f"max_batch {self.max_batch}")
+        if max_new_tokens < 0:
+            raise ValueError(f"max_new_tokens must be >= 0 (got {max_new_tokens})")
+        for p in prompts:
+            if not p:
+                raise ValueError("prompt_ids must not be empty")
+            if len(p) + max_new_tokens > self.max_seq_len:
+                raise ValueError(f"len(prompt_ids) ({len(p)}) + max_new_tokens ({max_new_tokens}) "
+                                 f"exceeds max_seq_len ({self.max_seq_len})")
+            if min(p) < 0 or max(p) >= self.model.cfg.vocab:
+                raise ValueError("a token id is outside the vocabulary")
+        return prompts
+
+    def _decoder(self, bt: torch.Tensor) -> paged.BatchDecoder:
+        cfg = self.model.cfg
+        return paged.BatchDecoder(self.pool, self.model.layers, bt, cfg.heads,
+                                  [0] * int(bt.shape[0]), eps=cfg.eps, freq_base=cfg.rope_base,
+                                  neox=cfg.rope_neox)
+
+    def generate_speculative_ids(
+        self,
+        batch_prompt_ids: Sequence[Sequence[int]],
+        drafter: Callable[[int, List[int]], Tuple[Sequence[int], Sequence[int]]],
+        max_new_tokens: int = 16,
+        stop_on_eos: bool = True,
+    ) -> Tuple[List[List[int]], Dict[str, float]]:
+        """Greedy generation that verifies drafted tokens, several per step.
+        ``drafter(i, ids)`` is given prompt i's ids so far and returns (tokens, parents) of
+        a drafted tree: parents[j] is the node above token j, smaller than j, or -1 for
+        a token right behind the ids; empty for no draft.  Every step runs the last
+        token and its draft through the layers at once (``BatchDecoder.verify``), follows
+        the drafted tokens that are the argmax of the node above them, keeps that path
+        (``commit``) and adds the argmax behind it: the ids are those of greedy decoding
+        whatever is drafted.  Metrics count the steps and the drafted and accepted tokens."""
+        cfg = self.model.cfg
+        prompts = self._check_prompts(batch_prompt_ids, 1, max_new_tokens)
+        b = len(prompts)
+        t0 = time.perf_counter()
+        outs: List[List[int]] = [[] for _ in range(b)]
+        stats = {"batch_size": float(b), "steps": 0.0, "drafted": 0.0, "accepted": 0.0}
+        if b and max_new_tokens:
+            stream = torch.cuda.current_stream(self.model.device)
+            dec = self._decoder(self.bt[:b].contiguous())
+            emb = self.model.embedding
+            try:
+                last = []
+                for i, p in enumerate(prompts):
+                    ids = torch.tensor(p, dtype=torch.long, device=emb.device)
+                    last.append(dec.prefill(i, emb[ids].contiguous(), stream=stream)[-1:])
+                first = torch.argmax(self._logits(torch.cat(last), stream).float(), dim=1).tolist()
+                for i in range(b):
+                    outs[i].append(int(first[i]))
+
+                def done(i: int) -> bool:
+                    return len(outs[i]) >= max_new_tokens or (
+                        stop_on_eos and outs[i][-1] == cfg.eos_token_id)
+
+                while not all(done(i) for i in range(b)):
+                    tokens, trees = [], []
+                    for i in range(b):
+                        if done(i):
+                            trees.append([])
+                            continue
+                        # node 0 is the last token, whose row is not cached yet
+                        toks, par = drafter(i, prompts[i] + outs[i])
+                        # a path of k tokens yields k + 1, and the cache holds all but the last
+                        room = min(max_new_tokens - len(outs[i]) - 1,
+                                   self.max_seq_len - int(dec.ctx[i]) - 1,
+                                   ffi.MAX_TREE_NODES - 1)
+                        toks, par = [int(t) for t in toks][:room], [int(q) for q in par][:room]
+                        if len(toks) != len(par) or any(not 0 <= t < cfg.vocab for t in toks):
+                            raise ValueError("the draft needs one parent per token of the vocabulary")
+                        tokens += [outs[i][-1]] + toks
+                        trees.append([-1] + [q + 1 for q in par])
+                        stats["drafted"] += len(toks)
+                    ids = torch.tensor(tokens, dtype=torch.long, device=emb.device)
+                    h = dec.verify(emb[ids].contiguous(), trees, stream=stream)
+                    best = torch.argmax(self._logits(h, stream).float(), dim=1).tolist()
+                    paths, o = [], 0
+                    for i, tree in enumerate(trees):
+                        path, at = [], 0
+                        if tree:
+                            path, new = [0], []
+                            while True:
+                                new.append(int(best[o + at]))
+                                nxt = [j for j in range(at + 1, len(tree))
+                                       if tree[j] == at and tokens[o + j] == new[-1]]
+                                if not nxt or (stop_on_eos and new[-1] == cfg.eos_token_id):
+                                    break
+                                at = nxt[0]
+                                path.append(at)
+                            outs[i] += new
+                            stats["accepted"] += len(path) - 1
+                        paths.append(path)
+                        o += len(tree)
+                    dec.commit(paths, stream=stream)
+                    stats["steps"] += 1
+            finally:
+                dec.close()
+        t = time.perf_counter() - t0
+        total = float(sum(len(o) for o in outs))
+        stats.update(total_tokens_generated=total, total_time_s=t, tokens_per_sec=total / max(t, 1e-9))
+        return outs, stats
+
+    def generate_beam_ids(
+        self,
+        batch_prompt_ids: Sequence[Sequence[int]],
+        num_beams: int = 4,
+        max_new_tokens: int = 16,
+        length_penalty: float = 1.0,
+        stop_on_eos: bool = True,
+    ) -> Tuple[List[List[int]], List[float]]:
+        """Beam search: for each prompt the ids of the best of ``num_beams`` beams and its
+        score, the sum of its tokens' log probabilities over len ** length_penalty.  Each
+        beam is a row of the batch (max_batch >= prompts * num_beams); every step picks
+        the continuations on the GPU (``beam.BeamSelector``) and lets the beams' cached
+        states follow their parents (``BatchDecoder.reorder``).  A prompt ends when
+        num_beams of its hypotheses have ended, or at max_new_tokens."""
+        import beam
+
+        cfg, k = self.model.cfg, int(num_beams)
+        if not 1 <= k <= ffi.MAX_BEAMS:
+            raise ValueError(f"num_beams must be in [1, {ffi.MAX_BEAMS}]")
+        if cfg.vocab < 2 * k:
+            raise ValueError("the vocabulary is smaller than two beams' continuations")
+        prompts = self._check_prompts(batch_prompt_ids, k, max_new_tokens)
+        n = len(prompts)
+        if n == 0 or max_new_tokens == 0:
+            return [[] for _ in prompts], [0.0] * n
+        stream = torch.cuda.current_stream(self.model.device)
+        emb = self.model.embedding
+        dec = self._decoder(self.bt[:n * k].clone())      # (reorder permutes the table)
+        sel = beam.BeamSelector(n, k, cfg.vocab, 2 * k, device=self.model.device)
+        ended: List[List[Tuple[float, List[int]]]] = [[] for _ in range(n)]
+        live: List[List[List[int]]] = [[[] for _ in range(k)] for _ in range(n)]
+
+        def norm(score: float, length: int) -> float:
+            return score / length ** length_penalty
+
+        try:
+            last = []
+            for i, p in enumerate(prompts):     # the prompt goes into the first beam's row
+                ids = torch.tensor(p, dtype=torch.long, device=emb.device)
+                h = dec.prefill(i * k, emb[ids].contiguous(), stream=stream)[-1:]
+                dec.ctx[i * k:(i + 1) * k] = len(p)
+                last.append(h.expand(k, -1))
+            h = torch.cat(last).contiguous()
+            scores = torch.full((n, k), -float("inf"), device=emb.device)
+            scores[:, 0] = 0.0
+            for step in range(max_new_tokens):
+                tok, par, best = sel.select(self._logits(h, stream), scores, 2 * k, stream=stream)
+                tok, par, best = tok.tolist(), par.tolist(), best.tolist()
+                parents = np.zeros((n, k), dtype=np.int32)
+                nxt = np.zeros((n, k), dtype=np.int64)
+                run = np.full((n, k), -np.inf, dtype=np.float32)
+                for i in range(n):
+                    if len(ended[i]) >= k:      # finished: rides along
+                        parents[i] = np.arange(k)
+                        continue
+                    grown = []
+                    for rank in range(2 * k):
+                        ids = live[i][par[i][rank]] + [tok[i][rank]]
+                        if stop_on_eos and tok[i][rank] == cfg.eos_token_id:
+                            if rank < k:
+                                ended[i].append((norm(best[i][rank], len(ids)), ids))
+                        elif len(grown) < k:
+                            j = len(grown)
+                            parents[i, j], nxt[i, j] = par[i][rank], tok[i][rank]
+                            run[i, j] = best[i][rank]
+                            grown.append(ids)
+                    live[i] = grown
+                if step + 1 == max_new_tokens or all(len(e) >= k for e in ended):
+                    break
+                dec.reorder(parents, stream=stream)
+                scores = torch.from_numpy(run).to(emb.device)
+                ids = torch.from_numpy(nxt.reshape(-1)).to(emb.device)
+                h = dec.step(emb[ids].contiguous(), stream=stream)
+        finally:
+            dec.close()
+            sel.close()
+        outs, finals = [], []
+        for i in range(n):
+            hyps = list(ended[i])
+            if len(hyps) < k:
+                hyps += [(norm(float(run[i, j]), len(ids)), ids) for j, ids in enumerate(live[i])
+                         if np.isfinite(run[i, j])]
+            score, ids = max(hyps, key=lambda x: x[0])
+            outs.append(ids)
+            finals.append(score)
+        return outs, finals
 
     def close(self):
         self.pool.close()

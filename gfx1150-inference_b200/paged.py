@@ -538,6 +538,8 @@ class BatchDecoder:
         self.ctx = np.asarray(ctx_lens, dtype=np.int64).copy()
         self.eps, self.freq_base, self.neox, self.scale = eps, freq_base, neox, scale
         self.plan = DecodePlan()
+        self.tree_plan: Optional[TreePlan] = None
+        self._drafted: Optional[list] = None      # node counts of the last verify
         self.capacity = int(block_tables.shape[1]) * cache.page_size
 
     def prefill(self, seq: int, x: torch.Tensor, stream=None) -> torch.Tensor:
@@ -569,6 +571,84 @@ class BatchDecoder:
         self.ctx += 1
         return y
 
+    def verify(self, x: torch.Tensor, trees: Sequence[Sequence[int]], stream=None) -> torch.Tensor:
+        """Run drafted tokens through every layer: trees[i] holds the parents of sequence
+        i's drafted tokens (tree_masks; empty for none), x (tokens, hidden) their
+        embeddings, sequence by sequence.  Each token attends over its sequence's
+        cached context, its ancestors and itself; returns the last layer's output
+        (tokens, hidden).  The context lengths stay until ``commit`` keeps a path."""
+        b = len(self.ctx)
+        if len(trees) != b:
+            raise ValueError(f"one tree per sequence is required ({b})")
+        counts = [len(t) for t in trees]
+        n = sum(counts)
+        if int(x.shape[0]) != n:
+            raise ValueError(f"x must hold one row per drafted token ({n})")
+        for c, k in zip(self.ctx, counts):
+            if k and int(c) + k > self.capacity:
+                raise IndexError("a tree exceeds its sequence's block-table capacity")
+        words = max(1, (max(counts, default=0) + 31) // 32)
+        masks = [tree_masks(t, words) for t in trees]
+        self._drafted = None
+        if n == 0:
+            self._drafted = counts
+            return x
+        pos = np.concatenate([int(c) + tree_depths(t) for c, t in zip(self.ctx, trees)])
+        dev = x.device
+        mask = torch.from_numpy(np.concatenate(masks)).to(dev)
+        rope_pos = torch.from_numpy(pos.astype(np.int32)).to(dev)
+        self.tree_plan = self.cache.plan_tree(self.ctx, counts, self.num_heads,
+                                              plan=self.tree_plan, stream=stream)
+        cur = x.contiguous()
+        bufs = (torch.empty_like(cur), torch.empty_like(cur))   # x itself is never written
+        for layer, lw in enumerate(self.layers):
+            nxt = bufs[layer % 2]
+            self.cache.forward_layer_tree(self.tree_plan, layer, cur, nxt, lw, mask, self.bt,
+                                          rope_pos, self.eps, self.freq_base, self.neox,
+                                          self.scale, stream)
+            cur = nxt
+        self._drafted = counts
+        return cur
+
+    def commit(self, paths: Sequence[Sequence[int]], stream=None) -> None:
+        """Keep paths[i], ascending node numbers of sequence i's last ``verify`` (empty:
+        none): their rows move together behind the context, which grows by them."""
+        if self._drafted is None:
+            raise RuntimeError("commit needs the trees of a verify before it")
+        if len(paths) != len(self.ctx):
+            raise ValueError(f"one path per sequence is required ({len(self.ctx)})")
+        for p, k in zip(paths, self._drafted):
+            if any(not 0 <= a < k for a in p) or any(a >= b for a, b in zip(p, p[1:])):
+                raise ValueError("a path holds ascending numbers of its tree's nodes")
+        lens = np.array([len(p) for p in paths], dtype=np.int32)
+        if lens.max(initial=0) > 0:
+            mat = np.zeros((len(paths), int(lens.max())), dtype=np.int32)
+            for i, p in enumerate(paths):
+                mat[i, :len(p)] = p
+            dev = self.bt.device
+            self.cache.commit_tree(self.bt, torch.from_numpy(self.ctx.astype(np.int32)).to(dev),
+                                   torch.from_numpy(mat).to(dev), torch.from_numpy(lens).to(dev),
+                                   stream=stream)
+        self.ctx += lens
+        self._drafted = None
+
+    def reorder(self, parents: np.ndarray, stream=None) -> None:
+        """Beam search: rows are sequences * beams, parents (sequences, beams) beam
+        numbers; every row takes its parent's cached states (reorder_beams).  The
+        block table is permuted in place: give the decoder one of its own."""
+        parents = np.ascontiguousarray(np.asarray(parents, dtype=np.int32))
+        if parents.ndim != 2 or parents.size != len(self.ctx):
+            raise ValueError("parents needs one entry per row, (sequences, beams)")
+        n, beams = parents.shape
+        if parents.size and (parents.min() < 0 or parents.max() >= beams):
+            raise ValueError("a parent is not a beam of its sequence")
+        ctx = self.ctx.reshape(n, beams)
+        if np.any(ctx != ctx[:, :1]):
+            raise ValueError("the beams of a sequence must have the same context length")
+        dev = self.bt.device
+        self.cache.reorder_beams(self.bt, torch.from_numpy(parents).to(dev),
+                                 torch.from_numpy(ctx[:, 0].astype(np.int32)).to(dev), stream=stream)
+
     def _layers(self, x: torch.Tensor, stream) -> torch.Tensor:
         cur = x.contiguous()
         bufs = (torch.empty_like(cur), torch.empty_like(cur))   # x itself is never written
@@ -577,10 +657,13 @@ class BatchDecoder:
             self.cache.forward_layer(self.plan, layer, cur, nxt, lw, self.bt, self.eps,
                                      self.freq_base, self.neox, self.scale, stream)
             cur = nxt
+        self._drafted = None
         return cur
 
     def close(self):
         self.plan.close()
+        if self.tree_plan is not None:
+            self.tree_plan.close()
 
 
 # -- drafted trees --------------------------------------------------------------------
