@@ -175,7 +175,6 @@ __device__ __forceinline__ float exp_diff(float x, float m) {
 // the instructions: nearly every batch of a run holds one that looks good so far.)
 template <typename T>
 __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const BeamArgs a) {
-  launch_dependents();
   // at most n_out lanes hold candidates, and each holds at most its logits
   __shared__ uint64_t s_keys[kMaxBeamOut * kPerLane * kMaxBatches];
   __shared__ uint64_t s_list[kChunkWarps][32];
@@ -192,6 +191,7 @@ __global__ void __launch_bounds__(32 * kChunkWarps) beam_chunk_kernel(const Beam
   const int batches = min(a.batches, (a.vocab - first + kBatch - 1) / kBatch);
   auto token = [&](int b, int i) { return first + b * kBatch + lane * N + (i / N) * 32 * N + i % N; };
   wait_prerequisites();
+  launch_dependents();
   const bool dead = !isfinite(a.cum[row]);   // a beam that is not in use
   float m = -INFINITY, sum = 0.f;
   int at = 0;                                // the batch of the lane's best
@@ -322,8 +322,8 @@ __device__ __forceinline__ Scored merge32(Scored x, const Scored& y, int lane) {
 // then the beams' lists are joined pairwise.  Scores are held in 64 bits so that
 // candidates of different beams that lie close together keep their order.
 __global__ void __launch_bounds__(32 * kMaxBeams) beam_merge_kernel(const BeamArgs a) {
-  launch_dependents();
   wait_prerequisites();
+  launch_dependents();
   __shared__ Scored s_list[kMaxBeams][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seq = blockIdx.x, row = seq * a.beams + warp;
@@ -382,7 +382,8 @@ __global__ void __launch_bounds__(32 * kMaxBeams) beam_merge_kernel(const BeamAr
 int beam_chunks(int vocab) { return (vocab + kMinChunk - 1) / kMinChunk; }
 
 namespace {
-// A launch that may begin before the one ahead of it has ended.
+// A launch that may begin before the one ahead of it has ended; it lets its successor begin
+// only once all before it has.
 template <typename K>
 cudaError_t launch_early(K kernel, dim3 grid, int threads, cudaStream_t s, const BeamArgs& a) {
   cudaLaunchAttribute attr[1];

@@ -83,8 +83,8 @@ __device__ __forceinline__ unsigned int ld_acquire_sys(const unsigned int* p) {
 }
 
 // ---- programmatic dependent launch ------------------------------------------------
-// The next launch on the stream may begin; the launches ahead of this one have ended and
-// their writes are visible.
+// launch_dependents: the next launch on the stream may begin.  wait_prerequisites: the
+// launches ahead of this one have ended and their writes are visible.
 __device__ __forceinline__ void launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

@@ -73,7 +73,6 @@ __global__ void __launch_bounds__(kAppendThreads) append_rope_kernel(const Appen
   constexpr int kTok = kAppendThreads / kPer;
   __shared__ float2 cs[kTok * kMaxRopePairs];
   __shared__ int s_page[kTok], s_slot[kTok];
-  launch_dependents();
   const int tok0 = blockIdx.x * kTok, half = a.head_dim / 2;
   const int toks = min(kTok, a.n - tok0);
   const int U = a.p.row_units, Hkv = a.p.num_kv_heads;
@@ -212,7 +211,6 @@ constexpr int kCommitCols = 8;      // columns of a thread in flight
 __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs a) {
   __shared__ int s_page[2][kMaxTreeNodes], s_t[2][kMaxTreeNodes];   // [source, target]
   __shared__ int s_bad;
-  launch_dependents();
   if (threadIdx.x == 0) s_bad = 0;
   wait_prerequisites();
   const int seq = blockIdx.y;
@@ -283,7 +281,6 @@ constexpr int kReorderThreads = 128;
 template <int kBeams>
 __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderArgs a) {
   __shared__ int s_parent[kMaxBeams], s_page[kMaxBeams], s_bad;
-  launch_dependents();
   if (threadIdx.x == 0) s_bad = 0;
   wait_prerequisites();
   const int seq = blockIdx.y, B = a.beams, ps = a.p.page_size;
@@ -354,7 +351,9 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderA
 }
 
 // A launch that may begin before the one ahead of it has ended: every kernel here touches
-// what others do only behind wait_prerequisites().
+// what others do only behind wait_prerequisites().  None lets its own successor begin
+// early: they write K/V rows, and a decode two launches on may stream those as soon as the
+// launch between them has begun.
 template <typename A>
 cudaError_t launch_early(void (*kernel)(A), dim3 grid, int threads, cudaStream_t s, const A& args) {
   cudaLaunchAttribute attr[1];

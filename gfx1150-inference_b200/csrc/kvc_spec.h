@@ -108,14 +108,16 @@ struct TreeArgs {
   float scale_log2;
 };
 
-// Tile shape of the kernel a pool takes: positions per tile and rows per block.
+// Tile shape of the kernel a batch takes: positions per tile and rows per block.
 struct TreeTile {
   int positions, rows;
   int ctas_per_sm;
   int piece_cost;                // start and end of a piece of work, in tiles
   bool tensor;                   // tcgen05 kernel
 };
-TreeTile tree_tile(const PoolGeom& g);
+// small_tiles: how many tiles of 32 rows x 32 positions (kTreeSmall) the batch has.
+constexpr int kTreeSmall = 32;
+TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms);
 cudaError_t launch_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s);
 
 // ---- beam selection ---------------------------------------------------------------------

@@ -191,9 +191,8 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   if (num_heads <= 0 || num_heads % g.num_kv_heads != 0)
     return set_error(KVC_ERR_INVALID_ARG, "num_heads must be divisible by num_kv_heads.");
   p->valid = false;
-  const TreeTile tile = tree_tile(g);
-  const int group = num_heads / g.num_kv_heads;
-  int64_t tokens = 0, tiles = 0, runs = 0, max_end = 0;
+  const int group = num_heads / g.num_kv_heads, sms = device_sms(pool->device);
+  int64_t tokens = 0, tiles = 0, runs = 0, max_end = 0, small = 0;
   int max_row = 0, max_nodes = 0;
   std::vector<int32_t> rows, slots;
   for (int i = 0; i < n_seqs; ++i) {
@@ -212,14 +211,19 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     if (h_nodes[i] > 0) max_end = std::max(max_end, end);
     max_row = std::max(max_row, row);
     max_nodes = std::max(max_nodes, h_nodes[i]);
+    small += (static_cast<int64_t>(h_nodes[i]) * group + kTreeSmall - 1) / kTreeSmall *
+             g.num_kv_heads * ((end + kTreeSmall - 1) / kTreeSmall);
+  }
+  const TreeTile tile = tree_tile(g, small, sms);
+  for (int i = 0; i < n_seqs; ++i) {
     const int64_t blocks = (static_cast<int64_t>(h_nodes[i]) * group + tile.rows - 1) / tile.rows;
+    const int64_t end = static_cast<int64_t>(h_ctx[i]) + h_nodes[i];
     runs += blocks * g.num_kv_heads;
     tiles += blocks * g.num_kv_heads * ((end + tile.positions - 1) / tile.positions);
   }
   if (tokens * num_heads > (1ll << 30) || tiles > (1ll << 30))
     return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
-  const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(device_sms(pool->device)) *
-                                             tile.ctas_per_sm, tiles);
+  const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(sms) * tile.ctas_per_sm, tiles);
   std::vector<TreeSeg> segs;
   std::vector<TreeMerge> merges;
   std::vector<int> cta_segs(1, 0);

@@ -7,7 +7,8 @@
 // tile, so a K/V byte is read once for all drafted tokens and the whole head group.
 //
 //   tree_mma_kernel     tcgen05 tensor cores: 16-bit pools, head dims 32 ... 256
-//   tree_simt_kernel    CUDA cores: fp32 pools and head dims without a tensor tile
+//   tree_f32_kernel     CUDA cores: fp32 pools
+//   tree_simt_kernel    CUDA cores: 16-bit pools with head dims without a tensor tile
 //   tree_merge_kernel   joins the pieces of rows whose positions were split over CTAs
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -158,8 +159,8 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = *s_tmem;
-  launch_dependents();
   wait_prerequisites();
+  launch_dependents();
 
   // false: some wait of this CTA gave up
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -718,11 +719,217 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
 }
 
 // =====================================================================================
+// fp32 kernel: 64 rows x 64 positions per step in fp32 throughout.  Thread (ty, tx) of
+// 16 x 16 takes rows 4 ty ... 4 ty + 3: their scores with positions tx, tx + 16, ..., then
+// 16-byte pieces tx, tx + 16, ... of their sums, so that 64 FMAs share 8 shared-memory
+// reads of 16 bytes.  A row's scores live in the 16 lanes of a half warp.  The next
+// tile's K and V are copied while this one is worked on, where two fit (head_dim <= 128).
+// =====================================================================================
+constexpr int kF32Rows = 64, kF32Pos = 64, kF32Threads = 256;
+
+template <int NJ>
+struct F32Shape {
+  static constexpr int kBuffers = NJ <= 2 ? 2 : 1;
+};
+
+template <int NJ>
+__global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs a) {
+  constexpr int kBuf = F32Shape<NJ>::kBuffers, kPld = kF32Pos + 4;
+  extern __shared__ float4 smem4[];
+  const int D = a.head_dim, ld = D + 4, U = a.p.row_units;
+  float* sq = reinterpret_cast<float*>(smem4);      // [64][D + 4]
+  float* sp = sq + kF32Rows * ld;                   // [64][68]
+  float* sk = sp + kF32Rows * kPld;                 // [kBuf][64][D + 4]
+  float* sv = sk + kBuf * kF32Pos * ld;             // [kBuf][64][D]
+  __shared__ size_t s_off[2][kF32Pos];              // byte offset of a position's row, ~0: none
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const uint32_t half = 0xffffu << (threadIdx.x & 16);
+  // (the plan's records are no kernel's output: they may be read before the wait)
+  const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
+  TreeSeg next = a.segs[seg0];
+  wait_prerequisites();
+  launch_dependents();
+
+  for (int si = seg0; si < seg1; ++si) {
+    const TreeSeg sg = next;
+    next = a.segs[min(si + 1, seg1 - 1)];
+    const int end = sg.ctx + sg.nodes, tiles = sg.tile1 - sg.tile0;
+    auto places = [&](int i) {   // threads 0 ... 63: where tile i's rows are
+      if (threadIdx.x >= kF32Pos || i >= tiles) return;
+      const int pos = (sg.tile0 + i) * kF32Pos + threadIdx.x;
+      size_t off = ~static_cast<size_t>(0);
+      if (pos < end)
+        off = (static_cast<size_t>(tree_page(a.p, sg.bt_row, pos)) * a.p.num_kv_heads + sg.kvh) *
+                  a.p.page_head_bytes +
+              static_cast<size_t>(pos % a.p.page_size) * U * 16;
+      s_off[i & 1][threadIdx.x] = off;
+    };
+    // positions behind the sequence's last are zero, whatever their page holds
+    auto fetch = [&](int i) {
+      float* k = sk + (i % kBuf) * kF32Pos * ld;
+      float* v = sv + (i % kBuf) * kF32Pos * D;
+      for (int x = threadIdx.x; x < kF32Pos * U; x += kF32Threads) {
+        const int t = x / U, u = x - t * U;
+        const size_t off = s_off[i & 1][t];
+        const bool there = off != ~static_cast<size_t>(0);
+        const size_t at = there ? off + u * 16 : 0;
+        copy16_async(smem_u32(k + t * ld + u * 4), a.p.k + at, there ? 16 : 0);
+        copy16_async(smem_u32(v + t * D + u * 4), a.p.v + at, there ? 16 : 0);
+      }
+    };
+    __syncthreads();
+    places(0);
+    for (int x = threadIdx.x; x < kF32Rows * U; x += kF32Threads) {
+      const int r = x / U, u = x - r * U;
+      const int row = sg.row0 + min(r, sg.rows - 1), node = row / a.group;
+      const float* src = reinterpret_cast<const float*>(a.q) +
+                         (static_cast<size_t>(sg.tok0 + node) * a.num_heads + sg.kvh * a.group + row -
+                          node * a.group) * D;
+      copy16_async(smem_u32(sq + r * ld + u * 4), src + u * 4, r < sg.rows ? 16 : 0);
+    }
+    __syncthreads();
+    fetch(0);
+    places(1);
+    const bool works = 4 * ty < sg.rows;
+    float m[4], l[4];
+    float4 acc[4][NJ];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = kNegBig;
+      l[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int it = 0; it < tiles; ++it) {
+      copy_async_wait();
+      __syncthreads();
+      if (kBuf == 2) {
+        if (it + 1 < tiles) fetch(it + 1);
+        places(it + 2);
+      }
+      const float* k = sk + (it % kBuf) * kF32Pos * ld;
+      const float* v = sv + (it % kBuf) * kF32Pos * D;
+      if (works) {
+        float s[4][4] = {};
+        for (int d = 0; d < D; d += 4) {
+          float4 q4[4], k4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q4[i] = *reinterpret_cast<const float4*>(sq + (4 * ty + i) * ld + d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) k4[j] = *reinterpret_cast<const float4*>(k + (tx + 16 * j) * ld + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              s[i][j] = fmaf(q4[i].x, k4[j].x, s[i][j]);
+              s[i][j] = fmaf(q4[i].y, k4[j].y, s[i][j]);
+              s[i][j] = fmaf(q4[i].z, k4[j].z, s[i][j]);
+              s[i][j] = fmaf(q4[i].w, k4[j].w, s[i][j]);
+            }
+        }
+        const int p0 = (sg.tile0 + it) * kF32Pos;
+        const bool edge = p0 + kF32Pos > sg.ctx;
+        const float sc = a.scale_log2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int node = (sg.row0 + min(4 * ty + i, sg.rows - 1)) / a.group;
+          float mx = m[i];
+          bool see[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int pos = p0 + tx + 16 * j;
+            see[j] = !edge || pos < sg.ctx || (pos < end && sees(a, sg.tok0, node, pos - sg.ctx));
+            s[i][j] *= sc;
+            if (see[j]) mx = fmaxf(mx, s[i][j]);
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(half, mx, o));
+          const float corr = fast_exp2(m[i] - mx);
+          m[i] = mx;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e = see[j] ? fast_exp2(s[i][j] - mx) : 0.f;
+            sum += e;
+            sp[(4 * ty + i) * kPld + tx + 16 * j] = e;
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(half, sum, o);
+          l[i] = l[i] * corr + sum;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            acc[i][j].x *= corr;
+            acc[i][j].y *= corr;
+            acc[i][j].z *= corr;
+            acc[i][j].w *= corr;
+          }
+        }
+        __syncwarp(half);
+#pragma unroll 2
+        for (int t = 0; t < kF32Pos; t += 4) {
+          float4 p4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p4[i] = *reinterpret_cast<const float4*>(sp + (4 * ty + i) * kPld + t);
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+            float4 v4[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+              v4[j] = 4 * (tx + 16 * j) < D
+                          ? *reinterpret_cast<const float4*>(v + (t + tt) * D + 4 * (tx + 16 * j))
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = (&p4[i].x)[tt];
+              // (a position without weight adds nothing, not even where its V is not finite)
+              if (edge && p == 0.f) continue;
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) {
+                acc[i][j].x = fmaf(p, v4[j].x, acc[i][j].x);
+                acc[i][j].y = fmaf(p, v4[j].y, acc[i][j].y);
+                acc[i][j].z = fmaf(p, v4[j].z, acc[i][j].z);
+                acc[i][j].w = fmaf(p, v4[j].w, acc[i][j].w);
+              }
+            }
+          }
+        }
+      }
+      if (kBuf == 1 && it + 1 < tiles) {
+        __syncthreads();
+        fetch(it + 1);
+        places(it + 2);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * ty + i;
+      if (r >= sg.rows) continue;
+      const int row = sg.row0 + r, node = row / a.group;
+      const int head = sg.kvh * a.group + row - node * a.group;
+      const float inv = l[i] > 0.f ? 1.0f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
+      float4* po = sg.part >= 0
+                       ? reinterpret_cast<float4*>(a.part_o + static_cast<size_t>(sg.part) * D) + r
+                       : reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) +
+                                                   (static_cast<size_t>(sg.tok0 + node) * a.num_heads + head) * D);
+      const int step = sg.part >= 0 ? sg.rows : 1;
+      const float f = sg.part >= 0 ? 1.0f : inv;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int c = tx + 16 * j;
+        if (4 * c < D)
+          po[c * step] = make_float4(acc[i][j].x * f, acc[i][j].y * f, acc[i][j].z * f, acc[i][j].w * f);
+      }
+      if (sg.part >= 0 && tx == 0) a.part_ml[sg.part + r] = make_float2(m[i], l[i]);
+    }
+  }
+}
+
+// =====================================================================================
 // CUDA-core kernel: 32 rows x 32 positions per step, eight warps of four rows.  A lane
 // owns one position for the scores and every 32nd dim for the sums; the running max
 // and sum of a row are the same in all lanes of its warp.
 // =====================================================================================
-constexpr int kSimtRows = 32, kSimtPos = 32, kSimtThreads = 256;
+constexpr int kSimtRows = kTreeSmall, kSimtPos = kTreeSmall, kSimtThreads = 256;
 
 template <typename T, int DPL>
 __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs a) {
@@ -734,11 +941,15 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int N = 16 / sizeof(T);
   const int U = a.p.row_units;
-  launch_dependents();
+  // (the plan's records are no kernel's output: they may be read before the wait)
+  const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
+  TreeSeg next = a.segs[seg0];
   wait_prerequisites();
+  launch_dependents();
 
-  for (int si = a.cta_segs[blockIdx.x]; si < a.cta_segs[blockIdx.x + 1]; ++si) {
-    const TreeSeg sg = a.segs[si];
+  for (int si = seg0; si < seg1; ++si) {
+    const TreeSeg sg = next;
+    next = a.segs[min(si + 1, seg1 - 1)];
     const int end = sg.ctx + sg.nodes;
     __syncthreads();
     for (int x = threadIdx.x; x < kSimtRows * U; x += kSimtThreads) {
@@ -877,8 +1088,8 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   constexpr int N = 16 / sizeof(T), F = N / 4;
   const TreeMerge mg = a.merges[blockIdx.x];
   const int D = a.head_dim;
-  launch_dependents();
   wait_prerequisites();
+  launch_dependents();
   const int x = blockIdx.y * kMergeThreads + threadIdx.x;
   const int c = x / mg.rows, r = x - c * mg.rows;   // 16 bytes c of row r
   if (c * N >= D) return;
@@ -939,7 +1150,8 @@ cudaError_t allow_smem(size_t smem) {
 }
 
 // A launch that may begin before the one ahead of it has ended: every kernel here reads
-// and writes what others do only behind wait_prerequisites().  The merge asks for the
+// and writes what others do only behind wait_prerequisites(), and lets its successor begin
+// only there, so that nothing written ahead of it is still on its way then.  The merge asks for the
 // attention kernels' shared-memory split, so that an SM passes from one to the other
 // without a change of it.
 template <typename A>
@@ -979,6 +1191,16 @@ cudaError_t run_simt(const TreeArgs& a, cudaStream_t s) {
   return launch_early(tree_simt_kernel<T, DPL>, dim3(a.n_ctas), kSimtThreads, smem, s, a);
 }
 
+template <int NJ>
+cudaError_t run_f32(const TreeArgs& a, cudaStream_t s) {
+  const size_t ld = a.head_dim + 4, buf = F32Shape<NJ>::kBuffers;
+  const size_t smem = sizeof(float) * (kF32Rows * ld + kF32Rows * (kF32Pos + 4) +
+                                       buf * kF32Pos * (ld + a.head_dim));
+  const cudaError_t e = allow_smem<tree_f32_kernel<NJ>>(smem);
+  if (e != cudaSuccess) return e;
+  return launch_early(tree_f32_kernel<NJ>, dim3(a.n_ctas), kF32Threads, smem, s, a);
+}
+
 template <typename T, int D>
 cudaError_t run_mma(const TreeArgs& a, cudaStream_t s) {
   using S = TreeShape<D>;
@@ -1006,16 +1228,26 @@ cudaError_t run_mma_any<float>(const TreeArgs&, cudaStream_t) {
 }
 
 template <typename T>
+cudaError_t run_cuda_cores(const TreeArgs& a, const TreeTile&, cudaStream_t s) {
+  if (a.head_dim <= 64) return run_simt<T, 2>(a, s);
+  if (a.head_dim <= 128) return run_simt<T, 4>(a, s);
+  return run_simt<T, 8>(a, s);
+}
+template <>
+cudaError_t run_cuda_cores<float>(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
+  if (t.rows == kSimtRows) {
+    if (a.head_dim <= 64) return run_simt<float, 2>(a, s);
+    if (a.head_dim <= 128) return run_simt<float, 4>(a, s);
+    return run_simt<float, 8>(a, s);
+  }
+  if (a.head_dim <= 64) return run_f32<1>(a, s);
+  if (a.head_dim <= 128) return run_f32<2>(a, s);
+  return run_f32<4>(a, s);
+}
+
+template <typename T>
 cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
-  cudaError_t e;
-  if (t.tensor)
-    e = run_mma_any<T>(a, s);
-  else if (a.head_dim <= 64)
-    e = run_simt<T, 2>(a, s);
-  else if (a.head_dim <= 128)
-    e = run_simt<T, 4>(a, s);
-  else
-    e = run_simt<T, 8>(a, s);
+  cudaError_t e = t.tensor ? run_mma_any<T>(a, s) : run_cuda_cores<T>(a, t, s);
   if (e != cudaSuccess || a.n_merges == 0) return e;
   if ((e = prefer_shared<tree_merge_kernel<T>>()) != cudaSuccess) return e;
   const int per = a.max_merge_rows * (a.head_dim * static_cast<int>(sizeof(T)) / 16);
@@ -1026,10 +1258,15 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
 
 }  // namespace
 
-TreeTile tree_tile(const PoolGeom& g) {
+// fp32: the larger tiles do 64 FMAs for 8 shared-memory reads (27 TFLOP/s where the small
+// ones reach 10, 32 drafted tokens of 4 sequences at 4000), the small ones start sooner and
+// spread further (14.8 against 17.3 us, 4 tokens of one sequence at 511): they are taken
+// while all of their tiles find a place on the GPU at once.
+TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms) {
   if (decode_uses_mma(g.dtype, g.head_dim, g.page_size) && g.layout == kLayoutCore)
     return g.head_dim <= 128 ? TreeTile{128, 256, 1, kPieceCost, true}
                              : TreeTile{64, 128, 1, kPieceCost, true};
+  if (g.elem_size == 4 && small_tiles > 2 * sms) return TreeTile{kF32Pos, kF32Rows, 1, 1, false};
   return TreeTile{kSimtPos, kSimtRows, 2, 0, false};
 }
 

@@ -614,7 +614,7 @@ KVC_API int kvc_forward_layer_tree(
  * j < d_path_lens[i], in block-table row d_rows[i] (NULL: row i).  Paths are
  * strictly ascending node numbers (an ancestor is drafted before its children), at
  * most path_stride long; a length of 0 keeps the sequence as it is.  Rows behind
- * the path stay as they were.  A path that does not ascend or leaves the table is
+ * the path stay as they were.  No two sequences of a call share a row.  A path that does not ascend or leaves the table is
  * reported (KVC_DEVERR_BAD_POSITION) and its sequence left alone. */
 KVC_API int kvc_commit_tree(kvc_pool_t* pool, const int32_t* d_block_tables, int bt_rows,
                             int bt_stride, const int32_t* d_rows, const int32_t* d_ctx_lens,

@@ -197,6 +197,75 @@ def test_tree_attention(case, dtype):
     check(*tree_case(dtype, d, h, hkv, ps, ctx, nodes, seed=11 + d + len(ctx)))
 
 
+LONG = [
+    (64, 32, 4, 16, [3000, 17, 700], [30, 64, 5]),
+    (128, 16, 2, 48, [2000, 0, 1, 3333], [33, 64, 7, 1]),
+    (256, 12, 2, 32, [1500, 900], [64, 21]),
+    (96, 8, 8, 16, [5000, 63, 64, 65], [9, 250, 3, 17]),
+    (12, 6, 2, 16, [4000, 1000], [64, 100]),          # fp32 only: 24-byte rows of 16-bit types
+]
+
+
+@pytest.mark.parametrize("case,dtype", [(c, t) for c in LONG for t in (F32, F16, BF16)
+                                        if c[0] != 12 or t == F32])
+def test_tree_long_batches(case, dtype):
+    """Batches with more tiles than the GPU takes at once: pieces are cut and joined."""
+    d, h, hkv, ps, ctx, nodes = case
+    check(*tree_case(dtype, d, h, hkv, ps, ctx, nodes, seed=100 + d))
+    check(*tree_case(dtype, d, h, hkv, ps, ctx, nodes, seed=200 + d, mask="any", scale=-0.05))
+
+    def poison(i, k, v, c):      # node 2 holds anything, and nobody sees it
+        if k.shape[0] > c + 2:
+            k[c + 2], v[c + 2] = math.nan, math.inf
+    orig = paged.tree_masks
+
+    def without_2(parents, words=None):
+        m = orig([-1] * len(parents), words)
+        if len(m) > 2:
+            m[2] = 0
+        return m
+    paged.tree_masks = without_2
+    try:
+        check(*tree_case(dtype, d, h, hkv, ps, ctx, nodes, seed=300 + d, tweak=poison))
+    finally:
+        paged.tree_masks = orig
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_tree_values_that_are_seen_come_through(dtype):
+    """A drafted V that is not finite reaches the rows that see it, and only there."""
+    dt = getattr(torch, dtype)
+    ctx, n, d = 200, 40, 128
+    pool = make_pool(1, 16, 16, 2, d, dtype, fill=0.0)
+    pool.fill_normal(seed=3)
+    bt = dev(np.arange(16).reshape(1, 16))
+    k = torch.randn(n, 2, d, device="cuda").to(dt)
+    v = torch.randn(n, 2, d, device="cuda").to(dt)
+    v[3, 1, 5], v[7, 0, 9], v[9, 0, 9] = math.inf, math.nan, -math.inf
+    pool.append(0, k, v, bt, torch.arange(ctx, ctx + n, dtype=torch.int32, device="cuda"))
+    par = [-1, 0, 1, 2, 3, 2, 5, 6, 2, 8] + [4] * 30      # 3 and 9 lie on different branches
+    q = torch.randn(n, 8, d, device="cuda").to(dt)
+    out = torch.zeros_like(q)
+    pool.decode_tree(pool.plan_tree([ctx], [n], 8), 0, q, dev(paged.tree_masks(par)), out, bt, 0.09)
+    no_error()
+    seen = [{j for j in range(n) if int(paged.tree_masks(par, 2)[i, j // 32]) >> (j % 32) & 1}
+            for i in range(n)]
+    o = out.float().cpu().numpy()
+    for i in range(n):
+        for h in range(8):
+            for x in (5, 9):
+                val = o[i, h, x]
+                if x == 5 and h >= 4 and 3 in seen[i]:
+                    assert val == np.inf
+                elif x == 9 and h < 4 and 7 in seen[i]:
+                    assert np.isnan(val)
+                elif x == 9 and h < 4 and 9 in seen[i]:
+                    assert val == -np.inf
+                else:
+                    assert np.isfinite(val)
+            assert np.all(np.isfinite(np.delete(o[i, h], [5, 9])))
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_tree_any_mask_and_empty_rows(dtype):
     got, ref, tol = tree_case(dtype, 128, 8, 2, 16, [0, 40, 0], [40, 33, 9], seed=3, mask="any")
