@@ -63,7 +63,10 @@ __device__ __forceinline__ void rotate(T& x0, T& x1, float2 cs) {
 // through sincospif in 32 bits.  A thread owns two 16-byte units that hold each other's
 // pairs (units 2i, 2i + 1, or i and i + half the row for NeoX), keeps their angles in
 // registers and goes through the heads of q, K and V, kAppendBatch of them on their way;
-// the first are asked for before the angles are computed.
+// the first are asked for before the angles are computed.  Bound by memory traffic: 8,895
+// tokens of 32 + 8 + 8 heads of 128 dims, bf16, 48 us for 219 MB (a plain copy of as many
+// bytes takes 37); the pool's layout puts a row's pieces 128 bytes apart, which costs 4 us
+// of it.  64 threads per token measured best of 32, 64, 128 and 256.
 // =====================================================================================
 constexpr int kAppendThreads = 256;
 constexpr int kAppendBatch = 3;
@@ -202,7 +205,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_rope_kernel(const Appen
 // All of a batch is read before any of it is written, and ascending paths keep the batches
 // apart: a later source lies behind every slot written before it.
 // The rows come in 16-byte pieces 128 bytes apart, and memory is read 64 bytes at a time:
-// the sources alone cost four times their bytes, which is what bounds this.
+// the sources alone cost four times their bytes, which is what bounds this (32 paths of up
+// to 8 nodes, 32 layers: 18 MB moved, 107 MB read, 23 us).
 // =====================================================================================
 constexpr int kCommitThreads = 256;
 constexpr int kCommitSteps = 8;     // of a path at a time
@@ -274,7 +278,8 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
 // head of one layer's K or V in the open pages.  A thread owns one 16-byte unit of a page
 // for all beams: it reads every moved beam's new value, then writes, so the permutation
 // happens in place without a second buffer.  The units in front of `tail` positions are
-// taken in the order of memory; of the last 8-position block only some rows are.
+// taken in the order of memory; of the last 8-position block only some rows are.  Bound by
+// memory traffic: 8 x 8 beams, 32 layers, 149 MB in 28.5 us (23 at the copy rate).
 // =====================================================================================
 constexpr int kReorderThreads = 128;
 
