@@ -102,6 +102,14 @@ __device__ __forceinline__ bool not_finite(uint32_t h) {
   return (h & e) == e;
 }
 
+// Whether one of two packed values may not be finite (never false when one is not).
+template <typename T>
+__device__ __forceinline__ bool maybe_odd(uint32_t two) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+  const uint32_t t = (two & e) ^ e;   // a half is zero where its exponent is all ones
+  return ((t - 0x00010001u) & ~t & 0x80008000u) != 0u;
+}
+
 // Mask word k (drafted tokens 32 k ... 32 k + 31) of a row; below 0: cached positions.
 __device__ __forceinline__ uint32_t mask_word(const TreeArgs& a, const TreeSeg& sg, int node, int k) {
   if (k < 0) return 0xffffffffu;
@@ -457,22 +465,31 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
           uint8_t* vt = stage_mem + st * S::kStageBytes;
           const int from = max(0, sg.ctx - p0), to = min(KP, (end - p0 + kSlab - 1) / kSlab * kSlab);
           bool dirty = false;
-          for (int i = from * U + lane; i < to * U; i += 32) {
+          auto cell = [&](int i) {
             const int pt = i / U, u = i - pt * U;
-            uint4* cell = reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            bool bad = p0 + pt >= end;
-            if (!bad) {
-              v = *cell;
-              uint32_t* e = &v.x;
+            return reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
+          };
+          const int live = min(to, end - p0) * U;      // units of drafted positions
+          for (int i0 = from * U + lane; i0 < live; i0 += 4 * 32) {
+            uint4 v[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if (not_finite<T>(e[k] & 0xffffu)) e[k] &= 0xffff0000u, bad = dirty = true;
-                if (not_finite<T>(e[k] >> 16)) e[k] &= 0x0000ffffu, bad = dirty = true;
+            for (int k = 0; k < 4; ++k)
+              v[k] = i0 + 32 * k < live ? *cell(i0 + 32 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (!(maybe_odd<T>(v[k].x) || maybe_odd<T>(v[k].y) || maybe_odd<T>(v[k].z) ||
+                    maybe_odd<T>(v[k].w)))
+                continue;
+              uint32_t e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                if (not_finite<T>(e[w] & 0xffffu)) e[w] &= 0xffff0000u, dirty = true;
+                if (not_finite<T>(e[w] >> 16)) e[w] &= 0x0000ffffu, dirty = true;
               }
+              *cell(i0 + 32 * k) = make_uint4(e[0], e[1], e[2], e[3]);
             }
-            if (bad) *cell = v;
           }
+          for (int i = live + lane; i < to * U; i += 32) *cell(i) = make_uint4(0, 0, 0, 0);
           if (dirty) s_dirty[si & 1] = si;
         }
         __threadfence_block();
@@ -1106,25 +1123,49 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   const int c = x / mg.rows, r = x - c * mg.rows;   // 16 bytes c of row r
   if (c * N >= D) return;
   const float2* ml = a.part_ml + mg.part + r;
-  float mx = kNegBig;
-  for (int k = 0; k < mg.n_parts; ++k) mx = fmaxf(mx, ml[static_cast<size_t>(k) * mg.rows].x);
-  float sum = 0.f;
+  const float4* po = reinterpret_cast<const float4*>(a.part_o + static_cast<size_t>(mg.part) * D) +
+                     c * F * mg.rows + r;
+  const size_t po_step = static_cast<size_t>(mg.rows) * D / 4;
+  float mx = kNegBig, sum = 0.f;
   float4 o[F];
 #pragma unroll
   for (int i = 0; i < F; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < mg.n_parts; ++k) {
-    const size_t at = static_cast<size_t>(k) * mg.rows;
-    const float2 e = ml[at];
-    const float w = fast_exp2(e.x - mx);
-    const float4* p = reinterpret_cast<const float4*>(a.part_o + (mg.part + at) * D) + c * F * mg.rows + r;
-    sum += e.y * w;
+  constexpr int kAtOnce = 4;   // pieces on their way together
+  for (int k0 = 0; k0 < mg.n_parts; k0 += kAtOnce) {
+    float2 e[kAtOnce];
+    float4 v[kAtOnce][F];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const bool there = k0 + k < mg.n_parts;
+      e[k] = there ? ml[static_cast<size_t>(k0 + k) * mg.rows] : make_float2(kNegBig, 0.f);
+#pragma unroll
+      for (int i = 0; i < F; ++i)
+        v[k][i] = there ? po[(k0 + k) * po_step + i * mg.rows] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float m2 = mx;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) m2 = fmaxf(m2, e[k].x);
+    const float f = fast_exp2(mx - m2);
+    mx = m2;
+    sum *= f;
 #pragma unroll
     for (int i = 0; i < F; ++i) {
-      const float4 v = p[i * mg.rows];
-      o[i].x += v.x * w;
-      o[i].y += v.y * w;
-      o[i].z += v.z * w;
-      o[i].w += v.w * w;
+      o[i].x *= f;
+      o[i].y *= f;
+      o[i].z *= f;
+      o[i].w *= f;
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float w = fast_exp2(e[k].x - mx);
+      sum += e[k].y * w;
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        o[i].x += v[k][i].x * w;
+        o[i].y += v[k][i].y * w;
+        o[i].z += v[k][i].z * w;
+        o[i].w += v[k][i].w * w;
+      }
     }
   }
   const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
