@@ -224,76 +224,92 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   if (tokens * num_heads > (1ll << 30) || tiles > (1ll << 30))
     return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
   const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(sms) * tile.ctas_per_sm, tiles);
-  std::vector<TreeSeg> segs;
-  std::vector<TreeMerge> merges;
-  std::vector<int> cta_segs(1, 0);
-  size_t part_rows = 0;
-  int max_merge_rows = 0;
-  // A piece costs its tiles and tile.piece_cost for its start and end.  CTA c's share ends
-  // where the cost laid out so far reaches (c + 1) / ctas of the total (the cuts' own
-  // pieces included); a cut that would leave less than piece_cost on either side moves
-  // to the end of the run.
-  const int64_t total_cost = tiles + (runs + ctas) * tile.piece_cost;
-  int64_t cost = 0, cta = 0;
-  auto share_end = [&](int64_t c) {
-    return c + 1 >= ctas ? INT64_MAX : (c + 1) * total_cost / ctas;
-  };
-  int tok0 = 0;
-  for (int i = 0; i < n_seqs; ++i) {
-    const int n_rows = h_nodes[i] * group;
-    const int run = (h_ctx[i] + h_nodes[i] + tile.positions - 1) / tile.positions;
-    for (int kvh = 0; kvh < g.num_kv_heads && n_rows > 0; ++kvh) {
-      for (int r0 = 0; r0 < n_rows; r0 += tile.rows) {
-        const int nr = std::min(tile.rows, n_rows - r0);
-        const size_t first = segs.size();
-        for (int t = 0; t < run;) {
-          const int64_t room = share_end(cta) - cost - tile.piece_cost;
-          if (room < std::max(1, tile.piece_cost) && room < run - t &&
-              cta_segs.back() < static_cast<int>(segs.size())) {
-            cta_segs.push_back(static_cast<int>(segs.size()));  // this share is full
-            ++cta;
-            continue;
+  // A piece costs its tiles and tile.piece_cost for its start and end; a CTA's pieces cost
+  // at most `limit` together, give or take a piece_cost: a cut that would leave less than that
+  // on either side moves to the end of the run or of the share.  walk() lays the runs out for
+  // a limit, calls emit(sequence, kvh, row0, rows, tile0, tiles) and close() for each piece
+  // and each full share, and returns the number of shares.
+  const int64_t pc = tile.piece_cost;
+  auto walk = [&](int64_t limit, auto&& emit, auto&& close) {
+    int64_t shares = 0, cost = 0;
+    for (int i = 0; i < n_seqs; ++i) {
+      const int n_rows = h_nodes[i] * group;
+      const int run = (h_ctx[i] + h_nodes[i] + tile.positions - 1) / tile.positions;
+      for (int kvh = 0; kvh < g.num_kv_heads && n_rows > 0; ++kvh) {
+        for (int r0 = 0; r0 < n_rows; r0 += tile.rows) {
+          for (int t = 0; t < run;) {
+            const int64_t room = limit - cost - pc;
+            if (cost > 0 && room < run - t && room < std::max<int64_t>(1, pc)) {
+              close();
+              ++shares;
+              cost = 0;
+              continue;
+            }
+            int take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(run - t, room)));
+            if (run - t - take < pc) take = run - t;
+            emit(i, kvh, r0, std::min(tile.rows, n_rows - r0), t, take);
+            t += take;
+            cost += take + pc;
           }
-          int take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(run - t, room)));
-          if (run - t - take < tile.piece_cost) take = run - t;
-          TreeSeg sg = {};
-          sg.bt_row = h_rows ? h_rows[i] : i;
-          sg.ctx = h_ctx[i];
-          sg.nodes = h_nodes[i];
-          sg.tok0 = tok0;
-          sg.kvh = kvh;
-          sg.row0 = r0;
-          sg.rows = nr;
-          sg.tile0 = t;
-          sg.tile1 = t + take;
-          sg.part = -1;
-          segs.push_back(sg);
-          t += take;
-          cost += take + tile.piece_cost;
-          if (cost >= share_end(cta)) {
-            cta_segs.push_back(static_cast<int>(segs.size()));
-            ++cta;
-          }
-        }
-        const size_t pieces = segs.size() - first;
-        if (pieces > 1) {
-          TreeMerge m = {};
-          m.part = static_cast<int>(part_rows);
-          m.n_parts = static_cast<int>(pieces);
-          m.tok0 = tok0;
-          m.row0 = r0;
-          m.kvh = kvh;
-          m.rows = nr;
-          merges.push_back(m);
-          for (size_t k = first; k < segs.size(); ++k) {
-            segs[k].part = static_cast<int>(part_rows);
-            part_rows += nr;
-          }
-          max_merge_rows = std::max(max_merge_rows, nr);
         }
       }
     }
-    tok0 += h_nodes[i];
+    return shares + (cost > 0 ? 1 : 0);
+  };
+  // the smallest limit that needs no more shares than there are CTAs
+  int64_t lo = 1, hi = tiles + runs * pc + 1;
+  if (ctas > 0) lo = std::max<int64_t>(1, (tiles + runs * pc) / ctas);
+  while (lo < hi) {
+    const int64_t mid = lo + (hi - lo) / 2;
+    if (walk(mid, [](int, int, int, int, int, int) {}, [] {}) <= ctas)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  std::vector<TreeSeg> segs;
+  std::vector<TreeMerge> merges;
+  std::vector<int> cta_segs(1, 0), tok0(std::max(1, n_seqs), 0);
+  for (int i = 1; i < n_seqs; ++i) tok0[i] = tok0[i - 1] + h_nodes[i - 1];
+  walk(
+      lo,
+      [&](int i, int kvh, int r0, int nr, int t, int take) {
+        TreeSeg sg = {};
+        sg.bt_row = h_rows ? h_rows[i] : i;
+        sg.ctx = h_ctx[i];
+        sg.nodes = h_nodes[i];
+        sg.tok0 = tok0[i];
+        sg.kvh = kvh;
+        sg.row0 = r0;
+        sg.rows = nr;
+        sg.tile0 = t;
+        sg.tile1 = t + take;
+        sg.part = -1;
+        segs.push_back(sg);
+      },
+      [&] { cta_segs.push_back(static_cast<int>(segs.size())); });
+  // runs in several pieces are joined from their partials
+  size_t part_rows = 0;
+  int max_merge_rows = 0;
+  for (size_t first = 0; first < segs.size();) {
+    size_t next = first + 1;
+    while (next < segs.size() && segs[next].tile0 > 0) ++next;
+    if (next - first > 1) {
+      const TreeSeg& sg = segs[first];
+      TreeMerge m = {};
+      m.part = static_cast<int>(part_rows);
+      m.n_parts = static_cast<int>(next - first);
+      m.tok0 = sg.tok0;
+      m.row0 = sg.row0;
+      m.kvh = sg.kvh;
+      m.rows = sg.rows;
+      merges.push_back(m);
+      max_merge_rows = std::max(max_merge_rows, sg.rows);
+      for (size_t k = first; k < next; ++k) {
+        segs[k].part = static_cast<int>(part_rows);
+        part_rows += sg.rows;
+      }
+    }
+    first = next;
   }
   if (cta_segs.back() < static_cast<int>(segs.size())) cta_segs.push_back(static_cast<int>(segs.size()));
   p->n_seqs = n_seqs;

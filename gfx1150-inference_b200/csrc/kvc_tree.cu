@@ -428,19 +428,28 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       if (ok) {
         const int rr = lane >> 2, uu = lane & 3;
         const int n_rows = two ? 256 : 128;
+        // node and head of row g0 + rr, carried along (a division takes as long as the copies)
+        int node = (sg.row0 + rr) / a.group, rem = sg.row0 + rr - node * a.group;
+        const int dn = 8 / a.group, dr = 8 - dn * a.group;
+        const T* base = reinterpret_cast<const T*>(a.q) +
+                        (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D + uu * 8;
+        const int row_step = a.num_heads * D;
+        const uint32_t dst0 = smem_u32(q_mem) + rr * 16 + uu * 128;
+#pragma unroll 2
         for (int g0 = 0; g0 < n_rows; g0 += 8) {
-          const int row = g0 + rr, grow = sg.row0 + min(row, sg.rows - 1), node = grow / a.group;
-          const T* src = reinterpret_cast<const T*>(a.q) +
-                         (static_cast<size_t>(sg.tok0 + node) * a.num_heads + sg.kvh * a.group +
-                          grow - node * a.group) * D;
-          const uint32_t dst = smem_u32(q_mem) + (row >> 7) * S::kQBytes +
-                               ((row & 127) >> 3) * U * 128 + rr * 16;
-          const uint32_t bytes = row < sg.rows ? 16 : 0;
+          const bool there = g0 + rr < sg.rows;
+          const T* src = there ? base + static_cast<size_t>(node) * row_step + rem * D : base;
+          const uint32_t dst = dst0 + (g0 >> 7) * S::kQBytes + ((g0 & 127) >> 3) * U * 128;
 #pragma unroll
           for (int i = 0; i < U / 4; ++i) {
-            copy16_async(dst + (4 * i + uu) * 128, src + (4 * i + uu) * 8, bytes);
-            if (S::kStreams == 2 && !two)
-              copy16_async(dst + S::kQBytes + (4 * i + uu) * 128, src + (4 * i + uu) * 8, bytes);
+            copy16_async(dst + i * 512, src + i * 32, there ? 16 : 0);
+            if (S::kStreams == 2 && !two) copy16_async(dst + S::kQBytes + i * 512, src + i * 32, there ? 16 : 0);
+          }
+          node += dn;
+          rem += dr;
+          if (rem >= a.group) {
+            rem -= a.group;
+            ++node;
           }
         }
         copy_async_wait();
