@@ -224,12 +224,15 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   if (tokens * num_heads > (1ll << 30) || tiles > (1ll << 30))
     return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
   const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(sms) * tile.ctas_per_sm, tiles);
-  // A piece costs its tiles and tile.piece_cost for its start and end; a CTA's pieces cost
-  // at most `limit` together, give or take a piece_cost: a cut that would leave less than that
-  // on either side moves to the end of the run or of the share.  walk() lays the runs out for
+  // A piece costs its tiles and `pc` for its start and end; a CTA's pieces cost at most `limit`
+  // together, give or take a pc: a cut that would leave less than that on either side moves
+  // to the end of the run or of the share.  pc is tile.piece_cost where CTAs have many tiles
+  // (4 against 1 there: 32 ragged trees 115 against 118 us), and less where they have few and
+  // short pieces spread the work further (63 drafted tokens at 511: 16 us at 1, 22 at 4).  walk() lays the runs out for
   // a limit, calls emit(sequence, kvh, row0, rows, tile0, tiles) and close() for each piece
   // and each full share, and returns the number of shares.
-  const int64_t pc = tile.piece_cost;
+  const int64_t pc = std::min<int64_t>(
+      tile.piece_cost, std::max<int64_t>(1, ctas > 0 ? tiles / (8 * ctas) : 1));
   auto walk = [&](int64_t limit, auto&& emit, auto&& close) {
     int64_t shares = 0, cost = 0;
     for (int i = 0; i < n_seqs; ++i) {

@@ -81,7 +81,7 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 // =====================================================================================
 constexpr int kTmemCols = 512;
 constexpr float kRescaleAt = 8.0f;   // log2
-constexpr int kPieceCost = 2;        // a piece's start and end, in tiles
+constexpr int kPieceCost = 4;        // a piece's start and end, in tiles
 
 template <int D>
 struct TreeShape {
