@@ -70,12 +70,12 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 // copying or issuing, and the kernel returns.
 //
 // Measured on B200 (replayed passes; in parentheses the time of the bytes at the copy rate of
-// 6.46 TB/s): 32 sequences of 5-16 nodes at 1K-8K, fp16, 113 us (111); 8 x 12 at 32K,
-// 168 us (167); 16 x 63 at 3K-9K, bf16, 119 us (67).  The first two are bound by memory, the
+// 6.46 TB/s): 32 sequences of 5-16 nodes at 1K-8K, fp16, 114 us (111); 8 x 12 at 32K,
+// 172 us (167); 16 x 63 at 3K-9K, bf16, 118 us (67).  The first two are bound by memory, the
 // last by the chain scores -> softmax -> sums of one stream: 3300 cycles for 256 rows x 128
 // positions, of which the tensor cores work 2050 and the exponentials of a stream alone
 // take 1024.  In seconds of calls without a pause the 1000 W limit holds the clock
-// at 1.55-1.7 GHz and the three take 125, 202 and 138 us.  Tiles of 128 positions fill the
+// at 1.55-1.7 GHz and the three take 128, 204 and 137 us.  Tiles of 128 positions fill the
 // 128 columns that two S and two O tiles leave each other; two streams because one alone
 // leaves the tensor cores idle through its softmax.
 // =====================================================================================
@@ -964,7 +964,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs
 // CUDA-core kernel: 32 rows x 32 positions per step, eight warps of four rows.  A lane
 // owns one position for the scores and every 32nd dim for the sums; the running max
 // and sum of a row are the same in all lanes of its warp.  Bound by latency in small
-// batches (4 nodes of one sequence at 511, fp32: 15 us with the join), by shared-memory
+// batches (4 nodes of one sequence at 511, fp32: 13.5 us with the join), by shared-memory
 // reads in large ones (10 TFLOP/s).
 // =====================================================================================
 constexpr int kSimtRows = kTreeSmall, kSimtPos = kTreeSmall, kSimtThreads = 256;
@@ -1322,8 +1322,8 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
 
 // fp32: the larger tiles do 64 FMAs for 8 shared-memory reads (27 TFLOP/s where the small
 // ones reach 10, 32 drafted tokens of 4 sequences at 4000), the small ones start sooner and
-// spread further (14.8 against 17.3 us, 4 tokens of one sequence at 511): they are taken
-// while all of their tiles find a place on the GPU at once.
+// spread further (14.8 against 17.3 us, 4 tokens of one sequence at 511, both with the join
+// as it was then, 1.3 us slower): they are taken while all of their tiles find a place on the GPU at once.
 TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms) {
   if (decode_uses_mma(g.dtype, g.head_dim, g.page_size) && g.layout == kLayoutCore)
     return g.head_dim <= 128 ? TreeTile{128, 256, 1, kPieceCost, true}
