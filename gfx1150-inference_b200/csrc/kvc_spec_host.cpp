@@ -260,11 +260,17 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     return shares + (cost > 0 ? 1 : 0);
   };
   // the smallest limit that needs no more shares than there are CTAs
-  int64_t lo = 1, hi = tiles + runs * pc + 1;
-  if (ctas > 0) lo = std::max<int64_t>(1, (tiles + runs * pc) / ctas);
+  auto fits = [&](int64_t limit) {
+    return walk(limit, [](int, int, int, int, int, int) {}, [] {}) <= ctas;
+  };
+  int64_t lo = 1, hi = 1;
+  if (ctas > 0) {
+    lo = std::max<int64_t>(1, (tiles + runs * pc) / ctas);
+    for (hi = (tiles + (runs + ctas) * pc) / ctas + 1; !fits(hi);) hi *= 2;
+  }
   while (lo < hi) {
     const int64_t mid = lo + (hi - lo) / 2;
-    if (walk(mid, [](int, int, int, int, int, int) {}, [] {}) <= ctas)
+    if (fits(mid))
       hi = mid;
     else
       lo = mid + 1;
@@ -274,7 +280,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   std::vector<int> cta_segs(1, 0), tok0(std::max(1, n_seqs), 0);
   for (int i = 1; i < n_seqs; ++i) tok0[i] = tok0[i - 1] + h_nodes[i - 1];
   walk(
-      lo,
+      hi,
       [&](int i, int kvh, int r0, int nr, int t, int take) {
         TreeSeg sg = {};
         sg.bt_row = h_rows ? h_rows[i] : i;

@@ -49,9 +49,9 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 // =====================================================================================
 // Tensor-core kernel.  One CTA per SM; each takes its share of the plan's position tiles.
 //
-// A tile of kTilePos positions of K and of V arrives by bulk copies, slab by slab, in the
-// pool's own layout: 8-position x 16-byte core matrices, which is the unswizzled
-// operand layout of tcgen05.mma, k-major for K (S = Q K^T) and mn-major for V (O = P V),
+// A tile of 128 positions (64 above head_dim 128) of K and of V arrives by bulk copies, slab
+// by slab, in the pool's own layout: 8-position x 16-byte core matrices, which is the
+// unswizzled operand layout of tcgen05.mma, k-major for K (S = Q K^T) and mn-major for V (O = P V),
 // so nothing is rearranged.  S, P and O live in tensor memory; P takes the place of its S.
 //
 // Two streams share the tensor cores, each with a softmax warpgroup whose thread r owns
@@ -65,9 +65,9 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 //
 // Warps: 0 and 2 bring K/V tiles into a ring of stages, 1 issues the MMAs, 3 loads each
 // piece's Q and looks through V tiles with drafted tokens, 4 ... 11 are the two softmax
-// warpgroups.  Every wait is bounded; a wait that gives up
-// raises the CTA's abort flag, all roles then run through their loops without waiting,
-// copying or issuing, and the kernel returns.
+// warpgroups.  Every wait is bounded; a wait that gives up raises the CTA's abort flag, all
+// roles then run through their loops without waiting, copying or issuing, and the kernel
+// returns.
 //
 // Measured on B200 (replayed passes; in parentheses the time of the bytes at the copy rate of
 // 6.46 TB/s): 32 sequences of 5-16 nodes at 1K-8K, fp16, 114 us (111); 8 x 12 at 32K,
@@ -170,15 +170,17 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     *s_abort = 0;
     s_dirty[0] = s_dirty[1] = -1;
   }
-  if (warp == 1) tmem_alloc(smem_u32(s_tmem), kTmemCols);
   // (the plan's records are no kernel's output: they may be read before the wait)
   const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
+  wait_prerequisites();
+  launch_dependents();
+  // Tensor memory is taken only here: a CTA that held it while it waits could keep a launch
+  // ahead of it from ever getting its own.
+  if (warp == 1) tmem_alloc(smem_u32(s_tmem), kTmemCols);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = *s_tmem;
-  wait_prerequisites();
-  launch_dependents();
 
   // false: some wait of this CTA gave up
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -200,315 +202,315 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
   // Registers move from the other warps to the softmax warpgroups: 128 x 104 + 256 x 200
   // is what 384 threads were launched with (168 each).
   if (warp < 4) {
-  if constexpr (S::kStreams == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == 0 || warp == 2) {
-    // ---- K/V tiles into the ring, in the order the MMAs take them: one warp issues the
-    // even entries, the other the odd ones (a tile of 16-position pages is eight copies,
-    // and issuing them takes a warp a quarter of the time that memory needs for them).
-    // A lane keeps the place of one slab: 32 slabs of page-table entries at a time, the
-    // next 32 on their way.
-    constexpr int kTileSlabs = KP / kSlab, kWinTiles = 32 / kTileSlabs;
-    const uint64_t policy = l2_policy_evict_first();
-    const int spp = a.p.page_size / kSlab;             // slabs of a page: neighbours are copied
-    const int run = spp % 8 == 0 ? 8 : spp % 4 == 0 ? 4 : spp % 2 == 0 ? 2 : 1;   // together
-    const uint32_t parity = warp >> 1;
-    uint32_t n = 0;  // ring entries so far
-    bool ok = true;
-    for (int si = seg0; si < seg1 && ok; ++si) {
-      const TreeSeg sg = a.segs[si];
-      const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
-      const int last_slab = (end - 1) / kSlab;
-      const int32_t* table = a.p.block_tables + static_cast<size_t>(sg.bt_row) * a.p.bt_stride;
-      auto entry_of = [&](int win) -> int {            // page-table entry of a window's slab
-        const int slab = (sg.tile0 + win * kWinTiles) * kTileSlabs + lane;
-        const int col = slab / spp;
-        return slab <= last_slab && col < a.p.bt_stride ? table[col] : -1;
-      };
-      int win = 0, now = entry_of(0), next = entry_of(1);
-      const int ahead = S::kStreams == 2 && sg.rows <= 128 ? 2 : 1;  // K runs this far ahead
-      for (int step = 0; step < tiles + ahead && ok; ++step) {
-        // step: V of tile step - ahead, then K of tile step
-        for (int kv = 1; kv >= 0 && ok; --kv) {
-          const int t = kv ? step - ahead : step;
-          if (t < 0 || t >= tiles) continue;
-          if ((n & 1) == parity) {
-            const int w = t / kWinTiles;
-            if (w != win) {
-              now = w == win + 1 ? next : entry_of(w);
-              next = entry_of(w + 1);
-              win = w;
-            }
-            const int slabs = min(kTileSlabs, last_slab + 1 - (sg.tile0 + t) * kTileSlabs);
-            int page = __shfl_sync(0xffffffffu, now, t % kWinTiles * kTileSlabs + (lane & (kTileSlabs - 1)));
-            const bool mine = lane < slabs && lane % run == 0;
-            const uint8_t* src = nullptr;
-            if (mine) {
-              if (page < 0 || page >= a.p.num_pages) {   // reported, and page 0 read instead
-                report_error_at(a.p.err, KVC_DEVERR_BAD_PAGE, static_cast<uint32_t>(page));
-                page = 0;
+    if constexpr (S::kStreams == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 0 || warp == 2) {
+      // ---- K/V tiles into the ring, in the order the MMAs take them: one warp issues the
+      // even entries, the other the odd ones (a tile of 16-position pages is eight copies,
+      // and issuing them takes a warp a quarter of the time that memory needs for them).
+      // A lane keeps the place of one slab: 32 slabs of page-table entries at a time, the
+      // next 32 on their way.
+      constexpr int kTileSlabs = KP / kSlab, kWinTiles = 32 / kTileSlabs;
+      const uint64_t policy = l2_policy_evict_first();
+      const int spp = a.p.page_size / kSlab;             // slabs of a page: neighbours are copied
+      const int run = spp % 8 == 0 ? 8 : spp % 4 == 0 ? 4 : spp % 2 == 0 ? 2 : 1;   // together
+      const uint32_t parity = warp >> 1;
+      uint32_t n = 0;  // ring entries so far
+      bool ok = true;
+      for (int si = seg0; si < seg1 && ok; ++si) {
+        const TreeSeg sg = a.segs[si];
+        const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
+        const int last_slab = (end - 1) / kSlab;
+        const int32_t* table = a.p.block_tables + static_cast<size_t>(sg.bt_row) * a.p.bt_stride;
+        auto entry_of = [&](int win) -> int {            // page-table entry of a window's slab
+          const int slab = (sg.tile0 + win * kWinTiles) * kTileSlabs + lane;
+          const int col = slab / spp;
+          return slab <= last_slab && col < a.p.bt_stride ? table[col] : -1;
+        };
+        int win = 0, now = entry_of(0), next = entry_of(1);
+        const int ahead = S::kStreams == 2 && sg.rows <= 128 ? 2 : 1;  // K runs this far ahead
+        for (int step = 0; step < tiles + ahead && ok; ++step) {
+          // step: V of tile step - ahead, then K of tile step
+          for (int kv = 1; kv >= 0 && ok; --kv) {
+            const int t = kv ? step - ahead : step;
+            if (t < 0 || t >= tiles) continue;
+            if ((n & 1) == parity) {
+              const int w = t / kWinTiles;
+              if (w != win) {
+                now = w == win + 1 ? next : entry_of(w);
+                next = entry_of(w + 1);
+                win = w;
               }
-              const int slab = (sg.tile0 + t) * kTileSlabs + lane;
-              src = (kv ? a.p.v : a.p.k) +
-                    (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) * a.p.page_head_bytes +
-                    slab % spp * kSlabBytes;
+              const int slabs = min(kTileSlabs, last_slab + 1 - (sg.tile0 + t) * kTileSlabs);
+              int page = __shfl_sync(0xffffffffu, now, t % kWinTiles * kTileSlabs + (lane & (kTileSlabs - 1)));
+              const bool mine = lane < slabs && lane % run == 0;
+              const uint8_t* src = nullptr;
+              if (mine) {
+                if (page < 0 || page >= a.p.num_pages) {   // reported, and page 0 read instead
+                  report_error_at(a.p.err, KVC_DEVERR_BAD_PAGE, static_cast<uint32_t>(page));
+                  page = 0;
+                }
+                const int slab = (sg.tile0 + t) * kTileSlabs + lane;
+                src = (kv ? a.p.v : a.p.k) +
+                      (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) * a.p.page_head_bytes +
+                      slab % spp * kSlabBytes;
+              }
+              const int st = n % S::kStages;
+              if (n >= S::kStages) ok = wait(empty(st), (n / S::kStages - 1) & 1);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              if (lane == 0) mbar_arrive_expect_tx(full(st), slabs * kSlabBytes);
+              __syncwarp();
+              if (mine)
+                bulk_g2s(smem_u32(stage_mem) + st * S::kStageBytes + lane * kSlabBytes, src,
+                         min(run, slabs - lane) * kSlabBytes, full(st), policy);
             }
-            const int st = n % S::kStages;
-            if (n >= S::kStages) ok = wait(empty(st), (n / S::kStages - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(full(st), slabs * kSlabBytes);
-            __syncwarp();
-            if (mine)
-              bulk_g2s(smem_u32(stage_mem) + st * S::kStageBytes + lane * kSlabBytes, src,
-                       min(run, slabs - lane) * kSlabBytes, full(st), policy);
+            ++n;
           }
-          ++n;
         }
       }
-    }
-    if (!ok) {  // copies in flight land before the CTA's memory goes
-      for (uint32_t i = n > 2 * S::kStages ? n - 2 * S::kStages : 0; i < n; ++i)
-        if ((i & 1) == parity) mbar_wait_bounded(full(i % S::kStages), (i / S::kStages) & 1);
-    }
-  } else if (warp == 1) {
-    // ---- MMAs: the warp waits together, one lane issues.  Everything an MMA takes is
-    // the same in all lanes (broadcast where the compiler could not tell), so it sits in
-    // uniform registers: with operands in ordinary ones an issue took over 100 cycles,
-    // twice as long as the MMA itself.
-    constexpr uint32_t kDescS = mma_desc<T>(128, KP, false);
-    constexpr uint32_t kDescO = mma_desc<T>(128, D, true);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    const uint64_t q_desc = operand_desc(smem_u32(q_mem), 128, U * 128);
-    const uint64_t k_desc = operand_desc(smem_u32(stage_mem), 128, U * 128);
-    const uint64_t v_desc = operand_desc(smem_u32(stage_mem), U * 128, 128);
-    const bool leader = elect_one();
-    uint32_t n = 0;                       // ring tiles consumed
-    uint32_t np[2] = {0, 0}, nq = 0, ng = 0, ne = 0;
-    bool ok = true;
-    auto wait_all = [&](uint32_t bar, uint32_t parity) {
-      ok = __all_sync(0xffffffffu, ok && wait(bar, parity));
-    };
-    auto take = [&]() -> int {            // the next tile of the ring
-      const int st = n % S::kStages;
-      wait_all(full(st), (n / S::kStages) & 1);
-      ++n;
-      return st;
-    };
-    auto commit = [&](uint32_t bar) {
-      if (leader) mma_commit(bar);
-    };
-    auto scores = [&](int x, int st) {    // S_x = Q_x K^T
-      const uint64_t qd = q_desc + x * (S::kQBytes / 16), kd = k_desc + st * (S::kStageBytes / 16);
-      if (leader) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)  // 16 dims: two core matrices on
-          mma_ss(tm + x * 128, qd + 16 * k, kd + 16 * k, kDescS, k > 0);
-        mma_commit(s_ready(x));
+      if (!ok) {  // copies in flight land before the CTA's memory goes
+        for (uint32_t i = n > 2 * S::kStages ? n - 2 * S::kStages : 0; i < n; ++i)
+          if ((i & 1) == parity) mbar_wait_bounded(full(i % S::kStages), (i / S::kStages) & 1);
       }
-    };
-    auto sums = [&](int x, int st, int slabs, bool accumulate) {   // O_x += P_x V
-      const uint64_t vd = v_desc + st * (S::kStageBytes / 16);
-      if (leader) {
-        if (slabs == KP / kSlab) {
-#pragma unroll
-          for (int k = 0; k < KP / kSlab; ++k)
-            mma_ts(tm + 256 + x * 128, tm + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
-                   accumulate || k > 0);
-        } else {
-#pragma unroll 1
-          for (int k = 0; k < slabs; ++k)
-            mma_ts(tm + 256 + x * 128, tm + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
-                   accumulate || k > 0);
-        }
-      }
-    };
-    for (int si = seg0; si < seg1 && ok; ++si) {
-      const TreeSeg sg = a.segs[si];
-      const int tiles = __shfl_sync(0xffffffffu, sg.tile1 - sg.tile0, 0);
-      const int left = __shfl_sync(0xffffffffu, sg.ctx + sg.nodes - sg.tile0 * KP, 0);
-      const bool two = __shfl_sync(0xffffffffu, sg.rows, 0) > 128;
-      const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-      const int edge0 = __shfl_sync(0xffffffffu, sg.ctx - sg.tile0 * KP, 0);
-      auto slabs_of = [&](int t) { return min(KP / kSlab, (left - t * KP + kSlab - 1) / kSlab); };
-      auto is_edge = [&](int t) { return (t + 1) * KP > edge0; };
-      // K of tile t is here: when the tile holds drafted positions the helper warps may
-      // take its V on, which the sums then wait for
-      auto take_k = [&](int t) {
-        const int st = take();
-        if (is_edge(t)) {
-          if (ok && leader) mbar_arrive(edge_go(ng));
-          ++ng;
-        }
+    } else if (warp == 1) {
+      // ---- MMAs: the warp waits together, one lane issues.  Everything an MMA takes is
+      // the same in all lanes (broadcast where the compiler could not tell), so it sits in
+      // uniform registers: with operands in ordinary ones an issue took over 100 cycles,
+      // twice as long as the MMA itself.
+      constexpr uint32_t kDescS = mma_desc<T>(128, KP, false);
+      constexpr uint32_t kDescO = mma_desc<T>(128, D, true);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t q_desc = operand_desc(smem_u32(q_mem), 128, U * 128);
+      const uint64_t k_desc = operand_desc(smem_u32(stage_mem), 128, U * 128);
+      const uint64_t v_desc = operand_desc(smem_u32(stage_mem), U * 128, 128);
+      const bool leader = elect_one();
+      uint32_t n = 0;                       // ring tiles consumed
+      uint32_t np[2] = {0, 0}, nq = 0, ng = 0, ne = 0;
+      bool ok = true;
+      auto wait_all = [&](uint32_t bar, uint32_t parity) {
+        ok = __all_sync(0xffffffffu, ok && wait(bar, parity));
+      };
+      auto take = [&]() -> int {            // the next tile of the ring
+        const int st = n % S::kStages;
+        wait_all(full(st), (n / S::kStages) & 1);
+        ++n;
         return st;
       };
-      auto edge_wait = [&](int t) {
-        if (is_edge(t)) {
-          wait_all(edge_done(ne), (ne >> 1) & 1);
-          ++ne;
+      auto commit = [&](uint32_t bar) {
+        if (leader) mma_commit(bar);
+      };
+      auto scores = [&](int x, int st) {    // S_x = Q_x K^T
+        const uint64_t qd = q_desc + x * (S::kQBytes / 16), kd = k_desc + st * (S::kStageBytes / 16);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)  // 16 dims: two core matrices on
+            mma_ss(tm + x * 128, qd + 16 * k, kd + 16 * k, kDescS, k > 0);
+          mma_commit(s_ready(x));
         }
       };
-      wait_all(q_ready, nq++ & 1);
-      if (two) {
-        int kst = take_k(0);
-        if (!ok) break;
-        scores(0, kst);
-        scores(1, kst);
-        commit(empty(kst));
-        if (tiles == 1) commit(q_free);
-        for (int t = 0; t < tiles && ok; ++t) {
-          const int vst = take();
-          edge_wait(t);
+      auto sums = [&](int x, int st, int slabs, bool accumulate) {   // O_x += P_x V
+        const uint64_t vd = v_desc + st * (S::kStageBytes / 16);
+        if (leader) {
+          if (slabs == KP / kSlab) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            wait_all(p_ready(x), np[x]++ & 1);
-            if (!ok) break;
-            tmem_fence_after();
-            sums(x, vst, slabs_of(t), t > 0);
-            if (x == 1) commit(empty(vst));
-            if (t + 1 == tiles) commit(o_ready(x));
-            if (t + 1 < tiles) {
-              if (x == 0) kst = take_k(t + 1);
-              if (!ok) break;
-              scores(x, kst);
-              if (x == 1) commit(empty(kst));
-              if (x == 1 && t + 2 == tiles) commit(q_free);
-            }
+            for (int k = 0; k < KP / kSlab; ++k)
+              mma_ts(tm + 256 + x * 128, tm + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
+                     accumulate || k > 0);
+          } else {
+#pragma unroll 1
+            for (int k = 0; k < slabs; ++k)
+              mma_ts(tm + 256 + x * 128, tm + x * 128 + 8 * k, vd + (kSlabBytes / 16) * k, kDescO,
+                     accumulate || k > 0);
           }
         }
-      } else {
-        for (int x = 0; x < ahead && x < tiles && ok; ++x) {
-          const int kst = take_k(x);
+      };
+      for (int si = seg0; si < seg1 && ok; ++si) {
+        const TreeSeg sg = a.segs[si];
+        const int tiles = __shfl_sync(0xffffffffu, sg.tile1 - sg.tile0, 0);
+        const int left = __shfl_sync(0xffffffffu, sg.ctx + sg.nodes - sg.tile0 * KP, 0);
+        const bool two = __shfl_sync(0xffffffffu, sg.rows, 0) > 128;
+        const int ahead = S::kStreams == 2 && !two ? 2 : 1;
+        const int edge0 = __shfl_sync(0xffffffffu, sg.ctx - sg.tile0 * KP, 0);
+        auto slabs_of = [&](int t) { return min(KP / kSlab, (left - t * KP + kSlab - 1) / kSlab); };
+        auto is_edge = [&](int t) { return (t + 1) * KP > edge0; };
+        // K of tile t is here: when the tile holds drafted positions the helper warps may
+        // take its V on, which the sums then wait for
+        auto take_k = [&](int t) {
+          const int st = take();
+          if (is_edge(t)) {
+            if (ok && leader) mbar_arrive(edge_go(ng));
+            ++ng;
+          }
+          return st;
+        };
+        auto edge_wait = [&](int t) {
+          if (is_edge(t)) {
+            wait_all(edge_done(ne), (ne >> 1) & 1);
+            ++ne;
+          }
+        };
+        wait_all(q_ready, nq++ & 1);
+        if (two) {
+          int kst = take_k(0);
           if (!ok) break;
-          scores(x, kst);
+          scores(0, kst);
+          scores(1, kst);
           commit(empty(kst));
-          if (x + 1 == tiles) commit(q_free);
-        }
-        for (int t = 0; t < tiles && ok; ++t) {
-          const int x = ahead == 2 ? t & 1 : 0;
-          const int vst = take();
-          edge_wait(t);
-          wait_all(p_ready(x), np[x]++ & 1);
-          if (!ok) break;
-          tmem_fence_after();
-          sums(x, vst, slabs_of(t), t >= ahead);
-          commit(empty(vst));
-          if (t + ahead < tiles) {
-            const int kst = take_k(t + ahead);
+          if (tiles == 1) commit(q_free);
+          for (int t = 0; t < tiles && ok; ++t) {
+            const int vst = take();
+            edge_wait(t);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              wait_all(p_ready(x), np[x]++ & 1);
+              if (!ok) break;
+              tmem_fence_after();
+              sums(x, vst, slabs_of(t), t > 0);
+              if (x == 1) commit(empty(vst));
+              if (t + 1 == tiles) commit(o_ready(x));
+              if (t + 1 < tiles) {
+                if (x == 0) kst = take_k(t + 1);
+                if (!ok) break;
+                scores(x, kst);
+                if (x == 1) commit(empty(kst));
+                if (x == 1 && t + 2 == tiles) commit(q_free);
+              }
+            }
+          }
+        } else {
+          for (int x = 0; x < ahead && x < tiles && ok; ++x) {
+            const int kst = take_k(x);
             if (!ok) break;
             scores(x, kst);
             commit(empty(kst));
-            if (t + ahead + 1 == tiles) commit(q_free);
-          } else {
-            commit(o_ready(x));
+            if (x + 1 == tiles) commit(q_free);
           }
-        }
-      }
-    }
-    if (!ok && leader) {  // MMAs in flight end before tensor memory is freed
-      mbar_init(bar0 + 8u * 40, 1);
-      fence_mbar_init();
-      mma_commit(bar0 + 8u * 40);
-      mbar_wait_bounded(bar0 + 8u * 40, 0);
-    }
-    __syncwarp();
-  } else {
-    // ---- helper: each piece's Q, and the V tiles that hold drafted positions --------------
-    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-    uint32_t ring = 0, nf = 0, ng = 0;
-    bool ok = true;
-    for (int si = seg0; si < seg1; ++si) {
-      const TreeSeg sg = a.segs[si];
-      const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
-      const bool two = sg.rows > 128;
-      const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-      // Q in k-major core matrices, all its copies in flight together: a warp's copy covers
-      // 8 rows x 64 bytes, rows past the block are zero.  Streams that share their rows get
-      // a copy each.
-      if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
-      if (ok) {
-        const int rr = lane >> 2, uu = lane & 3;
-        const int n_rows = two ? 256 : 128;
-        // node and head of row g0 + rr, carried along (a division takes as long as the copies)
-        int node = (sg.row0 + rr) / a.group, rem = sg.row0 + rr - node * a.group;
-        const int dn = 8 / a.group, dr = 8 - dn * a.group;
-        const T* base = reinterpret_cast<const T*>(a.q) +
-                        (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D + uu * 8;
-        const int row_step = a.num_heads * D;
-        const uint32_t dst0 = smem_u32(q_mem) + rr * 16 + uu * 128;
-#pragma unroll 2
-        for (int g0 = 0; g0 < n_rows; g0 += 8) {
-          const bool there = g0 + rr < sg.rows;
-          const T* src = there ? base + static_cast<size_t>(node) * row_step + rem * D : base;
-          const uint32_t dst = dst0 + (g0 >> 7) * S::kQBytes + ((g0 & 127) >> 3) * U * 128;
-#pragma unroll
-          for (int i = 0; i < U / 4; ++i) {
-            copy16_async(dst + i * 512, src + i * 32, there ? 16 : 0);
-            if (S::kStreams == 2 && !two) copy16_async(dst + S::kQBytes + i * 512, src + i * 32, there ? 16 : 0);
-          }
-          node += dn;
-          rem += dr;
-          if (rem >= a.group) {
-            rem -= a.group;
-            ++node;
-          }
-        }
-        copy_async_wait();
-        if (flip) {   // a negative scale turns q
-          for (int i = lane; i < S::kStreams * S::kQBytes / 4; i += 32)
-            reinterpret_cast<uint32_t*>(q_mem)[i] ^= flip;
-        }
-      }
-      fence_proxy_async();
-      mbar_arrive(q_ready);
-      // V of drafted tokens: what is not finite would spread through zero weights to rows
-      // that do not see it, so it leaves the tile here (and comes back at the end, to the
-      // rows that do); positions past the end hold anything, and go to zero.
-      for (int t = max(0, sg.ctx / KP - sg.tile0); t < tiles; ++t) {
-        const int p0 = (sg.tile0 + t) * KP;
-        ok = ok && wait(edge_go(ng), (ng >> 1) & 1);
-        // ring order of the piece: `ahead` K tiles, then V t, K t + ahead, ...
-        const uint32_t vi = ring + t + min(ahead + t, tiles);
-        const int st = vi % S::kStages;
-        ok = ok && wait(full(st), (vi / S::kStages) & 1);
-        if (ok) {
-          uint8_t* vt = stage_mem + st * S::kStageBytes;
-          const int from = max(0, sg.ctx - p0), to = min(KP, (end - p0 + kSlab - 1) / kSlab * kSlab);
-          bool dirty = false;
-          auto cell = [&](int i) {
-            const int pt = i / U, u = i - pt * U;
-            return reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
-          };
-          const int live = min(to, end - p0) * U;      // units of drafted positions
-          for (int i0 = from * U + lane; i0 < live; i0 += 4 * 32) {
-            uint4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              v[k] = i0 + 32 * k < live ? *cell(i0 + 32 * k) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (!(maybe_odd<T>(v[k].x) || maybe_odd<T>(v[k].y) || maybe_odd<T>(v[k].z) ||
-                    maybe_odd<T>(v[k].w)))
-                continue;
-              uint32_t e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                if (not_finite<T>(e[w] & 0xffffu)) e[w] &= 0xffff0000u, dirty = true;
-                if (not_finite<T>(e[w] >> 16)) e[w] &= 0x0000ffffu, dirty = true;
-              }
-              *cell(i0 + 32 * k) = make_uint4(e[0], e[1], e[2], e[3]);
+          for (int t = 0; t < tiles && ok; ++t) {
+            const int x = ahead == 2 ? t & 1 : 0;
+            const int vst = take();
+            edge_wait(t);
+            wait_all(p_ready(x), np[x]++ & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            sums(x, vst, slabs_of(t), t >= ahead);
+            commit(empty(vst));
+            if (t + ahead < tiles) {
+              const int kst = take_k(t + ahead);
+              if (!ok) break;
+              scores(x, kst);
+              commit(empty(kst));
+              if (t + ahead + 1 == tiles) commit(q_free);
+            } else {
+              commit(o_ready(x));
             }
           }
-          for (int i = live + lane; i < to * U; i += 32) *cell(i) = make_uint4(0, 0, 0, 0);
-          if (dirty) s_dirty[si & 1] = si;
         }
-        __threadfence_block();
-        fence_proxy_async();
-        mbar_arrive(edge_done(ng));
-        ++ng;
       }
-      ring += 2 * tiles;
+      if (!ok && leader) {  // MMAs in flight end before tensor memory is freed
+        mbar_init(bar0 + 8u * 40, 1);
+        fence_mbar_init();
+        mma_commit(bar0 + 8u * 40);
+        mbar_wait_bounded(bar0 + 8u * 40, 0);
+      }
+      __syncwarp();
+    } else {
+      // ---- helper: each piece's Q, and the V tiles that hold drafted positions --------------
+      const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+      uint32_t ring = 0, nf = 0, ng = 0;
+      bool ok = true;
+      for (int si = seg0; si < seg1; ++si) {
+        const TreeSeg sg = a.segs[si];
+        const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
+        const bool two = sg.rows > 128;
+        const int ahead = S::kStreams == 2 && !two ? 2 : 1;
+        // Q in k-major core matrices, all its copies in flight together: a warp's copy covers
+        // 8 rows x 64 bytes, rows past the block are zero.  Streams that share their rows get
+        // a copy each.
+        if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
+        if (ok) {
+          const int rr = lane >> 2, uu = lane & 3;
+          const int n_rows = two ? 256 : 128;
+          // node and head of row g0 + rr, carried along (a division takes as long as the copies)
+          int node = (sg.row0 + rr) / a.group, rem = sg.row0 + rr - node * a.group;
+          const int dn = 8 / a.group, dr = 8 - dn * a.group;
+          const T* base = reinterpret_cast<const T*>(a.q) +
+                          (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D + uu * 8;
+          const int row_step = a.num_heads * D;
+          const uint32_t dst0 = smem_u32(q_mem) + rr * 16 + uu * 128;
+#pragma unroll 2
+          for (int g0 = 0; g0 < n_rows; g0 += 8) {
+            const bool there = g0 + rr < sg.rows;
+            const T* src = there ? base + static_cast<size_t>(node) * row_step + rem * D : base;
+            const uint32_t dst = dst0 + (g0 >> 7) * S::kQBytes + ((g0 & 127) >> 3) * U * 128;
+#pragma unroll
+            for (int i = 0; i < U / 4; ++i) {
+              copy16_async(dst + i * 512, src + i * 32, there ? 16 : 0);
+              if (S::kStreams == 2 && !two) copy16_async(dst + S::kQBytes + i * 512, src + i * 32, there ? 16 : 0);
+            }
+            node += dn;
+            rem += dr;
+            if (rem >= a.group) {
+              rem -= a.group;
+              ++node;
+            }
+          }
+          copy_async_wait();
+          if (flip) {   // a negative scale turns q
+            for (int i = lane; i < S::kStreams * S::kQBytes / 4; i += 32)
+              reinterpret_cast<uint32_t*>(q_mem)[i] ^= flip;
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(q_ready);
+        // V of drafted tokens: what is not finite would spread through zero weights to rows
+        // that do not see it, so it leaves the tile here (and comes back at the end, to the
+        // rows that do); positions past the end hold anything, and go to zero.
+        for (int t = max(0, sg.ctx / KP - sg.tile0); t < tiles; ++t) {
+          const int p0 = (sg.tile0 + t) * KP;
+          ok = ok && wait(edge_go(ng), (ng >> 1) & 1);
+          // ring order of the piece: `ahead` K tiles, then V t, K t + ahead, ...
+          const uint32_t vi = ring + t + min(ahead + t, tiles);
+          const int st = vi % S::kStages;
+          ok = ok && wait(full(st), (vi / S::kStages) & 1);
+          if (ok) {
+            uint8_t* vt = stage_mem + st * S::kStageBytes;
+            const int from = max(0, sg.ctx - p0), to = min(KP, (end - p0 + kSlab - 1) / kSlab * kSlab);
+            bool dirty = false;
+            auto cell = [&](int i) {
+              const int pt = i / U, u = i - pt * U;
+              return reinterpret_cast<uint4*>(vt + (pt >> 3) * U * 128 + u * 128 + (pt & 7) * 16);
+            };
+            const int live = min(to, end - p0) * U;      // units of drafted positions
+            for (int i0 = from * U + lane; i0 < live; i0 += 4 * 32) {
+              uint4 v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                v[k] = i0 + 32 * k < live ? *cell(i0 + 32 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (!(maybe_odd<T>(v[k].x) || maybe_odd<T>(v[k].y) || maybe_odd<T>(v[k].z) ||
+                      maybe_odd<T>(v[k].w)))
+                  continue;
+                uint32_t e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                  if (not_finite<T>(e[w] & 0xffffu)) e[w] &= 0xffff0000u, dirty = true;
+                  if (not_finite<T>(e[w] >> 16)) e[w] &= 0x0000ffffu, dirty = true;
+                }
+                *cell(i0 + 32 * k) = make_uint4(e[0], e[1], e[2], e[3]);
+              }
+            }
+            for (int i = live + lane; i < to * U; i += 32) *cell(i) = make_uint4(0, 0, 0, 0);
+            if (dirty) s_dirty[si & 1] = si;
+          }
+          __threadfence_block();
+          fence_proxy_async();
+          mbar_arrive(edge_done(ng));
+          ++ng;
+        }
+        ring += 2 * tiles;
+      }
     }
-  }
   } else {
     if constexpr (S::kStreams == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---- softmax: thread r of stream x owns row r ---------------------------------------------
@@ -1323,7 +1325,8 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
 // fp32: the larger tiles do 64 FMAs for 8 shared-memory reads (27 TFLOP/s where the small
 // ones reach 10, 32 drafted tokens of 4 sequences at 4000), the small ones start sooner and
 // spread further (14.8 against 17.3 us, 4 tokens of one sequence at 511, both with the join
-// as it was then, 1.3 us slower): they are taken while all of their tiles find a place on the GPU at once.
+// as it was then, 1.3 us slower): they are taken while all of their tiles find a place on
+// the GPU at once.
 TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms) {
   if (decode_uses_mma(g.dtype, g.head_dim, g.page_size) && g.layout == kLayoutCore)
     return g.head_dim <= 128 ? TreeTile{128, 256, 1, kPieceCost, true}

@@ -522,7 +522,7 @@ def check_select(logits, scores, n_out, sel=None):
     got = best.double().cpu().numpy()
     fin = np.isfinite(rs)
     assert np.array_equal(fin, np.isfinite(got)) and np.all(got[~fin] == -np.inf)
-    assert np.all(np.abs(got - rs)[fin] <= 2.0 ** -20 + 2.0 ** -24 * np.abs(rs[fin]))
+    assert np.all(np.abs(got[fin] - rs[fin]) <= 2.0 ** -20 + 2.0 ** -24 * np.abs(rs[fin]))
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
