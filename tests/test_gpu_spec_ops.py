@@ -345,6 +345,63 @@ def test_tree_graph_streams_and_repeats(dtype):
     assert torch.equal(a, b) and torch.equal(a, c)
 
 
+@pytest.mark.parametrize("d", [32, 128])
+def test_tree_on_two_streams_at_once(d):
+    """Two plans on two streams share the SMs and their tensor memory."""
+    pool = make_pool(1, 512, 16, 4, d, F16, fill=0.0)
+    pool.fill_normal(seed=9)
+    bt = dev(np.random.default_rng(1).permutation(512).reshape(4, 128))
+    qs = [torch.randn(n, 16, d, device="cuda").half() for n in (4 * 20, 4 * 63)]
+    plans = [pool.plan_tree([1900, 700, 33, 1200], [n] * 4, 16) for n in (20, 63)]
+    want = [torch.zeros_like(q) for q in qs]
+    for p, q, o in zip(plans, qs, want):
+        pool.decode_tree(p, 0, q, None, o, bt, 0.1)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [torch.zeros_like(q) for q in qs]
+    for _ in range(30):
+        for st, p, q, o in zip(streams, plans, qs, got):
+            pool.decode_tree(p, 0, q, None, o, bt, 0.1, stream=st)
+    no_error()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_pages_past_four_gigabytes():
+    """Every operator on pages whose byte offsets need more than 32 bits."""
+    pages, ps, hkv, d = 140000, 16, 8, 128                  # 4.6 GB of K, and of V
+    pool = paged.PagedKVCache(1, pages, ps, hkv, d)
+    ctx, n, h = 100, 20, 32
+    table = np.arange(pages - 8, pages, dtype=np.int32)[::-1].copy().reshape(1, 8)
+    bt = dev(table)
+    k = torch.randn(ctx + n, hkv, d, device="cuda").half()
+    v = torch.randn(ctx + n, hkv, d, device="cuda").half()
+    q = torch.randn(n, h, d, device="cuda").half()
+    pos = torch.arange(ctx + n, dtype=torch.int32, device="cuda")
+    zero = torch.zeros_like(pos)
+    # angle 0 leaves the rows as they are
+    pool.append_rope(0, None, k, v, bt, pos, rope_positions=zero)
+    gk, gv = pool.gather(0, bt, 0, 0, ctx + n)
+    assert torch.equal(gk, k) and torch.equal(gv, v)
+    out = torch.zeros_like(q)
+    pool.decode_tree(pool.plan_tree([ctx], [n], h), 0, q, None, out, bt, 0.09)
+    low = paged.PagedKVCache(1, 8, ps, hkv, d)
+    bt2, want = dev(np.arange(8).reshape(1, 8)), torch.zeros_like(q)
+    low.append_rope(0, None, k, v, bt2, pos, rope_positions=zero)
+    low.decode_tree(low.plan_tree([ctx], [n], h), 0, q, None, want, bt2, 0.09)
+    no_error()
+    assert torch.equal(out, want)
+    pool.commit_tree(bt, dev([ctx]), dev([[3, 7, 19]]), dev([3]))
+    gk, _ = pool.gather(0, bt, 0, ctx, 3)
+    assert torch.equal(gk, k[[ctx + 3, ctx + 7, ctx + 19]])
+    beams = dev(np.arange(pages - 8, pages).reshape(2, 4))   # rows of 4 pages, 37 positions
+    old = [pool.gather(0, beams, r, 0, 37) for r in range(2)]
+    pool.reorder_beams(beams, dev([[1, 0]]), dev([37]))
+    for r in range(2):
+        for x, y in zip(old[1 - r], pool.gather(0, beams, r, 0, 37)):
+            assert torch.equal(x, y)
+    no_error()
+
+
 def test_tree_bad_page_is_reported():
     pool = make_pool(1, 8, 16, 2, 64, F16, fill=0.0)
     bt = dev([[0, 99, 2, 3]])
