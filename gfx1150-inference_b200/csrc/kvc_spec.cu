@@ -64,15 +64,16 @@ __device__ __forceinline__ void rotate(T& x0, T& x1, float2 cs) {
 // pairs (units 2i, 2i + 1, or i and i + half the row for NeoX), keeps their angles in
 // registers and goes through the heads of q, K and V, kAppendBatch of them on their way;
 // the first are asked for before the angles are computed.  Bound by memory traffic: 8,895
-// tokens of 32 + 8 + 8 heads of 128 dims, bf16, 48 us for 219 MB (a plain copy of as many
+// tokens of 32 + 8 + 8 heads of 128 dims, bf16, 45 us for 219 MB (a plain copy of as many
 // bytes takes 37); the pool's layout puts a row's pieces 128 bytes apart, which costs 4 us
-// of it.  64 threads per token measured best of 32, 64, 128 and 256.
+// of it.  64 threads per token measured best of 32, 64, 128 and 256, and four CTAs of two
+// pairs a thread better than three of three (47 us).
 // =====================================================================================
 constexpr int kAppendThreads = 256;
-constexpr int kAppendBatch = 3;
+constexpr int kAppendBatch = 2;
 
 template <typename T, bool kNeox, int kPer>
-__global__ void __launch_bounds__(kAppendThreads) append_rope_kernel(const AppendRopeArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 4) append_rope_kernel(const AppendRopeArgs a) {
   constexpr int kTok = kAppendThreads / kPer;
   __shared__ float2 cs[kTok * kMaxRopePairs];
   __shared__ int s_page[kTok], s_slot[kTok];
