@@ -62,6 +62,10 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 //
 // O is rescaled only when a row's max has grown by more than 2^8 since the last time: the
 // probabilities then stay below 2^8 and a tile normally touches O with the MMA alone.
+// fp16 probabilities are 2^7 times that, at most 2^15: fp16 keeps 11 bits of those down to
+// 2^-21 of the row's largest, and of smaller ones all but 2^-32 of it, so a flat tail of
+// 10^5 positions far below one peak loses less than the output's rounding.  As 2^-14 and
+// 2^-25 (without the factor) it lost a hundredth of the output and more.
 //
 // Warps: 0 and 2 bring K/V tiles into a ring of stages, 1 issues the MMAs, 3 loads each
 // piece's Q and looks through V tiles with drafted tokens, 4 ... 11 are the two softmax
@@ -81,6 +85,9 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int 
 // =====================================================================================
 constexpr int kTmemCols = 512;
 constexpr float kRescaleAt = 8.0f;   // log2
+// log2 of the factor on the probabilities of a storage type (bf16 has fp32's exponents).
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr int kPieceCost = 4;        // a piece's start and end, in tiles
 
 template <int D>
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const bool joint = ahead == 2;
       const int row = (two ? x * 128 : 0) + r;
       const bool live = (two ? x * 128 : 0) + w4 * 32 < seg->rows;   // some row of the warp
-      float m = kNegBig, l = 0.f;     // max in log2 units
+      float m = kNegBig, l = 0.f;     // max in log2 units, less kLift
       // One tile of the stream: scores to probabilities, in place, and the running max and
       // sum.  Edge tiles hold positions that some rows do not see.
       auto softmax = [&](auto edge_tag, int t, const uint32_t* vis) {
@@ -576,7 +583,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
             }
           }
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          mt = mx == -INFINITY ? kNegBig : mx * sc;
+          mt = mx == -INFINITY ? kNegBig : mx * sc - kLift<T>;
         };
         if (t < ahead) {
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -591,7 +598,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
               if (!kEdge || ((vis[w] >> i) & 1u)) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[i]));
           }
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          m = mx == -INFINITY ? kNegBig : mx * sc;
+          m = mx == -INFINITY ? kNegBig : mx * sc - kLift<T>;
         }
         for (;;) {
           pass();
