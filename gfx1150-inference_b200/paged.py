@@ -402,6 +402,8 @@ class PagedKVCache:
         if mask.dim() != 2:
             raise ValueError("mask must be (tokens, words)")
         words = mask.shape[1]
+        if words == 0 and tokens:   # (its address is null, which the library takes for a chain)
+            raise ValueError("a mask needs at least one word per token")
         return _on(mask, "mask", torch.int32, tokens * words, self.device), words
 
     def _table(self, block_tables: torch.Tensor, plan: TreePlan) -> None:
