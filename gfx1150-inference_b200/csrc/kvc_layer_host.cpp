@@ -17,6 +17,8 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <cmath>
+
 #include "kvc_common.h"
 #include "kvc_internal.h"
 #include "kvc_spec.h"
@@ -402,12 +404,14 @@ extern "C" int kvc_forward_layer_tree(
     int intermediate_size, float rms_norm_eps, float rope_freq_base, int rope_neox, float scale,
     void* stream) {
   if (!pool || !plan) return set_error(KVC_ERR_INVALID_ARG, "pool and plan must not be null.");
-  if (!plan->valid) return set_error(KVC_ERR_INVALID_ARG, "plan has not been built.");
+  // (everything is checked before the first launch: a refused call leaves the cache alone)
+  if (const int rc = check_tree_call(pool, plan, layer_idx, d_mask, mask_words, bt_stride, scale))
+    return rc;
   const PoolGeom& g = pool->g;
   if (g.dtype != KVC_DTYPE_F16)
     return set_error(KVC_ERR_INVALID_ARG, "the layer pipeline needs an fp16 KV pool.");
-  if (layer_idx < 0 || layer_idx >= g.num_layers)
-    return set_error(KVC_ERR_OUT_OF_RANGE, "layer_idx out of range for the KV pool.");
+  if (!(rope_freq_base > 0.0f) || !std::isfinite(rope_freq_base))
+    return set_error(KVC_ERR_INVALID_ARG, "freq_base must be positive.");
   LayerDims d;
   d.layer = layer_idx;
   d.seq = plan->n_tokens;
@@ -431,6 +435,8 @@ extern "C" int kvc_forward_layer_tree(
   LayerIO io;
   for (int i = 0; i < 7; ++i) {
     if (!w[i]) return set_error(KVC_ERR_INVALID_ARG, "weight buffers must not be null.");
+    if (reinterpret_cast<uintptr_t>(w[i]) & 15u)
+      return set_error(KVC_ERR_INVALID_ARG, "weights must be 16-byte aligned.");
     io.w[i] = w[i];
     io.type[i] = types[i];
   }

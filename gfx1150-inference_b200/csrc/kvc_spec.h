@@ -149,6 +149,9 @@ int do_append_rope(kvc_pool* pool, int layer, const void* d_q, int q_stride, voi
                    const int32_t* d_rows, const int32_t* d_positions,
                    const int32_t* d_rope_positions, int n, float freq_base, int neox,
                    cudaStream_t s);
+// The plan, the layer and the sizes of a call, before anything of it is launched.
+int check_tree_call(const kvc_pool* pool, const kvc_tree_plan* plan, int layer,
+                    const int32_t* d_mask, int mask_words, int bt_stride, float scale);
 int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
                    const int32_t* d_mask, int mask_words, void* d_out, const int32_t* d_bt,
                    int bt_stride, float scale, cudaStream_t s);

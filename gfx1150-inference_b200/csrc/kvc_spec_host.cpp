@@ -132,9 +132,8 @@ int do_append_rope(kvc_pool* pool, int layer, const void* d_q, int q_stride, voi
   return e == cudaSuccess ? KVC_OK : cuda_error(e, "append + rope kernel");
 }
 
-int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
-                   const int32_t* d_mask, int mask_words, void* d_out, const int32_t* d_bt,
-                   int bt_stride, float scale, cudaStream_t s) {
+int check_tree_call(const kvc_pool* pool, const kvc_tree_plan* plan, int layer,
+                    const int32_t* d_mask, int mask_words, int bt_stride, float scale) {
   const PoolGeom& g = pool->g;
   if (!plan->valid) return set_error(KVC_ERR_INVALID_ARG, "plan has not been built.");
   if (layer < 0 || layer >= g.num_layers)
@@ -144,15 +143,24 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
       pg.page_size != g.page_size || pg.dtype != g.dtype || plan->device != pool->device)
     return set_error(KVC_ERR_INVALID_ARG, "plan was built for a pool of another geometry.");
   if (plan->n_tokens == 0) return KVC_OK;
-  if (!d_q || !d_out || !d_bt)
-    return set_error(KVC_ERR_INVALID_ARG, "q, out and block tables must not be null.");
-  if (!aligned16(d_q) || !aligned16(d_out))
-    return set_error(KVC_ERR_INVALID_ARG, "q and out must be 16-byte aligned.");
   if (d_mask && mask_words <= 0)
     return set_error(KVC_ERR_INVALID_ARG, "mask_words must be positive.");
   if (!std::isfinite(scale)) return set_error(KVC_ERR_INVALID_ARG, "scale must be finite.");
   if (bt_stride <= 0 || plan->max_end > static_cast<int64_t>(bt_stride) * g.page_size)
     return set_error(KVC_ERR_OUT_OF_RANGE, "a sequence exceeds the block-table width.");
+  return KVC_OK;
+}
+
+int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
+                   const int32_t* d_mask, int mask_words, void* d_out, const int32_t* d_bt,
+                   int bt_stride, float scale, cudaStream_t s) {
+  const PoolGeom& g = pool->g;
+  if (int rc = check_tree_call(pool, plan, layer, d_mask, mask_words, bt_stride, scale)) return rc;
+  if (plan->n_tokens == 0) return KVC_OK;
+  if (!d_q || !d_out || !d_bt)
+    return set_error(KVC_ERR_INVALID_ARG, "q, out and block tables must not be null.");
+  if (!aligned16(d_q) || !aligned16(d_out))
+    return set_error(KVC_ERR_INVALID_ARG, "q and out must be 16-byte aligned.");
   TreeArgs a = {};
   if (int rc = paged_view(pool, layer, d_bt, plan->max_row + 1, bt_stride, &a.p)) return rc;
   a.q = d_q;

@@ -16,8 +16,10 @@ pytestmark = pytest.mark.gpu
 if HAS_GPU:
     import torch
 
+    import batch_generate as BG
     import paged
-    from test_gpu_spec_ops import BF16, F16, dev, no_error
+    from test_gpu_batch_generate import _model
+    from test_gpu_spec_ops import BF16, F16, dev, no_error, raw
 
 
 # -- tree attention: a flat tail far below one peak ------------------------------------------
@@ -68,3 +70,42 @@ def test_tree_keeps_a_flat_tail_below_a_peak(dtype, at):
         assert float(err.max()) <= 0, f"{x} nats: over by {float(err.max()):.3g}"
     plan.close()
     pool.close()
+
+
+# -- the whole layer: a refused call leaves the cache alone ---------------------------------------
+def test_refused_layer_calls_launch_nothing():
+    cfg, tensors = _model()
+    model = BG.BatchModel.from_tensors(cfg, tensors)
+    pool = paged.PagedKVCache(cfg.layers, 8, 16, cfg.kv_heads, cfg.head_dim)
+    bt, n = dev(np.arange(8).reshape(2, 4)), 3
+    x = model.embedding[:n].contiguous()
+    out = torch.full_like(x, 7.0)
+    for m in raw(pool):
+        m.fill_(3.0)
+    plan = pool.plan_tree([20], [n], cfg.heads)
+    good = dict(plan=plan, layer=0, weights=model.layers[0], mask=None, block_tables=bt)
+    others = []
+    for layers, ps, hkv, d in ((cfg.layers, 32, cfg.kv_heads, cfg.head_dim),
+                               (cfg.layers, 16, 2 * cfg.kv_heads, cfg.head_dim),
+                               (cfg.layers, 16, cfg.kv_heads, 2 * cfg.head_dim)):
+        o = paged.PagedKVCache(layers, 8, ps, hkv, d)
+        others.append((o, o.plan_tree([20], [n], cfg.heads if hkv == cfg.kv_heads else 2 * cfg.heads)))
+    off = torch.zeros(model.layers[0].w[6].numel() + 2, dtype=torch.uint8, device="cuda")[2:]
+    lw = model.layers[0]
+    crooked = paged.DeviceLayerWeights(lw.attn_norm, lw.ffn_norm, list(lw.w[:6]) + [off], lw.types,
+                                       lw.hidden, lw.intermediate)
+    bad = [dict(plan=p) for _, p in others]
+    bad += [dict(layer=cfg.layers), dict(layer=-1), dict(block_tables=bt[:, :1].contiguous()),
+            dict(mask=torch.zeros(n, 0, dtype=torch.int32, device="cuda")),
+            dict(scale=math.nan), dict(freq_base=0.0), dict(freq_base=math.inf),
+            dict(weights=crooked), dict(plan=paged.TreePlan())]
+    for change in bad:
+        with pytest.raises((ValueError, IndexError)):
+            pool.forward_layer_tree(**{**dict(x=x, out=out), **good, **change})
+        no_error()
+        assert torch.all(out == 7.0), change
+        for m in raw(pool):
+            assert torch.all(m == 3.0), change
+    pool.forward_layer_tree(x=x, out=out, **good)
+    no_error()
+    assert not torch.any(out == 7.0) and int((raw(pool)[1] != 3.0).sum()) == n * cfg.kv_heads * cfg.head_dim
