@@ -428,8 +428,8 @@ class PagedKVCache:
         if len(weights.w) != 7 or len(weights.types) != 7:
             raise ValueError("a layer has seven weights: q, k, v, o, gate, up, down")
         for w in weights.w:
-            if not w.is_cuda or not w.is_contiguous():
-                raise ValueError("weights must be contiguous CUDA tensors")
+            if w.get_device() != dev or not w.is_contiguous():
+                raise ValueError(f"weights must be contiguous tensors on cuda:{dev}")
         wt = [x for w, ty in zip(weights.w, weights.types) for x in (int(w.data_ptr()), int(ty))]
         mp, words = self._mask(mask, t)
         self._table(block_tables, plan)
