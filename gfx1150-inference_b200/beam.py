@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 import kvcache_ffi as ffi
-from paged import _TORCH_CODE, _on, _stream_on
+from paged import _TORCH_CODE, _made_on, _on, _stream_on
 
 
 class BeamSelector:
@@ -52,9 +52,10 @@ class BeamSelector:
         if (vocab > 1 and st[1] != 1) or (n * beams > 1 and st[0] < vocab):
             raise ValueError("a row of logits must be packed")
         if out is None:
-            tokens = torch.empty((n, n_out), dtype=torch.int32, device=logits.device)
-            out = (tokens, torch.empty_like(tokens),
-                   torch.empty((n, n_out), dtype=torch.float32, device=logits.device))
+            with _made_on(stream, dev):
+                tokens = torch.empty((n, n_out), dtype=torch.int32, device=logits.device)
+                out = (tokens, torch.empty_like(tokens),
+                       torch.empty((n, n_out), dtype=torch.float32, device=logits.device))
         tokens, parents, best = out
         m = n * n_out
         ffi.check(ffi.lib.kvc_beam_select(

@@ -16,6 +16,7 @@ building each rank's pool with its own ``num_kv_heads`` slice (see
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -79,6 +80,22 @@ def _stream_on(stream, device: int) -> Optional[int]:
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(device) or None
     return int(stream.cuda_stream) or None
+
+
+def _made_on(stream, device):
+    """What is allocated or uploaded inside belongs to `stream` (None: the current one), so
+    that its memory goes to another tensor only behind the kernels enqueued there."""
+    if stream is None:
+        return contextlib.nullcontext()
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(stream.cuda_stream), device=device)
+    return torch.cuda.stream(stream)
+
+
+def _upload(a: np.ndarray, dev: torch.device) -> torch.Tensor:
+    """A tensor of `a` on `dev`, without waiting for the stream's earlier work."""
+    t = torch.from_numpy(np.ascontiguousarray(a))
+    return t.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else t
 
 
 @dataclass
@@ -346,7 +363,8 @@ class PagedKVCache:
             heads = q.shape[1]
             qp, qs = _token_rows(q, "q", dt, (n, heads, d), dev)
             if q_out is None:
-                q_out = torch.empty((n, heads, d), dtype=dt, device=q.device)
+                with _made_on(stream, dev):
+                    q_out = torch.empty((n, heads, d), dtype=dt, device=q.device)
             op = _on(q_out, "q_out", dt, n * heads * d, dev)
         if block_tables.dim() != 2:
             raise ValueError("block_tables must be (rows, pages)")
@@ -484,9 +502,10 @@ class PagedKVCache:
 
     def gather(self, layer: int, block_tables: torch.Tensor, row: int, start: int, count: int,
                stream=None):
-        k = torch.empty((count, self.num_kv_heads, self.head_dim), dtype=self.dtype,
-                        device=f"cuda:{self.device}")
-        v = torch.empty_like(k)
+        with _made_on(stream, self.device):
+            k = torch.empty((count, self.num_kv_heads, self.head_dim), dtype=self.dtype,
+                            device=f"cuda:{self.device}")
+            v = torch.empty_like(k)
         ffi.check(ffi.lib.kvc_gather(self.handle, layer, _i32(block_tables),
                                      int(block_tables.shape[-1]), row, start, count,
                                      int(k.data_ptr()), int(v.data_ptr()), _sp(stream)))
@@ -525,7 +544,10 @@ class BatchDecoder:
     of the batch advances by one token per step, one kvc_forward_layer_paged
     call per layer for the whole batch.  Sequence i owns block-table row i;
     ``ctx_lens[i]`` counts its cached positions.  The embedding lookup, the
-    final norm, the LM head and sampling stay with the caller."""
+    final norm, the LM head and sampling stay with the caller.
+
+    With ``stream`` a call's whole work runs there: its inputs must be ready on that
+    stream, and what it returns belongs to it, as after ``torch.cuda.stream(stream)``."""
 
     def __init__(self, cache: PagedKVCache, layers: Sequence[DeviceLayerWeights],
                  block_tables: torch.Tensor, num_heads: int, ctx_lens: Sequence[int],
@@ -596,13 +618,13 @@ class BatchDecoder:
             self._drafted = counts
             return x
         pos = np.concatenate([int(c) + tree_depths(t) for c, t in zip(self.ctx, trees)])
-        dev = x.device
-        mask = torch.from_numpy(np.concatenate(masks)).to(dev)
-        rope_pos = torch.from_numpy(pos.astype(np.int32)).to(dev)
+        with _made_on(stream, self.bt.device):
+            mask = _upload(np.concatenate(masks), x.device)
+            rope_pos = _upload(pos.astype(np.int32), x.device)
+            cur = x.contiguous()
+            bufs = (torch.empty_like(cur), torch.empty_like(cur))   # x itself is never written
         self.tree_plan = self.cache.plan_tree(self.ctx, counts, self.num_heads,
                                               plan=self.tree_plan, stream=stream)
-        cur = x.contiguous()
-        bufs = (torch.empty_like(cur), torch.empty_like(cur))   # x itself is never written
         for layer, lw in enumerate(self.layers):
             nxt = bufs[layer % 2]
             self.cache.forward_layer_tree(self.tree_plan, layer, cur, nxt, lw, mask, self.bt,
@@ -627,10 +649,10 @@ class BatchDecoder:
             mat = np.zeros((len(paths), int(lens.max())), dtype=np.int32)
             for i, p in enumerate(paths):
                 mat[i, :len(p)] = p
-            dev = self.bt.device
-            self.cache.commit_tree(self.bt, torch.from_numpy(self.ctx.astype(np.int32)).to(dev),
-                                   torch.from_numpy(mat).to(dev), torch.from_numpy(lens).to(dev),
-                                   stream=stream)
+            with _made_on(stream, self.bt.device):
+                ctx, mat, n = (_upload(a, self.bt.device)
+                               for a in (self.ctx.astype(np.int32), mat, lens))
+            self.cache.commit_tree(self.bt, ctx, mat, n, stream=stream)
         self.ctx += lens
         self._drafted = None
 
@@ -647,13 +669,15 @@ class BatchDecoder:
         ctx = self.ctx.reshape(n, beams)
         if np.any(ctx != ctx[:, :1]):
             raise ValueError("the beams of a sequence must have the same context length")
-        dev = self.bt.device
-        self.cache.reorder_beams(self.bt, torch.from_numpy(parents).to(dev),
-                                 torch.from_numpy(ctx[:, 0].astype(np.int32)).to(dev), stream=stream)
+        with _made_on(stream, self.bt.device):
+            par = _upload(parents, self.bt.device)
+            lens = _upload(ctx[:, 0].astype(np.int32), self.bt.device)
+        self.cache.reorder_beams(self.bt, par, lens, stream=stream)
 
     def _layers(self, x: torch.Tensor, stream) -> torch.Tensor:
-        cur = x.contiguous()
-        bufs = (torch.empty_like(cur), torch.empty_like(cur))   # x itself is never written
+        with _made_on(stream, self.bt.device):
+            cur = x.contiguous()
+            bufs = (torch.empty_like(cur), torch.empty_like(cur))   # x itself is never written
         for layer, lw in enumerate(self.layers):
             nxt = bufs[layer % 2]
             self.cache.forward_layer(self.plan, layer, cur, nxt, lw, self.bt, self.eps,

@@ -17,9 +17,11 @@ if HAS_GPU:
     import torch
 
     import batch_generate as BG
+    import beam
     import paged
     from test_gpu_batch_generate import _model
     from test_gpu_spec_ops import BF16, F16, dev, no_error, raw
+    from test_gpu_spec_generate import gen  # noqa: F401  (a fixture)
 
 
 # -- tree attention: a flat tail far below one peak ------------------------------------------
@@ -109,3 +111,69 @@ def test_refused_layer_calls_launch_nothing():
     pool.forward_layer_tree(x=x, out=out, **good)
     no_error()
     assert not torch.any(out == 7.0) and int((raw(pool)[1] != 3.0).sum()) == n * cfg.kv_heads * cfg.head_dim
+
+
+# -- another stream than the current one ----------------------------------------------------------
+def _litter():
+    """Small tensors of every size on the current stream, full of what no call can use."""
+    for n in (1, 3, 8, 64, 200, 1024, 4096, 1 << 16):
+        for _ in range(4):
+            torch.full((n,), 0x7E7E7E7E, dtype=torch.int32, device="cuda")
+
+
+def _run(gen, stream, busy):
+    bt = gen.bt[:3].clone()
+    dec = gen._decoder(bt)
+    x = lambda ids: gen.model.embedding[torch.tensor(ids, device="cuda")].contiguous()  # noqa: E731
+    prompt, drafts = x([3, 14, 15, 9, 2, 6, 5]), x([5, 9, 11, 3, 60, 7, 8, 2, 4])
+    nxt = x([1, 2, 3])
+    outs = []
+    torch.cuda.synchronize()
+    if busy:
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(100_000_000)        # some 50 ms, so that all below waits its turn
+    for i in range(3):
+        outs.append(dec.prefill(i, prompt, stream=stream))
+        _litter()
+    outs.append(dec.verify(drafts, [[-1, 0, 0]] * 3, stream=stream))
+    _litter()
+    dec.commit([[0, 2], [0, 1], [0, 2]], stream=stream)
+    _litter()
+    dec.reorder([[2, 0, 0]], stream=stream)
+    _litter()
+    outs.append(dec.step(nxt, stream=stream))
+    _litter()
+    outs += [t for r in range(3) for t in gen.pool.gather(1, bt, r, 0, 10, stream=stream)]
+    _litter()
+    torch.cuda.synchronize()
+    dec.close()
+    return outs, bt
+
+
+def test_decoder_on_a_busy_side_stream(gen):  # noqa: F811
+    want, table = _run(gen, None, False)
+    for _ in range(3):
+        got, bt = _run(gen, torch.cuda.Stream(), True)
+        assert torch.equal(table, bt)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    no_error()
+
+
+def test_outputs_made_for_a_side_stream_are_its_own():
+    """The current stream still has writes under way to memory that it has freed."""
+    pool = paged.PagedKVCache(1, 8, 16, 2, 64)
+    bt, pos = dev([[0, 1, 2, 3]]), dev(np.arange(40))
+    k = torch.randn(40, 2, 64, device="cuda").half()
+    q = torch.randn(40, 4, 64, device="cuda").half()
+    logits, scores = torch.randn(4, 5000, device="cuda"), torch.zeros(1, 4, device="cuda")
+    sel = beam.BeamSelector(1, 4, 5000, 8)
+    want = [pool.append_rope(0, q, k, k, bt, pos), *sel.select(logits, scores, 8)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    shapes = [(t.shape, t.dtype) for t in want]
+    torch.cuda._sleep(100_000_000)
+    late = [torch.full(s, 9, dtype=d, device="cuda") for s, d in shapes]
+    del late
+    got = [pool.append_rope(0, q, k, k, bt, pos, stream=side), *sel.select(logits, scores, 8, stream=side)]
+    no_error()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))

@@ -42,3 +42,67 @@ def test_layer_weights_on_another_device_are_refused():
     with pytest.raises(ValueError, match="weights"):
         pool.forward_layer_tree(plan, 0, x, x, lw, None, torch.zeros(1, 4, dtype=torch.int32))
     plan.close()
+
+
+class _Cache:
+    """Takes a decoder's calls and remembers the streams that they name."""
+    num_layers, page_size = 2, 16
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name not in ("plan", "plan_tree", "forward_layer", "forward_layer_tree", "commit_tree",
+                        "reorder_beams"):
+            raise AttributeError(name)
+
+        def call(*args, **kw):
+            self.calls.append((name, kw.get("stream", args[-1] if args else None)))
+            return paged.TreePlan() if name == "plan_tree" else None
+        return call
+
+
+def _decoder(rows=3, ctx=10):
+    return paged.BatchDecoder(_Cache(), [object(), object()], torch.zeros((rows, 4), dtype=torch.int32),
+                              8, [ctx] * rows)
+
+
+def test_what_a_decoder_makes_belongs_to_the_stream_it_is_given(monkeypatch):
+    """The allocator may hand memory of the current stream to another tensor as soon as the
+    call has returned, so nothing that the kernels on `stream` use is made elsewhere."""
+    state = {"on": None}
+    made = []
+
+    class On:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            state["on"] = self.stream
+
+        def __exit__(self, *_):
+            state["on"] = None
+
+    class Stream:
+        cuda_stream = 77
+
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda ptr, device=None: ("stream", ptr))
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    for name in ("from_numpy", "empty_like"):
+        real = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda *a, _real=real, _name=name, **k: (
+            made.append((_name, state["on"])), _real(*a, **k))[1])
+    dec, s = _decoder(), Stream()
+    x = torch.zeros((3, 16), dtype=torch.float16)
+    dec.verify(x, [[-1], [-1], [-1]], stream=s)
+    dec.commit([[0], [0], [0]], stream=s)
+    dec.reorder([[1, 1, 2]], stream=s)
+    dec.step(x, stream=s)
+    dec.prefill(0, x, stream=s)
+    assert {n for n, _ in made} == {"from_numpy", "empty_like"} and len(made) >= 13
+    assert all(on == ("stream", 77) for _, on in made)
+    assert all(at is s for _, at in dec.cache.calls) and len(dec.cache.calls) == 11
+    made.clear()
+    dec.verify(x, [[-1], [-1], [-1]])          # none given: the current stream
+    assert made and all(on is None for _, on in made)
+    dec.close()
