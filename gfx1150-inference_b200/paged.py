@@ -659,7 +659,8 @@ class BatchDecoder:
     def reorder(self, parents: np.ndarray, stream=None) -> None:
         """Beam search: rows are sequences * beams, parents (sequences, beams) beam
         numbers; every row takes its parent's cached states (reorder_beams).  The
-        block table is permuted in place: give the decoder one of its own."""
+        block table is permuted in place: give the decoder one of its own.  The rows of
+        a ``verify`` that was not committed do not follow: it is dropped."""
         parents = np.ascontiguousarray(np.asarray(parents, dtype=np.int32))
         if parents.ndim != 2 or parents.size != len(self.ctx):
             raise ValueError("parents needs one entry per row, (sequences, beams)")
@@ -672,6 +673,7 @@ class BatchDecoder:
         with _made_on(stream, self.bt.device):
             par = _upload(parents, self.bt.device)
             lens = _upload(ctx[:, 0].astype(np.int32), self.bt.device)
+        self._drafted = None      # (drafted rows lie behind the positions that move)
         self.cache.reorder_beams(self.bt, par, lens, stream=stream)
 
     def _layers(self, x: torch.Tensor, stream) -> torch.Tensor:

@@ -106,3 +106,21 @@ def test_what_a_decoder_makes_belongs_to_the_stream_it_is_given(monkeypatch):
     dec.verify(x, [[-1], [-1], [-1]])          # none given: the current stream
     assert made and all(on is None for _, on in made)
     dec.close()
+
+
+def test_a_reorder_drops_the_verify_before_it():
+    """Only cached positions follow their parents: the drafted rows behind them stay, and a
+    commit would keep another beam's."""
+    dec = _decoder()
+    x = torch.zeros((6, 16), dtype=torch.float16)
+    dec.verify(x, [[-1, 0]] * 3)
+    dec.reorder([[1, 2, 0]])
+    with pytest.raises(RuntimeError, match="verify"):
+        dec.commit([[0, 1]] * 3)
+    assert list(dec.ctx) == [10] * 3
+    dec.verify(x, [[-1, 0]] * 3)
+    with pytest.raises(ValueError):
+        dec.reorder([[1, 2, 3]])              # refused: nothing moved, the verify stands
+    dec.commit([[0, 1], [0], []])
+    assert list(dec.ctx) == [12, 11, 10]
+    dec.close()
