@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
   volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(smem + 512);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + 516);
-  volatile int* s_dirty = reinterpret_cast<volatile int*>(smem + 520);   // [2]
+  volatile int* s_dirty = reinterpret_cast<volatile int*>(smem + 520);   // [4]
   float2* s_ml = reinterpret_cast<float2*>(smem + 1024);                 // [2][128]
   uint8_t* q_mem = smem + S::kHeadBytes;
   uint8_t* stage_mem = q_mem + S::kStreams * S::kQBytes;
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     }
     fence_mbar_init();
     *s_abort = 0;
-    s_dirty[0] = s_dirty[1] = -1;
+    for (int i = 0; i < 4; ++i) s_dirty[i] = -1;
   }
   // (the plan's records are no kernel's output: they may be read before the wait)
   const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
@@ -508,7 +508,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
               }
             }
             for (int i = live + lane; i < to * U; i += 32) *cell(i) = make_uint4(0, 0, 0, 0);
-            if (dirty) s_dirty[si & 1] = si;
+            // The helper is in piece p once the MMAs are, when softmax group 0 is past piece
+            // p - 2.  Group 1 is too, or still at the end of p - 2 (if p - 1 is one tile, all of
+            // it group 0's).  So three places suffice for a piece's flag to be read before it
+            // is written again; two do not.
+            if (dirty) s_dirty[si & 3] = si;
           }
           __threadfence_block();
           fence_proxy_async();
@@ -682,7 +686,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
           w1 = fast_exp2(e1.x - mm);
           ll = e0.y * w0 + e1.y * w1;
         }
-        const bool dirty = s_dirty[si & 1] == si;
+        const bool dirty = s_dirty[si & 3] == si;
         // rare: what was taken out of V comes back, for the nodes that this row sees
         auto restore = [&](int c, float* f) {
           const int t0 = max(sg.tile0 * KP, sg.ctx), t1 = min(sg.tile1 * KP, sg.ctx + sg.nodes);

@@ -177,3 +177,44 @@ def test_outputs_made_for_a_side_stream_are_its_own():
     got = [pool.append_rope(0, q, k, k, bt, pos, stream=side), *sel.select(logits, scores, 8, stream=side)]
     no_error()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+# -- pieces of every kind after one another on one CTA ---------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_tree_restores_values_in_every_piece_of_a_cta(dtype):
+    """Wide trees (two groups of rows) and single tokens (one tile) in turn, several pieces a
+    CTA, each with drafted V that are not finite: they reach the rows that see them, and the
+    rest is what it is with zeros in their place."""
+    dt = getattr(torch, dtype)
+    seqs, d, h, ps, cols = 1200, 64, 4, 16, 8
+    rng = np.random.default_rng(5)
+    ctx = rng.integers(0, 60, seqs)
+    nodes = np.where(np.arange(seqs) % 2 == 0, 60, 1 + np.arange(seqs) % 5)
+    pool = paged.PagedKVCache(1, seqs * cols, ps, 1, d, dtype=dt)
+    pool.fill_normal(seed=2)
+    bt = dev(rng.permutation(seqs * cols).reshape(seqs, cols))
+    total = int(nodes.sum())
+    rows = dev(np.repeat(np.arange(seqs), nodes))
+    first = np.concatenate([[0], np.cumsum(nodes)[:-1]])
+    node = np.arange(total) - np.repeat(first, nodes)
+    slots = dev(np.repeat(ctx, nodes) + node)
+    k = torch.randn(total, 1, d, device="cuda").to(dt)
+    clean = torch.randn(total, 1, d, device="cuda").to(dt)
+    hurt = torch.from_numpy(first + rng.integers(0, nodes)).cuda()      # one node of each sequence
+    clean[hurt, 0, 7] = 0.0
+    odd = clean.clone()
+    odd[hurt, 0, 7] = math.inf
+    q = torch.randn(total, h, d, device="cuda").to(dt)
+    plan = pool.plan_tree(ctx, nodes, h)
+    assert plan.info().n_items * 4 <= seqs
+    out = []
+    for v in (clean, odd):
+        pool.append(0, k, v, bt, slots, rows)
+        o = torch.zeros_like(q)
+        pool.decode_tree(plan, 0, q, None, o, bt, 0.1)
+        no_error()
+        out.append(o)
+    want = out[0].clone()
+    at = np.repeat((hurt.cpu().numpy() - first), nodes)
+    want[torch.from_numpy(node >= at).cuda(), :, 7] = math.inf
+    assert torch.equal(out[1], want)
