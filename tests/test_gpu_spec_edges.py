@@ -20,7 +20,7 @@ if HAS_GPU:
     import beam
     import paged
     from test_gpu_batch_generate import _model
-    from test_gpu_spec_ops import BF16, F16, dev, no_error, raw
+    from test_gpu_spec_ops import BF16, F16, F32, dev, no_error, raw
     from test_gpu_spec_generate import gen  # noqa: F401  (a fixture)
 
 
@@ -218,3 +218,149 @@ def test_tree_restores_values_in_every_piece_of_a_cta(dtype):
     at = np.repeat((hurt.cpu().numpy() - first), nodes)
     want[torch.from_numpy(node >= at).cuda(), :, 7] = math.inf
     assert torch.equal(out[1], want)
+
+
+# -- rotate + append: the variant for many tokens ---------------------------------------------------
+@pytest.mark.parametrize("neox", [False, True])
+@pytest.mark.parametrize("dtype,d,hkv,h,ps", [
+    (F32, 64, 2, 6, 16), (F16, 128, 8, 32, 16), (BF16, 96, 3, 7, 48), (F16, 40, 2, 4, 16),
+    (BF16, 256, 1, 3, 32), (F32, 256, 2, 2, 16), (F16, 8, 3, 5, 16), (F32, 12, 1, 2, 16)])
+def test_append_rope_of_many_tokens(dtype, d, hkv, h, ps, neox):
+    """From 592 tokens on four of them share a CTA; the last CTA has one, two or three."""
+    dt = getattr(torch, dtype)
+    half = torch.finfo(dt).eps / 2
+    slack = 2.0 ** -22 + 3 * 2.0 ** -24 + 2.0 ** -23
+    rng = np.random.default_rng(d + h)
+    for counts, ctx in (([400, 1, 260], [5, ps - 1, 100000]), ([592], [0]), ([3, 700, 11], [7, 0, 64]),
+                        ([1201], [33])):
+        n = sum(counts)
+        need = [-(-(c + k) // ps) for c, k in zip(ctx, counts)]
+        bt = np.zeros((len(ctx), max(need)), dtype=np.int32)
+        pages = sum(b - c // ps for b, c in zip(need, ctx))
+        perm = iter(rng.permutation(pages))
+        for i, c in enumerate(ctx):
+            for p in range(c // ps, need[i]):
+                bt[i, p] = next(perm)
+        pool = paged.PagedKVCache(1, pages, ps, hkv, d, dtype=dt)
+        pos = np.concatenate([c + np.arange(k) for c, k in zip(ctx, counts)])
+        rows = np.repeat(np.arange(len(ctx)), counts)
+        pad = np.unique(np.concatenate([rng.integers(0, n, 9), [n - 1]]))
+        slots = pos.copy()
+        slots[pad] = -1
+        g = torch.Generator(device="cuda")
+        g.manual_seed(n)
+        qkv = torch.randn(n, h + 2 * hkv, d, generator=g, device="cuda").to(dt)
+        q, k, v = qkv[:, :h], qkv[:, h:h + hkv], qkv[:, h + hkv:]
+        ang = pos + rng.integers(-3, 4, n)
+        args = lambda a, b: dict(rows=dev(rows[a:b]), rope_positions=dev(ang[a:b]),  # noqa: E731
+                                 freq_base=500000.0, neox=neox)
+        for m in raw(pool):
+            m.fill_(3.0)
+        q_out = torch.full((n, h, d), 5.0, dtype=dt, device="cuda")
+        pool.append_rope(0, q, k, v, dev(bt), dev(slots), q_out=q_out, **args(0, n))
+        no_error()
+        freq = 500000.0 ** (-2.0 * np.arange(d // 2) / d)
+        th = torch.from_numpy(ang[:, None].astype(np.float64) * freq).cuda()[:, None]
+
+        def rot(x):
+            x = x.double()
+            a, b = (x[..., :d // 2], x[..., d // 2:]) if neox else (x[..., 0::2], x[..., 1::2])
+            y = [a * th.cos() - b * th.sin(), a * th.sin() + b * th.cos()]
+            t = [a.abs() + b.abs()] * 2
+            if neox:
+                return torch.cat(y, -1), torch.cat(t, -1)
+            return torch.stack(y, -1).flatten(-2), torch.stack(t, -1).flatten(-2)
+
+        live = np.setdiff1d(np.arange(n), pad)
+        kk, vv = torch.empty_like(k), torch.empty_like(v)
+        o = 0
+        for i, (c, m) in enumerate(zip(ctx, counts)):
+            gk, gv = pool.gather(0, dev(bt), i, c, m)
+            kk[o:o + m], vv[o:o + m] = gk, gv
+            o += m
+        for got, src in ((q_out, q), (kk, k)):
+            ref, mag = rot(src)
+            tol = half * ref.abs() + slack * mag + (2.0 ** -25 if dtype == F16 else 0)
+            assert torch.all((got.double() - ref).abs()[live] <= tol[live])
+        assert torch.equal(vv[live], v[live])
+        assert torch.all(q_out[pad] == 5.0) and torch.all(kk[pad] == 3.0) and torch.all(vv[pad] == 3.0)
+        for m in raw(pool):   # nothing else is written
+            assert int((m != 3.0).sum()) <= len(live) * hkv * d
+        # few tokens at a time, a CTA each: the same bits
+        whole = [m.clone() for m in raw(pool)]
+        again = torch.full_like(q_out, 5.0)
+        for m in raw(pool):
+            m.fill_(3.0)
+        for a in range(0, n, 400):
+            b = min(n, a + 400)
+            pool.append_rope(0, q[a:b], k[a:b], v[a:b], dev(bt), dev(slots[a:b]), q_out=again[a:b],
+                             **args(a, b))
+        no_error()
+        assert torch.equal(again, q_out) and all(torch.equal(a, b) for a, b in zip(whole, raw(pool)))
+        pool.close()
+
+
+# -- selection: many rows over a large vocabulary ---------------------------------------------------
+def _select_ref(logits, scores, n_out):
+    """Tokens, parents and scores in 64 bits, on the GPU; lower candidates win ties."""
+    n, b = scores.shape
+    x = logits.double()
+    fin = torch.isfinite(x)
+    x = torch.where(fin, x, -math.inf)
+    top = x.amax(1, keepdim=True)
+    some = torch.isfinite(top)
+    lse = torch.where(some, top + (x - torch.where(some, top, 0.0)).exp().sum(1, keepdim=True).log(), 0.0)
+    cum = scores.double().view(-1, 1)
+    s = torch.where(fin & torch.isfinite(cum), cum + (x - lse), -math.inf).view(n, -1)
+    best, at = torch.sort(s, dim=1, descending=True, stable=True)
+    v = logits.shape[1]
+    return at[:, :n_out] % v, at[:, :n_out] // v, best[:, :n_out]
+
+
+def _check_select(logits, scores, n_out):
+    n, b = scores.shape
+    sel = beam.BeamSelector(n, b, logits.shape[1], n_out)
+    tok, par, best = sel.select(logits, scores, n_out)
+    no_error()
+    rt, rp, rs = _select_ref(logits, scores, n_out)
+    assert torch.equal(par.long(), rp) and torch.equal(tok.long(), rt)
+    fin = torch.isfinite(rs)
+    assert torch.equal(fin, torch.isfinite(best)) and torch.all(best[~fin] == -math.inf)
+    assert torch.all((best.double() - rs).abs()[fin] <= (2.0 ** -17 + 2.0 ** -24 * rs.abs())[fin])
+    sel.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,b,v,k", [(12, 8, 65537, 8), (24, 4, 120000, 32), (24, 8, 100003, 16),
+                                     (16, 16, 77777, 32)])
+def test_beam_select_many_rows(n, b, v, k, dtype):
+    """2, 4, 8 and 8 batches of 512 logits a warp: the running max and sum go over several."""
+    dt = getattr(torch, dtype)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(v)
+    logits = (3 * torch.randn(n * b, v, generator=g, device="cuda")).to(dt)
+    scores = -5 * torch.rand(n, b, generator=g, device="cuda")
+    _check_select(logits, scores, k)
+    wide = torch.full((n * b, v + 13), math.inf, dtype=dt, device="cuda")    # rows on every alignment
+    wide[:, 5:5 + v] = logits
+    _check_select(wide[:, 5:5 + v], scores, k)
+    # a max that grows with every batch, one that falls, masks, values that are not finite
+    ramp = torch.linspace(-20, 20, v, device="cuda")
+    logits[0::5] = (logits[0::5].float() + ramp).to(dt)
+    logits[1::5] = (logits[1::5].float() - ramp).to(dt)
+    logits[2, :v - 3] = -math.inf
+    logits[3, 100:] = -math.inf
+    logits[4] = -math.inf
+    logits[7, ::3] = math.nan
+    logits[8, 1::2] = math.inf
+    logits[9] = torch.finfo(dt).min
+    logits[9, v // 2] = 0.0
+    _check_select(logits, scores, k)
+    scores[:, 1:] = -math.inf
+    scores[1, 0], scores[2, 0] = math.nan, -math.inf
+    _check_select(logits, scores, k)
+    same = torch.zeros(n * b, v, dtype=dt, device="cuda")      # every candidate ties
+    _check_select(same, torch.zeros(n, b, device="cuda"), k)
+    peak = same.clone()
+    peak[:, 4090:4100] = 7.0                                   # across two warps' runs
+    _check_select(peak, torch.zeros(n, b, device="cuda"), k)
