@@ -6,6 +6,7 @@
 // All three are bound by memory traffic: each byte is read once and written once,
 // in 16-byte units, and the address arithmetic of a row is shared by its units.
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -226,8 +227,9 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
   __syncthreads();
   for (int j = threadIdx.x; j < min(len, a.path_stride); j += kCommitThreads) {
     const int node = path[j];
+    // (a context near 2^31 would overflow the sums below, and with them page_of's checks)
     const bool ok = node >= j && node < kMaxTreeNodes && (j == 0 || path[j - 1] < node) && ctx >= 0 &&
-                    len <= a.path_stride;
+                    ctx <= INT_MAX - kMaxTreeNodes && len <= a.path_stride;
     const int sp = ok ? page_of(a.p, row, ctx + node) : -1, dp = ok ? page_of(a.p, row, ctx + j) : -1;
     if (sp < 0 || dp < 0) {
       report_error_at(a.p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(node));
@@ -235,8 +237,8 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
     }
     s_page[0][j] = sp;
     s_page[1][j] = node == j ? -1 : dp;   // a row that stays is not touched
-    s_t[0][j] = (ctx + node) % a.p.page_size;
-    s_t[1][j] = (ctx + j) % a.p.page_size;
+    s_t[0][j] = ok ? (ctx + node) % a.p.page_size : 0;
+    s_t[1][j] = ok ? (ctx + j) % a.p.page_size : 0;
   }
   if (len > a.path_stride && threadIdx.x == 0) {
     report_error_at(a.p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(len));

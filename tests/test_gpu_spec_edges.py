@@ -18,6 +18,7 @@ if HAS_GPU:
 
     import batch_generate as BG
     import beam
+    import kvcache_ffi as ffi
     import paged
     from test_gpu_batch_generate import _model
     from test_gpu_spec_ops import BF16, F16, F32, dev, no_error, raw
@@ -364,3 +365,16 @@ def test_beam_select_many_rows(n, b, v, k, dtype):
     peak = same.clone()
     peak[:, 4090:4100] = 7.0                                   # across two warps' runs
     _check_select(peak, torch.zeros(n, b, device="cuda"), k)
+
+
+# -- commit: contexts that no table holds -------------------------------------------------------------
+@pytest.mark.parametrize("ctx", [2 ** 31 - 1, 2 ** 31 - 257, 2 ** 31 - 256, 2 ** 30, -1, -2 ** 31])
+def test_commit_reports_contexts_past_every_table(ctx):
+    pool = paged.PagedKVCache(1, 4, 16, 1, 64)
+    pool.fill_normal(seed=1)
+    before = [m.clone() for m in raw(pool)]
+    bt = dev([[0, 1], [2, 3]])
+    pool.commit_tree(bt, dev([ctx, 3]), dev([[1, 200], [0, 0]]), dev([2, 0]))
+    torch.cuda.synchronize()
+    assert ffi.device_error(0)[0] == 3
+    assert all(torch.equal(a, b) for a, b in zip(before, raw(pool)))
