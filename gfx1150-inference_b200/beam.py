@@ -33,9 +33,11 @@ class BeamSelector:
                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """The ``n_out`` best (beam, token) pairs of each sequence by scores[seq, beam] +
         log softmax(logits)[token], best first; equal scores go to the lower beam, then
-        the lower token.  logits: (sequences * beams, vocab) fp16, bf16 or fp32, rows may
-        be strided; scores: (sequences, beams) fp32, -inf for a beam not in use.  Returns
-        (tokens int32, parents int32, scores fp32), each (sequences, n_out)."""
+        the lower token.  Scores are within 2^-17 (and their rounding), so candidates of
+        different beams less than 2^-16 apart may change places.  logits: (sequences *
+        beams, vocab) fp16, bf16 or fp32, rows may be strided; scores: (sequences, beams)
+        fp32, -inf for a beam not in use.  Returns (tokens int32, parents int32, scores
+        fp32), each (sequences, n_out)."""
         dev = self.device
         code = _TORCH_CODE.get(logits.dtype)
         if code is None:

@@ -614,8 +614,9 @@ KVC_API int kvc_forward_layer_tree(
  * j < d_path_lens[i], in block-table row d_rows[i] (NULL: row i).  Paths are
  * strictly ascending node numbers (an ancestor is drafted before its children), at
  * most path_stride long; a length of 0 keeps the sequence as it is.  Rows behind
- * the path stay as they were.  No two sequences of a call share a row.  A path that does not ascend or leaves the table is
- * reported (KVC_DEVERR_BAD_POSITION) and its sequence left alone. */
+ * the path stay as they were.  No two sequences of a call share a row.  A path that
+ * does not ascend or leaves the table is reported (KVC_DEVERR_BAD_POSITION) and its
+ * sequence left alone. */
 KVC_API int kvc_commit_tree(kvc_pool_t* pool, const int32_t* d_block_tables, int bt_rows,
                             int bt_stride, const int32_t* d_rows, const int32_t* d_ctx_lens,
                             const int32_t* d_paths, int path_stride, const int32_t* d_path_lens,
@@ -634,8 +635,11 @@ KVC_API int kvc_beam_destroy(kvc_beam_t* beam);
  * d_scores_out: (n_seqs, n_out).  Equal scores go to the lower beam, then the
  * lower token.  A logit that is not finite takes no part in the softmax and scores
  * -inf, and so does every token of a beam whose score is not finite (a beam that
- * is not in use yet).  n_beams * vocab must be at least n_out.  Calls sharing a handle must be ordered
- * on one stream. */
+ * is not in use yet).  The exponentials are added in 32 bits, which leaves a beam's
+ * scores within 2^-17 of the exact ones: the order within a beam is exact, and so is
+ * that of candidates of different beams further apart than twice that; beams of equal
+ * rows and scores tie exactly.  n_beams * vocab must be at least n_out.  Calls sharing
+ * a handle must be ordered on one stream. */
 KVC_API int kvc_beam_select(kvc_beam_t* beam, const void* d_logits, int dtype, int64_t row_stride,
                             const float* d_scores_in, int n_seqs, int n_beams, int vocab,
                             int n_out, int32_t* d_tokens, int32_t* d_parents,

@@ -378,3 +378,82 @@ def test_commit_reports_contexts_past_every_table(ctx):
     torch.cuda.synchronize()
     assert ffi.device_error(0)[0] == 3
     assert all(torch.equal(a, b) for a, b in zip(before, raw(pool)))
+
+
+# -- selection: candidates of different beams that nearly tie -------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("v", [700, 32000, 128256])
+def test_beam_select_keeps_the_order_of_near_ties(dtype, v):
+    """Beams are 2^-16 and more apart, up and down in turn (each is within 2^-17 of its score)."""
+    n = 100
+    g = torch.Generator(device="cuda")
+    g.manual_seed(v)
+    x = torch.randn(2 * n, v, generator=g, device="cuda")
+    x *= torch.linspace(0.1, 4.0, n, device="cuda").repeat_interleave(2)[:, None]     # flat to peaked
+    x[:, 5] = x.amax(1) + 1.0 + torch.rand(2 * n, generator=g, device="cuda")
+    logits = x.to(getattr(torch, dtype))
+    logp = torch.log_softmax(logits.double(), 1).amax(1).view(n, 2)
+    gap = 2.0 ** -16 * (1 + torch.arange(n, device="cuda") % 3) * (1 - 2 * (torch.arange(n, device="cuda") % 2))
+    cum = torch.zeros(n, 2, device="cuda")
+    cum[:, 1] = (logp[:, 0] - logp[:, 1] + gap).float()
+    apart = cum[:, 1].double() + logp[:, 1] - logp[:, 0]
+    wide = apart.abs() >= 2.0 ** -16          # (what the scores' own fp32 leaves of the gap)
+    assert int(wide.sum()) >= n // 3
+    tok, par, _ = beam.BeamSelector(n, 2, v, 2).select(logits, cum, 2)
+    no_error()
+    assert torch.all(tok == 5)
+    assert torch.equal(par[wide, 0].long(), (apart > 0).long()[wide])
+    assert torch.equal(par[:, 0] + par[:, 1], torch.ones_like(par[:, 0]))
+
+
+# -- beam search against a search of its own over the same logits ---------------------------------------
+def _search(steps, k, most, penalty, eos):
+    """Beam search of one prompt: steps[t] are the (k, vocab) logits of the beams after t tokens."""
+    beams, ended = [(0.0, [])], []
+    for t in range(most):
+        logp = torch.log_softmax(steps[t].double(), 1).cpu().numpy()
+        found = sorted(((s + logp[b, w], -b, -w) for b, (s, _) in enumerate(beams)
+                        for w in range(logp.shape[1])), reverse=True)[:2 * k]
+        kept = []
+        for rank, (s, b, w) in enumerate(found):
+            ids = beams[-b][1] + [-w]
+            if -w == eos:
+                if rank < k:
+                    ended.append((s / len(ids) ** penalty, ids))
+            elif len(kept) < k:
+                kept.append((s, ids))
+        beams = kept
+        if len(ended) >= k:
+            break
+    else:
+        ended += [(s / len(ids) ** penalty, ids) for s, ids in beams]
+    return max(ended, key=lambda e: e[0])
+
+
+@pytest.mark.parametrize("k,penalty,eos_at", [(2, 1.0, None), (3, 0.0, None), (4, 1.0, 1), (4, 2.0, 0),
+                                              (3, -0.5, 3), (2, 0.7, 2)])
+def test_beam_search_against_a_search_over_the_same_logits(gen, monkeypatch, k, penalty, eos_at):  # noqa: F811
+    prompts = [[3, 14, 15, 9, 2, 6, 5], [1] * 17]
+    cfg = gen.model.cfg
+    old = cfg.eos_token_id
+    if eos_at is not None:
+        plain, _ = gen.generate_beam_ids(prompts, num_beams=k, max_new_tokens=6, stop_on_eos=False)
+        cfg.eos_token_id = plain[0][eos_at]
+    seen, real = [], gen._logits
+
+    def logits(h, stream):
+        out = real(h, stream)
+        seen.append(out.view(len(prompts), k, -1).clone())
+        return out
+    monkeypatch.setattr(gen, "_logits", logits)
+    try:
+        ids, scores = gen.generate_beam_ids(prompts, num_beams=k, max_new_tokens=12,
+                                            length_penalty=penalty, stop_on_eos=eos_at is not None)
+    finally:
+        eos, cfg.eos_token_id = cfg.eos_token_id, old
+    for i in range(len(prompts)):
+        score, want = _search([s[i] for s in seen], k, 12, penalty, eos if eos_at is not None else -1)
+        assert ids[i] == want
+        # 12 selections, each within 2^-17 and one rounding of a sum below 64
+        n = len(want) ** penalty
+        assert abs(scores[i] - score) <= 12 * (2.0 ** -17 + 2.0 ** -18) / n + 2.0 ** -40
