@@ -424,12 +424,21 @@ extern "C" int kvc_plan_tree(kvc_tree_plan_t* plan, const kvc_pool_t* pool, cons
                              int num_heads, void* stream) {
   if (!plan || !pool) return set_error(KVC_ERR_INVALID_ARG, "plan and pool must not be null.");
   return guarded("kvc_plan_tree", [&]() -> int {
+    DeviceScope dev(pool->device);
+    if (dev.rc()) return dev.rc();
+    // A captured upload would read the staging buffer at every replay, whatever a later build
+    // has put there (the capture stays valid).
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    const cudaError_t e = cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &cap);
+    if (e != cudaSuccess) return cuda_error(e, "cudaStreamIsCapturing");
+    if (cap != cudaStreamCaptureStatusNone)
+      return set_error(KVC_ERR_INVALID_ARG,
+                       "a tree plan cannot be built on a stream that is being captured: build it "
+                       "before the capture and capture the calls that use it.");
     if (plan->device >= 0 && plan->device != pool->device) {  // its buffers are elsewhere
       DeviceScope old(plan->device);
       plan->release();
     }
-    DeviceScope dev(pool->device);
-    if (dev.rc()) return dev.rc();
     return tree_build(plan, pool, h_rows, h_ctx_lens, h_node_counts, n_seqs, num_heads,
                       static_cast<cudaStream_t>(stream));
   });

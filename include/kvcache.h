@@ -569,7 +569,8 @@ KVC_API int kvc_append_rope(kvc_pool_t* pool, int layer, const void* d_q, int q_
  * h_ctx_lens[i] cached positions and h_node_counts[i] drafted tokens (0 to
  * KVC_MAX_TREE_NODES) whose K/V rows are in slots [ctx, ctx + nodes) of
  * block-table row h_rows[i] (NULL: row i); its tokens follow those of sequence
- * i - 1 in q, mask and out.  Built on the host and uploaded on `stream`. */
+ * i - 1 in q, mask and out.  Built on the host and uploaded on `stream`, which must not
+ * be capturing (KVC_ERR_INVALID_ARG: the plan and the capture stay as they are). */
 KVC_API int kvc_tree_plan_create(kvc_tree_plan_t** out);
 KVC_API int kvc_tree_plan_destroy(kvc_tree_plan_t* plan);
 KVC_API int kvc_plan_tree(kvc_tree_plan_t* plan, const kvc_pool_t* pool, const int32_t* h_rows,

@@ -457,3 +457,30 @@ def test_beam_search_against_a_search_over_the_same_logits(gen, monkeypatch, k, 
         # 12 selections, each within 2^-17 and one rounding of a sum below 64
         n = len(want) ** penalty
         assert abs(scores[i] - score) <= 12 * (2.0 ** -17 + 2.0 ** -18) / n + 2.0 ** -40
+
+
+# -- plans and captures ---------------------------------------------------------------------------------
+def test_a_tree_plan_is_not_built_inside_a_capture():
+    """An upload from the plan's staging buffer, replayed, would bring what a later build left
+    there.  The call is refused, and the capture around it goes on."""
+    pool = paged.PagedKVCache(1, 16, 16, 2, 64)
+    pool.fill_normal(seed=4)
+    bt = dev(np.arange(16).reshape(2, 8))
+    q = torch.randn(12, 8, 64, device="cuda").half()
+    plan = pool.plan_tree([50, 9], [5, 7], 8)
+    want, got = torch.zeros_like(q), torch.zeros_like(q)
+    pool.decode_tree(plan, 0, q, None, want, bt, 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for p in (plan, None):
+            with pytest.raises(ValueError, match="captured"):
+                pool.plan_tree([3, 4], [2, 2], 8, plan=p)
+        pool.decode_tree(plan, 0, q, None, got, bt, 0.1)
+    graph.replay()
+    no_error()
+    assert plan.n_tokens == 12 and torch.equal(want, got)
+    pool.plan_tree([50, 9], [5, 7], 8, plan=plan)      # and builds again outside
+    pool.decode_tree(plan, 0, q, None, got.zero_(), bt, 0.1)
+    no_error()
+    assert torch.equal(want, got)
