@@ -73,6 +73,8 @@ def _token_rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device: i
     s0, s1, s2 = t.stride()
     if (s2 != 1 and dim > 1) or (s1 != dim and heads > 1) or (s0 < heads * dim and n > 1):
         raise ValueError(f"the heads of a token of {name} must be packed")
+    if s0 >= 1 << 31 and n > 1:     # (the call takes it in 32 bits)
+        raise ValueError(f"the tokens of {name} are 2^31 elements apart or more")
     return t.data_ptr(), (s0 if n > 1 else heads * dim)
 
 

@@ -124,3 +124,14 @@ def test_a_reorder_drops_the_verify_before_it():
     dec.commit([[0, 1], [0], []])
     assert list(dec.ctx) == [12, 11, 10]
     dec.close()
+
+
+@pytest.mark.parametrize("apart", [2 ** 31, 2 ** 32, 2 ** 32 + 512])
+def test_tokens_too_far_apart_are_refused(apart):
+    """2^32 would arrive as 0 (packed rows), 2^32 + 512 as 512."""
+    t = torch.empty(apart + 128, dtype=torch.float16, device="meta").as_strided((2, 2, 64), (apart, 64, 1))
+    with pytest.raises(ValueError, match="apart"):
+        paged._token_rows(t, "q", torch.float16, (2, 2, 64), t.get_device())
+    near = t.as_strided((2, 2, 64), (2 ** 31 - 8, 64, 1))
+    assert paged._token_rows(near, "q", torch.float16, (2, 2, 64), t.get_device())[1] == 2 ** 31 - 8
+    assert paged._token_rows(t[:1], "q", torch.float16, (1, 2, 64), t.get_device())[1] == 128
