@@ -78,6 +78,15 @@ def _token_rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device: i
     return t.data_ptr(), (s0 if n > 1 else heads * dim)
 
 
+def _counts(a, name: str) -> np.ndarray:
+    """Whole numbers as int32, none of them cut to fit."""
+    wide = np.asarray(a, dtype=np.int64)
+    got = np.ascontiguousarray(wide.astype(np.int32))
+    if not np.array_equal(got, wide):
+        raise ValueError(f"{name} must fit 32 bits")
+    return got
+
+
 def _stream_on(stream, device: int) -> Optional[int]:
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(device) or None
@@ -386,12 +395,11 @@ class PagedKVCache:
                   stream=None) -> TreePlan:
         """Plan the attention of node_counts[i] drafted tokens per sequence behind
         ctx_lens[i] cached positions of block-table row rows[i] (default i)."""
-        p = plan if plan is not None else TreePlan()
-        ctx = np.ascontiguousarray(np.asarray(ctx_lens, dtype=np.int32))
-        cnt = np.ascontiguousarray(np.asarray(node_counts, dtype=np.int32))
-        r = None if rows is None else np.ascontiguousarray(np.asarray(rows, dtype=np.int32))
+        ctx, cnt = _counts(ctx_lens, "ctx_lens"), _counts(node_counts, "node_counts")
+        r = None if rows is None else _counts(rows, "rows")
         if ctx.shape != cnt.shape or ctx.ndim != 1 or (r is not None and r.shape != ctx.shape):
             raise ValueError("ctx_lens, node_counts and rows must have one entry per sequence")
+        p = plan if plan is not None else TreePlan()
         ffi.check(ffi.lib.kvc_plan_tree(p.handle, self.handle, ffi.np_ptr(r), ffi.np_ptr(ctx),
                                         ffi.np_ptr(cnt), ctx.size, int(num_heads),
                                         _stream_on(stream, self.device)))

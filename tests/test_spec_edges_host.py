@@ -3,6 +3,7 @@ calls that are refused before any device work, and what the decoder remembers.""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -135,3 +136,14 @@ def test_tokens_too_far_apart_are_refused(apart):
     near = t.as_strided((2, 2, 64), (2 ** 31 - 8, 64, 1))
     assert paged._token_rows(near, "q", torch.float16, (2, 2, 64), t.get_device())[1] == 2 ** 31 - 8
     assert paged._token_rows(t[:1], "q", torch.float16, (1, 2, 64), t.get_device())[1] == 128
+
+
+@pytest.mark.parametrize("kind", [list, lambda a: np.array(a, dtype=np.int64)])
+def test_lengths_past_32_bits_are_refused(kind):
+    """2^32 + 5 cached positions are not 5."""
+    pool = _pool()
+    for args in (([2 ** 32 + 5], [3]), ([5], [2 ** 32 + 3]), ([2 ** 31], [1])):
+        with pytest.raises(ValueError, match="32 bits"):
+            pool.plan_tree(kind(args[0]), kind(args[1]), 4)
+    with pytest.raises(ValueError, match="32 bits"):
+        pool.plan_tree([5], [3], 4, rows=kind([2 ** 32]))
