@@ -24,8 +24,8 @@ prompt i, exactly like the sequential loop.  A sequence that has stopped (EOS)
 keeps riding along in the batch; its extra tokens are discarded.
 
 Two loops have no counterpart in the reference: ``generate_speculative_ids`` verifies
-a tree of drafted tokens per step and yields greedy decoding's tokens in fewer
-steps, and ``generate_beam_ids`` is beam search.
+a tree of drafted tokens per step and yields greedy decoding's tokens (up to rounding)
+in fewer steps, and ``generate_beam_ids`` is beam search.
 """
 
 from __future__ import annotations
@@ -324,7 +324,10 @@ class BatchGenerator:
         token and its draft through the layers at once (``BatchDecoder.verify``), follows
         the drafted tokens that are the argmax of the node above them, keeps that path
         (``commit``) and adds the argmax behind it: the ids are those of greedy decoding
-        whatever is drafted.  Metrics count the steps and the drafted and accepted tokens."""
+        whatever is drafted, up to rounding.  (Several tokens of a step are rotated by angles of
+        64 bits where single ones have the reference's 32, and their sums run in another
+        order, so where two logits are within a few fp16 steps the other may win.)
+        Metrics count the steps and the drafted and accepted tokens."""
         cfg = self.model.cfg
         prompts = self._check_prompts(batch_prompt_ids, 1, max_new_tokens)
         b = len(prompts)
@@ -360,9 +363,11 @@ class BatchGenerator:
                         room = min(max_new_tokens - len(outs[i]) - 1,
                                    self.max_seq_len - int(dec.ctx[i]) - 1,
                                    ffi.MAX_TREE_NODES - 1)
+                        if len(toks) != len(par):
+                            raise ValueError("the draft needs one parent per token")
                         toks, par = [int(t) for t in toks][:room], [int(q) for q in par][:room]
-                        if len(toks) != len(par) or any(not 0 <= t < cfg.vocab for t in toks):
-                            raise ValueError("the draft needs one parent per token of the vocabulary")
+                        if any(not 0 <= t < cfg.vocab for t in toks):
+                            raise ValueError("a drafted token id is outside the vocabulary")
                         tokens += [outs[i][-1]] + toks
                         trees.append([-1] + [q + 1 for q in par])
                         stats["drafted"] += len(toks)

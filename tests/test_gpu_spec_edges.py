@@ -484,3 +484,21 @@ def test_a_tree_plan_is_not_built_inside_a_capture():
     pool.decode_tree(plan, 0, q, None, got.zero_(), bt, 0.1)
     no_error()
     assert torch.equal(want, got)
+
+
+# -- drafts ---------------------------------------------------------------------------------------------
+def test_drafts_with_missing_parents_are_refused(gen):  # noqa: F811
+    """Also where the missing ones lie behind what there is room for."""
+    prompts = [[3, 14, 15, 9, 2, 6, 5]]
+    for draft in (([1, 2, 3, 4], [-1, 0, 1]), ([1, 2, 3, 4, 5, 6], [-1, 0, 1, 2]), ([1], []), ([], [-1])):
+        with pytest.raises(ValueError, match="parent"):
+            gen.generate_speculative_ids(prompts, lambda i, ids: draft, max_new_tokens=4,
+                                         stop_on_eos=False)
+    for draft in (([64], [-1]), ([-1], [-1])):
+        with pytest.raises(ValueError, match="vocabulary"):
+            gen.generate_speculative_ids(prompts, lambda i, ids: draft, max_new_tokens=4,
+                                         stop_on_eos=False)
+    want, _ = gen.generate_batch_ids(prompts, max_new_tokens=4, stop_on_eos=False)
+    got, _ = gen.generate_speculative_ids(prompts, lambda i, ids: ([1] * 90, [-1] * 90), max_new_tokens=4,
+                                          stop_on_eos=False)
+    assert got == want
