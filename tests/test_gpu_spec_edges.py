@@ -10,6 +10,8 @@ import numpy as np
 import pytest
 
 from conftest import HAS_GPU
+from test_gpu_spec_generate import gen  # noqa: F401  (a fixture)
+from test_gpu_spec_ops import BF16, F16, F32, dev, no_error, raw
 
 pytestmark = pytest.mark.gpu
 
@@ -21,8 +23,6 @@ if HAS_GPU:
     import kvcache_ffi as ffi
     import paged
     from test_gpu_batch_generate import _model
-    from test_gpu_spec_ops import BF16, F16, F32, dev, no_error, raw
-    from test_gpu_spec_generate import gen  # noqa: F401  (a fixture)
 
 
 # -- tree attention: a flat tail far below one peak ------------------------------------------
