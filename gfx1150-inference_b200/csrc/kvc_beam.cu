@@ -390,40 +390,23 @@ __global__ void __launch_bounds__(32 * kMaxBeams) beam_merge_kernel(const BeamAr
 
 int beam_chunks(int vocab) { return (vocab + kMinChunk - 1) / kMinChunk; }
 
-namespace {
-// A launch that may begin before the one ahead of it has ended; it lets its successor begin
-// only once all before it has.
-template <typename K>
-cudaError_t launch_early(K kernel, dim3 grid, int threads, cudaStream_t s, const BeamArgs& a) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
-}
-}  // namespace
-
+// (both kernels let their successor begin only once all before them has ended)
 cudaError_t launch_beam_select(BeamArgs a, cudaStream_t s) {
   // Longer runs spread a warp's sorting over more logits; shorter ones fill the GPU.
   const int rows = a.n * a.beams, most = beam_chunks(a.vocab);
   a.batches = kMaxBatches;
-  while (a.batches > 1 && static_cast<int64_t>(rows) * most / a.batches < 4 * 148) a.batches /= 2;
+  while (a.batches > 1 && static_cast<int64_t>(rows) * most / a.batches < 4 * a.sms) a.batches /= 2;
   a.n_chunks = (most + a.batches - 1) / a.batches;
   const dim3 grid(static_cast<unsigned>(a.n_chunks), static_cast<unsigned>(rows));
   cudaError_t e;
   switch (a.dtype) {
-    case KVC_DTYPE_F16: e = launch_early(beam_chunk_kernel<__half>, grid, 32 * kChunkWarps, s, a); break;
-    case KVC_DTYPE_BF16: e = launch_early(beam_chunk_kernel<__nv_bfloat16>, grid, 32 * kChunkWarps, s, a); break;
-    case KVC_DTYPE_F32: e = launch_early(beam_chunk_kernel<float>, grid, 32 * kChunkWarps, s, a); break;
+    case KVC_DTYPE_F16: e = launch_early(beam_chunk_kernel<__half>, grid, 32 * kChunkWarps, 0, s, a); break;
+    case KVC_DTYPE_BF16: e = launch_early(beam_chunk_kernel<__nv_bfloat16>, grid, 32 * kChunkWarps, 0, s, a); break;
+    case KVC_DTYPE_F32: e = launch_early(beam_chunk_kernel<float>, grid, 32 * kChunkWarps, 0, s, a); break;
     default: return cudaErrorInvalidValue;
   }
   if (e != cudaSuccess) return e;
-  return launch_early(beam_merge_kernel, dim3(static_cast<unsigned>(a.n)), 32 * a.beams, s, a);
+  return launch_early(beam_merge_kernel, dim3(static_cast<unsigned>(a.n)), 32 * a.beams, 0, s, a);
 }
 
 }  // namespace kvc

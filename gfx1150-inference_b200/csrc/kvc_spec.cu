@@ -359,30 +359,15 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderA
   }
 }
 
-// A launch that may begin before the one ahead of it has ended: every kernel here touches
-// what others do only behind wait_prerequisites().  None lets its own successor begin
-// early: they write K/V rows, and a decode two launches on may stream those as soon as the
-// launch between them has begun.
-template <typename A>
-cudaError_t launch_early(void (*kernel)(A), dim3 grid, int threads, cudaStream_t s, const A& args) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args);
-}
+// No kernel here lets its successor begin early: they write K/V rows, and a decode two
+// launches on may stream those as soon as the launch between them has begun.
 
 // Many tokens: 64 threads each, four in a CTA; few tokens: a CTA each.
 template <typename T, bool kNeox>
 cudaError_t run_append_rope(const AppendRopeArgs& a, cudaStream_t s) {
-  if (a.n >= 4 * 148)
-    return launch_early(append_rope_kernel<T, kNeox, 64>, dim3((a.n + 3) / 4), kAppendThreads, s, a);
-  return launch_early(append_rope_kernel<T, kNeox, kAppendThreads>, dim3(a.n), kAppendThreads, s, a);
+  if (a.n >= 4 * a.sms)
+    return launch_early(append_rope_kernel<T, kNeox, 64>, dim3((a.n + 3) / 4), kAppendThreads, 0, s, a);
+  return launch_early(append_rope_kernel<T, kNeox, kAppendThreads>, dim3(a.n), kAppendThreads, 0, s, a);
 }
 
 }  // namespace
@@ -400,14 +385,14 @@ cudaError_t launch_append_rope(const AppendRopeArgs& a, cudaStream_t s) {
 
 cudaError_t launch_commit(const CommitArgs& a, cudaStream_t s) {
   return launch_early(commit_kernel, dim3(static_cast<unsigned>(a.n_layers), static_cast<unsigned>(a.n)),
-                      kCommitThreads, s, a);
+                      kCommitThreads, 0, s, a);
 }
 
 cudaError_t launch_reorder(const ReorderArgs& a, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(2 * a.n_layers * a.p.num_kv_heads + 1), static_cast<unsigned>(a.n));
-  if (a.beams <= 4) return launch_early(reorder_kernel<4>, grid, kReorderThreads, s, a);
-  if (a.beams <= 8) return launch_early(reorder_kernel<8>, grid, kReorderThreads, s, a);
-  return launch_early(reorder_kernel<16>, grid, kReorderThreads, s, a);
+  if (a.beams <= 4) return launch_early(reorder_kernel<4>, grid, kReorderThreads, 0, s, a);
+  if (a.beams <= 8) return launch_early(reorder_kernel<8>, grid, kReorderThreads, 0, s, a);
+  return launch_early(reorder_kernel<16>, grid, kReorderThreads, 0, s, a);
 }
 
 }  // namespace kvc

@@ -51,6 +51,7 @@ struct AppendRopeArgs {
   int head_dim;
   int dtype;
   int neox;
+  int sms;                       // of the device
   double turns[kMaxRopePairs];   // inv_freq / 2 pi
 };
 
@@ -127,6 +128,7 @@ struct BeamArgs {
   int dtype;
   const float* cum;              // (n, beams)
   int n, beams, vocab, n_out;
+  int sms;                       // of the device
   int32_t* tokens;               // (n, n_out)
   int32_t* parents;
   float* scores;
@@ -137,6 +139,25 @@ struct BeamArgs {
 };
 int beam_chunks(int vocab);   // at most
 cudaError_t launch_beam_select(BeamArgs a, cudaStream_t s);
+
+// A launch that may begin before the one ahead of it has ended.  The kernels launched so
+// touch what others do only behind wait_prerequisites(); where each lets its own successor
+// begin is said beside them.
+template <typename A>
+cudaError_t launch_early(void (*kernel)(A), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                         const A& args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args);
+}
 
 cudaError_t launch_append_rope(const AppendRopeArgs& a, cudaStream_t s);
 cudaError_t launch_commit(const CommitArgs& a, cudaStream_t s);
@@ -179,6 +200,8 @@ class DeviceScope {
 
 // Device error word of `device` (which is current); looked up once.
 int device_error_word(int device, uint32_t** out);
+// SMs of `device`; looked up once.
+int sms_of(int device);
 
 }  // namespace kvc
 
@@ -217,6 +240,7 @@ struct kvc_tree_plan {
 struct kvc_beam {
   int device = 0;
   int max_seqs = 0, max_beams = 0, max_vocab = 0, max_out = 0;
+  int sms = 0;
   kvc::DevBuf ws;
   size_t ml_bytes = 0;
 };

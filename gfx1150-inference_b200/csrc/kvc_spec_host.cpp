@@ -32,6 +32,14 @@ int device_error_word(int device, uint32_t** out) {
   return KVC_OK;
 }
 
+int sms_of(int device) {
+  static std::atomic<int> sms[64];
+  if (device < 0 || device >= 64) return device_sms(device);
+  int n = sms[device].load(std::memory_order_relaxed);
+  if (n == 0) sms[device].store(n = device_sms(device), std::memory_order_relaxed);
+  return n;
+}
+
 namespace {
 
 // No C++ exception leaves a C entry point.
@@ -125,6 +133,7 @@ int do_append_rope(kvc_pool* pool, int layer, const void* d_q, int q_stride, voi
   a.head_dim = g.head_dim;
   a.dtype = g.dtype;
   a.neox = neox ? 1 : 0;
+  a.sms = sms_of(pool->device);
   for (int i = 0; i < g.head_dim / 2; ++i)
     a.turns[i] = std::pow(static_cast<double>(freq_base), -2.0 * i / g.head_dim) /
                  6.283185307179586476925286766559;
@@ -199,7 +208,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   if (num_heads <= 0 || num_heads % g.num_kv_heads != 0)
     return set_error(KVC_ERR_INVALID_ARG, "num_heads must be divisible by num_kv_heads.");
   p->valid = false;
-  const int group = num_heads / g.num_kv_heads, sms = device_sms(pool->device);
+  const int group = num_heads / g.num_kv_heads, sms = sms_of(pool->device);
   int64_t tokens = 0, tiles = 0, runs = 0, max_end = 0, small = 0;
   int max_row = 0, max_nodes = 0;
   std::vector<int32_t> rows, slots;
@@ -551,6 +560,7 @@ extern "C" int kvc_beam_create(int max_seqs, int max_beams, int max_vocab, int m
     b->max_beams = max_beams;
     b->max_vocab = max_vocab;
     b->max_out = max_out;
+    b->sms = sms_of(device);
     b->ml_bytes = (sizeof(float2) * slots + 255) & ~static_cast<size_t>(255);
     const cudaError_t e = b->ws.ensure(b->ml_bytes + sizeof(uint64_t) * slots * max_out);
     if (e != cudaSuccess) {
@@ -605,6 +615,7 @@ extern "C" int kvc_beam_select(kvc_beam_t* beam, const void* d_logits, int dtype
     a.beams = n_beams;
     a.vocab = vocab;
     a.n_out = n_out;
+    a.sms = beam->sms;
     a.tokens = d_tokens;
     a.parents = d_parents;
     a.scores = d_scores_out;

@@ -1224,27 +1224,9 @@ cudaError_t allow_smem(size_t smem) {
   return e;
 }
 
-// A launch that may begin before the one ahead of it has ended: every kernel here reads
-// and writes what others do only behind wait_prerequisites(), and lets its successor begin
-// only there, so that nothing written ahead of it is still on its way then.  The merge asks for the
-// attention kernels' shared-memory split, so that an SM passes from one to the other
-// without a change of it.
-template <typename A>
-cudaError_t launch_early(void (*kernel)(A), dim3 grid, int threads, size_t smem, cudaStream_t s,
-                         const A& args) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args);
-}
-
+// Every kernel here lets its successor begin right behind its own wait, so that nothing
+// written ahead of it is still on its way then.  The merge asks for the attention kernels'
+// shared-memory split, so that an SM passes from one to the other without a change of it.
 template <auto Kernel>
 cudaError_t prefer_shared() {
   static std::atomic<bool> done[64];
