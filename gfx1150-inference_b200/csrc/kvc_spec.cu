@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_rope_kernel(const Ap
 // apart: a later source lies behind every slot written before it.
 // The rows come in 16-byte pieces 128 bytes apart, and memory is read 64 bytes at a time:
 // the sources alone cost four times their bytes, which is what bounds this (32 paths of up
-// to 8 nodes, 32 layers: 18 MB moved, 107 MB read, 22 us).
+// to 8 nodes, 32 layers: 18 MB moved, 107 MB read; 27 us over states in turn that do not stay
+// in L2, 22 on one that does).
 // =====================================================================================
 constexpr int kCommitThreads = 128;
 constexpr int kCommitSteps = 8;     // of a path at a time
@@ -281,9 +282,10 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
 // head of one layer's K or V in the open pages.  A thread owns one 16-byte unit of a page
 // for all beams: it reads every moved beam's new value, then writes, so the permutation
 // happens in place without a second buffer.  The units in front of `tail` positions are
-// taken in the order of memory; of the last 8-position block only some rows are.  Bound by
-// memory traffic: 8 x 8 beams, 32 layers, 149 MB in 27.7 us (23 at the copy rate; 28.4 with
-// 128 threads, 44 with 256).
+// taken in the order of memory; of the last 8-position block only some rows are.  8 x 8
+// beams, 32 layers, 149 MB: 32.4 us over states in turn (23 at the copy rate), where each of
+// the 4,104 short CTAs makes its sequence's checks before its first byte moves; replayed on
+// one state, part of which stays in L2, 27 (28.4 with 128 threads, 44 with 256).
 // =====================================================================================
 constexpr int kReorderThreads = 64;
 
