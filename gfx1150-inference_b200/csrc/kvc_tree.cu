@@ -462,7 +462,8 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
             }
           }
           copy_async_wait();
-          if (flip) {   // a negative scale turns q
+          if (flip) {   // a negative scale turns q: what other lanes have copied, too
+            __syncwarp();
             for (int i = lane; i < S::kStreams * S::kQBytes / 4; i += 32)
               reinterpret_cast<uint32_t*>(q_mem)[i] ^= flip;
           }

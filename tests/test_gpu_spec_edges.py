@@ -502,3 +502,24 @@ def test_drafts_with_missing_parents_are_refused(gen):  # noqa: F811
     got, _ = gen.generate_speculative_ids(prompts, lambda i, ids: ([1] * 90, [-1] * 90), max_new_tokens=4,
                                           stop_on_eos=False)
     assert got == want
+
+
+# -- a negative scale ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d,nodes", [(64, 3), (128, 60), (256, 33), (80, 20)])
+def test_tree_with_a_negative_scale_is_the_tree_of_negated_queries(dtype, d, nodes):
+    """Bit for bit, in every piece of a CTA: q changes sign where it is copied, and again and
+    again for new queries in the same place."""
+    dt = getattr(torch, dtype)
+    seqs, ctx, cols = 300, 40, 8
+    pool = paged.PagedKVCache(1, seqs * cols, 16, 1, d, dtype=dt)
+    pool.fill_normal(seed=6)
+    bt = dev(np.random.default_rng(d).permutation(seqs * cols).reshape(seqs, cols))
+    plan = pool.plan_tree([ctx] * seqs, [nodes] * seqs, 4)
+    for k in range(3):
+        q = torch.randn(seqs * nodes, 4, d, device="cuda").to(dt)
+        a, b = torch.zeros_like(q), torch.zeros_like(q)
+        pool.decode_tree(plan, 0, q, None, a, bt, -0.1)
+        pool.decode_tree(plan, 0, -q, None, b, bt, 0.1)
+        no_error()
+        assert torch.equal(a, b)
