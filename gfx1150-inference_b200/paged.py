@@ -684,7 +684,8 @@ class BatchDecoder:
             par = _upload(parents, self.bt.device)
             lens = _upload(ctx[:, 0].astype(np.int32), self.bt.device)
         self._drafted = None      # (drafted rows lie behind the positions that move)
-        self.cache.reorder_beams(self.bt, par, lens, stream=stream)
+        # (the table may have rows behind the decoder's)
+        self.cache.reorder_beams(self.bt[:parents.size], par, lens, stream=stream)
 
     def _layers(self, x: torch.Tensor, stream) -> torch.Tensor:
         with _made_on(stream, self.bt.device):

@@ -147,3 +147,17 @@ def test_lengths_past_32_bits_are_refused(kind):
             pool.plan_tree(kind(args[0]), kind(args[1]), 4)
     with pytest.raises(ValueError, match="32 bits"):
         pool.plan_tree([5], [3], 4, rows=kind([2 ** 32]))
+
+
+def test_reorder_takes_the_decoder_s_rows_of_a_longer_table():
+    seen = []
+
+    class Cache(_Cache):
+        def reorder_beams(self, table, parents, lens, stream=None):
+            seen.append((table.data_ptr(), table.shape, parents.tolist(), lens.tolist()))
+
+    bt = torch.zeros((6, 4), dtype=torch.int32)
+    dec = paged.BatchDecoder(Cache(), [object(), object()], bt, 8, [10, 10, 7, 7])
+    dec.reorder([[1, 0], [1, 1]])
+    assert seen == [(bt.data_ptr(), (4, 4), [[1, 0], [1, 1]], [10, 7])]
+    dec.close()
