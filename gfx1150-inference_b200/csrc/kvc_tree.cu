@@ -88,6 +88,15 @@ constexpr float kRescaleAt = 8.0f;   // log2
 // log2 of the factor on the probabilities of a storage type (bf16 has fp32's exponents).
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+// What a row's largest scaled score (log2 units) is taken for.  Past 2^22, where the
+// rounding of the score itself comes on top and counts, the factor would take probabilities
+// out of fp16's range.
+template <typename T>
+__device__ __forceinline__ float row_max(float score, float scale) {
+  if (score == -INFINITY) return kNegBig;
+  const float x = score * scale;
+  return fabsf(x) < 4194304.0f ? x - kLift<T> : x;
+}
 constexpr int kPieceCost = 4;        // a piece's start and end, in tiles
 
 template <int D>
@@ -588,7 +597,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
             }
           }
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          mt = mx == -INFINITY ? kNegBig : mx * sc - kLift<T>;
+          mt = row_max<T>(mx, sc);
         };
         if (t < ahead) {
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -603,7 +612,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
               if (!kEdge || ((vis[w] >> i) & 1u)) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[i]));
           }
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          m = mx == -INFINITY ? kNegBig : mx * sc - kLift<T>;
+          m = row_max<T>(mx, sc);
         }
         for (;;) {
           pass();

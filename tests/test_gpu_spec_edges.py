@@ -523,3 +523,57 @@ def test_tree_with_a_negative_scale_is_the_tree_of_negated_queries(dtype, d, nod
         pool.decode_tree(plan, 0, -q, None, b, bt, 0.1)
         no_error()
         assert torch.equal(a, b)
+
+
+# -- scores whose rounding outweighs every difference -------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("size", [100.0, 700.0, 1100.0, 1500.0, 2000.0, 2600.0])
+def test_tree_with_huge_scores_stays_a_weighted_mean(dtype, size):
+    """Scores of 1e5 to 8e7, all nearly equal: whatever the weights, equal values come out as
+    they are, up to the probabilities' rounding (h relative each) and the output's.  The max
+    creeps up along the context, several tiles a piece."""
+    dt = getattr(torch, dtype)
+    seqs, hkv, d, ctx, n = 40, 8, 128, 700, 2
+    cols = -(-(ctx + n) // 16)
+    pool = paged.PagedKVCache(1, seqs * cols, 16, hkv, d, dtype=dt)
+    bt = dev(np.arange(seqs * cols).reshape(seqs, cols))
+    g = torch.Generator(device="cuda")
+    g.manual_seed(int(size))
+    pos = torch.arange(ctx + n, dtype=torch.int32, device="cuda")
+    v = torch.full((ctx + n, hkv, d), 3.0, dtype=dt, device="cuda")
+    creep = torch.linspace(1.0, 1.0 + 2.0 ** -7, ctx + n, device="cuda")[:, None, None]
+    for i in range(seqs):
+        k = size * creep * (1 + 2.0 ** -10 * torch.randn(ctx + n, hkv, d, generator=g, device="cuda"))
+        pool.append(0, k.to(dt), v, bt, pos, torch.full_like(pos, i))
+    q = torch.full((seqs * n, hkv, d), size, device="cuda").to(dt)
+    out = torch.zeros_like(q)
+    pool.decode_tree(pool.plan_tree([ctx] * seqs, [n] * seqs, hkv), 0, q, None, out, bt, 0.088)
+    no_error()
+    half = torch.finfo(dt).eps / 2
+    assert float((out.double() - 3.0).abs().max()) <= 3.0 * (2 * half + 2.0 ** -14)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_tree_with_huge_scores_that_grow_by_less_than_a_rescaling(dtype):
+    """Scores of 6e7 (a step of fp32 is worth 2^4), the later half 2^7.9 above the first: O is
+    not rescaled for that, and the probabilities must still fit their type."""
+    dt = getattr(torch, dtype)
+    seqs, hkv, d, ctx, n = 40, 8, 128, 700, 2
+    cols = -(-(ctx + n) // 16)
+    pool = paged.PagedKVCache(1, seqs * cols, 16, hkv, d, dtype=dt)
+    bt = dev(np.arange(seqs * cols).reshape(seqs, cols))
+    pos = torch.arange(ctx + n, dtype=torch.int32, device="cuda")
+    v = torch.full((ctx + n, hkv, d), 3.0, dtype=dt, device="cuda")
+    for i in range(seqs):
+        k = torch.full((ctx + n, hkv, d), 2000.0 - 8 * i, device="cuda")
+        k[:, :, 0] = 0.0
+        k[256:, :, 0] = 64.0
+        pool.append(0, k.to(dt), v, bt, pos, torch.full_like(pos, i))
+    q = torch.full((seqs * n, hkv, d), 1.0, device="cuda")
+    q[:, :, 1:] = (1960.0 + 8 * torch.arange(hkv, device="cuda"))[:, None]
+    q = q.to(dt)
+    out = torch.zeros_like(q)
+    pool.decode_tree(pool.plan_tree([ctx] * seqs, [n] * seqs, hkv), 0, q, None, out, bt, 0.0856)
+    no_error()
+    half = torch.finfo(dt).eps / 2
+    assert float((out.double() - 3.0).abs().max()) <= 3.0 * (2 * half + 2.0 ** -14)
