@@ -1,0 +1,556 @@
+// Kernels of a serving step around the attention itself:
+//   norm_rope_kernel    RMSNorm and rotation of q and the new K heads fused with the scatter
+//                       of the K/V rows into the paged pool
+//   evict_select_kernel the slots that stay, by their summed attention weights
+//   evict_move_kernel   their K/V rows moved together, all layers
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "kvc_device.cuh"
+#include "kvc_paged.cuh"
+#include "kvc_serve.h"
+
+namespace kvc {
+namespace {
+
+// =====================================================================================
+// Norm + rotate + append.  y = R(p) (x w / sqrt(mean(x^2) + eps)) for the heads of q and K,
+// V as it is.  kPer threads take a token: its angles are computed once and serve all its
+// heads (turns in 64 bits with the whole ones removed, then sincospif, as append_rope_kernel
+// does), each pair with the position of its own axis.  A head belongs to kLanes lanes of one
+// warp, each of which owns two 16-byte units that hold each other's pairs, so the sum of
+// squares is a few shuffles and the head is read once.  All in 32 bits, rounded once.
+// =====================================================================================
+constexpr int kNormThreads = 256;
+constexpr int kNormBatch = 2;      // heads of a lane group on their way
+
+template <typename T, bool kNeox, int kPer, int kLanes>
+__global__ void __launch_bounds__(kNormThreads) norm_rope_kernel(const NormRopeArgs a) {
+  constexpr int kTok = kNormThreads / kPer, kAtOnce = kPer / kLanes;
+  constexpr int N = Unit<T>::N;
+  __shared__ float2 cs[kTok * kMaxRopePairs];
+  __shared__ int s_page[kTok], s_slot[kTok];
+  const int tok0 = blockIdx.x * kTok;
+  const int toks = min(kTok, a.n - tok0);
+  const int U = a.p.row_units, Hkv = a.p.num_kv_heads, H = a.num_heads;
+  const int heads = H + 2 * Hkv;                     // q, K and V heads
+  const int tok = threadIdx.x / kPer, me = threadIdx.x % kPer;
+  const int row0 = me / kLanes, i = me % kLanes;     // first head, unit pair
+  const bool works = i < U / 2 && tok < toks;
+  const int turned = a.pairs / N;                    // unit pairs that are rotated
+  const bool turns = i < turned;
+  // the rotated front of a NeoX head: units i and i + turned; neighbours otherwise
+  const int u0 = kNeox && turns ? i : 2 * i, du = kNeox && turns ? turned : 1;
+  const size_t t = tok0 + tok;
+  const size_t row_bytes = static_cast<size_t>(U) * 16;
+  wait_prerequisites();
+
+  struct Item {
+    Unit<T> x0, x1;
+  };
+  const uint8_t* q_src = a.q + t * a.q_stride + u0 * 16;
+  const uint8_t* k_src = a.k_new + t * a.k_stride + u0 * 16;
+  const uint8_t* v_src = a.v_new + t * a.v_stride + u0 * 16;
+  auto load = [&](int head, Item& it) {
+    if (!works || head >= heads) {
+      it.x0.raw = it.x1.raw = make_uint4(0, 0, 0, 0);
+      return;
+    }
+    const uint8_t* src = head < H         ? q_src + head * row_bytes
+                         : head < H + Hkv ? k_src + (head - H) * row_bytes
+                                          : v_src + (head - H - Hkv) * row_bytes;
+    it.x0.raw = *reinterpret_cast<const uint4*>(src);
+    it.x1.raw = *reinterpret_cast<const uint4*>(src + du * 16);
+  };
+  Item items[kNormBatch];
+#pragma unroll
+  for (int k = 0; k < kNormBatch; ++k) load(row0 + k * kAtOnce, items[k]);
+  Item wq = {}, wk = {};
+  if (works && a.q_weight) {
+    wq.x0.raw = *reinterpret_cast<const uint4*>(a.q_weight + u0 * 16);
+    wq.x1.raw = *reinterpret_cast<const uint4*>(a.q_weight + (u0 + du) * 16);
+  }
+  if (works && a.k_weight) {
+    wk.x0.raw = *reinterpret_cast<const uint4*>(a.k_weight + u0 * 16);
+    wk.x1.raw = *reinterpret_cast<const uint4*>(a.k_weight + (u0 + du) * 16);
+  }
+
+  for (int x = threadIdx.x; x < toks * a.pairs; x += kNormThreads) {
+    const int tk = kTok == 1 ? 0 : x / a.pairs, j = x - tk * a.pairs;
+    double turn = static_cast<double>(a.rope_positions[static_cast<size_t>(tok0 + tk) * a.axes +
+                                                       a.axis[j]]) * a.turns[j];
+    turn -= rint(turn);
+    // (by pair of a unit pair, then unit pair: neighbouring threads read neighbouring angles)
+    float2& out = cs[tk * kMaxRopePairs + j % N * turned + j / N];
+    sincospif(2.0f * static_cast<float>(turn), &out.y, &out.x);
+  }
+  if (threadIdx.x < toks) {
+    const int pos = a.positions[tok0 + threadIdx.x];
+    s_page[threadIdx.x] = pos < 0 ? -1 : page_of(a.p, a.rows ? a.rows[tok0 + threadIdx.x] : 0, pos);
+    s_slot[threadIdx.x] = pos < 0 ? 0 : pos % a.p.page_size;
+  }
+  __syncthreads();
+  if (tok >= toks) return;                           // (a warp has one token)
+  const int page = s_page[tok];
+  if (page < 0) return;                              // padding, or reported
+  float2 c[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    c[k] = turns ? cs[tok * kMaxRopePairs + k * turned + i] : make_float2(1.f, 0.f);
+  uint8_t* q_dst = a.q_out + t * H * row_bytes + u0 * 16;
+  const size_t place = unit_at(a.p, page, 0, s_slot[tok], u0);
+  const int dp = du * (a.p.layout == kLayoutCore ? 128 : 16);
+  const float inv_d = 1.0f / a.head_dim;
+  const int last = heads - 1;
+  // (every lane of a warp goes through every round: the shuffles need them all)
+  for (int h0 = row0; h0 - row0 <= last; h0 += kNormBatch * kAtOnce) {
+#pragma unroll
+    for (int k = 0; k < kNormBatch; ++k) {
+      const int head = h0 + k * kAtOnce;
+      Item& it = items[k];
+      const bool is_q = head < H, is_k = !is_q && head < H + Hkv;
+      const bool normed = is_q ? a.q_weight != nullptr : is_k && a.k_weight != nullptr;
+      float x0[N], x1[N], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        x0[e] = to_f32<T>(it.x0.v[e]);
+        x1[e] = to_f32<T>(it.x1.v[e]);
+        sum = fmaf(x0[e], x0[e], sum);
+        sum = fmaf(x1[e], x1[e], sum);
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (works && head < heads) {
+        if (normed) {
+          const float r = rsqrtf(fmaf(sum, inv_d, a.eps));
+          const Item& w = is_q ? wq : wk;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            x0[e] = x0[e] * r * to_f32<T>(w.x0.v[e]);
+            x1[e] = x1[e] * r * to_f32<T>(w.x1.v[e]);
+          }
+        }
+        if ((is_q || is_k) && turns) {
+          if constexpr (kNeox) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) turn_pair(x0[e], x1[e], c[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) {
+              turn_pair(x0[2 * e], x0[2 * e + 1], c[e]);
+              turn_pair(x1[2 * e], x1[2 * e + 1], c[N / 2 + e]);
+            }
+          }
+        }
+        if (is_q || is_k) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            it.x0.v[e] = from_f32<T>(x0[e]);
+            it.x1.v[e] = from_f32<T>(x1[e]);
+          }
+        }
+        if (is_q) {
+          uint8_t* d = q_dst + head * row_bytes;
+          *reinterpret_cast<uint4*>(d) = it.x0.raw;
+          *reinterpret_cast<uint4*>(d + du * 16) = it.x1.raw;
+        } else {
+          uint8_t* d = (is_k ? a.p.k : a.p.v) + place +
+                       (head - H - (is_k ? 0 : Hkv)) * a.p.page_head_bytes;
+          *reinterpret_cast<uint4*>(d) = it.x0.raw;
+          *reinterpret_cast<uint4*>(d + dp) = it.x1.raw;
+        }
+      }
+    }
+    const int next = h0 + kNormBatch * kAtOnce;
+#pragma unroll
+    for (int k = 0; k < kNormBatch; ++k) load(next + k * kAtOnce, items[k]);
+  }
+}
+
+// Any even head dim and any number of rotated pairs: a warp takes a head, a lane every 32nd
+// pair of its dims.
+template <typename T, bool kNeox>
+__global__ void __launch_bounds__(kNormThreads) norm_rope_any_kernel(const NormRopeArgs a) {
+  constexpr int N = Unit<T>::N, kHeld = kMaxRopePairs / 32;
+  __shared__ float2 cs[kMaxRopePairs];
+  const int Hkv = a.p.num_kv_heads, H = a.num_heads, heads = H + 2 * Hkv, half = a.head_dim / 2;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const size_t t = blockIdx.x;
+  wait_prerequisites();
+  for (int j = threadIdx.x; j < a.pairs; j += kNormThreads) {
+    double turn = static_cast<double>(a.rope_positions[t * a.axes + a.axis[j]]) * a.turns[j];
+    turn -= rint(turn);
+    sincospif(2.0f * static_cast<float>(turn), &cs[j].y, &cs[j].x);
+  }
+  __shared__ int s_page;
+  const int pos = a.positions[t];
+  if (threadIdx.x == 0) s_page = pos < 0 ? -1 : page_of(a.p, a.rows ? a.rows[t] : 0, pos);
+  __syncthreads();
+  const int page = s_page;
+  if (page < 0) return;                              // padding, or reported
+  const int slot = pos % a.p.page_size;
+  for (int head = warp; head < heads; head += kNormThreads / 32) {
+    const bool is_q = head < H, is_k = !is_q && head < H + Hkv;
+    const int h = head - (is_q ? 0 : is_k ? H : H + Hkv);
+    const T* src = reinterpret_cast<const T*>(is_q   ? a.q + t * a.q_stride
+                                              : is_k ? a.k_new + t * a.k_stride
+                                                     : a.v_new + t * a.v_stride) +
+                   static_cast<size_t>(h) * a.head_dim;
+    const T* w = reinterpret_cast<const T*>(is_q ? a.q_weight : is_k ? a.k_weight : nullptr);
+    auto dims = [&](int j, int& i0, int& i1) {
+      const bool apart = kNeox && j < a.pairs;
+      i0 = apart ? j : 2 * j;
+      i1 = apart ? j + a.pairs : 2 * j + 1;
+    };
+    T x[kHeld][2];
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int j = lane + 32 * k;
+      if (j >= half) continue;
+      int i0, i1;
+      dims(j, i0, i1);
+      x[k][0] = src[i0];
+      x[k][1] = src[i1];
+      const float f0 = to_f32<T>(x[k][0]), f1 = to_f32<T>(x[k][1]);
+      sum = fmaf(f0, f0, sum);
+      sum = fmaf(f1, f1, sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float r = rsqrtf(fmaf(sum, 1.0f / a.head_dim, a.eps));
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int j = lane + 32 * k;
+      if (j >= half) continue;
+      int i0, i1;
+      dims(j, i0, i1);
+      if (is_q || is_k) {
+        float f0 = to_f32<T>(x[k][0]), f1 = to_f32<T>(x[k][1]);
+        if (w) {
+          f0 = f0 * r * to_f32<T>(w[i0]);
+          f1 = f1 * r * to_f32<T>(w[i1]);
+        }
+        if (j < a.pairs) turn_pair(f0, f1, cs[j]);
+        x[k][0] = from_f32<T>(f0);
+        x[k][1] = from_f32<T>(f1);
+      }
+      if (is_q) {
+        T* dst = reinterpret_cast<T*>(a.q_out) + (t * H + h) * a.head_dim;
+        dst[i0] = x[k][0];
+        dst[i1] = x[k][1];
+      } else {
+        uint8_t* dst = is_k ? a.p.k : a.p.v;
+        reinterpret_cast<T*>(dst + unit_at(a.p, page, h, slot, i0 / N))[i0 % N] = x[k][0];
+        reinterpret_cast<T*>(dst + unit_at(a.p, page, h, slot, i1 / N))[i1 % N] = x[k][1];
+      }
+    }
+  }
+}
+
+// Many tokens: 64 threads each, four in a CTA; few tokens: a CTA each.
+template <typename T, bool kNeox, int kLanes>
+cudaError_t run_norm_rope(const NormRopeArgs& a, int sms, cudaStream_t s) {
+  if (a.n >= 4 * sms)
+    return launch_early(norm_rope_kernel<T, kNeox, 64, kLanes>, dim3((a.n + 3) / 4), kNormThreads, 0, s, a);
+  return launch_early(norm_rope_kernel<T, kNeox, kNormThreads, kLanes>, dim3(a.n), kNormThreads, 0, s, a);
+}
+
+template <typename T, bool kNeox>
+cudaError_t run_norm_rope_any(const NormRopeArgs& a, int sms, cudaStream_t s) {
+  const int units = a.p.row_units;
+  if (units % 2 == 0 && a.pairs % Unit<T>::N == 0) {
+    if (units <= 8) return run_norm_rope<T, kNeox, 4>(a, sms, s);
+    if (units <= 16) return run_norm_rope<T, kNeox, 8>(a, sms, s);
+    if (units <= 32) return run_norm_rope<T, kNeox, 16>(a, sms, s);
+    return run_norm_rope<T, kNeox, 32>(a, sms, s);
+  }
+  return launch_early(norm_rope_any_kernel<T, kNeox>, dim3(a.n), kNormThreads, 0, s, a);
+}
+
+template <typename T>
+cudaError_t run_norm_rope_type(const NormRopeArgs& a, bool neox, int sms, cudaStream_t s) {
+  return neox ? run_norm_rope_any<T, true>(a, sms, s) : run_norm_rope_any<T, false>(a, sms, s);
+}
+
+// =====================================================================================
+// Which slots stay.  A CTA takes one (layer, sequence, KV head): of the slots in front of
+// the last `recent` it keeps the budget - recent heaviest, found by a radix search for the
+// weight of the last of them, eight bits a pass, over keys that wait in shared memory; equal
+// weights at the border go to the lowest slots.  One ordered pass then writes the kept slots
+// and their weights, which may go to where they came from: a slot never moves up.
+// =====================================================================================
+constexpr int kSelectThreads = 256;
+constexpr int kSelectKeys = 8192;    // kept in shared memory; longer rows are read again
+
+// Larger for a larger weight; what is not a number comes last.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return 0u;
+  w += 0.0f;                          // (-0 ties with 0)
+  const uint32_t u = __float_as_uint(w);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
+  extern __shared__ uint32_t s_key[];
+  __shared__ uint32_t s_hist[kSelectThreads];
+  __shared__ uint32_t s_digit, s_need;
+  __shared__ int s_warp[2][kSelectThreads / 32];
+  constexpr int kWarps = kSelectThreads / 32;
+  const int head = blockIdx.x, seq = blockIdx.y, layer = blockIdx.z;
+  const int Hkv = a.p.num_kv_heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  wait_prerequisites();
+  const int n = a.ctx[seq], row = a.rows ? a.rows[seq] : seq;
+  int32_t* kept = a.kept + ((static_cast<size_t>(layer) * a.n + seq) * Hkv + head) * a.budget;
+  const bool fits = row >= 0 && row < a.p.bt_rows && row < a.weight_rows && n >= 0 &&
+                    n <= a.weight_slots && n <= static_cast<int64_t>(a.p.bt_stride) * a.p.page_size;
+  if (!fits) {
+    if (tid == 0) report_error_at(a.p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(n));
+    for (int j = tid; j < a.budget; j += kSelectThreads) kept[j] = -1;
+    return;
+  }
+  const size_t base = ((static_cast<size_t>(layer) * a.weight_rows + row) * Hkv + head) * a.weight_slots;
+  const float* w = a.weights + base;
+  float* left = a.weights_out + base;
+  if (n <= a.budget) {
+    for (int j = tid; j < a.budget; j += kSelectThreads) {
+      kept[j] = j < n ? j : -1;
+      if (j < n && left != w) left[j] = w[j];
+    }
+    return;
+  }
+  const int old = n - a.recent, take = a.budget - a.recent;   // take of [0, old), all behind
+  uint32_t need = take, border = 0;                           // keys above it: take - need
+  const bool held = old <= kSelectKeys;
+  if (held)
+    for (int i = tid; i < old; i += kSelectThreads) s_key[i] = weight_key(w[i]);
+  auto key = [&](int i) { return held ? s_key[i] : weight_key(w[i]); };
+  if (take > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      s_hist[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < old; i += kSelectThreads) {
+        const uint32_t k = key(i);
+        if (shift == 24 || (k >> (shift + 8)) == (border >> (shift + 8)))
+          atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+      }
+      __syncthreads();
+      // the digit of the need-th largest: thread d sums the bins above its own
+      if (warp == 0) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) mine += s_hist[lane * 8 + b];
+        uint32_t above = mine;                       // of this lane's bins and those above
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t v = __shfl_down_sync(0xffffffffu, above, o);
+          if (lane + o < 32) above += v;
+        }
+        uint32_t over = above - mine;
+        if (over < need && need <= above) {
+          for (int b = 7; b >= 0; --b) {
+            const uint32_t cnt = s_hist[lane * 8 + b];
+            if (need <= over + cnt) {
+              s_digit = lane * 8 + b;
+              s_need = need - over;
+              break;
+            }
+            over += cnt;
+          }
+        }
+      }
+      __syncthreads();
+      border |= s_digit << shift;
+      need = s_need;
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  // In order: slots above the border, and the first `need` on it.
+  int at = 0, ties = 0;                                       // written and ties so far
+  for (int i0 = 0; i0 < old && take > 0; i0 += kSelectThreads) {
+    const int i = i0 + tid;
+    const uint32_t k = i < old ? key(i) : 0u;
+    const bool over = i < old && k > border, tie = i < old && k == border;
+    const float wi = i < old ? w[i] : 0.f;
+    const uint32_t b_over = __ballot_sync(0xffffffffu, over), b_tie = __ballot_sync(0xffffffffu, tie);
+    if (lane == 0) {
+      s_warp[0][warp] = __popc(b_over);
+      s_warp[1][warp] = __popc(b_tie);
+    }
+    __syncthreads();                                          // (w[i] is read by all, too)
+    int my_over = 0, my_tie = 0, all_over = 0, all_tie = 0;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+      if (v == warp) {
+        my_over = all_over;
+        my_tie = all_tie;
+      }
+      all_over += s_warp[0][v];
+      all_tie += s_warp[1][v];
+    }
+    const uint32_t below = (1u << lane) - 1u;
+    my_over += __popc(b_over & below);
+    my_tie += __popc(b_tie & below);
+    const int ties_before = min(ties + my_tie, static_cast<int>(need));
+    if (over || (tie && ties + my_tie < static_cast<int>(need))) {
+      const int j = at + my_over + ties_before - min(ties, static_cast<int>(need));
+      kept[j] = i;
+      left[j] = wi;
+    }
+    const int ties_now = min(ties + all_tie, static_cast<int>(need));
+    at += all_over + ties_now - min(ties, static_cast<int>(need));
+    ties += all_tie;
+    __syncthreads();
+  }
+  for (int i0 = 0; i0 < a.recent; i0 += kSelectThreads) {
+    const int i = i0 + tid;
+    const float wi = i < a.recent ? w[old + i] : 0.f;
+    __syncthreads();
+    if (i < a.recent) {
+      kept[take + i] = old + i;
+      left[take + i] = wi;
+    }
+    __syncthreads();
+  }
+}
+
+// =====================================================================================
+// The kept rows move together.  A CTA takes some of the 16-byte columns of one head of one
+// layer's K or V and goes through the kept slots in order, a chunk at a time.  A slot never
+// moves up, so a later chunk's sources lie behind every place written before it: the next
+// chunk is read before this one is written, and only the reads of one chunk have to be done
+// (a barrier) before its first write.  Rows in front of the first one that leaves stay.
+// =====================================================================================
+constexpr int kMoveThreads = 256;
+constexpr int kMoveUnits = 8;        // 16-byte units of a thread on their way
+constexpr int kMoveRows = 256;       // rows of a chunk at most
+
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a, const int parts) {
+  __shared__ size_t s_src[3][kMoveRows], s_dst[3][kMoveRows];
+  constexpr size_t kNone = ~static_cast<size_t>(0);
+  const int seq = blockIdx.y, tid = threadIdx.x;
+  const int part = blockIdx.x % parts, head = blockIdx.x / parts, kv = blockIdx.z & 1, layer = blockIdx.z >> 1;
+  const int Hkv = a.p.num_kv_heads, U = a.p.row_units / parts, ps = a.p.page_size;
+  wait_prerequisites();
+  const int n = a.ctx[seq], m = a.budget, row = a.rows ? a.rows[seq] : seq;
+  const int32_t* kept = a.kept + ((static_cast<size_t>(layer) * a.n + seq) * Hkv + head) * m;
+  if (n <= m || kept[0] < 0) return;       // nothing leaves, or reported
+  int lo = 0, hi = m;                      // the first row that moves
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (kept[mid] > mid)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  const bool core = a.p.layout == kLayoutCore;
+  const int first = core ? lo & ~7 : lo;
+  if (lo >= m) return;
+  uint8_t* base = (kv ? a.p.v : a.p.k) + static_cast<size_t>(layer) * a.layer_bytes;
+  int chunk = kMoveThreads * kMoveUnits / U;                 // rows of a chunk
+  chunk = chunk > kMoveRows ? kMoveRows : (chunk & ~7);
+  const int chunks = (m - first + chunk - 1) / chunk;
+  auto place = [&](int pos) {
+    const int page = page_of(a.p, row, pos);
+    return page < 0 ? kNone : unit_at(a.p, page, head, pos % ps, part * U);
+  };
+  auto places = [&](int c) {               // where chunk c's rows are and go
+    for (int r = tid; r < chunk && c < chunks; r += kMoveThreads) {
+      const int j = first + c * chunk + r;
+      size_t src = kNone, dst = kNone;
+      if (j < m && kept[j] > j) {
+        src = place(kept[j]);
+        dst = place(j);
+      }
+      s_src[c % 3][r] = src == kNone || dst == kNone ? kNone : src;
+      s_dst[c % 3][r] = dst;
+    }
+  };
+  const int step = core ? 128 : 16, units = chunk * U;
+  // unit x of a chunk in the order of memory: row and byte offset within the row
+  auto split = [&](int x, int& r, int& u) {
+    if (core) {
+      r = x & 7;
+      const int y = x >> 3;
+      u = y % U;
+      r += (y / U) << 3;
+    } else {
+      r = x / U;
+      u = x - r * U;
+    }
+  };
+  uint4 now[kMoveUnits], next[kMoveUnits];
+  auto load = [&](int c, uint4* v) {
+#pragma unroll
+    for (int k = 0; k < kMoveUnits; ++k) {
+      const int x = tid + k * kMoveThreads;
+      int r, u;
+      split(x, r, u);
+      if (x < units && c < chunks && s_src[c % 3][r] != kNone)
+        v[k] = *reinterpret_cast<const uint4*>(base + s_src[c % 3][r] + u * step);
+    }
+  };
+  places(0);
+  places(1);
+  __syncthreads();
+  load(0, now);
+  for (int c = 0; c < chunks; ++c) {
+    __syncthreads();                       // chunk c has been read, chunk c - 1 written
+    places(c + 2);
+    load(c + 1, next);
+#pragma unroll
+    for (int k = 0; k < kMoveUnits; ++k) {
+      const int x = tid + k * kMoveThreads;
+      int r, u;
+      split(x, r, u);
+      if (x < units && s_src[c % 3][r] != kNone)
+        *reinterpret_cast<uint4*>(base + s_dst[c % 3][r] + u * step) = now[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kMoveUnits; ++k) now[k] = next[k];
+  }
+}
+
+}  // namespace
+
+// (No kernel here lets its successor begin early: they write K/V rows, and a decode two
+// launches on may stream those as soon as the launch between them has begun.)
+
+cudaError_t launch_norm_rope(const NormRopeArgs& a, int dtype, bool neox, int sms, cudaStream_t s) {
+  switch (dtype) {
+    case KVC_DTYPE_F16: return run_norm_rope_type<__half>(a, neox, sms, s);
+    case KVC_DTYPE_BF16: return run_norm_rope_type<__nv_bfloat16>(a, neox, sms, s);
+    case KVC_DTYPE_F32: return run_norm_rope_type<float>(a, neox, sms, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_evict(const EvictArgs& a, int sms, cudaStream_t s) {
+  const size_t keys = sizeof(uint32_t) * std::min(kSelectKeys, a.weight_slots);
+  cudaError_t e = launch_early(evict_select_kernel,
+                               dim3(static_cast<unsigned>(a.p.num_kv_heads), static_cast<unsigned>(a.n),
+                                    static_cast<unsigned>(a.n_layers)),
+                               kSelectThreads, keys, s, a);
+  if (e != cudaSuccess) return e;
+  // few heads: their columns are spread over more CTAs
+  const int64_t heads = 2ll * a.n_layers * a.n * a.p.num_kv_heads;
+  int parts = 1;
+  while (heads * parts < 2 * sms && a.p.row_units % (2 * parts) == 0) parts *= 2;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.p.num_kv_heads * parts), static_cast<unsigned>(a.n),
+                     static_cast<unsigned>(2 * a.n_layers));
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, evict_move_kernel, a, parts);
+}
+
+}  // namespace kvc

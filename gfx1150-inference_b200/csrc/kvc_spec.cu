@@ -12,42 +12,12 @@
 #include <algorithm>
 
 #include "kvc_device.cuh"
+#include "kvc_paged.cuh"
 #include "kvc_spec.h"
 #include "kvcache.h"
 
 namespace kvc {
 namespace {
-
-// Byte offset of unit u of position t of a page's KV head h.
-__device__ __forceinline__ size_t unit_at(const PagedView& p, int page, int h, int t, int u) {
-  return (static_cast<size_t>(page) * p.num_kv_heads + h) * p.page_head_bytes +
-         unit_offset(p.layout, t, u, p.row_units) * 16;
-}
-
-// The page of `pos` in block-table row `row`, or -1 with the error reported.
-__device__ __forceinline__ int page_of(const PagedView& p, int row, int pos) {
-  const int col = pos / p.page_size;
-  if (row < 0 || row >= p.bt_rows || pos < 0 || col >= p.bt_stride) {
-    report_error_at(p.err, KVC_DEVERR_BAD_POSITION, static_cast<uint32_t>(pos));
-    return -1;
-  }
-  const int page = p.block_tables[static_cast<size_t>(row) * p.bt_stride + col];
-  if (page < 0 || page >= p.num_pages) {
-    report_error_at(p.err, KVC_DEVERR_BAD_PAGE, static_cast<uint32_t>(page));
-    return -1;
-  }
-  return page;
-}
-
-template <typename T>
-struct Unit {
-  static constexpr int N = 16 / sizeof(T);
-  union {
-    uint4 raw;
-    T v[N];
-  };
-  __device__ Unit() {}
-};
 
 // (x0, x1) rotated by the pair's (cos, sin), in 32 bits, rounded once.
 template <typename T>

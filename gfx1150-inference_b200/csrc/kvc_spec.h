@@ -6,11 +6,13 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <exception>
 #include <new>
 #include <vector>
 
 #include "kvc_common.h"
 #include "kvc_internal.h"
+#include "kvcache.h"
 
 struct kvc_tree_plan;
 
@@ -79,18 +81,38 @@ struct ReorderArgs {
 };
 
 // ---- tree attention -----------------------------------------------------------------
-// One piece of work of one CTA: tiles [tile0, tile1) of the positions of one
-// sequence for one KV head and a block of its (node, q-head) rows.  Row r of the
-// sequence is node r / group, q-head kvh * group + r % group.
+// One piece of work of one CTA: tiles [tile0, tile1) of the positions from `base` (a whole
+// number of slabs) to ctx + nodes of one block-table row, for one KV head and a block of
+// (node, q-head) rows.  Row r is node r / group, q-head kvh * group + r % group; node n is
+// token tok0 + n of the batch.  Every row sees the positions below ctx, the mask names
+// those that it sees of the `nodes` behind them.
 struct alignas(16) TreeSeg {
   int bt_row, ctx, nodes, tok0;
   int kvh, row0, rows, tile0;
-  int tile1, part, pad0, pad1;   // part: first row of its partials, -1: writes the output
+  int tile1, part, base;         // part: first row of its partials, -1: writes the output
+  int scores;                    // 16 floats: where row 0's scores start (TreeArgs::scores)
 };
 // Rows whose partials are joined: n_parts pieces, `rows` partial rows apart.
 struct alignas(16) TreeMerge {
   int part, n_parts, tok0, row0;
   int kvh, rows, pad0, pad1;
+};
+
+// The pieces of one row run: partial rows `part` on, n pieces `rows` partial rows apart, the
+// run's first row at `row` of each.
+struct JoinPieces {
+  int part, n, rows, row;
+};
+// Rows of one sequence and KV head: token, first q-head and number of q-heads.
+struct alignas(16) SharedJoin {
+  JoinPieces prefix, own;
+  int token, head, rows, pad;
+};
+// kTreeWeighSlots slots of one (sequence, KV head) whose weights are added up.
+constexpr int kTreeWeighSlots = 512;
+struct alignas(16) TreeWeigh {
+  int bt_row, ctx, nodes, tok0;
+  int kvh, slot0, scores, pad;   // scores: as in TreeSeg
 };
 
 struct TreeArgs {
@@ -107,6 +129,17 @@ struct TreeArgs {
   float2* part_ml;               // (partial rows) max (log2 units) and sum
   int num_heads, group, head_dim, dtype;
   float scale_log2;
+  const SharedJoin* joins;       // instead of merges, for shared prefixes
+  int n_joins;
+  // Attention that adds its weights up (null otherwise): the raw scores and final (max, sum)
+  // of every row, and where the sums go, (table rows, KV heads, weight_slots).
+  float* scores;
+  float2* row_ml;                // (tokens, H)
+  const TreeWeigh* weighs;
+  int n_weighs;
+  float* weights;
+  int weight_slots;
+  float score_scale;             // what a kept score is multiplied by, log2 units
 };
 
 // Tile shape of the kernel a batch takes: positions per tile and rows per block.
@@ -173,9 +206,45 @@ int do_append_rope(kvc_pool* pool, int layer, const void* d_q, int q_stride, voi
 // The plan, the layer and the sizes of a call, before anything of it is launched.
 int check_tree_call(const kvc_pool* pool, const kvc_tree_plan* plan, int layer,
                     const int32_t* d_mask, int mask_words, int bt_stride, float scale);
+// What the attention kernels take of a call, without its mask and its joins.
+int tree_args(const kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
+              void* d_out, const int32_t* d_bt, int bt_stride, float scale, TreeArgs* out);
+// A plan is not built while its stream is being captured.
+int refuse_capture(cudaStream_t s, const char* what);
+// d_weights: null, or (weight_rows, KV heads, weight_slots) sums that the weights are added to.
 int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
                    const int32_t* d_mask, int mask_words, void* d_out, const int32_t* d_bt,
-                   int bt_stride, float scale, cudaStream_t s);
+                   int bt_stride, float scale, cudaStream_t s, float* d_weights = nullptr,
+                   int weight_rows = 0, int weight_slots = 0);
+
+// Floats that the scores of one plan take at most.
+constexpr int64_t kMaxScores = 1ll << 30;
+// Cuts whole runs (tile0 0, tile1 their tiles) into the CTAs' shares.
+void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
+              std::vector<TreeSeg>* segs, std::vector<int>* cta_segs);
+// A plan's records go to its device buffer in one copy; dev[i]: where parts[i] will be.
+struct PlanPart {
+  const void* data;
+  size_t bytes;
+};
+int upload_plan(kvc_tree_plan* p, const PlanPart* parts, int n, const uint8_t** dev, cudaStream_t s);
+
+// No C++ exception leaves a C entry point.
+template <typename F>
+int guarded(const char* what, F&& f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return set_error(KVC_ERR_RUNTIME, "%s: %s", what, e.what());
+  } catch (...) {
+    return set_error(KVC_ERR_RUNTIME, "%s: unknown exception", what);
+  }
+}
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int check_table(const int32_t* d_bt, int bt_rows, int bt_stride);
+// The view of `layer` of a pool (its device is current).
+int paged_view(const kvc_pool* pool, int layer, const int32_t* d_bt, int bt_rows, int bt_stride,
+               PagedView* v);
 
 // The device current at construction comes back at the end of the scope.
 class DeviceScope {
@@ -219,7 +288,11 @@ struct kvc_tree_plan {
   const kvc::TreeMerge* dev_merges = nullptr;
   const int32_t* dev_rows = nullptr;   // (n_tokens) block-table row of each token
   const int32_t* dev_slots = nullptr;  // (n_tokens) cache slot of each token
-  kvc::DevBuf d_blob, d_part_o, d_part_ml;
+  // kvc_tree_plan_set_weights: builds make room for the scores; has_scores: the last did
+  bool keep_scores = false, has_scores = false;
+  int n_weighs = 0;
+  const kvc::TreeWeigh* dev_weighs = nullptr;
+  kvc::DevBuf d_blob, d_part_o, d_part_ml, d_scores, d_row_ml;
   kvc::DevBuf d_layer;                 // activations of kvc_forward_layer_tree
   kvc::HostBuf h_stage;
   cudaEvent_t upload_done = nullptr;
@@ -228,6 +301,8 @@ struct kvc_tree_plan {
     d_blob.release();
     d_part_o.release();
     d_part_ml.release();
+    d_scores.release();
+    d_row_ml.release();
     d_layer.release();
     h_stage.release();
     if (upload_done) cudaEventDestroy(upload_done);

@@ -40,22 +40,6 @@ int sms_of(int device) {
   return n;
 }
 
-namespace {
-
-// No C++ exception leaves a C entry point.
-template <typename F>
-int guarded(const char* what, F&& f) {
-  try {
-    return f();
-  } catch (const std::exception& e) {
-    return set_error(KVC_ERR_RUNTIME, "%s: %s", what, e.what());
-  } catch (...) {
-    return set_error(KVC_ERR_RUNTIME, "%s: unknown exception", what);
-  }
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 int check_table(const int32_t* d_bt, int bt_rows, int bt_stride) {
   if (!d_bt) return set_error(KVC_ERR_INVALID_ARG, "block tables must not be null.");
   if (bt_rows <= 0 || bt_stride <= 0)
@@ -80,8 +64,6 @@ int paged_view(const kvc_pool* pool, int layer, const int32_t* d_bt, int bt_rows
   v->page_head_bytes = g.page_head_bytes;
   return device_error_word(pool->device, &v->err);
 }
-
-}  // namespace
 
 int do_append_rope(kvc_pool* pool, int layer, const void* d_q, int q_stride, void* d_q_out,
                    int num_heads, const void* d_k_new, int k_stride, const void* d_v_new,
@@ -160,28 +142,20 @@ int check_tree_call(const kvc_pool* pool, const kvc_tree_plan* plan, int layer,
   return KVC_OK;
 }
 
-int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
-                   const int32_t* d_mask, int mask_words, void* d_out, const int32_t* d_bt,
-                   int bt_stride, float scale, cudaStream_t s) {
+int tree_args(const kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
+              void* d_out, const int32_t* d_bt, int bt_stride, float scale, TreeArgs* out) {
   const PoolGeom& g = pool->g;
-  if (int rc = check_tree_call(pool, plan, layer, d_mask, mask_words, bt_stride, scale)) return rc;
-  if (plan->n_tokens == 0) return KVC_OK;
   if (!d_q || !d_out || !d_bt)
     return set_error(KVC_ERR_INVALID_ARG, "q, out and block tables must not be null.");
   if (!aligned16(d_q) || !aligned16(d_out))
     return set_error(KVC_ERR_INVALID_ARG, "q and out must be 16-byte aligned.");
-  TreeArgs a = {};
+  TreeArgs& a = *out;
   if (int rc = paged_view(pool, layer, d_bt, plan->max_row + 1, bt_stride, &a.p)) return rc;
   a.q = d_q;
   a.out = d_out;
-  a.mask = reinterpret_cast<const uint32_t*>(d_mask);
-  a.mask_words = d_mask ? mask_words : 0;
   a.segs = plan->dev_segs;
   a.cta_segs = plan->dev_cta_segs;
-  a.merges = plan->dev_merges;
   a.n_ctas = plan->n_ctas;
-  a.n_merges = plan->n_merges;
-  a.max_merge_rows = plan->max_merge_rows;
   a.part_o = static_cast<float*>(plan->d_part_o.ptr);
   a.part_ml = static_cast<float2*>(plan->d_part_ml.ptr);
   a.num_heads = plan->num_heads;
@@ -189,15 +163,153 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
   a.head_dim = g.head_dim;
   a.dtype = g.dtype;
   a.scale_log2 = scale * kLog2e;
+  return KVC_OK;
+}
+
+int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const void* d_q,
+                   const int32_t* d_mask, int mask_words, void* d_out, const int32_t* d_bt,
+                   int bt_stride, float scale, cudaStream_t s, float* d_weights, int weight_rows,
+                   int weight_slots) {
+  if (int rc = check_tree_call(pool, plan, layer, d_mask, mask_words, bt_stride, scale)) return rc;
+  if (plan->n_tokens == 0) return KVC_OK;
+  TreeArgs a = {};
+  if (int rc = tree_args(pool, plan, layer, d_q, d_out, d_bt, bt_stride, scale, &a)) return rc;
+  a.mask = reinterpret_cast<const uint32_t*>(d_mask);
+  a.mask_words = d_mask ? mask_words : 0;
+  a.merges = plan->dev_merges;
+  a.n_merges = plan->n_merges;
+  a.max_merge_rows = plan->max_merge_rows;
+  if (d_weights) {
+    if (!plan->has_scores)
+      return set_error(KVC_ERR_INVALID_ARG, "the plan was built without kvc_tree_plan_set_weights.");
+    if (plan->max_row >= weight_rows)
+      return set_error(KVC_ERR_OUT_OF_RANGE, "a sequence's row is outside the weights.");
+    if (plan->max_end > weight_slots)
+      return set_error(KVC_ERR_OUT_OF_RANGE, "a sequence exceeds the weights' slots.");
+    a.scores = static_cast<float*>(plan->d_scores.ptr);
+    a.row_ml = static_cast<float2*>(plan->d_row_ml.ptr);
+    a.weighs = plan->dev_weighs;
+    a.n_weighs = plan->n_weighs;
+    a.weights = d_weights;
+    a.weight_slots = weight_slots;
+    // (the tensor cores' kernel takes the scale's sign into q)
+    a.score_scale = plan->tile.tensor ? std::fabs(a.scale_log2) : a.scale_log2;
+  }
   const cudaError_t e = launch_tree(a, plan->tile, s);
   return e == cudaSuccess ? KVC_OK : cuda_error(e, "tree attention kernel");
 }
 
+int refuse_capture(cudaStream_t s, const char* what) {
+  // A captured upload would read the staging buffer at every replay, whatever a later build
+  // has put there (the capture stays valid).
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(s, &cap);
+  if (e != cudaSuccess) return cuda_error(e, "cudaStreamIsCapturing");
+  if (cap != cudaStreamCaptureStatusNone)
+    return set_error(KVC_ERR_INVALID_ARG,
+                     "%s cannot be built on a stream that is being captured: build it "
+                     "before the capture and capture the calls that use it.", what);
+  return KVC_OK;
+}
+
+// The work list: the runs of position tiles are laid end to end and cut into shares of
+// equal cost, one per CTA.  A run that falls into several shares is joined from its pieces'
+// partials.
+void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
+              std::vector<TreeSeg>* segs, std::vector<int>* cta_segs) {
+  segs->clear();
+  cta_segs->assign(1, 0);
+  int64_t tiles = 0;
+  for (const TreeSeg& r : runs) tiles += r.tile1;
+  const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(sms) * tile.ctas_per_sm, tiles);
+  // A piece costs its tiles and `pc` for its start and end; a CTA's pieces cost at most `limit`
+  // together, give or take a pc: a cut that would leave less than that on either side moves
+  // to the end of the run or of the share.  pc is tile.piece_cost where CTAs have many tiles
+  // (4 against 1 there: 32 ragged trees 115 against 118 us), and less where they have few and
+  // short pieces spread the work further (63 drafted tokens at 511: 16 us at 1, 22 at 4).
+  // walk() lays the runs out for a limit, calls emit(run, tile, tiles) and close() for each
+  // piece and each full share, and returns the number of shares.
+  const int64_t pc = std::min<int64_t>(
+      tile.piece_cost, std::max<int64_t>(1, ctas > 0 ? tiles / (8 * ctas) : 1));
+  auto walk = [&](int64_t limit, auto&& emit, auto&& close) {
+    int64_t shares = 0, cost = 0;
+    for (const TreeSeg& r : runs) {
+      const int run = r.tile1;
+      for (int t = 0; t < run;) {
+        const int64_t room = limit - cost - pc;
+        if (cost > 0 && room < run - t && room < std::max<int64_t>(1, pc)) {
+          close();
+          ++shares;
+          cost = 0;
+          continue;
+        }
+        int take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(run - t, room)));
+        if (run - t - take < pc) take = run - t;
+        emit(r, t, take);
+        t += take;
+        cost += take + pc;
+      }
+    }
+    return shares + (cost > 0 ? 1 : 0);
+  };
+  // the smallest limit that needs no more shares than there are CTAs
+  auto fits = [&](int64_t limit) {
+    return walk(limit, [](const TreeSeg&, int, int) {}, [] {}) <= ctas;
+  };
+  const int64_t n_runs = static_cast<int64_t>(runs.size());
+  int64_t lo = 1, hi = 1;
+  if (ctas > 0) {
+    lo = std::max<int64_t>(1, (tiles + n_runs * pc) / ctas);
+    for (hi = (tiles + (n_runs + ctas) * pc) / ctas + 1; !fits(hi);) hi *= 2;
+  }
+  while (lo < hi) {
+    const int64_t mid = lo + (hi - lo) / 2;
+    if (fits(mid))
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  walk(
+      hi,
+      [&](const TreeSeg& r, int t, int take) {
+        TreeSeg sg = r;
+        sg.tile0 = t;
+        sg.tile1 = t + take;
+        segs->push_back(sg);
+      },
+      [&] { cta_segs->push_back(static_cast<int>(segs->size())); });
+  if (cta_segs->back() < static_cast<int>(segs->size()))
+    cta_segs->push_back(static_cast<int>(segs->size()));
+}
+
+int upload_plan(kvc_tree_plan* p, const PlanPart* parts, int n, const uint8_t** dev, cudaStream_t s) {
+  cudaError_t e;
+  auto al = [](size_t b) { return (b + 255) & ~static_cast<size_t>(255); };
+  size_t total = 0;
+  for (int i = 0; i < n; ++i) total += al(parts[i].bytes);
+  if ((e = p->d_blob.ensure(total))) return cuda_error(e, "plan buffers");
+  if (p->upload_done) {  // the staging is free once the previous upload has landed
+    if (const int rc = wait_event(p->upload_done, "plan upload")) return rc;
+  } else if ((e = cudaEventCreateWithFlags(&p->upload_done, cudaEventDisableTiming))) {
+    return cuda_error(e, "cudaEventCreate");
+  }
+  if ((e = p->h_stage.ensure(total))) return cuda_error(e, "cudaMallocHost(plan)");
+  uint8_t* h = static_cast<uint8_t*>(p->h_stage.ptr);
+  size_t at = 0;
+  for (int i = 0; i < n; ++i) {
+    if (parts[i].bytes) memcpy(h + at, parts[i].data, parts[i].bytes);
+    dev[i] = static_cast<const uint8_t*>(p->d_blob.ptr) + at;
+    at += al(parts[i].bytes);
+  }
+  if ((e = cudaMemcpyAsync(p->d_blob.ptr, h, total, cudaMemcpyHostToDevice, s)))
+    return cuda_error(e, "plan upload");
+  if ((e = cudaEventRecord(p->upload_done, s))) return cuda_error(e, "cudaEventRecord(plan)");
+  return KVC_OK;
+}
+
 namespace {
 
-// The work list: every (sequence, KV head, row block) is a run of position tiles;
-// the runs are laid end to end and cut into shares of equal cost, one per CTA.  A run
-// that falls into several shares is joined from its pieces' partials.
+// Every (sequence, KV head, row block) is a run of position tiles.
 int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
                const int32_t* h_ctx, const int32_t* h_nodes, int n_seqs, int num_heads,
                cudaStream_t s) {
@@ -209,9 +321,10 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     return set_error(KVC_ERR_INVALID_ARG, "num_heads must be divisible by num_kv_heads.");
   p->valid = false;
   const int group = num_heads / g.num_kv_heads, sms = sms_of(pool->device);
-  int64_t tokens = 0, tiles = 0, runs = 0, max_end = 0, small = 0;
+  int64_t tokens = 0, tiles = 0, scores = 0, max_end = 0, small = 0;
   int max_row = 0, max_nodes = 0;
   std::vector<int32_t> rows, slots;
+  std::vector<int> seen;
   for (int i = 0; i < n_seqs; ++i) {
     const int row = h_rows ? h_rows[i] : i;
     if (h_ctx[i] < 0) return set_error(KVC_ERR_INVALID_ARG, "context length must be non-negative.");
@@ -227,92 +340,57 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     tokens += h_nodes[i];
     if (h_nodes[i] > 0) max_end = std::max(max_end, end);
     max_row = std::max(max_row, row);
+    if (p->keep_scores && h_nodes[i] > 0) seen.push_back(row);
     max_nodes = std::max(max_nodes, h_nodes[i]);
     small += (static_cast<int64_t>(h_nodes[i]) * group + kTreeSmall - 1) / kTreeSmall *
              g.num_kv_heads * ((end + kTreeSmall - 1) / kTreeSmall);
   }
+  std::sort(seen.begin(), seen.end());
+  const bool rows_apart = std::adjacent_find(seen.begin(), seen.end()) == seen.end();
   const TreeTile tile = tree_tile(g, small, sms);
   for (int i = 0; i < n_seqs; ++i) {
     const int64_t blocks = (static_cast<int64_t>(h_nodes[i]) * group + tile.rows - 1) / tile.rows;
     const int64_t end = static_cast<int64_t>(h_ctx[i]) + h_nodes[i];
-    runs += blocks * g.num_kv_heads;
     tiles += blocks * g.num_kv_heads * ((end + tile.positions - 1) / tile.positions);
+    scores += static_cast<int64_t>(h_nodes[i]) * num_heads * ((end + 15) / 16);
   }
   if (tokens * num_heads > (1ll << 30) || tiles > (1ll << 30))
     return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
-  const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(sms) * tile.ctas_per_sm, tiles);
-  // A piece costs its tiles and `pc` for its start and end; a CTA's pieces cost at most `limit`
-  // together, give or take a pc: a cut that would leave less than that on either side moves
-  // to the end of the run or of the share.  pc is tile.piece_cost where CTAs have many tiles
-  // (4 against 1 there: 32 ragged trees 115 against 118 us), and less where they have few and
-  // short pieces spread the work further (63 drafted tokens at 511: 16 us at 1, 22 at 4).  walk() lays the runs out for
-  // a limit, calls emit(sequence, kvh, row0, rows, tile0, tiles) and close() for each piece
-  // and each full share, and returns the number of shares.
-  const int64_t pc = std::min<int64_t>(
-      tile.piece_cost, std::max<int64_t>(1, ctas > 0 ? tiles / (8 * ctas) : 1));
-  auto walk = [&](int64_t limit, auto&& emit, auto&& close) {
-    int64_t shares = 0, cost = 0;
-    for (int i = 0; i < n_seqs; ++i) {
-      const int n_rows = h_nodes[i] * group;
-      const int run = (h_ctx[i] + h_nodes[i] + tile.positions - 1) / tile.positions;
-      for (int kvh = 0; kvh < g.num_kv_heads && n_rows > 0; ++kvh) {
-        for (int r0 = 0; r0 < n_rows; r0 += tile.rows) {
-          for (int t = 0; t < run;) {
-            const int64_t room = limit - cost - pc;
-            if (cost > 0 && room < run - t && room < std::max<int64_t>(1, pc)) {
-              close();
-              ++shares;
-              cost = 0;
-              continue;
-            }
-            int take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(run - t, room)));
-            if (run - t - take < pc) take = run - t;
-            emit(i, kvh, r0, std::min(tile.rows, n_rows - r0), t, take);
-            t += take;
-            cost += take + pc;
-          }
-        }
+  if (p->keep_scores && scores > kMaxScores / 16)
+    return set_error(KVC_ERR_INVALID_ARG, "the batch keeps more scores than one plan holds (2^30).");
+  if (p->keep_scores && !rows_apart)
+    return set_error(KVC_ERR_INVALID_ARG,
+                     "two sequences of one block-table row cannot add their weights up together.");
+  std::vector<TreeSeg> runs, segs;
+  std::vector<TreeMerge> merges;
+  std::vector<TreeWeigh> weighs;
+  std::vector<int> cta_segs;
+  int tok0 = 0, score0 = 0;
+  for (int i = 0; i < n_seqs; tok0 += h_nodes[i++]) {
+    const int n_rows = h_nodes[i] * group, end = h_ctx[i] + h_nodes[i];
+    for (int kvh = 0; kvh < g.num_kv_heads && n_rows > 0; ++kvh) {
+      TreeSeg sg = {};
+      sg.bt_row = h_rows ? h_rows[i] : i;
+      sg.ctx = h_ctx[i];
+      sg.nodes = h_nodes[i];
+      sg.tok0 = tok0;
+      sg.kvh = kvh;
+      sg.tile1 = (end + tile.positions - 1) / tile.positions;
+      sg.part = -1;
+      if (p->keep_scores) {
+        sg.scores = score0;
+        score0 += n_rows * ((end + 15) / 16);
+        for (int slot = 0; slot < end; slot += kTreeWeighSlots)
+          weighs.push_back(TreeWeigh{sg.bt_row, sg.ctx, sg.nodes, sg.tok0, kvh, slot, sg.scores, 0});
+      }
+      for (int r0 = 0; r0 < n_rows; r0 += tile.rows) {
+        sg.row0 = r0;
+        sg.rows = std::min(tile.rows, n_rows - r0);
+        runs.push_back(sg);
       }
     }
-    return shares + (cost > 0 ? 1 : 0);
-  };
-  // the smallest limit that needs no more shares than there are CTAs
-  auto fits = [&](int64_t limit) {
-    return walk(limit, [](int, int, int, int, int, int) {}, [] {}) <= ctas;
-  };
-  int64_t lo = 1, hi = 1;
-  if (ctas > 0) {
-    lo = std::max<int64_t>(1, (tiles + runs * pc) / ctas);
-    for (hi = (tiles + (runs + ctas) * pc) / ctas + 1; !fits(hi);) hi *= 2;
   }
-  while (lo < hi) {
-    const int64_t mid = lo + (hi - lo) / 2;
-    if (fits(mid))
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  std::vector<TreeSeg> segs;
-  std::vector<TreeMerge> merges;
-  std::vector<int> cta_segs(1, 0), tok0(std::max(1, n_seqs), 0);
-  for (int i = 1; i < n_seqs; ++i) tok0[i] = tok0[i - 1] + h_nodes[i - 1];
-  walk(
-      hi,
-      [&](int i, int kvh, int r0, int nr, int t, int take) {
-        TreeSeg sg = {};
-        sg.bt_row = h_rows ? h_rows[i] : i;
-        sg.ctx = h_ctx[i];
-        sg.nodes = h_nodes[i];
-        sg.tok0 = tok0[i];
-        sg.kvh = kvh;
-        sg.row0 = r0;
-        sg.rows = nr;
-        sg.tile0 = t;
-        sg.tile1 = t + take;
-        sg.part = -1;
-        segs.push_back(sg);
-      },
-      [&] { cta_segs.push_back(static_cast<int>(segs.size())); });
+  cut_runs(runs, tile, sms, &segs, &cta_segs);
   // runs in several pieces are joined from their partials
   size_t part_rows = 0;
   int max_merge_rows = 0;
@@ -337,7 +415,6 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     }
     first = next;
   }
-  if (cta_segs.back() < static_cast<int>(segs.size())) cta_segs.push_back(static_cast<int>(segs.size()));
   p->n_seqs = n_seqs;
   p->n_tokens = static_cast<int>(tokens);
   p->num_heads = num_heads;
@@ -349,6 +426,8 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   p->n_merges = static_cast<int>(merges.size());
   p->max_merge_rows = max_merge_rows;
   p->part_rows = part_rows;
+  p->n_weighs = static_cast<int>(weighs.size());
+  p->has_scores = p->keep_scores;
   p->pool_geom = g;
   p->device = pool->device;
   if (tokens == 0) {
@@ -359,33 +438,24 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   if ((e = p->d_part_o.ensure(sizeof(float) * std::max<size_t>(1, part_rows) * g.head_dim)) ||
       (e = p->d_part_ml.ensure(sizeof(float2) * std::max<size_t>(1, part_rows))))
     return cuda_error(e, "plan buffers");
-  auto al = [](size_t b) { return (b + 255) & ~static_cast<size_t>(255); };
-  const size_t segs_n = sizeof(TreeSeg) * segs.size(), cta_n = sizeof(int) * cta_segs.size();
-  const size_t mrg_n = sizeof(TreeMerge) * merges.size(), row_n = sizeof(int32_t) * rows.size();
-  const size_t o_cta = al(segs_n), o_mrg = o_cta + al(cta_n), o_row = o_mrg + al(mrg_n);
-  const size_t o_slot = o_row + al(row_n), total = o_slot + al(row_n);
-  if ((e = p->d_blob.ensure(total))) return cuda_error(e, "plan buffers");
-  if (p->upload_done) {  // the staging is free once the previous upload has landed
-    if (const int rc = wait_event(p->upload_done, "plan upload")) return rc;
-  } else if ((e = cudaEventCreateWithFlags(&p->upload_done, cudaEventDisableTiming))) {
-    return cuda_error(e, "cudaEventCreate");
-  }
-  if ((e = p->h_stage.ensure(total))) return cuda_error(e, "cudaMallocHost(plan)");
-  uint8_t* h = static_cast<uint8_t*>(p->h_stage.ptr);
-  memcpy(h, segs.data(), segs_n);
-  memcpy(h + o_cta, cta_segs.data(), cta_n);
-  if (mrg_n) memcpy(h + o_mrg, merges.data(), mrg_n);
-  memcpy(h + o_row, rows.data(), row_n);
-  memcpy(h + o_slot, slots.data(), row_n);
-  if ((e = cudaMemcpyAsync(p->d_blob.ptr, h, total, cudaMemcpyHostToDevice, s)))
-    return cuda_error(e, "plan upload");
-  if ((e = cudaEventRecord(p->upload_done, s))) return cuda_error(e, "cudaEventRecord(plan)");
-  const uint8_t* d = static_cast<const uint8_t*>(p->d_blob.ptr);
-  p->dev_segs = reinterpret_cast<const TreeSeg*>(d);
-  p->dev_cta_segs = reinterpret_cast<const int*>(d + o_cta);
-  p->dev_merges = reinterpret_cast<const TreeMerge*>(d + o_mrg);
-  p->dev_rows = reinterpret_cast<const int32_t*>(d + o_row);
-  p->dev_slots = reinterpret_cast<const int32_t*>(d + o_slot);
+  if (p->keep_scores &&
+      ((e = p->d_scores.ensure(sizeof(float) * 16 * static_cast<size_t>(score0))) ||
+       (e = p->d_row_ml.ensure(sizeof(float2) * static_cast<size_t>(tokens) * num_heads))))
+    return cuda_error(e, "plan buffers");
+  const PlanPart parts[] = {{segs.data(), sizeof(TreeSeg) * segs.size()},
+                            {cta_segs.data(), sizeof(int) * cta_segs.size()},
+                            {merges.data(), sizeof(TreeMerge) * merges.size()},
+                            {rows.data(), sizeof(int32_t) * rows.size()},
+                            {slots.data(), sizeof(int32_t) * slots.size()},
+                            {weighs.data(), sizeof(TreeWeigh) * weighs.size()}};
+  const uint8_t* d[6];
+  if (const int rc = upload_plan(p, parts, 6, d, s)) return rc;
+  p->dev_segs = reinterpret_cast<const TreeSeg*>(d[0]);
+  p->dev_cta_segs = reinterpret_cast<const int*>(d[1]);
+  p->dev_merges = reinterpret_cast<const TreeMerge*>(d[2]);
+  p->dev_rows = reinterpret_cast<const int32_t*>(d[3]);
+  p->dev_slots = reinterpret_cast<const int32_t*>(d[4]);
+  p->dev_weighs = reinterpret_cast<const TreeWeigh*>(d[5]);
   p->valid = true;
   return KVC_OK;
 }
@@ -435,15 +505,7 @@ extern "C" int kvc_plan_tree(kvc_tree_plan_t* plan, const kvc_pool_t* pool, cons
   return guarded("kvc_plan_tree", [&]() -> int {
     DeviceScope dev(pool->device);
     if (dev.rc()) return dev.rc();
-    // A captured upload would read the staging buffer at every replay, whatever a later build
-    // has put there (the capture stays valid).
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    const cudaError_t e = cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &cap);
-    if (e != cudaSuccess) return cuda_error(e, "cudaStreamIsCapturing");
-    if (cap != cudaStreamCaptureStatusNone)
-      return set_error(KVC_ERR_INVALID_ARG,
-                       "a tree plan cannot be built on a stream that is being captured: build it "
-                       "before the capture and capture the calls that use it.");
+    if (int rc = refuse_capture(static_cast<cudaStream_t>(stream), "a tree plan")) return rc;
     if (plan->device >= 0 && plan->device != pool->device) {  // its buffers are elsewhere
       DeviceScope old(plan->device);
       plan->release();
@@ -458,7 +520,14 @@ extern "C" int kvc_tree_plan_info(const kvc_tree_plan_t* plan, int* n_tokens, in
   if (!plan) return set_error(KVC_ERR_INVALID_ARG, "plan must not be null.");
   if (n_tokens) *n_tokens = plan->n_tokens;
   if (n_ctas) *n_ctas = plan->n_ctas;
-  if (scratch_bytes) *scratch_bytes = plan->d_part_o.cap + plan->d_part_ml.cap;
+  if (scratch_bytes)
+    *scratch_bytes = plan->d_part_o.cap + plan->d_part_ml.cap + plan->d_scores.cap + plan->d_row_ml.cap;
+  return KVC_OK;
+}
+
+extern "C" int kvc_tree_plan_set_weights(kvc_tree_plan_t* plan, int on) {
+  if (!plan) return set_error(KVC_ERR_INVALID_ARG, "plan must not be null.");
+  plan->keep_scores = on != 0;
   return KVC_OK;
 }
 
@@ -472,6 +541,24 @@ extern "C" int kvc_decode_tree(kvc_pool_t* pool, const kvc_tree_plan_t* plan, in
     if (dev.rc()) return dev.rc();
     return do_decode_tree(pool, plan, layer, d_q, d_mask, mask_words, d_out, d_block_tables,
                           bt_stride, scale, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int kvc_decode_tree_weights(kvc_pool_t* pool, const kvc_tree_plan_t* plan, int layer,
+                                       const void* d_q, const int32_t* d_mask, int mask_words,
+                                       float* d_weights, int weight_rows, int weight_slots,
+                                       void* d_out, const int32_t* d_block_tables, int bt_stride,
+                                       float scale, void* stream) {
+  if (!pool || !plan) return set_error(KVC_ERR_INVALID_ARG, "pool and plan must not be null.");
+  return guarded("kvc_decode_tree_weights", [&]() -> int {
+    if (!d_weights) return set_error(KVC_ERR_INVALID_ARG, "weights must not be null.");
+    if (!aligned16(d_weights))
+      return set_error(KVC_ERR_INVALID_ARG, "weights must be 16-byte aligned.");
+    DeviceScope dev(pool->device);
+    if (dev.rc()) return dev.rc();
+    return do_decode_tree(pool, plan, layer, d_q, d_mask, mask_words, d_out, d_block_tables,
+                          bt_stride, scale, static_cast<cudaStream_t>(stream), d_weights,
+                          weight_rows, weight_slots);
   });
 }
 

@@ -10,6 +10,10 @@
 //   tree_f32_kernel     CUDA cores: fp32 pools
 //   tree_simt_kernel    CUDA cores: 16-bit pools with head dims without a tensor tile
 //   tree_merge_kernel   joins the pieces of rows whose positions were split over CTAs
+//   shared_join_kernel  the same for rows of a shared prefix and their own positions
+//                       (kvc_decode_shared)
+//   tree_weights_kernel adds the probabilities up per slot (kvc_decode_tree_weights),
+//                       from scores that the attention kernels' kScores variants keep
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -126,6 +130,14 @@ __device__ __forceinline__ bool maybe_odd(uint32_t two) {
   return ((t - 0x00010001u) & ~t & 0x80008000u) != 0u;
 }
 
+// A score that the row does not see, as it is kept (-inf).
+constexpr uint32_t kUnseen = 0xff800000u;
+// Where row r of a (sequence, KV head) keeps its scores: rows of whole 16s, in a row.
+__device__ __forceinline__ size_t score_row(const TreeSeg& sg, int r) {
+  const int pitch = (sg.ctx + sg.nodes + 15) & ~15;
+  return static_cast<size_t>(sg.scores) * 16 + static_cast<size_t>(r) * pitch;
+}
+
 // Mask word k (drafted tokens 32 k ... 32 k + 31) of a row; below 0: cached positions.
 __device__ __forceinline__ uint32_t mask_word(const TreeArgs& a, const TreeSeg& sg, int node, int k) {
   if (k < 0) return 0xffffffffu;
@@ -141,7 +153,7 @@ __device__ __forceinline__ uint32_t mask_word(const TreeArgs& a, const TreeSeg& 
   return left < 32 ? w & ((1u << left) - 1u) : w;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kScores>
 __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(const TreeArgs a) {
   using S = TreeShape<D>;
   constexpr int U = D / 8, KP = S::kPos;
@@ -235,10 +247,10 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       for (int si = seg0; si < seg1 && ok; ++si) {
         const TreeSeg sg = a.segs[si];
         const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
-        const int last_slab = (end - 1) / kSlab;
+        const int last_slab = (end - 1) / kSlab, slab0 = sg.base / kSlab + sg.tile0 * kTileSlabs;
         const int32_t* table = a.p.block_tables + static_cast<size_t>(sg.bt_row) * a.p.bt_stride;
         auto entry_of = [&](int win) -> int {            // page-table entry of a window's slab
-          const int slab = (sg.tile0 + win * kWinTiles) * kTileSlabs + lane;
+          const int slab = slab0 + win * kWinTiles * kTileSlabs + lane;
           const int col = slab / spp;
           return slab <= last_slab && col < a.p.bt_stride ? table[col] : -1;
         };
@@ -256,7 +268,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
                 next = entry_of(w + 1);
                 win = w;
               }
-              const int slabs = min(kTileSlabs, last_slab + 1 - (sg.tile0 + t) * kTileSlabs);
+              const int slabs = min(kTileSlabs, last_slab + 1 - slab0 - t * kTileSlabs);
               int page = __shfl_sync(0xffffffffu, now, t % kWinTiles * kTileSlabs + (lane & (kTileSlabs - 1)));
               const bool mine = lane < slabs && lane % run == 0;
               const uint8_t* src = nullptr;
@@ -265,7 +277,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
                   report_error_at(a.p.err, KVC_DEVERR_BAD_PAGE, static_cast<uint32_t>(page));
                   page = 0;
                 }
-                const int slab = (sg.tile0 + t) * kTileSlabs + lane;
+                const int slab = slab0 + t * kTileSlabs + lane;
                 src = (kv ? a.p.v : a.p.k) +
                       (static_cast<size_t>(page) * a.p.num_kv_heads + sg.kvh) * a.p.page_head_bytes +
                       slab % spp * kSlabBytes;
@@ -343,10 +355,10 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       for (int si = seg0; si < seg1 && ok; ++si) {
         const TreeSeg sg = a.segs[si];
         const int tiles = __shfl_sync(0xffffffffu, sg.tile1 - sg.tile0, 0);
-        const int left = __shfl_sync(0xffffffffu, sg.ctx + sg.nodes - sg.tile0 * KP, 0);
+        const int left = __shfl_sync(0xffffffffu, sg.ctx + sg.nodes - sg.base - sg.tile0 * KP, 0);
         const bool two = __shfl_sync(0xffffffffu, sg.rows, 0) > 128;
         const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-        const int edge0 = __shfl_sync(0xffffffffu, sg.ctx - sg.tile0 * KP, 0);
+        const int edge0 = __shfl_sync(0xffffffffu, sg.ctx - sg.base - sg.tile0 * KP, 0);
         auto slabs_of = [&](int t) { return min(KP / kSlab, (left - t * KP + kSlab - 1) / kSlab); };
         auto is_edge = [&](int t) { return (t + 1) * KP > edge0; };
         // K of tile t is here: when the tile holds drafted positions the helper warps may
@@ -482,8 +494,8 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         // V of drafted tokens: what is not finite would spread through zero weights to rows
         // that do not see it, so it leaves the tile here (and comes back at the end, to the
         // rows that do); positions past the end hold anything, and go to zero.
-        for (int t = max(0, sg.ctx / KP - sg.tile0); t < tiles; ++t) {
-          const int p0 = (sg.tile0 + t) * KP;
+        for (int t = max(0, (sg.ctx - sg.base) / KP - sg.tile0); t < tiles; ++t) {
+          const int p0 = sg.base + (sg.tile0 + t) * KP;
           ok = ok && wait(edge_go(ng), (ng >> 1) & 1);
           // ring order of the piece: `ahead` K tiles, then V t, K t + ahead, ...
           const uint32_t vi = ring + t + min(ahead + t, tiles);
@@ -543,7 +555,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     bool ok = true;
     for (int si = seg0; si < seg1; ++si) {
       const TreeSeg* seg = a.segs + si;   // (read again where it is needed again: no spills)
-      const int tiles = seg->tile1 - seg->tile0, p00 = seg->tile0 * KP, ctx = seg->ctx;
+      const int tiles = seg->tile1 - seg->tile0, p00 = seg->base + seg->tile0 * KP, ctx = seg->ctx;
       const bool two = seg->rows > 128;
       const int ahead = S::kStreams == 2 && !two ? 2 : 1;
       const bool joint = ahead == 2;
@@ -554,6 +566,17 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       // sum.  Edge tiles hold positions that some rows do not see.
       auto softmax = [&](auto edge_tag, int t, const uint32_t* vis) {
         constexpr bool kEdge = decltype(edge_tag)::value;
+        // (a row's scores are 16 to a store of 64 bytes; its pitch is a multiple of that)
+        float* keep = nullptr;
+        int keep_n = 0;
+        if constexpr (kScores) {
+          const TreeSeg sg = *seg;
+          const int p0 = p00 + t * KP;
+          if (row < sg.rows) {
+            keep = a.scores + score_row(sg, sg.row0 + row) + p0;
+            keep_n = min(KP, sg.ctx + sg.nodes - p0);
+          }
+        }
         // One pass with the max as it was: the probabilities wait in registers, and only
         // when a row's max turns out to have grown too far is the pass made again.  The
         // first tile has no such max: it looks for one.
@@ -572,6 +595,22 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
             tmem_wait_ld();
             tmem_loaded<16>(s[w & 1]);
             if (w + 1 < KP / 16) tmem_ld16(t_s + 16 * (w + 1), s[(w + 1) & 1]);
+            if constexpr (kScores) {
+              if (16 * w < keep_n) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                  uint4 v = make_uint4(now[i], now[i + 1], now[i + 2], now[i + 3]);
+                  if constexpr (kEdge) {
+                    const uint32_t bits = vis[w >> 1] >> ((w & 1) * 16 + i);
+                    if (!(bits & 1u)) v.x = kUnseen;
+                    if (!(bits & 2u)) v.y = kUnseen;
+                    if (!(bits & 4u)) v.z = kUnseen;
+                    if (!(bits & 8u)) v.w = kUnseen;
+                  }
+                  *reinterpret_cast<uint4*>(keep + 16 * w + i) = v;
+                }
+              }
+            }
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               const float a0 = __uint_as_float(now[i]), a1 = __uint_as_float(now[i + 1]);
@@ -699,7 +738,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const bool dirty = s_dirty[si & 3] == si;
         // rare: what was taken out of V comes back, for the nodes that this row sees
         auto restore = [&](int c, float* f) {
-          const int t0 = max(sg.tile0 * KP, sg.ctx), t1 = min(sg.tile1 * KP, sg.ctx + sg.nodes);
+          const int t0 = max(sg.base + sg.tile0 * KP, sg.ctx), t1 = min(sg.base + sg.tile1 * KP, sg.ctx + sg.nodes);
           for (int pos = t0; pos < t1; ++pos) {
             const int j = pos - sg.ctx;
             if (!((mask_word(a, sg, node, j >> 5) >> (j & 31)) & 1u)) continue;
@@ -720,6 +759,9 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const float inv = ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);
         if (live_row && sg.part >= 0 && (!joint || x == 0))
           a.part_ml[sg.part + row] = make_float2(mm, ll);
+        if constexpr (kScores) {
+          if (live_row && sg.part < 0 && (!joint || x == 0)) a.row_ml[io_row / D] = make_float2(mm, ll);
+        }
         const bool add = joint && tiles > 1;
         auto load = [&](int c, uint32_t* o, uint32_t* q) {
           tmem_ld16(o0 + c, o);
@@ -791,7 +833,7 @@ struct F32Shape {
   static constexpr int kBuffers = NJ <= 2 ? 2 : 1;
 };
 
-template <int NJ>
+template <int NJ, bool kScores>
 __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs a) {
   constexpr int kBuf = F32Shape<NJ>::kBuffers, kPld = kF32Pos + 4;
   extern __shared__ float4 smem4[];
@@ -815,7 +857,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs
     const int end = sg.ctx + sg.nodes, tiles = sg.tile1 - sg.tile0;
     auto places = [&](int i) {   // threads 0 ... 63: where tile i's rows are
       if (threadIdx.x >= kF32Pos || i >= tiles) return;
-      const int pos = (sg.tile0 + i) * kF32Pos + threadIdx.x;
+      const int pos = sg.base + (sg.tile0 + i) * kF32Pos + threadIdx.x;
       size_t off = ~static_cast<size_t>(0);
       if (pos < end)
         off = (static_cast<size_t>(tree_page(a.p, sg.bt_row, pos)) * a.p.num_kv_heads + sg.kvh) *
@@ -886,7 +928,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs
               s[i][j] = fmaf(q4[i].w, k4[j].w, s[i][j]);
             }
         }
-        const int p0 = (sg.tile0 + it) * kF32Pos;
+        const int p0 = sg.base + (sg.tile0 + it) * kF32Pos;
         const bool edge = p0 + kF32Pos > sg.ctx;
         const float sc = a.scale_log2;
 #pragma unroll
@@ -898,6 +940,10 @@ __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs
           for (int j = 0; j < 4; ++j) {
             const int pos = p0 + tx + 16 * j;
             see[j] = !edge || pos < sg.ctx || (pos < end && sees(a, sg.tok0, node, pos - sg.ctx));
+            if constexpr (kScores) {
+              if (4 * ty + i < sg.rows && pos < end)
+                a.scores[score_row(sg, sg.row0 + 4 * ty + i) + pos] = see[j] ? s[i][j] : -INFINITY;
+            }
             s[i][j] *= sc;
             if (see[j]) mx = fmaxf(mx, s[i][j]);
           }
@@ -979,6 +1025,10 @@ __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs
           po[c * step] = make_float4(acc[i][j].x * f, acc[i][j].y * f, acc[i][j].z * f, acc[i][j].w * f);
       }
       if (sg.part >= 0 && tx == 0) a.part_ml[sg.part + r] = make_float2(m[i], l[i]);
+      if constexpr (kScores) {
+        if (sg.part < 0 && tx == 0)
+          a.row_ml[static_cast<size_t>(sg.tok0 + node) * a.num_heads + head] = make_float2(m[i], l[i]);
+      }
     }
   }
 }
@@ -992,7 +1042,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs
 // =====================================================================================
 constexpr int kSimtRows = kTreeSmall, kSimtPos = kTreeSmall, kSimtThreads = 256;
 
-template <typename T, int DPL>
+template <typename T, int DPL, bool kScores>
 __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs a) {
   extern __shared__ float4 smem4[];
   const int D = a.head_dim, ld = D + 4;
@@ -1041,7 +1091,7 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
       for (int d = 0; d < DPL; ++d) acc[i][d] = 0.f;
     }
     for (int tile = sg.tile0; tile < sg.tile1; ++tile) {
-      const int p0 = tile * kSimtPos;
+      const int p0 = sg.base + tile * kSimtPos;
       __syncthreads();
       // rows behind the sequence's last position are zero, whatever their page holds
       for (int x = threadIdx.x; x < kSimtPos * U; x += kSimtThreads) {
@@ -1081,6 +1131,10 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
       for (int i = 0; i < 4; ++i) {
         const int node = (sg.row0 + min(warp * 4 + i, sg.rows - 1)) / a.group;
         const bool vis = j < 0 || (pos < end && sees(a, sg.tok0, node, j));
+        if constexpr (kScores) {
+          if (warp * 4 + i < sg.rows && pos < end)
+            a.scores[score_row(sg, sg.row0 + warp * 4 + i) + pos] = vis ? s[i] : -INFINITY;
+        }
         const float sc = vis ? s[i] * a.scale_log2 : kNegBig;
         float mx = fmaxf(sc, m[i]);
 #pragma unroll
@@ -1127,6 +1181,10 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
         T* po = reinterpret_cast<T*>(a.out) +
                 (static_cast<size_t>(sg.tok0 + node) * a.num_heads + head) * D;
         const float inv = l[i] > 0.f ? 1.0f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
+        if constexpr (kScores) {
+          if (lane == 0)
+            a.row_ml[static_cast<size_t>(sg.tok0 + node) * a.num_heads + head] = make_float2(m[i], l[i]);
+        }
 #pragma unroll
         for (int d = 0; d < DPL; ++d)
           if (lane + 32 * d < D) po[lane + 32 * d] = from_f32<T>(acc[i][d] * inv);
@@ -1144,76 +1202,167 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
 // =====================================================================================
 constexpr int kMergeThreads = 256;
 
+// 16 bytes of output of one row, gathered from pieces.
+template <typename T>
+struct Join {
+  static constexpr int N = 16 / sizeof(T), F = N / 4;
+  static constexpr int kAtOnce = 4;   // pieces on their way together
+  float mx = kNegBig, sum = 0.f;
+  float4 o[F];
+
+  __device__ __forceinline__ Join() {
+#pragma unroll
+    for (int i = 0; i < F; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // n pieces from partial row `part` on, of `rows` rows each; 16 bytes c of their row r.
+  __device__ __forceinline__ void add(const TreeArgs& a, int part, int n, int rows, int r, int c) {
+    const float2* ml = a.part_ml + part + r;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + static_cast<size_t>(part) * a.head_dim) +
+                       c * F * rows + r;
+    const size_t po_step = static_cast<size_t>(rows) * a.head_dim / 4;
+    for (int k0 = 0; k0 < n; k0 += kAtOnce) {
+      float2 e[kAtOnce];
+      float4 v[kAtOnce][F];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const bool there = k0 + k < n;
+        e[k] = there ? ml[static_cast<size_t>(k0 + k) * rows] : make_float2(kNegBig, 0.f);
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+          v[k][i] = there ? po[(k0 + k) * po_step + i * rows] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float m2 = mx;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) m2 = fmaxf(m2, e[k].x);
+      const float f = fast_exp2(mx - m2);
+      mx = m2;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        o[i].x *= f;
+        o[i].y *= f;
+        o[i].z *= f;
+        o[i].w *= f;
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float w = fast_exp2(e[k].x - mx);
+        sum += e[k].y * w;
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+          o[i].x += v[k][i].x * w;
+          o[i].y += v[k][i].y * w;
+          o[i].z += v[k][i].z * w;
+          o[i].w += v[k][i].w * w;
+        }
+      }
+    }
+  }
+  // into 16 bytes c of row `row` of the output, (tokens * heads) rows
+  __device__ __forceinline__ void store(const TreeArgs& a, size_t row, int c) const {
+    const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+    T v[N];
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      v[4 * i] = from_f32<T>(o[i].x * inv);
+      v[4 * i + 1] = from_f32<T>(o[i].y * inv);
+      v[4 * i + 2] = from_f32<T>(o[i].z * inv);
+      v[4 * i + 3] = from_f32<T>(o[i].w * inv);
+    }
+    T* out = reinterpret_cast<T*>(a.out) + row * a.head_dim + c * N;
+    *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);
+  }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
-  constexpr int N = 16 / sizeof(T), F = N / 4;
   const TreeMerge mg = a.merges[blockIdx.x];
-  const int D = a.head_dim;
   wait_prerequisites();
   launch_dependents();
   const int x = blockIdx.y * kMergeThreads + threadIdx.x;
   const int c = x / mg.rows, r = x - c * mg.rows;   // 16 bytes c of row r
-  if (c * N >= D) return;
-  const float2* ml = a.part_ml + mg.part + r;
-  const float4* po = reinterpret_cast<const float4*>(a.part_o + static_cast<size_t>(mg.part) * D) +
-                     c * F * mg.rows + r;
-  const size_t po_step = static_cast<size_t>(mg.rows) * D / 4;
-  float mx = kNegBig, sum = 0.f;
-  float4 o[F];
-#pragma unroll
-  for (int i = 0; i < F; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int kAtOnce = 4;   // pieces on their way together
-  for (int k0 = 0; k0 < mg.n_parts; k0 += kAtOnce) {
-    float2 e[kAtOnce];
-    float4 v[kAtOnce][F];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const bool there = k0 + k < mg.n_parts;
-      e[k] = there ? ml[static_cast<size_t>(k0 + k) * mg.rows] : make_float2(kNegBig, 0.f);
-#pragma unroll
-      for (int i = 0; i < F; ++i)
-        v[k][i] = there ? po[(k0 + k) * po_step + i * mg.rows] : make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c * Join<T>::N >= a.head_dim) return;
+  Join<T> join;
+  join.add(a, mg.part, mg.n_parts, mg.rows, r, c);
+  const int row = mg.row0 + r, node = row / a.group;
+  const int head = mg.kvh * a.group + row - node * a.group;
+  const size_t out_row = static_cast<size_t>(mg.tok0 + node) * a.num_heads + head;
+  join.store(a, out_row, c);
+  if (a.row_ml && c == 0) a.row_ml[out_row] = make_float2(join.mx, join.sum);
+}
+
+// =====================================================================================
+// Join of a shared prefix and what follows it: a row's pieces are those of its group's
+// prefix, then those of its own positions.  A CTA joins one run of rows (a sequence's
+// q-heads of one KV head) with 16 bytes of one row a thread.
+// =====================================================================================
+constexpr int kSharedJoinThreads = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const TreeArgs a) {
+  const SharedJoin j = a.joins[blockIdx.x];
+  wait_prerequisites();
+  launch_dependents();
+  const int n = j.rows * (a.head_dim / Join<T>::N);
+  for (int x = threadIdx.x; x < n; x += kSharedJoinThreads) {
+    const int c = x / j.rows, r = x - c * j.rows;
+    Join<T> join;
+    join.add(a, j.prefix.part, j.prefix.n, j.prefix.rows, j.prefix.row + r, c);
+    join.add(a, j.own.part, j.own.n, j.own.rows, j.own.row + r, c);
+    join.store(a, static_cast<size_t>(j.token) * a.num_heads + j.head + r, c);
+  }
+}
+
+// =====================================================================================
+// Weights per slot: weights[row, kvh, p] += sum over the tokens and the head group of
+// 2^(s scale log2(e) - max) / sum, from the kept scores and the rows' final statistics.  A
+// thread owns four slots and adds the rows in order, so the sums do not depend on the
+// schedule; slots of the call's own tokens start from zero.  The statistics of 256 rows
+// at a time wait in shared memory.
+// =====================================================================================
+constexpr int kWeighThreads = 128, kWeighSlots = 4 * kWeighThreads, kWeighRows = 256;
+static_assert(kWeighSlots == kTreeWeighSlots, "the plan cuts the slots as the kernel takes them");
+
+__global__ void __launch_bounds__(kWeighThreads) tree_weights_kernel(const TreeArgs a) {
+  __shared__ float2 s_ml[kWeighRows];
+  const TreeWeigh w = a.weighs[blockIdx.x];
+  wait_prerequisites();
+  launch_dependents();
+  const int end = w.ctx + w.nodes, rows = w.nodes * a.group, pitch = (end + 15) & ~15;
+  const int p = w.slot0 + 4 * threadIdx.x;
+  const float* s = a.scores + static_cast<size_t>(w.scores) * 16 + p;
+  const float sc = a.score_scale;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r0 = 0; r0 < rows; r0 += kWeighRows) {
+    const int n = min(kWeighRows, rows - r0);
+    __syncthreads();
+    for (int r = threadIdx.x; r < n; r += kWeighThreads) {
+      const int node = (r0 + r) / a.group, head = w.kvh * a.group + r0 + r - node * a.group;
+      const float2 e = a.row_ml[static_cast<size_t>(w.tok0 + node) * a.num_heads + head];
+      s_ml[r] = make_float2(e.x, e.y > 0.f ? 1.0f / e.y : (e.y == 0.f ? 0.f : e.y));
     }
-    float m2 = mx;
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) m2 = fmaxf(m2, e[k].x);
-    const float f = fast_exp2(mx - m2);
-    mx = m2;
-    sum *= f;
-#pragma unroll
-    for (int i = 0; i < F; ++i) {
-      o[i].x *= f;
-      o[i].y *= f;
-      o[i].z *= f;
-      o[i].w *= f;
-    }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const float w = fast_exp2(e[k].x - mx);
-      sum += e[k].y * w;
-#pragma unroll
-      for (int i = 0; i < F; ++i) {
-        o[i].x += v[k][i].x * w;
-        o[i].y += v[k][i].y * w;
-        o[i].z += v[k][i].z * w;
-        o[i].w += v[k][i].w * w;
+    __syncthreads();
+    if (p < end) {
+      auto weight = [&](float x, float2 e) {
+        return x == -INFINITY ? 0.f : fast_exp2(fmaf(x, sc, -e.x)) * e.y;
+      };
+#pragma unroll 8
+      for (int r = 0; r < n; ++r) {
+        const float4 x = __ldcs(reinterpret_cast<const float4*>(s + static_cast<size_t>(r0 + r) * pitch));
+        const float2 e = s_ml[r];
+        sum.x += weight(x.x, e);
+        sum.y += weight(x.y, e);
+        sum.z += weight(x.z, e);
+        sum.w += weight(x.w, e);
       }
     }
   }
-  const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
-  const int row = mg.row0 + r, node = row / a.group;
-  const int head = mg.kvh * a.group + row - node * a.group;
-  T v[N];
+  if (p >= end) return;
+  float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
+  const float add[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-  for (int i = 0; i < F; ++i) {
-    v[4 * i] = from_f32<T>(o[i].x * inv);
-    v[4 * i + 1] = from_f32<T>(o[i].y * inv);
-    v[4 * i + 2] = from_f32<T>(o[i].z * inv);
-    v[4 * i + 3] = from_f32<T>(o[i].w * inv);
-  }
-  T* out = reinterpret_cast<T*>(a.out) +
-           (static_cast<size_t>(mg.tok0 + node) * a.num_heads + head) * D + c * N;
-  *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);
+  for (int i = 0; i < 4; ++i)
+    if (p + i < end) out[i] = p + i < w.ctx ? out[i] + add[i] : add[i];
 }
 
 // Dynamic shared memory opt-in, once per kernel, device and size.
@@ -1249,78 +1398,89 @@ cudaError_t prefer_shared() {
   return e;
 }
 
-template <typename T, int DPL>
+template <typename T, int DPL, bool kScores>
 cudaError_t run_simt(const TreeArgs& a, cudaStream_t s) {
   const size_t smem = sizeof(float) * (static_cast<size_t>(kSimtRows + kSimtPos) * (a.head_dim + 4) +
                                        static_cast<size_t>(kSimtPos) * a.head_dim);
-  const cudaError_t e = allow_smem<tree_simt_kernel<T, DPL>>(smem);
+  const cudaError_t e = allow_smem<tree_simt_kernel<T, DPL, kScores>>(smem);
   if (e != cudaSuccess) return e;
-  return launch_early(tree_simt_kernel<T, DPL>, dim3(a.n_ctas), kSimtThreads, smem, s, a);
+  return launch_early(tree_simt_kernel<T, DPL, kScores>, dim3(a.n_ctas), kSimtThreads, smem, s, a);
 }
 
-template <int NJ>
+template <int NJ, bool kScores>
 cudaError_t run_f32(const TreeArgs& a, cudaStream_t s) {
   const size_t ld = a.head_dim + 4, buf = F32Shape<NJ>::kBuffers;
   const size_t smem = sizeof(float) * (kF32Rows * ld + kF32Rows * (kF32Pos + 4) +
                                        buf * kF32Pos * (ld + a.head_dim));
-  const cudaError_t e = allow_smem<tree_f32_kernel<NJ>>(smem);
+  const cudaError_t e = allow_smem<tree_f32_kernel<NJ, kScores>>(smem);
   if (e != cudaSuccess) return e;
-  return launch_early(tree_f32_kernel<NJ>, dim3(a.n_ctas), kF32Threads, smem, s, a);
+  return launch_early(tree_f32_kernel<NJ, kScores>, dim3(a.n_ctas), kF32Threads, smem, s, a);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kScores>
 cudaError_t run_mma(const TreeArgs& a, cudaStream_t s) {
   using S = TreeShape<D>;
-  const cudaError_t e = allow_smem<tree_mma_kernel<T, D>>(S::kSmem);
+  const cudaError_t e = allow_smem<tree_mma_kernel<T, D, kScores>>(S::kSmem);
   if (e != cudaSuccess) return e;
-  return launch_early(tree_mma_kernel<T, D>, dim3(a.n_ctas), S::kThreads, S::kSmem, s, a);
+  return launch_early(tree_mma_kernel<T, D, kScores>, dim3(a.n_ctas), S::kThreads, S::kSmem, s, a);
 }
 
-template <typename T>
+template <typename T, bool kScores>
 cudaError_t run_mma_any(const TreeArgs& a, cudaStream_t s) {
-  switch (a.head_dim) {
-    case 32: return run_mma<T, 32>(a, s);
-    case 64: return run_mma<T, 64>(a, s);
-    case 96: return run_mma<T, 96>(a, s);
-    case 128: return run_mma<T, 128>(a, s);
-    case 160: return run_mma<T, 160>(a, s);
-    case 192: return run_mma<T, 192>(a, s);
-    case 256: return run_mma<T, 256>(a, s);
-    default: return cudaErrorInvalidValue;
+  if constexpr (sizeof(T) == 2) {
+    switch (a.head_dim) {
+      case 32: return run_mma<T, 32, kScores>(a, s);
+      case 64: return run_mma<T, 64, kScores>(a, s);
+      case 96: return run_mma<T, 96, kScores>(a, s);
+      case 128: return run_mma<T, 128, kScores>(a, s);
+      case 160: return run_mma<T, 160, kScores>(a, s);
+      case 192: return run_mma<T, 192, kScores>(a, s);
+      case 256: return run_mma<T, 256, kScores>(a, s);
+      default: break;
+    }
   }
-}
-template <>
-cudaError_t run_mma_any<float>(const TreeArgs&, cudaStream_t) {
   return cudaErrorInvalidValue;
 }
 
-template <typename T>
-cudaError_t run_cuda_cores(const TreeArgs& a, const TreeTile&, cudaStream_t s) {
-  if (a.head_dim <= 64) return run_simt<T, 2>(a, s);
-  if (a.head_dim <= 128) return run_simt<T, 4>(a, s);
-  return run_simt<T, 8>(a, s);
-}
-template <>
-cudaError_t run_cuda_cores<float>(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
-  if (t.rows == kSimtRows) {
-    if (a.head_dim <= 64) return run_simt<float, 2>(a, s);
-    if (a.head_dim <= 128) return run_simt<float, 4>(a, s);
-    return run_simt<float, 8>(a, s);
+template <typename T, bool kScores>
+cudaError_t run_cuda_cores(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4) {
+    if (t.rows != kSimtRows) {
+      if (a.head_dim <= 64) return run_f32<1, kScores>(a, s);
+      if (a.head_dim <= 128) return run_f32<2, kScores>(a, s);
+      return run_f32<4, kScores>(a, s);
+    }
   }
-  if (a.head_dim <= 64) return run_f32<1>(a, s);
-  if (a.head_dim <= 128) return run_f32<2>(a, s);
-  return run_f32<4>(a, s);
+  if (a.head_dim <= 64) return run_simt<T, 2, kScores>(a, s);
+  if (a.head_dim <= 128) return run_simt<T, 4, kScores>(a, s);
+  return run_simt<T, 8, kScores>(a, s);
 }
 
 template <typename T>
 cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
-  cudaError_t e = t.tensor ? run_mma_any<T>(a, s) : run_cuda_cores<T>(a, t, s);
-  if (e != cudaSuccess || a.n_merges == 0) return e;
-  if ((e = prefer_shared<tree_merge_kernel<T>>()) != cudaSuccess) return e;
-  const int per = a.max_merge_rows * (a.head_dim * static_cast<int>(sizeof(T)) / 16);
-  return launch_early(tree_merge_kernel<T>,
-                      dim3(a.n_merges, (per + kMergeThreads - 1) / kMergeThreads), kMergeThreads, 0,
-                      s, a);
+  cudaError_t e = cudaSuccess;
+  if (a.n_ctas > 0) {
+    if (a.scores)
+      e = t.tensor ? run_mma_any<T, true>(a, s) : run_cuda_cores<T, true>(a, t, s);
+    else
+      e = t.tensor ? run_mma_any<T, false>(a, s) : run_cuda_cores<T, false>(a, t, s);
+  }
+  if (e == cudaSuccess && a.n_merges > 0) {
+    if ((e = prefer_shared<tree_merge_kernel<T>>()) != cudaSuccess) return e;
+    const int per = a.max_merge_rows * (a.head_dim * static_cast<int>(sizeof(T)) / 16);
+    e = launch_early(tree_merge_kernel<T>,
+                     dim3(a.n_merges, (per + kMergeThreads - 1) / kMergeThreads), kMergeThreads, 0,
+                     s, a);
+  }
+  if (e == cudaSuccess && a.n_joins > 0) {
+    if ((e = prefer_shared<shared_join_kernel<T>>()) != cudaSuccess) return e;
+    e = launch_early(shared_join_kernel<T>, dim3(a.n_joins), kSharedJoinThreads, 0, s, a);
+  }
+  if (e == cudaSuccess && a.n_weighs > 0) {
+    if ((e = prefer_shared<tree_weights_kernel>()) != cudaSuccess) return e;
+    e = launch_early(tree_weights_kernel, dim3(a.n_weighs), kWeighThreads, 0, s, a);
+  }
+  return e;
 }
 
 }  // namespace
@@ -1339,7 +1499,6 @@ TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms) {
 }
 
 cudaError_t launch_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
-  if (a.n_ctas <= 0) return cudaSuccess;
   switch (a.dtype) {
     case KVC_DTYPE_F16: return run_tree<__half>(a, t, s);
     case KVC_DTYPE_BF16: return run_tree<__nv_bfloat16>(a, t, s);

@@ -174,11 +174,26 @@ SIGNATURES = {
     "kvc_beam_select": (_c_int, [_vp, _vp, _c_int, _i64, _vp, _c_int, _c_int, _c_int, _c_int, _vp,
                                  _vp, _vp, _vp]),
     "kvc_reorder_beams": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
+    "kvc_append_norm_rope": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp,
+                                      _vp, _c_int, _c_float, _vp, _c_int, _c_int, _vp, _vp, _vp,
+                                      _c_int, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
+    "kvc_shared_plan_create": (_c_int, [ctypes.POINTER(_vp)]),
+    "kvc_shared_plan_destroy": (_c_int, [_vp]),
+    "kvc_plan_shared": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
+    "kvc_shared_plan_info": (_c_int, [_vp, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
+                                      ctypes.POINTER(_c_size)]),
+    "kvc_decode_shared": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_float, _vp]),
+    "kvc_tree_plan_set_weights": (_c_int, [_vp, _c_int]),
+    "kvc_decode_tree_weights": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_int, _vp, _c_int, _c_int,
+                                         _vp, _vp, _c_int, _c_float, _vp]),
+    "kvc_evict": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_int, _c_int,
+                           _c_int, _c_int, _vp, _vp]),
 }
 
 MAX_TREE_NODES = 256
 MAX_BEAMS = 16
 MAX_BEAM_OUT = 32
+MAX_ROPE_AXES = 4
 
 XCHG_HANDLE_BYTES = 64
 

@@ -203,6 +203,89 @@ class TreePlan:
             pass
 
 
+class SharedPlan:
+    """Work list of one decode step over shared prefixes (see kvc_plan_shared)."""
+
+    def __init__(self):
+        h = ctypes.c_void_p()
+        ffi.check(ffi.lib.kvc_shared_plan_create(ctypes.byref(h)))
+        self.handle = h
+        self.n_tokens = 0
+        self.num_heads = 0
+        self.max_row = 0
+        self.lens: Optional[np.ndarray] = None
+
+    def info(self) -> PlanInfo:
+        n, ctas, scratch = ctypes.c_int(), ctypes.c_int(), ctypes.c_size_t()
+        ffi.check(ffi.lib.kvc_shared_plan_info(self.handle, ctypes.byref(n), ctypes.byref(ctas),
+                                               ctypes.byref(scratch)))
+        return PlanInfo(n.value, ctas.value, ctas.value, scratch.value)
+
+    def close(self):
+        if self.handle is not None:
+            ffi.check(ffi.lib.kvc_shared_plan_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Rotation:
+    """Which pairs of a head are rotated, how fast, and by which of a token's positions
+    (see kvc_append_norm_rope).
+
+    The first ``rotary_dim`` dims of a head are rotated, pair j of them by
+    ``freq_base^(-2j / rotary_dim)`` a position.  ``sections`` deals the pairs out to the
+    axes of a position (time, height, width: how many each turns, rotary_dim / 2 in sum):
+
+    * order "blocks": the first axis takes the first pairs, the next one those behind them;
+    * order "cyclic": the axes take turns, pair j going to axis j % axes while that axis
+      has pairs left and to the first one after that;
+    * order "ladders": as "blocks", but every axis starts its own frequencies,
+      ``freq_base^(-i / pairs of the axis)`` for its i-th pair.
+
+    ``inv_freq`` (rotary_dim / 2 numbers) replaces the frequencies, for stretched or scaled
+    ones.  ``neox``: pair j is dims j and j + rotary_dim / 2, else 2j and 2j + 1."""
+
+    def __init__(self, rotary_dim: int, freq_base: float = 10000.0,
+                 sections: Optional[Sequence[int]] = None, order: str = "blocks",
+                 neox: bool = True, inv_freq: Optional[Sequence[float]] = None):
+        if rotary_dim <= 0 or rotary_dim % 2:
+            raise ValueError("rotary_dim must be a positive even integer.")
+        if not (freq_base > 0.0 and math.isfinite(freq_base)):
+            raise ValueError("freq_base must be positive.")
+        if order not in ("blocks", "cyclic", "ladders"):
+            raise ValueError(f"unknown order of the axes {order!r}")
+        half = rotary_dim // 2
+        sec = [half] if sections is None else [int(x) for x in sections]
+        if not 1 <= len(sec) <= ffi.MAX_ROPE_AXES or min(sec) < 0 or sum(sec) != half:
+            raise ValueError(f"sections must deal {half} pairs out to 1 to {ffi.MAX_ROPE_AXES} axes")
+        j = np.arange(half)
+        inv = np.power(float(freq_base), -j / half)
+        if order == "cyclic":
+            axis = j % len(sec)
+            axis[j // len(sec) >= np.asarray(sec)[axis]] = 0
+            if np.bincount(axis, minlength=len(sec)).tolist() != sec:
+                raise ValueError(f"the sections {sec} cannot take turns")
+        else:
+            axis = np.repeat(np.arange(len(sec)), sec)
+            if order == "ladders":
+                inv = np.concatenate([np.power(float(freq_base), -np.arange(n) / n)
+                                      for n in sec if n])
+        if inv_freq is not None:
+            inv = np.asarray(inv_freq, dtype=np.float64)
+            if inv.shape != (half,) or not np.all(np.isfinite(inv)):
+                raise ValueError(f"inv_freq must be {half} finite numbers")
+        self.rotary_dim, self.pairs, self.axes, self.neox = rotary_dim, half, len(sec), bool(neox)
+        self.inv_freq = np.array(inv, dtype=np.float64)
+        self.axis = np.array(axis, dtype=np.uint8)
+        self.inv_freq.setflags(write=False)
+        self.axis.setflags(write=False)
+
+
 class PagedKVCache:
     """Paged K/V pool for ``num_layers`` layers on one GPU."""
 
@@ -392,14 +475,16 @@ class PagedKVCache:
 
     def plan_tree(self, ctx_lens: Sequence[int], node_counts: Sequence[int], num_heads: int,
                   rows: Optional[Sequence[int]] = None, plan: Optional[TreePlan] = None,
-                  stream=None) -> TreePlan:
+                  stream=None, weights: bool = False) -> TreePlan:
         """Plan the attention of node_counts[i] drafted tokens per sequence behind
-        ctx_lens[i] cached positions of block-table row rows[i] (default i)."""
+        ctx_lens[i] cached positions of block-table row rows[i] (default i); with
+        ``weights`` for decode_tree_weights."""
         ctx, cnt = _counts(ctx_lens, "ctx_lens"), _counts(node_counts, "node_counts")
         r = None if rows is None else _counts(rows, "rows")
         if ctx.shape != cnt.shape or ctx.ndim != 1 or (r is not None and r.shape != ctx.shape):
             raise ValueError("ctx_lens, node_counts and rows must have one entry per sequence")
         p = plan if plan is not None else TreePlan()
+        ffi.check(ffi.lib.kvc_tree_plan_set_weights(p.handle, 1 if weights else 0))
         ffi.check(ffi.lib.kvc_plan_tree(p.handle, self.handle, ffi.np_ptr(r), ffi.np_ptr(ctx),
                                         ffi.np_ptr(cnt), ctx.size, int(num_heads),
                                         _stream_on(stream, self.device)))
@@ -424,6 +509,158 @@ class PagedKVCache:
             _on(out, "out", dt, n, dev), block_tables.data_ptr(), block_tables.shape[1], scale,
             _stream_on(stream, dev)))
 
+    def decode_tree_weights(self, plan: TreePlan, layer: int, q: torch.Tensor,
+                            mask: Optional[torch.Tensor], weights: torch.Tensor,
+                            out: torch.Tensor, block_tables: torch.Tensor, scale: float,
+                            stream=None):
+        """decode_tree that also adds its attention weights up (kvc_decode_tree_weights):
+        weights (table rows, kv_heads, slots) fp32, weights[r, h, p] += what the tokens of
+        the sequence in row r gave position p through KV head h's q-heads; slots of the
+        plan's own tokens start from zero.  The plan is one with ``weights``."""
+        dev, dt, t = self.device, self.dtype, plan.n_tokens
+        n = t * plan.num_heads * self.head_dim
+        mp, words = self._mask(mask, t)
+        self._table(block_tables, plan)
+        if weights.dim() != 3 or weights.shape[1] != self.num_kv_heads:
+            raise ValueError("weights must be (rows, kv_heads, slots)")
+        ffi.check(ffi.lib.kvc_decode_tree_weights(
+            self.handle, plan.handle, layer, _on(q, "q", dt, n, dev), mp, words,
+            _on(weights, "weights", torch.float32, 0, dev), weights.shape[0], weights.shape[2],
+            _on(out, "out", dt, n, dev), block_tables.data_ptr(), block_tables.shape[1], scale,
+            _stream_on(stream, dev)))
+
+    def append_norm_rope(self, layer: int, q: Optional[torch.Tensor], k_new: torch.Tensor,
+                         v_new: torch.Tensor, block_tables: torch.Tensor,
+                         positions: torch.Tensor, rotation: Optional[Rotation],
+                         rows: Optional[torch.Tensor] = None,
+                         rope_positions: Optional[torch.Tensor] = None,
+                         q_weight: Optional[torch.Tensor] = None,
+                         k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                         q_out: Optional[torch.Tensor] = None,
+                         stream=None) -> Optional[torch.Tensor]:
+        """append_rope with every head of q and K normalised first (RMSNorm with q_weight /
+        k_weight (head_dim); None: not normalised) and rotated as ``rotation`` says (None:
+        not at all), in one launch (kvc_append_norm_rope).  rope_positions: (n) or
+        (n, axes) int32, the token's position on every axis of the rotation; without them
+        all axes count ``positions``.  The rest as in append_rope; returns q_out."""
+        dev, dt, d = self.device, self.dtype, self.head_dim
+        n = positions.numel()
+        rows_shape = (n, self.num_kv_heads, d)
+        kp, ks = _token_rows(k_new, "k_new", dt, rows_shape, dev)
+        vp, vs = _token_rows(v_new, "v_new", dt, rows_shape, dev)
+        qp = op = None
+        heads = qs = 0
+        if q is not None:
+            if q.dim() != 3:
+                raise ValueError("q must be (n, heads, head_dim)")
+            heads = q.shape[1]
+            qp, qs = _token_rows(q, "q", dt, (n, heads, d), dev)
+            if q_out is None:
+                with _made_on(stream, dev):
+                    q_out = torch.empty((n, heads, d), dtype=dt, device=q.device)
+            op = _on(q_out, "q_out", dt, n * heads * d, dev)
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be (rows, pages)")
+        axes = 1 if rotation is None else rotation.axes
+        rp = None
+        if rope_positions is not None:
+            if rope_positions.shape != (n, axes) and (axes > 1 or rope_positions.shape != (n,)):
+                raise ValueError(f"rope_positions must be ({n}, {axes}), got "
+                                 f"{tuple(rope_positions.shape)}")
+            rp = _on(rope_positions, "rope_positions", torch.int32, n * axes, dev)
+        for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            if w is not None and w.shape != (d,):
+                raise ValueError(f"{name} must be ({d},), got {tuple(w.shape)}")
+        ffi.check(ffi.lib.kvc_append_norm_rope(
+            self.handle, layer, qp, qs, op, heads,
+            None if q_weight is None else _on(q_weight, "q_weight", dt, d, dev), kp, ks,
+            None if k_weight is None else _on(k_weight, "k_weight", dt, d, dev), vp, vs, eps,
+            _on(block_tables, "block_tables", torch.int32, 0, dev), block_tables.shape[0],
+            block_tables.shape[1],
+            None if rows is None else _on(rows, "rows", torch.int32, n, dev),
+            _on(positions, "positions", torch.int32, n, dev), rp, axes, n,
+            None if rotation is None else ffi.np_ptr(rotation.inv_freq),
+            None if rotation is None else ffi.np_ptr(rotation.axis),
+            0 if rotation is None else rotation.pairs,
+            1 if rotation is not None and rotation.neox else 0, _stream_on(stream, dev)))
+        return q_out
+
+    def plan_shared(self, lens: Sequence[int], group_sizes: Sequence[int],
+                    prefix_lens: Sequence[int], num_heads: int,
+                    rows: Optional[Sequence[int]] = None, plan: Optional[SharedPlan] = None,
+                    stream=None) -> SharedPlan:
+        """Plan a decode step whose query i attends over positions [0, lens[i]) of
+        block-table row rows[i] (default i).  The batch is cut into runs of
+        group_sizes[k] queries that have their first prefix_lens[k] positions (whole pages)
+        in common; those are read once for all of them (kvc_plan_shared)."""
+        ln, sz = _counts(lens, "lens"), _counts(group_sizes, "group_sizes")
+        pre = _counts(prefix_lens, "prefix_lens")
+        r = None if rows is None else _counts(rows, "rows")
+        if ln.ndim != 1 or (r is not None and r.shape != ln.shape):
+            raise ValueError("lens and rows must have one entry per query")
+        if sz.ndim != 1 or sz.shape != pre.shape:
+            raise ValueError("group_sizes and prefix_lens must have one entry per group")
+        p = plan if plan is not None else SharedPlan()
+        ffi.check(ffi.lib.kvc_plan_shared(p.handle, self.handle, ffi.np_ptr(r), ffi.np_ptr(ln),
+                                          ln.size, ffi.np_ptr(sz), ffi.np_ptr(pre), sz.size,
+                                          int(num_heads), _stream_on(stream, self.device)))
+        p.n_tokens = ln.size
+        p.num_heads = int(num_heads)
+        p.max_row = int(r.max(initial=0)) if r is not None else max(0, ln.size - 1)
+        p.lens = ln
+        return p
+
+    def decode_shared(self, plan: SharedPlan, layer: int, q: torch.Tensor, out: torch.Tensor,
+                      block_tables: torch.Tensor, scale: float, stream=None):
+        """Attention of a shared plan's queries (kvc_decode_shared): q, out (queries, heads,
+        D).  Their K/V rows must be appended already."""
+        dev, dt = self.device, self.dtype
+        n = plan.n_tokens * plan.num_heads * self.head_dim
+        self._table(block_tables, plan)
+        ffi.check(ffi.lib.kvc_decode_shared(
+            self.handle, plan.handle, layer, _on(q, "q", dt, n, dev), _on(out, "out", dt, n, dev),
+            block_tables.data_ptr(), block_tables.shape[1], scale, _stream_on(stream, dev)))
+
+    def evict(self, block_tables: torch.Tensor, ctx_lens: torch.Tensor, weights: torch.Tensor,
+              budget: int, recent: int = 0, rows: Optional[torch.Tensor] = None,
+              weights_out: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None,
+              stream=None) -> torch.Tensor:
+        """Cut sequences back to ``budget`` cached positions in every layer (kvc_evict): the
+        last ``recent`` and those with the largest weights stay and move together.  weights
+        (layers, table rows, kv_heads, slots) fp32, as decode_tree_weights adds them up, go
+        along into weights_out (default: in place).  Returns the positions that stayed,
+        (layers, sequences, kv_heads, budget) int32, -1 behind a shorter sequence's; the
+        cached lengths are min(ctx_lens, budget) from then on.  ctx_lens and rows int32."""
+        dev, n = self.device, ctx_lens.numel()
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be (rows, pages)")
+        if rows is None and n > block_tables.shape[0]:
+            raise IndexError("a sequence's block-table row is outside the table")
+        if weights.dim() != 4 or weights.shape[0] != self.num_layers or \
+                weights.shape[2] != self.num_kv_heads:
+            raise ValueError("weights must be (layers, rows, kv_heads, slots)")
+        if weights_out is None:
+            weights_out = weights
+        if weights_out.shape != weights.shape:
+            raise ValueError("weights_out must have the shape of weights")
+        shape = (self.num_layers, n, self.num_kv_heads, int(budget))
+        if kept is None:
+            with _made_on(stream, dev):
+                kept = torch.empty(tuple(max(0, x) for x in shape), dtype=torch.int32,
+                                   device=f"cuda:{dev}")
+        elif kept.shape != shape:
+            raise ValueError(f"kept must be {shape}, got {tuple(kept.shape)}")
+        ffi.check(ffi.lib.kvc_evict(
+            self.handle, _on(block_tables, "block_tables", torch.int32, 0, dev),
+            block_tables.shape[0], block_tables.shape[1],
+            None if rows is None else _on(rows, "rows", torch.int32, n, dev),
+            _on(ctx_lens, "ctx_lens", torch.int32, n, dev), n,
+            _on(weights, "weights", torch.float32, 0, dev),
+            _on(weights_out, "weights_out", torch.float32, 0, dev), weights.shape[1],
+            weights.shape[3], int(budget), int(recent), _on(kept, "kept", torch.int32, 0, dev),
+            _stream_on(stream, dev)))
+        return kept
+
     def _mask(self, mask: Optional[torch.Tensor], tokens: int):
         if mask is None:
             return None, 0
@@ -434,7 +671,7 @@ class PagedKVCache:
             raise ValueError("a mask needs at least one word per token")
         return _on(mask, "mask", torch.int32, tokens * words, self.device), words
 
-    def _table(self, block_tables: torch.Tensor, plan: TreePlan) -> None:
+    def _table(self, block_tables: torch.Tensor, plan) -> None:
         _on(block_tables, "block_tables", torch.int32, 0, self.device)
         if block_tables.dim() != 2:
             raise ValueError("block_tables must be (rows, pages)")

@@ -660,6 +660,106 @@ KVC_API int kvc_reorder_beams(kvc_pool_t* pool, int32_t* d_block_tables, int bt_
                               const int32_t* d_parents, const int32_t* d_ctx_lens, int n_seqs,
                               int n_beams, void* stream);
 
+/* ==== 7. Head norms, shared prefixes and eviction on the paged pool =============
+ * No counterpart in the reference.  kvc_append_norm_rope is kvc_append_rope for
+ * models that normalise each head of q and K, rotate a part of it, or count
+ * positions on several axes (time, height and width of images and video).
+ * kvc_decode_shared is a decode step's attention for sequences that share long
+ * prefixes.  kvc_decode_tree_weights is kvc_decode_tree that also adds its
+ * attention weights up per cached slot, and kvc_evict cuts a cache back to its
+ * heaviest slots by those sums.  Memory, streams and devices as in section 6. */
+
+#define KVC_MAX_ROPE_AXES 4
+
+typedef struct kvc_shared_plan kvc_shared_plan_t;
+
+/* Normalises, rotates and appends n tokens in one pass: K row = R(N(d_k_new[i])) and
+ * V row = d_v_new[i] at slot d_positions[i] of block-table row d_rows[i] (NULL: row
+ * 0), and, when d_q is given, d_q_out[i] = R(N(d_q[i])).
+ * N, per head: x * w / sqrt(mean(x^2) + eps) over the head_dim values, w = d_q_weight
+ * or d_k_weight, (head_dim) in the pool's type; NULL leaves that tensor as it is.
+ * R, per head: pair j < n_pairs is turned by p_a * h_inv_freq[j], a = h_axes[j]
+ * (NULL: 0) and p_a = d_rope_positions[i * n_axes + a]; without d_rope_positions
+ * every axis counts d_positions[i].  Pair j is dims (j, j + n_pairs) if neox, else
+ * (2 j, 2 j + 1); dims from 2 n_pairs on are not rotated, and n_pairs 0 rotates
+ * nothing.  h_inv_freq and h_axes are host memory, read before the call returns.
+ * Angles are reduced in 64 bits and so exact at any position; norm and rotation are
+ * in 32 bits (a head whose squares pass 3.4e38 in sum becomes zero), rounded once to
+ * the pool's type.  Strides, padding, errors and alignment as in kvc_append_rope; eps
+ * must be positive. */
+KVC_API int kvc_append_norm_rope(
+    kvc_pool_t* pool, int layer, const void* d_q, int q_stride, void* d_q_out, int num_heads,
+    const void* d_q_weight, const void* d_k_new, int k_stride, const void* d_k_weight,
+    const void* d_v_new, int v_stride, float eps, const int32_t* d_block_tables, int bt_rows,
+    int bt_stride, const int32_t* d_rows, const int32_t* d_positions,
+    const int32_t* d_rope_positions, int n_axes, int n, const double* h_inv_freq,
+    const uint8_t* h_axes, int n_pairs, int neox, void* stream);
+
+/* The work list of one decode step, used by all its layers.  Query i attends over
+ * positions [0, h_lens[i]) of block-table row h_rows[i] (NULL: row i), its own row
+ * appended already.  The batch is cut into n_groups runs of consecutive queries:
+ * group k has h_group_sizes[k] members whose first h_prefix_lens[k] positions (a
+ * whole number of pages, none longer than a member) are the same, in the pages that
+ * the first member's row names; they are read once for the whole group.  A query
+ * without company is a group of one, whose prefix does not matter.  Built on the host
+ * and uploaded on `stream`, which must not be capturing. */
+KVC_API int kvc_shared_plan_create(kvc_shared_plan_t** out);
+KVC_API int kvc_shared_plan_destroy(kvc_shared_plan_t* plan);
+KVC_API int kvc_plan_shared(kvc_shared_plan_t* plan, const kvc_pool_t* pool,
+                            const int32_t* h_rows, const int32_t* h_lens, int n_seqs,
+                            const int32_t* h_group_sizes, const int32_t* h_prefix_lens,
+                            int n_groups, int num_heads, void* stream);
+/* Of the last build: queries, CTAs of the attention kernel, bytes of partials. */
+KVC_API int kvc_shared_plan_info(const kvc_shared_plan_t* plan, int* n_queries, int* n_ctas,
+                                 size_t* scratch_bytes);
+
+/* Attention of a shared plan's queries for one layer: d_q, d_out (n_seqs, num_heads,
+ * head_dim) in the pool's type.  A query of length 0 gets a zero row.  Numerics, and
+ * what calls that share a plan have to mind, as in kvc_decode_tree. */
+KVC_API int kvc_decode_shared(kvc_pool_t* pool, const kvc_shared_plan_t* plan, int layer,
+                              const void* d_q, void* d_out, const int32_t* d_block_tables,
+                              int bt_stride, float scale, void* stream);
+
+/* Builds of the plan from now on (do not) make room for kvc_decode_tree_weights: 4
+ * bytes for each token, q-head and position it may see, at most 2^30 of them.  Such a
+ * plan's sequences must be in different block-table rows. */
+KVC_API int kvc_tree_plan_set_weights(kvc_tree_plan_t* plan, int on);
+
+/* kvc_decode_tree that also adds its softmax weights up: d_weights is (weight_rows,
+ * num_kv_heads, weight_slots) in fp32, and for the sequence in block-table row r,
+ * d_weights[r, h, p] += the weight of position p summed over the sequence's tokens and
+ * the q-heads of KV head h, for its cached positions p < ctx; the slots of its drafted
+ * tokens, [ctx, ctx + nodes), are set to that sum instead.  Other slots and rows stay
+ * as they were.  The weights are in 32 bits, not rounded to the pool's type, and the
+ * rows are added in order, so a call repeats bit by bit.  The plan needs
+ * kvc_tree_plan_set_weights before its build; its score buffer, too, is its own. */
+KVC_API int kvc_decode_tree_weights(kvc_pool_t* pool, const kvc_tree_plan_t* plan, int layer,
+                                    const void* d_q, const int32_t* d_mask, int mask_words,
+                                    float* d_weights, int weight_rows, int weight_slots,
+                                    void* d_out, const int32_t* d_block_tables, int bt_stride,
+                                    float scale, void* stream);
+
+/* Cuts sequences back to `budget` cached positions, in every layer and KV head by
+ * itself.  Of the d_ctx_lens[i] positions of block-table row d_rows[i] (NULL: row i)
+ * the last `recent` stay, and of the others the budget - recent with the largest
+ * d_weights[layer, row, head, position] (equal ones: the lower position; not a number
+ * counts as the lowest), d_weights being (layers, weight_rows, num_kv_heads,
+ * weight_slots) in fp32.  Their K and V rows move together, in order, to positions
+ * [0, budget), and their weights to the same places of d_weights_out (the same shape;
+ * it may be d_weights).  d_kept, (layers, n_seqs, num_kv_heads, budget), gets the
+ * positions that stayed, ascending.  A sequence of at most `budget` positions stays as
+ * it is; its kept positions are its own, then -1.  Positions behind the kept ones are
+ * left as they were, so the cached length is min(d_ctx_lens[i], budget) from then on.
+ * Rows keep the rotation that they were appended with.  No two sequences of a call
+ * share a row or a page below their length: pages that are read by others (a shared
+ * prefix) must be copied first.  A row, length or page out of range is reported
+ * (KVC_DEVERR_BAD_POSITION / _BAD_PAGE); a sequence with a bad row or length is left
+ * alone, and its d_kept is -1. */
+KVC_API int kvc_evict(kvc_pool_t* pool, const int32_t* d_block_tables, int bt_rows,
+                      int bt_stride, const int32_t* d_rows, const int32_t* d_ctx_lens, int n_seqs,
+                      const float* d_weights, float* d_weights_out, int weight_rows,
+                      int weight_slots, int budget, int recent, int32_t* d_kept, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
