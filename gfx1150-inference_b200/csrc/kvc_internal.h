@@ -195,6 +195,8 @@ struct DecodeArgs {
   // the plan is rebuilt for grown contexts.  The decode grid then spans every SM
   // and the merge grid n_queries x num_heads.  Null: the values above are used.
   const int* plan_hdr = nullptr;
+  // The caller joins the partial states itself, and re-arms the unit counter: no merge.
+  int no_merge = 0;
 };
 // Slots of the plan's device header (int32).
 constexpr int kHdrUnits = 0;

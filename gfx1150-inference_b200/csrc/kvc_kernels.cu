@@ -1368,6 +1368,7 @@ cudaError_t run_persistent(const DecodeArgs& a, cudaStream_t s) {
     cfg.numAttrs = 1;
     if ((e = cudaLaunchKernelEx(&cfg, kern, a)) != cudaSuccess) return e;
   }
+  if (a.no_merge) return cudaSuccess;
   // merge (and counter re-arm) as a programmatic dependent launch: scheduled while
   // the decode grid drains
   cudaLaunchConfig_t cfg = {};

@@ -6,6 +6,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <exception>
 #include <new>
 #include <vector>
@@ -90,7 +91,8 @@ struct alignas(16) TreeSeg {
   int bt_row, ctx, nodes, tok0;
   int kvh, row0, rows, tile0;
   int tile1, part, base;         // part: first row of its partials, -1: writes the output
-  int scores;                    // 16 floats: where row 0's scores start (TreeArgs::scores)
+  int scores;                    // 16 floats: where row 0's scores start (TreeArgs::scores),
+                                 // -1: not kept
 };
 // Rows whose partials are joined: n_parts pieces, `rows` partial rows apart.
 struct alignas(16) TreeMerge {
@@ -99,7 +101,7 @@ struct alignas(16) TreeMerge {
 };
 
 // The pieces of one row run: partial rows `part` on, n pieces `rows` partial rows apart, the
-// run's first row at `row` of each.
+// run's first row at `row` of each.  Of the decode kernel: its n splits from `part` on.
 struct JoinPieces {
   int part, n, rows, row;
 };
@@ -108,12 +110,15 @@ struct alignas(16) SharedJoin {
   JoinPieces prefix, own;
   int token, head, rows, pad;
 };
-// kTreeWeighSlots slots of one (sequence, KV head) whose weights are added up.
-constexpr int kTreeWeighSlots = 512;
+// Slots of one (sequence, KV head) whose weights are added up: kWeighSlots from slot0 on from
+// kept scores, kRecountSlots where they are computed again.
+constexpr int kWeighSlots = 512, kRecountSlots = 128;
 struct alignas(16) TreeWeigh {
   int bt_row, ctx, nodes, tok0;
   int kvh, slot0, scores, pad;   // scores: as in TreeSeg
 };
+// (token, q-head) rows up to which a sequence keeps its scores on the tensor cores.
+constexpr int kKeepRows = 32;
 
 struct TreeArgs {
   PagedView p;
@@ -131,13 +136,18 @@ struct TreeArgs {
   float scale_log2;
   const SharedJoin* joins;       // instead of merges, for shared prefixes
   int n_joins;
-  // Attention that adds its weights up (null otherwise): the raw scores and final (max, sum)
-  // of every row, and where the sums go, (table rows, KV heads, weight_slots).
-  float* scores;
-  float2* row_ml;                // (tokens, H)
-  const TreeWeigh* weighs;
-  int n_weighs;
+  // Own positions that the decode kernel attends to: its partial states, (splits, H, D) and
+  // (splits, H), and the counter of its work list, which the join re-arms; null: none.
+  const float* own_o;
+  const float2* own_ml;
+  unsigned int* own_queue;
+  // Attention that adds its weights up (null otherwise): where the sums go, (table rows, KV
+  // heads, weight_slots), every row's final (max, sum), and kept raw scores.
   float* weights;
+  float2* row_ml;                // (tokens, H)
+  float* scores;
+  const TreeWeigh* weighs;       // those with kept scores, then those without
+  int n_weighs, n_recounts;
   int weight_slots;
   float score_scale;             // what a kept score is multiplied by, log2 units
 };
@@ -153,6 +163,9 @@ struct TreeTile {
 constexpr int kTreeSmall = 32;
 TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms);
 cudaError_t launch_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s);
+cudaError_t launch_shared_join(const TreeArgs& a, cudaStream_t s);
+// The weights of what launch_tree has just attended to.
+cudaError_t launch_weigh(const TreeArgs& a, const TreeTile& t, cudaStream_t s);
 
 // ---- beam selection ---------------------------------------------------------------------
 struct BeamArgs {
@@ -190,6 +203,37 @@ cudaError_t launch_early(void (*kernel)(A), dim3 grid, int threads, size_t smem,
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+// Dynamic shared memory opt-in, once per kernel, device and size.
+template <auto Kernel>
+cudaError_t allow_smem(size_t smem) {
+  static std::atomic<size_t> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire) >= smem) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem));
+  if (e == cudaSuccess && dev >= 0 && dev < 64) {
+    size_t cur = done[dev].load(std::memory_order_relaxed);
+    while (cur < smem && !done[dev].compare_exchange_weak(cur, smem)) {
+    }
+  }
+  return e;
+}
+
+// Asks for the attention kernels' split of shared memory and L1, once per kernel and device.
+template <auto Kernel>
+cudaError_t prefer_shared() {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire))) return e;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                           cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+  return e;
 }
 
 cudaError_t launch_append_rope(const AppendRopeArgs& a, cudaStream_t s);
@@ -290,7 +334,7 @@ struct kvc_tree_plan {
   const int32_t* dev_slots = nullptr;  // (n_tokens) cache slot of each token
   // kvc_tree_plan_set_weights: builds make room for the scores; has_scores: the last did
   bool keep_scores = false, has_scores = false;
-  int n_weighs = 0;
+  int n_weighs = 0, n_recounts = 0;
   const kvc::TreeWeigh* dev_weighs = nullptr;
   kvc::DevBuf d_blob, d_part_o, d_part_ml, d_scores, d_row_ml;
   kvc::DevBuf d_layer;                 // activations of kvc_forward_layer_tree

@@ -190,6 +190,7 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
     a.row_ml = static_cast<float2*>(plan->d_row_ml.ptr);
     a.weighs = plan->dev_weighs;
     a.n_weighs = plan->n_weighs;
+    a.n_recounts = plan->n_recounts;
     a.weights = d_weights;
     a.weight_slots = weight_slots;
     // (the tensor cores' kernel takes the scale's sign into q)
@@ -348,11 +349,12 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   std::sort(seen.begin(), seen.end());
   const bool rows_apart = std::adjacent_find(seen.begin(), seen.end()) == seen.end();
   const TreeTile tile = tree_tile(g, small, sms);
+  auto keeps = [&](int nodes) { return p->keep_scores && (!tile.tensor || nodes * group <= kKeepRows); };
   for (int i = 0; i < n_seqs; ++i) {
     const int64_t blocks = (static_cast<int64_t>(h_nodes[i]) * group + tile.rows - 1) / tile.rows;
     const int64_t end = static_cast<int64_t>(h_ctx[i]) + h_nodes[i];
     tiles += blocks * g.num_kv_heads * ((end + tile.positions - 1) / tile.positions);
-    scores += static_cast<int64_t>(h_nodes[i]) * num_heads * ((end + 15) / 16);
+    if (keeps(h_nodes[i])) scores += static_cast<int64_t>(h_nodes[i]) * num_heads * ((end + 15) / 16);
   }
   if (tokens * num_heads > (1ll << 30) || tiles > (1ll << 30))
     return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
@@ -363,7 +365,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
                      "two sequences of one block-table row cannot add their weights up together.");
   std::vector<TreeSeg> runs, segs;
   std::vector<TreeMerge> merges;
-  std::vector<TreeWeigh> weighs;
+  std::vector<TreeWeigh> weighs, recounts;
   std::vector<int> cta_segs;
   int tok0 = 0, score0 = 0;
   for (int i = 0; i < n_seqs; tok0 += h_nodes[i++]) {
@@ -378,10 +380,12 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
       sg.tile1 = (end + tile.positions - 1) / tile.positions;
       sg.part = -1;
       if (p->keep_scores) {
-        sg.scores = score0;
-        score0 += n_rows * ((end + 15) / 16);
-        for (int slot = 0; slot < end; slot += kTreeWeighSlots)
-          weighs.push_back(TreeWeigh{sg.bt_row, sg.ctx, sg.nodes, sg.tok0, kvh, slot, sg.scores, 0});
+        const bool keep = keeps(h_nodes[i]);
+        sg.scores = keep ? score0 : -1;
+        if (keep) score0 += n_rows * ((end + 15) / 16);
+        std::vector<TreeWeigh>& list = keep ? weighs : recounts;
+        for (int slot = 0; slot < end; slot += keep ? kWeighSlots : kRecountSlots)
+          list.push_back(TreeWeigh{sg.bt_row, sg.ctx, sg.nodes, sg.tok0, kvh, slot, sg.scores, 0});
       }
       for (int r0 = 0; r0 < n_rows; r0 += tile.rows) {
         sg.row0 = r0;
@@ -427,6 +431,11 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   p->max_merge_rows = max_merge_rows;
   p->part_rows = part_rows;
   p->n_weighs = static_cast<int>(weighs.size());
+  p->n_recounts = static_cast<int>(recounts.size());
+  // (those with the most rows first: the last CTAs are short ones)
+  std::stable_sort(recounts.begin(), recounts.end(),
+                   [](const TreeWeigh& x, const TreeWeigh& y) { return x.nodes > y.nodes; });
+  weighs.insert(weighs.end(), recounts.begin(), recounts.end());
   p->has_scores = p->keep_scores;
   p->pool_geom = g;
   p->device = pool->device;
@@ -439,7 +448,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
       (e = p->d_part_ml.ensure(sizeof(float2) * std::max<size_t>(1, part_rows))))
     return cuda_error(e, "plan buffers");
   if (p->keep_scores &&
-      ((e = p->d_scores.ensure(sizeof(float) * 16 * static_cast<size_t>(score0))) ||
+      ((e = p->d_scores.ensure(sizeof(float) * 16 * static_cast<size_t>(std::max(1, score0)))) ||
        (e = p->d_row_ml.ensure(sizeof(float2) * static_cast<size_t>(tokens) * num_heads))))
     return cuda_error(e, "plan buffers");
   const PlanPart parts[] = {{segs.data(), sizeof(TreeSeg) * segs.size()},

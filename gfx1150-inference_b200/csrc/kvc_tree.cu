@@ -12,8 +12,8 @@
 //   tree_merge_kernel   joins the pieces of rows whose positions were split over CTAs
 //   shared_join_kernel  the same for rows of a shared prefix and their own positions
 //                       (kvc_decode_shared)
-//   tree_weights_kernel adds the probabilities up per slot (kvc_decode_tree_weights),
-//                       from scores that the attention kernels' kScores variants keep
+// The kScores variants also keep what kvc_weigh.cu makes the weights per slot of
+// (kvc_decode_tree_weights): every row's final max and sum, and the scores of short row lists.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -24,23 +24,11 @@
 #include "kvc_device.cuh"
 #include "kvc_spec.h"
 #include "kvc_tcgen05.cuh"
+#include "kvc_tree.cuh"
 #include "kvcache.h"
 
 namespace kvc {
 namespace {
-
-// Page of `pos` of a sequence; a bad entry is reported and reads page 0.
-__device__ __forceinline__ int tree_page(const PagedView& p, int bt_row, int pos) {
-  const int col = pos / p.page_size;
-  const int page = col < p.bt_stride
-                       ? p.block_tables[static_cast<size_t>(bt_row) * p.bt_stride + col]
-                       : -1;
-  if (page < 0 || page >= p.num_pages) {
-    report_error_at(p.err, KVC_DEVERR_BAD_PAGE, static_cast<uint32_t>(page));
-    return 0;
-  }
-  return page;
-}
 
 // Whether node `node` of a sequence sees its drafted token j.
 __device__ __forceinline__ bool sees(const TreeArgs& a, int tok0, int node, int j) {
@@ -128,29 +116,6 @@ __device__ __forceinline__ bool maybe_odd(uint32_t two) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
   const uint32_t t = (two & e) ^ e;   // a half is zero where its exponent is all ones
   return ((t - 0x00010001u) & ~t & 0x80008000u) != 0u;
-}
-
-// A score that the row does not see, as it is kept (-inf).
-constexpr uint32_t kUnseen = 0xff800000u;
-// Where row r of a (sequence, KV head) keeps its scores: rows of whole 16s, in a row.
-__device__ __forceinline__ size_t score_row(const TreeSeg& sg, int r) {
-  const int pitch = (sg.ctx + sg.nodes + 15) & ~15;
-  return static_cast<size_t>(sg.scores) * 16 + static_cast<size_t>(r) * pitch;
-}
-
-// Mask word k (drafted tokens 32 k ... 32 k + 31) of a row; below 0: cached positions.
-__device__ __forceinline__ uint32_t mask_word(const TreeArgs& a, const TreeSeg& sg, int node, int k) {
-  if (k < 0) return 0xffffffffu;
-  const int left = sg.nodes - 32 * k;
-  if (left <= 0) return 0u;
-  uint32_t w;
-  if (a.mask) {
-    w = k < a.mask_words ? a.mask[static_cast<size_t>(sg.tok0 + node) * a.mask_words + k] : 0u;
-  } else {
-    const int upto = node - 32 * k;  // a chain
-    w = upto < 0 ? 0u : (upto >= 31 ? 0xffffffffu : (2u << upto) - 1u);
-  }
-  return left < 32 ? w & ((1u << left) - 1u) : w;
 }
 
 template <typename T, int D, bool kScores>
@@ -452,12 +417,12 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const bool two = sg.rows > 128;
         const int ahead = S::kStreams == 2 && !two ? 2 : 1;
         // Q in k-major core matrices, all its copies in flight together: a warp's copy covers
-        // 8 rows x 64 bytes, rows past the block are zero.  Streams that share their rows get
-        // a copy each.
+        // 8 rows x 64 bytes.  Rows behind the last are zero up to a group of 8; what lies
+        // further on reaches no live row.  Streams that share their rows get a copy each.
         if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
         if (ok) {
           const int rr = lane >> 2, uu = lane & 3;
-          const int n_rows = two ? 256 : 128;
+          const int n_rows = (sg.rows + 7) & ~7;
           // node and head of row g0 + rr, carried along (a division takes as long as the copies)
           int node = (sg.row0 + rr) / a.group, rem = sg.row0 + rr - node * a.group;
           const int dn = 8 / a.group, dr = 8 - dn * a.group;
@@ -485,8 +450,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
           copy_async_wait();
           if (flip) {   // a negative scale turns q: what other lanes have copied, too
             __syncwarp();
-            for (int i = lane; i < S::kStreams * S::kQBytes / 4; i += 32)
-              reinterpret_cast<uint32_t*>(q_mem)[i] ^= flip;
+            for (int x = 0; x < S::kStreams; ++x) {
+              const int n = !two ? n_rows : x == 0 ? 128 : n_rows - 128;
+              uint32_t* words = reinterpret_cast<uint32_t*>(q_mem + x * S::kQBytes);
+              for (int i = lane; i < n * D / 2; i += 32) words[i] ^= flip;
+            }
           }
         }
         fence_proxy_async();
@@ -561,6 +529,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const bool joint = ahead == 2;
       const int row = (two ? x * 128 : 0) + r;
       const bool live = (two ? x * 128 : 0) + w4 * 32 < seg->rows;   // some row of the warp
+      const bool mine = row < seg->rows;   // (rows behind the last hold whatever Q's memory does)
       float m = kNegBig, l = 0.f;     // max in log2 units, less kLift
       // One tile of the stream: scores to probabilities, in place, and the running max and
       // sum.  Edge tiles hold positions that some rows do not see.
@@ -572,7 +541,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         if constexpr (kScores) {
           const TreeSeg sg = *seg;
           const int p0 = p00 + t * KP;
-          if (row < sg.rows) {
+          if (row < sg.rows && sg.scores >= 0) {
             keep = a.scores + score_row(sg, sg.row0 + row) + p0;
             keep_n = min(KP, sg.ctx + sg.nodes - p0);
           }
@@ -655,7 +624,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         }
         for (;;) {
           pass();
-          const bool grew = mt > m + kRescaleAt;
+          const bool grew = mine && mt > m + kRescaleAt;
           if (!__any_sync(0xffffffffu, grew)) break;
           const float m2 = grew ? mt : m;
           const float f = fast_exp2(m - m2);
@@ -1231,31 +1200,52 @@ struct Join {
         for (int i = 0; i < F; ++i)
           v[k][i] = there ? po[(k0 + k) * po_step + i * rows] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      float m2 = mx;
+      take(e, v);
+    }
+  }
+  __device__ __forceinline__ void take(const float2 (&e)[kAtOnce], const float4 (&v)[kAtOnce][F]) {
+    float m2 = mx;
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) m2 = fmaxf(m2, e[k].x);
-      const float f = fast_exp2(mx - m2);
-      mx = m2;
-      sum *= f;
+    for (int k = 0; k < kAtOnce; ++k) m2 = fmaxf(m2, e[k].x);
+    const float f = fast_exp2(mx - m2);
+    mx = m2;
+    sum *= f;
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      o[i].x *= f;
+      o[i].y *= f;
+      o[i].z *= f;
+      o[i].w *= f;
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float w = fast_exp2(e[k].x - mx);
+      sum += e[k].y * w;
 #pragma unroll
       for (int i = 0; i < F; ++i) {
-        o[i].x *= f;
-        o[i].y *= f;
-        o[i].z *= f;
-        o[i].w *= f;
+        o[i].x += v[k][i].x * w;
+        o[i].y += v[k][i].y * w;
+        o[i].z += v[k][i].z * w;
+        o[i].w += v[k][i].w * w;
       }
+    }
+  }
+  // n splits from `split` on of the decode kernel, whose rows are plain; head `head`.
+  __device__ __forceinline__ void add_splits(const TreeArgs& a, int split, int n, int head, int c) {
+    for (int k0 = 0; k0 < n; k0 += kAtOnce) {
+      float2 e[kAtOnce];
+      float4 v[kAtOnce][F];
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
-        const float w = fast_exp2(e[k].x - mx);
-        sum += e[k].y * w;
+        const bool there = k0 + k < n;
+        const size_t row = static_cast<size_t>(split + k0 + k) * a.num_heads + head;
+        e[k] = there ? a.own_ml[row] : make_float2(kNegBig, 0.f);
 #pragma unroll
-        for (int i = 0; i < F; ++i) {
-          o[i].x += v[k][i].x * w;
-          o[i].y += v[k][i].y * w;
-          o[i].z += v[k][i].z * w;
-          o[i].w += v[k][i].w * w;
-        }
+        for (int i = 0; i < F; ++i)
+          v[k][i] = there ? reinterpret_cast<const float4*>(a.own_o + row * a.head_dim)[c * F + i]
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+      take(e, v);
     }
   }
   // into 16 bytes c of row `row` of the output, (tokens * heads) rows
@@ -1300,104 +1290,35 @@ constexpr int kSharedJoinThreads = 128;
 
 template <typename T>
 __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const TreeArgs a) {
-  const SharedJoin j = a.joins[blockIdx.x];
+  const bool mine = blockIdx.x < a.n_joins;
+  SharedJoin j = {};
+  if (mine) j = a.joins[blockIdx.x];
   wait_prerequisites();
+  if (a.own_queue && blockIdx.x == 0) {   // the decode is done: its work list for the next call
+    if (threadIdx.x == 0) {
+      *a.own_queue = 0u;
+      __threadfence();
+    }
+    __syncthreads();
+  }
   launch_dependents();
+  if (!mine) return;
   const int n = j.rows * (a.head_dim / Join<T>::N);
   for (int x = threadIdx.x; x < n; x += kSharedJoinThreads) {
     const int c = x / j.rows, r = x - c * j.rows;
     Join<T> join;
     join.add(a, j.prefix.part, j.prefix.n, j.prefix.rows, j.prefix.row + r, c);
-    join.add(a, j.own.part, j.own.n, j.own.rows, j.own.row + r, c);
+    if (a.own_o)
+      join.add_splits(a, j.own.part, j.own.n, j.head + r, c);
+    else
+      join.add(a, j.own.part, j.own.n, j.own.rows, j.own.row + r, c);
     join.store(a, static_cast<size_t>(j.token) * a.num_heads + j.head + r, c);
   }
 }
 
-// =====================================================================================
-// Weights per slot: weights[row, kvh, p] += sum over the tokens and the head group of
-// 2^(s scale log2(e) - max) / sum, from the kept scores and the rows' final statistics.  A
-// thread owns four slots and adds the rows in order, so the sums do not depend on the
-// schedule; slots of the call's own tokens start from zero.  The statistics of 256 rows
-// at a time wait in shared memory.
-// =====================================================================================
-constexpr int kWeighThreads = 128, kWeighSlots = 4 * kWeighThreads, kWeighRows = 256;
-static_assert(kWeighSlots == kTreeWeighSlots, "the plan cuts the slots as the kernel takes them");
-
-__global__ void __launch_bounds__(kWeighThreads) tree_weights_kernel(const TreeArgs a) {
-  __shared__ float2 s_ml[kWeighRows];
-  const TreeWeigh w = a.weighs[blockIdx.x];
-  wait_prerequisites();
-  launch_dependents();
-  const int end = w.ctx + w.nodes, rows = w.nodes * a.group, pitch = (end + 15) & ~15;
-  const int p = w.slot0 + 4 * threadIdx.x;
-  const float* s = a.scores + static_cast<size_t>(w.scores) * 16 + p;
-  const float sc = a.score_scale;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int r0 = 0; r0 < rows; r0 += kWeighRows) {
-    const int n = min(kWeighRows, rows - r0);
-    __syncthreads();
-    for (int r = threadIdx.x; r < n; r += kWeighThreads) {
-      const int node = (r0 + r) / a.group, head = w.kvh * a.group + r0 + r - node * a.group;
-      const float2 e = a.row_ml[static_cast<size_t>(w.tok0 + node) * a.num_heads + head];
-      s_ml[r] = make_float2(e.x, e.y > 0.f ? 1.0f / e.y : (e.y == 0.f ? 0.f : e.y));
-    }
-    __syncthreads();
-    if (p < end) {
-      auto weight = [&](float x, float2 e) {
-        return x == -INFINITY ? 0.f : fast_exp2(fmaf(x, sc, -e.x)) * e.y;
-      };
-#pragma unroll 8
-      for (int r = 0; r < n; ++r) {
-        const float4 x = __ldcs(reinterpret_cast<const float4*>(s + static_cast<size_t>(r0 + r) * pitch));
-        const float2 e = s_ml[r];
-        sum.x += weight(x.x, e);
-        sum.y += weight(x.y, e);
-        sum.z += weight(x.z, e);
-        sum.w += weight(x.w, e);
-      }
-    }
-  }
-  if (p >= end) return;
-  float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
-  const float add[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (p + i < end) out[i] = p + i < w.ctx ? out[i] + add[i] : add[i];
-}
-
-// Dynamic shared memory opt-in, once per kernel, device and size.
-template <auto Kernel>
-cudaError_t allow_smem(size_t smem) {
-  static std::atomic<size_t> done[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire) >= smem) return cudaSuccess;
-  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem));
-  if (e == cudaSuccess && dev >= 0 && dev < 64) {
-    size_t cur = done[dev].load(std::memory_order_relaxed);
-    while (cur < smem && !done[dev].compare_exchange_weak(cur, smem)) {
-    }
-  }
-  return e;
-}
-
 // Every kernel here lets its successor begin right behind its own wait, so that nothing
-// written ahead of it is still on its way then.  The merge asks for the attention kernels'
+// written ahead of it is still on its way then.  The joins ask for the attention kernels'
 // shared-memory split, so that an SM passes from one to the other without a change of it.
-template <auto Kernel>
-cudaError_t prefer_shared() {
-  static std::atomic<bool> done[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire))) return e;
-  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                           cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
-  return e;
-}
-
 template <typename T, int DPL, bool kScores>
 cudaError_t run_simt(const TreeArgs& a, cudaStream_t s) {
   const size_t smem = sizeof(float) * (static_cast<size_t>(kSimtRows + kSimtPos) * (a.head_dim + 4) +
@@ -1460,7 +1381,7 @@ template <typename T>
 cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (a.n_ctas > 0) {
-    if (a.scores)
+    if (a.weights)
       e = t.tensor ? run_mma_any<T, true>(a, s) : run_cuda_cores<T, true>(a, t, s);
     else
       e = t.tensor ? run_mma_any<T, false>(a, s) : run_cuda_cores<T, false>(a, t, s);
@@ -1472,15 +1393,7 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
                      dim3(a.n_merges, (per + kMergeThreads - 1) / kMergeThreads), kMergeThreads, 0,
                      s, a);
   }
-  if (e == cudaSuccess && a.n_joins > 0) {
-    if ((e = prefer_shared<shared_join_kernel<T>>()) != cudaSuccess) return e;
-    e = launch_early(shared_join_kernel<T>, dim3(a.n_joins), kSharedJoinThreads, 0, s, a);
-  }
-  if (e == cudaSuccess && a.n_weighs > 0) {
-    if ((e = prefer_shared<tree_weights_kernel>()) != cudaSuccess) return e;
-    e = launch_early(tree_weights_kernel, dim3(a.n_weighs), kWeighThreads, 0, s, a);
-  }
-  return e;
+  return e == cudaSuccess && a.weights ? launch_weigh(a, t, s) : e;
 }
 
 }  // namespace
@@ -1496,6 +1409,25 @@ TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms) {
                              : TreeTile{64, 128, 1, kPieceCost, true};
   if (g.elem_size == 4 && small_tiles > 2 * sms) return TreeTile{kF32Pos, kF32Rows, 1, 1, false};
   return TreeTile{kSimtPos, kSimtRows, 2, 0, false};
+}
+
+namespace {
+template <typename T>
+cudaError_t run_shared_join(const TreeArgs& a, cudaStream_t s) {
+  const cudaError_t e = prefer_shared<shared_join_kernel<T>>();
+  if (e != cudaSuccess) return e;
+  return launch_early(shared_join_kernel<T>, dim3(std::max(1, a.n_joins)), kSharedJoinThreads, 0, s, a);
+}
+}  // namespace
+
+cudaError_t launch_shared_join(const TreeArgs& a, cudaStream_t s) {
+  if (a.n_joins == 0 && !a.own_queue) return cudaSuccess;
+  switch (a.dtype) {
+    case KVC_DTYPE_F16: return run_shared_join<__half>(a, s);
+    case KVC_DTYPE_BF16: return run_shared_join<__nv_bfloat16>(a, s);
+    case KVC_DTYPE_F32: return run_shared_join<float>(a, s);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 cudaError_t launch_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {

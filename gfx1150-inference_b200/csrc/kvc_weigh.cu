@@ -1,0 +1,325 @@
+// Attention weights summed per cached slot (kvc_decode_tree_weights), behind the attention
+// of kvc_tree.cu, which leaves every row's final max and sum (and, of short row lists, the
+// scores):
+//
+//   weights[row, kvh, p] += sum over the rows (token, q-head of kvh) of
+//                           2^(s scale log2(e) - max) / sum
+//
+//   weigh_kernel         from kept scores
+//   recount_mma_kernel   computes the scores again on the tensor cores
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "kvc_device.cuh"
+#include "kvc_spec.h"
+#include "kvc_tcgen05.cuh"
+#include "kvc_tree.cuh"
+
+namespace kvc {
+namespace {
+
+// =====================================================================================
+// Weights per slot: weights[row, kvh, p] += sum over the tokens and the head group of
+// 2^(s scale log2(e) - max) / sum, from the kept scores and the rows' final statistics.  A
+// thread owns four slots and adds the rows in order, so the sums do not depend on the
+// schedule; slots of the call's own tokens start from zero.  The statistics of 256 rows
+// at a time wait in shared memory.
+// =====================================================================================
+constexpr int kWeighThreads = kWeighSlots / 4, kWeighRows = 256;
+
+__global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const TreeArgs a) {
+  __shared__ float2 s_ml[kWeighRows];
+  const TreeWeigh w = a.weighs[blockIdx.x];
+  wait_prerequisites();
+  launch_dependents();
+  const int end = w.ctx + w.nodes, rows = w.nodes * a.group, pitch = (end + 15) & ~15;
+  const int p = w.slot0 + 4 * threadIdx.x;
+  const float* s = a.scores + static_cast<size_t>(w.scores) * 16 + p;
+  const float sc = a.score_scale;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r0 = 0; r0 < rows; r0 += kWeighRows) {
+    const int n = min(kWeighRows, rows - r0);
+    __syncthreads();
+    for (int r = threadIdx.x; r < n; r += kWeighThreads) {
+      const int node = (r0 + r) / a.group, head = w.kvh * a.group + r0 + r - node * a.group;
+      const float2 e = a.row_ml[static_cast<size_t>(w.tok0 + node) * a.num_heads + head];
+      s_ml[r] = make_float2(e.x, e.y > 0.f ? 1.0f / e.y : (e.y == 0.f ? 0.f : e.y));
+    }
+    __syncthreads();
+    if (p < end) {
+      auto weight = [&](float x, float2 e) {
+        return x == -INFINITY ? 0.f : fast_exp2(fmaf(x, sc, -e.x)) * e.y;
+      };
+#pragma unroll 8
+      for (int r = 0; r < n; ++r) {
+        const float4 x = __ldcs(reinterpret_cast<const float4*>(s + static_cast<size_t>(r0 + r) * pitch));
+        const float2 e = s_ml[r];
+        sum.x += weight(x.x, e);
+        sum.y += weight(x.y, e);
+        sum.z += weight(x.z, e);
+        sum.w += weight(x.w, e);
+      }
+    }
+  }
+  if (p >= end) return;
+  float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
+  const float add[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (p + i < end) out[i] = p + i < w.ctx ? out[i] + add[i] : add[i];
+}
+
+// =====================================================================================
+// Recount.  With many rows, writing the scores out and reading them back (8 bytes a score)
+// costs more than computing them again from K (2 D bytes a position and KV head, once).
+// The product is turned round, S^T = K Q^T: a tensor memory lane is a position, so a thread
+// owns one and adds its row of 128 columns up in registers, without a sum across threads.
+// 1 / sum goes into the exponent: the weight is 2^(s scale log2(e) - (max + log2(sum))).
+//
+// A CTA takes one tile of 128 positions and goes through the (token, q-head) rows in blocks
+// of 128, two warpgroups taking every other one by themselves: each copies its block of Q,
+// has it multiplied into its half of tensor memory and adds it up while the next block of Q
+// is on its way.  So an SM's two CTAs have four products and sums in different phases.
+// =====================================================================================
+constexpr int kRecountThreads = 256, kRecountRows = 128, kRecountCols = 256;
+
+template <int D>
+struct RecountShape {
+  static constexpr int kTileBytes = 128 * D * 2;
+  static constexpr int kHeadBytes = 6144;    // barriers, shifts, visibility
+  static constexpr int kSmem = kHeadBytes + 3 * kTileBytes;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
+    recount_mma_kernel(const TreeArgs a) {
+  using S = RecountShape<D>;
+  constexpr int U = D / 8;
+  constexpr uint32_t kSlabBytes = kSlab * D * 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);          // K, the two warpgroups' products
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + 64);
+  volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(smem + 68);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wg = warp >> 2, wt = tid & 127, ww = warp & 3;     // warpgroup; thread and warp in it
+  float* s_shift = reinterpret_cast<float*>(smem + 1024) + wg * kRecountRows;
+  uint4* s_vis = reinterpret_cast<uint4*>(smem + 2048) + wg * kRecountRows;   // of the 128 positions
+  uint8_t* k_mem = smem + S::kHeadBytes;
+  uint8_t* q_mem = k_mem + (1 + wg) * S::kTileBytes;
+  const uint32_t bar0 = smem_u32(bars), done = bar0 + 8 * (1 + wg);
+  const TreeWeigh w = a.weighs[a.n_weighs + blockIdx.x];
+  const int end = w.ctx + w.nodes, rows = w.nodes * a.group, p0 = w.slot0;
+  const int blocks = (rows + kRecountRows - 1) / kRecountRows;
+  const bool edge = p0 + kRecountSlots > w.ctx;
+  if (tid == 0) {
+    for (int i = 0; i < 3; ++i) mbar_init(bar0 + 8 * i, 1);
+    fence_mbar_init();
+    *s_abort = 0;
+  }
+  wait_prerequisites();
+  launch_dependents();
+  // (tensor memory only here: see tree_mma_kernel)
+  if (warp == 0) tmem_alloc(smem_u32(s_tmem), kRecountCols);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = *s_tmem + wg * kRecountRows;
+
+  if (warp == 0) {
+    const int slabs = min(kRecountSlots / kSlab, (end - p0 + kSlab - 1) / kSlab);
+    if (lane == 0) mbar_arrive_expect_tx(bar0, slabs * kSlabBytes);
+    __syncwarp();
+    if (lane < slabs) {
+      const int pos = p0 + lane * kSlab;
+      const uint8_t* src = a.p.k + (static_cast<size_t>(tree_page(a.p, w.bt_row, pos)) * a.p.num_kv_heads + w.kvh) *
+                                       a.p.page_head_bytes +
+                           pos % a.p.page_size / kSlab * kSlabBytes;
+      bulk_g2s(smem_u32(k_mem) + lane * kSlabBytes, src, kSlabBytes, bar0, l2_policy_evict_first());
+    }
+  }
+  // Block b's rows of Q (zero behind the last), in k-major core matrices: a warp's copy covers
+  // 8 rows x 64 bytes; node and head are carried along.
+  auto copy_q = [&](int b) {
+    const int dn = 32 / a.group, dr = 32 - dn * a.group;
+    int row = b * kRecountRows + ww * 8 + (lane >> 2), node = row / a.group, rem = row - node * a.group;
+    const T* base = reinterpret_cast<const T*>(a.q) +
+                    (static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group) * D + (lane & 3) * 8;
+    uint32_t dst = smem_u32(q_mem) + ww * U * 128 + (lane & 3) * 128 + (lane >> 2) * 16;
+    for (int g = 0; g < kRecountRows / 32; ++g) {
+      const bool there = row < rows;
+      const T* src = there ? base + (static_cast<size_t>(node) * a.num_heads + rem) * D : base;
+#pragma unroll
+      for (int i = 0; i < U / 4; ++i) copy16_async(dst + i * 512, src + i * 32, there ? 16 : 0);
+      dst += 4 * U * 128;
+      row += 32;
+      node += dn;
+      rem += dr;
+      if (rem >= a.group) {
+        rem -= a.group;
+        ++node;
+      }
+    }
+  };
+  // Thread r: row r's max and sum.
+  auto statistics = [&](int b) {
+    const int row = b * kRecountRows + wt, node = row / a.group;
+    return row < rows ? a.row_ml[static_cast<size_t>(w.tok0 + node) * a.num_heads + w.kvh * a.group + row -
+                                 node * a.group]
+                      : make_float2(0.f, 0.f);
+  };
+  // Thread r: what row r's scores are shifted by, and which positions of an edge tile it sees.
+  auto constants = [&](int b, float2 e) {
+    const int row = b * kRecountRows + wt;
+    uint32_t vis[4] = {0, 0, 0, 0};
+    if (edge && row < rows) {
+      const int node = row / a.group;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j0 = p0 + 32 * k - w.ctx, m = j0 >> 5;
+        vis[k] = __funnelshift_r(mask_word(a, w.tok0, w.nodes, node, m),
+                                 mask_word(a, w.tok0, w.nodes, node, m + 1), j0 & 31);
+      }
+    }
+    s_shift[wt] = e.y == 0.f ? INFINITY : e.x + log2f(e.y);     // (infinity: no weight)
+    if (edge) s_vis[wt] = make_uint4(vis[0], vis[1], vis[2], vis[3]);
+  };
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!mbar_wait_bounded(bar, parity)) {
+      report_error_at(a.p.err, KVC_DEVERR_WAIT_LIMIT, blockIdx.x);
+      *s_abort = 1;
+    }
+  };
+  auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory"); };
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 sc = make_float2(a.scale_log2, a.scale_log2);   // (q as it is, whatever the sign)
+  bool issued = false;
+  float2 next = make_float2(0.f, 0.f);
+  if (wg < blocks) {
+    copy_q(wg);
+    next = statistics(wg);
+    wait(bar0, 0);                     // K is here
+  }
+  for (int b = wg, n = 0; b < blocks; b += 2, ++n) {
+    constants(b, next);
+    copy_async_wait();
+    fence_proxy_async();
+    tmem_fence_before();
+    group_sync();                      // the block is here, and the last one's sums are made
+    tmem_fence_after();
+    if (*s_abort) break;
+    if (ww == 0 && elect_one()) {
+      constexpr uint32_t kDesc = mma_desc<T>(128, kRecountRows, false);
+      const uint64_t kd = operand_desc(smem_u32(k_mem), 128, U * 128);
+      const uint64_t qd = operand_desc(smem_u32(q_mem), 128, U * 128);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) mma_ss(tmem, kd + 16 * k, qd + 16 * k, kDesc, k > 0);
+      mma_commit(done);
+    }
+    __syncwarp();
+    issued = true;
+    if (b + 2 < blocks) next = statistics(b + 2);
+    wait(done, n & 1);
+    tmem_fence_after();
+    if (b + 2 < blocks) copy_q(b + 2);   // (the product has read the last block)
+    const uint32_t* vis = reinterpret_cast<const uint32_t*>(s_vis) + ww;
+    const uint32_t t_s = tmem + (static_cast<uint32_t>(ww * 32) << 16);
+    const int cols = min(kRecountRows, (rows - b * kRecountRows + 31) & ~31);
+    // 32 columns at a time, the next ones on their way
+    auto add = [&](int c, const uint32_t* s) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(s_shift + c + i);
+        float2 e0 = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc, make_float2(-m.x, -m.y));
+        float2 e1 = fma2(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), sc, make_float2(-m.z, -m.w));
+        e0.x = fast_exp2(e0.x);
+        e0.y = fast_exp2(e0.y);
+        e1.x = fast_exp2(e1.x);
+        e1.y = fast_exp2(e1.y);
+        if (edge) {
+          if (!((vis[4 * (c + i)] >> lane) & 1u)) e0.x = 0.f;
+          if (!((vis[4 * (c + i + 1)] >> lane) & 1u)) e0.y = 0.f;
+          if (!((vis[4 * (c + i + 2)] >> lane) & 1u)) e1.x = 0.f;
+          if (!((vis[4 * (c + i + 3)] >> lane) & 1u)) e1.y = 0.f;
+        }
+        sum[0] = add2(sum[0], e0);
+        sum[1] = add2(sum[1], e1);
+      }
+    };
+    uint32_t sa[32], sb[32];
+    tmem_ld32(t_s, sa);
+#pragma unroll 1
+    for (int c = 0; c < cols; c += 64) {
+      tmem_wait_ld();
+      tmem_loaded<32>(sa);
+      if (c + 32 < cols) tmem_ld32(t_s + c + 32, sb);
+      add(c, sa);
+      if (c + 32 < cols) {
+        tmem_wait_ld();
+        tmem_loaded<32>(sb);
+        if (c + 64 < cols) tmem_ld32(t_s + c + 64, sa);
+        add(c + 32, sb);
+      }
+    }
+    tmem_fence_before();
+    group_sync();                      // the shifts have been read by all
+    if (*s_abort) break;
+  }
+  copy_async_wait();
+  float* s_sum = reinterpret_cast<float*>(smem + 1024) + kRecountRows;   // (the second group's shifts)
+  const float add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+  if (wg == 1) s_sum[wt] = add;
+  tmem_fence_before();
+  __syncthreads();
+  const int p = p0 + wt;
+  if (wg == 0 && p < end && !*s_abort) {
+    float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
+    const float total = add + s_sum[wt];
+    *out = p < w.ctx ? *out + total : total;
+  }
+  if (*s_abort && wt == 0) {           // what is in flight lands before the memory goes
+    mbar_wait_bounded(bar0, 0);
+    if (issued) mbar_wait_bounded(done, 0);
+  }
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 0) tmem_dealloc(*s_tmem, kRecountCols);
+}
+
+template <typename T, int D>
+cudaError_t run_recount(const TreeArgs& a, cudaStream_t s) {
+  using S = RecountShape<D>;
+  const cudaError_t e = allow_smem<recount_mma_kernel<T, D>>(S::kSmem);
+  if (e != cudaSuccess) return e;
+  return launch_early(recount_mma_kernel<T, D>, dim3(a.n_recounts), kRecountThreads, S::kSmem, s, a);
+}
+
+template <typename T>
+cudaError_t run_recount_any(const TreeArgs& a, cudaStream_t s) {
+  switch (a.head_dim) {
+    case 32: return run_recount<T, 32>(a, s);
+    case 64: return run_recount<T, 64>(a, s);
+    case 96: return run_recount<T, 96>(a, s);
+    case 128: return run_recount<T, 128>(a, s);
+    case 160: return run_recount<T, 160>(a, s);
+    case 192: return run_recount<T, 192>(a, s);
+    case 256: return run_recount<T, 256>(a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_weigh(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
+  cudaError_t e = cudaSuccess;
+  if (a.n_weighs > 0) {
+    if ((e = prefer_shared<weigh_kernel>()) != cudaSuccess) return e;
+    e = launch_early(weigh_kernel, dim3(a.n_weighs), kWeighThreads, 0, s, a);
+  }
+  if (e != cudaSuccess || a.n_recounts == 0) return e;
+  if (!t.tensor) return cudaErrorInvalidValue;
+  return a.dtype == KVC_DTYPE_F16 ? run_recount_any<__half>(a, s) : run_recount_any<__nv_bfloat16>(a, s);
+}
+
+}  // namespace kvc

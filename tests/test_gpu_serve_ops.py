@@ -461,6 +461,9 @@ WEIGH = [
     (32, 4, 4, 16, [600, 31], [256, 200]),
     (64, 7, 1, 16, [100, 383, 384], [64, 1, 40]),
     (80, 4, 2, 16, [77, 200], [6, 20]),
+    (160, 4, 2, 16, [130, 0], [40, 129]),
+    (192, 6, 2, 32, [700, 130], [33, 200]),
+    (128, 32, 4, 16, [2000, 300, 64], [40, 4, 5]),         # 320, 32 and 40 rows
 ]
 
 
@@ -477,11 +480,13 @@ def test_weights_masks_rows_scales(dtype):
     weigh_case(dtype, 64, 8, 4, 16, [50, 400], [7, 9], seed=4, rows=[3, 1])
     for s in (0.0, -0.1, 1.0):
         weigh_case(dtype, 128, 4, 2, 16, [130, 9], [7, 9], seed=5, scale=s)
+        weigh_case(dtype, 128, 8, 2, 16, [130, 9], [40, 70], seed=5, scale=s, mask="any")
 
     def grow(k, v, c):
         ramp = torch.linspace(0.1, 5.0, k.shape[0], device="cuda")[:, None, None]
         k.copy_((k.float() * ramp).to(k.dtype))
     weigh_case(dtype, 128, 8, 2, 16, [2500, 700], [1, 20], seed=6, tweak=grow)
+    weigh_case(dtype, 64, 8, 2, 16, [1500], [90], seed=6, tweak=grow)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -505,6 +510,7 @@ def test_weights_of_unseen_values(dtype):
     np.random.default_rng = Rng
     try:
         me.weigh_case(dtype, 128, 8, 2, 16, [300, 60], [9, 6], seed=7, mask="any", tweak=poison)
+        me.weigh_case(dtype, 128, 8, 2, 16, [300, 60], [40, 29], seed=8, mask="any", tweak=poison)
     finally:
         np.random.default_rng = orig
 
