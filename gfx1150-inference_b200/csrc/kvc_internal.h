@@ -197,6 +197,12 @@ struct DecodeArgs {
   const int* plan_hdr = nullptr;
   // The caller joins the partial states itself, and re-arms the unit counter: no merge.
   int no_merge = 0;
+  // Scores kept for the sums of attention weights (null: not kept), scaled, in log2 units:
+  // query i's q-head h from float 16 score_base[i] + h * (context rounded up to 16) on; and
+  // the (max, sum) of rows in one split, (n_queries, H).
+  float* scores = nullptr;
+  const int* score_base = nullptr;
+  float2* row_ml = nullptr;
 };
 // Slots of the plan's device header (int32).
 constexpr int kHdrUnits = 0;

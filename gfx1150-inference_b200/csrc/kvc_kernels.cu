@@ -468,9 +468,10 @@ constexpr int persist_stages() {
              : (196608 / (kPersistWarpsPerSm * 2 * kSlab * D * 2));
 }
 
-template <typename T, int D, int NW, int NS>
+template <typename T, int D, int NW, int NS, bool kScores>
 __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     decode_persistent_kernel(const DecodeArgs a) {
+  // kScores: the scores and final statistics are kept for kvc_decode_tree_weights
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int SLAB_BYTES = kSlab * D * 2;
   constexpr int STAGE_BYTES = 2 * SLAB_BYTES;
@@ -710,6 +711,9 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     const float l_hi = __shfl_sync(0xffffffffu, l_run, (2 * tig + 1) * 4);
     const int h_lo = 2 * tig, h_hi = 2 * tig + 1;
     if (n_splits == 1 && a.xchg_peers == 0) {  // exchanged outputs all go through the merge
+      if constexpr (kScores) {
+        if (tig == 0 && gid < nh) a.row_ml[static_cast<size_t>(query) * H + hq0 + gid] = make_float2(m_run, l_run);
+      }
       const float i_lo = l_lo > 0.f ? 1.0f / l_lo : 0.f;
       const float i_hi = l_hi > 0.f ? 1.0f / l_hi : 0.f;
       T* out = reinterpret_cast<T*>(a.out) + (static_cast<size_t>(query) * H + hq0) * D;
@@ -742,6 +746,7 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     if (tig == 0 && gid < nh) a.part_ml[slot + gid] = make_float2(m_run, l_run);
   };
 
+  float* score_row = nullptr;   // of q-head gid of the unit
   constexpr int K2 = D / 32;
   constexpr bool kAllFragsFirst = D <= 128;  // registers allow holding a whole slab
   bool dead = false;  // a wait ran past its limit: stop computing
@@ -774,6 +779,9 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
         }
       }
       if (!have_q) load_q(c_r0, c_r2, qa);
+      if constexpr (kScores)
+        score_row = a.scores + static_cast<size_t>(a.score_base[c_r0.x]) * 16 +
+                    static_cast<size_t>(c_r2.z + gid) * ((c_r1.y + 15) & ~15);
       m_run = kNegBig;
       l_run = 0.f;
 #pragma unroll
@@ -881,6 +889,12 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     const float x1 = (sc[0][0][1] + sc[0][1][1]) * a.scale_log2;
     const float x2 = (sc[1][0][0] + sc[1][1][0]) * a.scale_log2;
     const float x3 = (sc[1][0][1] + sc[1][1][1]) * a.scale_log2;
+    if constexpr (kScores) {
+      if (gid < c_r2.w) {   // (whole slabs: a row has room for them)
+        *reinterpret_cast<float2*>(score_row + j * kSlab + t0) = make_float2(x0, x1);
+        *reinterpret_cast<float2*>(score_row + j * kSlab + t0 + 8) = make_float2(x2, x3);
+      }
+    }
     float mx = fmaxf(fmaxf(v0 ? x0 : kNegBig, v1 ? x1 : kNegBig),
                      fmaxf(v2 ? x2 : kNegBig, v3 ? x3 : kNegBig));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -1344,13 +1358,13 @@ cudaError_t set_smem_once(F kern, size_t smem) {
   return e;
 }
 
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, bool kScores>
 cudaError_t run_persistent(const DecodeArgs& a, cudaStream_t s) {
   constexpr int NS = persist_stages<D>();
   const size_t smem =
       kPersistBarBytes + kPersistMetaBytes + static_cast<size_t>(NW) * NS * 2 * kSlab * D * 2;
-  auto kern = decode_persistent_kernel<T, D, NW, NS>;
-  cudaError_t e = set_smem_once<decode_persistent_kernel<T, D, NW, NS>>(kern, smem);
+  auto kern = decode_persistent_kernel<T, D, NW, NS, kScores>;
+  cudaError_t e = set_smem_once<decode_persistent_kernel<T, D, NW, NS, kScores>>(kern, smem);
   if (e != cudaSuccess) return e;
   if (a.n_sched_ctas <= 0) return cudaSuccess;
   cudaLaunchAttribute attr[1];
@@ -1397,7 +1411,8 @@ cudaError_t run_persistent(const DecodeArgs& a, cudaStream_t s) {
 
 template <typename T, int D>
 cudaError_t run_mma(const DecodeArgs& a, cudaStream_t s) {
-  return run_persistent<T, D, kPersistWarps>(a, s);
+  if (a.scores) return run_persistent<T, D, kPersistWarps, true>(a, s);
+  return run_persistent<T, D, kPersistWarps, false>(a, s);
 }
 
 template <typename T, int EPL>

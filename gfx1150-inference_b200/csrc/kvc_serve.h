@@ -54,17 +54,4 @@ cudaError_t launch_evict(const EvictArgs& a, int sms, cudaStream_t s);
 // Work list of one decode step over shared prefixes (kvc_plan_shared), used by every layer.
 struct kvc_shared_plan {
   kvc_tree_plan t;                 // its pieces, their partials and its upload
-  // Own positions on the decode kernel: unit records and their counter in t's upload
-  const int4* dev_units = nullptr;
-  unsigned int* dev_queue = nullptr;
-  int n_units = 0, n_unit_ctas = 0;
-  kvc::DevBuf d_own_o, d_own_ml;
-  const kvc::SharedJoin* dev_joins = nullptr;
-  int n_joins = 0;
-
-  void release() {
-    t.release();
-    d_own_o.release();
-    d_own_ml.release();
-  }
 };

@@ -168,38 +168,11 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   // warps an SM each work on a piece of their own, and a short piece (96 x 30-700 positions, 64 x
   // 128 heads: 39 us) costs it half of what it costs a CTA of the tree kernel (74 us), which
   // is made for many rows.
-  std::vector<JoinPieces> splits(tile.tensor ? n_seqs : 0);
-  std::vector<int4> units;
-  int n_splits = 0;
+  UnitList units;
   if (tile.tensor) {
-    std::vector<int> own(n_seqs), refine(n_seqs);
-    for (int i = 0; i < n_seqs; ++i) own[i] = h_lens[i] - base[i];
-    const int chunks = (group + 7) / 8;
-    const int C = split_partition_sms(g.page_size, own.data(), n_seqs, Hkv * chunks, sms, refine.data());
-    std::vector<int4> items;
-    for (int i = 0; i < n_seqs; ++i) {
-      if (own[i] == 0) continue;
-      splits[i].part = n_splits;
-      splits[i].n = emit_splits(i, own[i], C, refine[i], [&](int4 it) {
-        it.z += base[i];
-        it.w += base[i];
-        items.push_back(it);
-      });
-      n_splits += splits[i].n;
-    }
-    std::stable_sort(items.begin(), items.end(),
-                     [](const int4& x, const int4& y) { return x.w - x.z > y.w - y.z; });
-    for (const int4& it : items) {
-      const int i = it.x;
-      // (more than one split: the kernel leaves partial states)
-      const int n = splits[i].n + (base[i] > 0 ? 1 : 0);
-      for (int kvh = 0; kvh < Hkv; ++kvh)
-        for (int c = 0; c < chunks; ++c) {
-          units.push_back(it);
-          units.push_back(make_int4(h_rows ? h_rows[i] : i, h_lens[i], splits[i].part, n));
-          units.push_back(make_int4(kvh, c, kvh * group + c * 8, std::min(8, group - c * 8)));
-        }
-    }
+    std::vector<int> rows(n_seqs);
+    for (int i = 0; i < n_seqs; ++i) rows[i] = h_rows ? h_rows[i] : i;
+    build_units(g, group, sms, rows, base, std::vector<int>(h_lens, h_lens + n_seqs), &units);
   }
   for (int i = 0; i < n_seqs && !tile.tensor; ++i) {
     if (h_lens[i] <= base[i]) continue;
@@ -252,7 +225,7 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
             j.prefix.row = row % tile.rows;
           }
           if (tile.tensor) {
-            if (base[i] > 0 || splits[i].n > 1) j.own = splits[i];   // (else it is written already)
+            if (base[i] > 0 || units.splits[i].n > 1) j.own = units.splits[i];   // (else it is written already)
           } else if (own_run[i] >= 0) {
             j.own = pieces[own_run[i] + kvh * own_blocks + r / tile.rows];
             j.own.row = r % tile.rows;
@@ -273,7 +246,7 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   p->part_rows = part_rows;
   p->pool_geom = g;
   p->device = pool->device;
-  sp->n_joins = static_cast<int>(joins.size());
+  p->n_joins = static_cast<int>(joins.size());
   if (n_seqs == 0) {
     p->valid = true;
     return KVC_OK;
@@ -282,55 +255,27 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   if ((e = p->d_part_o.ensure(sizeof(float) * std::max<size_t>(1, part_rows) * g.head_dim)) ||
       (e = p->d_part_ml.ensure(sizeof(float2) * std::max<size_t>(1, part_rows))))
     return cuda_error(e, "plan buffers");
-  if (tile.tensor &&
-      ((e = sp->d_own_o.ensure(sizeof(float) * std::max<size_t>(1, n_splits) * num_heads * g.head_dim)) ||
-       (e = sp->d_own_ml.ensure(sizeof(float2) * std::max<size_t>(1, n_splits) * num_heads))))
+  const size_t split_rows = std::max<size_t>(1, units.n_splits) * num_heads;
+  if (tile.tensor && ((e = p->d_own_o.ensure(sizeof(float) * split_rows * g.head_dim)) ||
+                      (e = p->d_own_ml.ensure(sizeof(float2) * split_rows))))
     return cuda_error(e, "plan buffers");
   const unsigned int zero = 0;
   const PlanPart parts[] = {{segs.data(), sizeof(TreeSeg) * segs.size()},
                             {cta_segs.data(), sizeof(int) * cta_segs.size()},
                             {joins.data(), sizeof(SharedJoin) * joins.size()},
-                            {units.data(), sizeof(int4) * units.size()},
+                            {units.recs.data(), sizeof(int4) * units.recs.size()},
                             {&zero, sizeof(zero)}};
   const uint8_t* d[5];
   if (const int rc = upload_plan(p, parts, 5, d, s)) return rc;
-  sp->dev_units = reinterpret_cast<const int4*>(d[3]);
-  sp->dev_queue = reinterpret_cast<unsigned int*>(const_cast<uint8_t*>(d[4]));
-  sp->n_units = static_cast<int>(units.size() / 3);
-  sp->n_unit_ctas = std::min(sms * kPersistCtasPerSm, (sp->n_units + kPersistWarps - 1) / kPersistWarps);
+  p->dev_units = reinterpret_cast<const int4*>(d[3]);
+  p->dev_queue = reinterpret_cast<unsigned int*>(const_cast<uint8_t*>(d[4]));
+  p->n_units = static_cast<int>(units.recs.size() / 3);
+  p->n_unit_ctas = std::min(sms * kPersistCtasPerSm, (p->n_units + kPersistWarps - 1) / kPersistWarps);
   p->dev_segs = reinterpret_cast<const TreeSeg*>(d[0]);
   p->dev_cta_segs = reinterpret_cast<const int*>(d[1]);
-  sp->dev_joins = reinterpret_cast<const SharedJoin*>(d[2]);
+  p->dev_joins = reinterpret_cast<const SharedJoin*>(d[2]);
   p->valid = true;
   return KVC_OK;
-}
-
-// The decode kernel's part of a call whose attention takes `a`.
-DecodeArgs own_args(const kvc_shared_plan* sp, const TreeArgs& a, bool behind_prefix) {
-  DecodeArgs d = {};
-  d.k_layer = a.p.k;
-  d.v_layer = a.p.v;
-  d.q = a.q;
-  d.out = a.out;
-  d.block_tables = a.p.block_tables;
-  d.bt_stride = a.p.bt_stride;
-  d.part_o = static_cast<float*>(sp->d_own_o.ptr);
-  d.part_ml = static_cast<float2*>(sp->d_own_ml.ptr);
-  d.sched_recs = sp->dev_units;
-  d.n_units = d.n_items = d.sched_cap = sp->n_units;
-  d.queue = sp->dev_queue;
-  d.n_sched_ctas = sp->n_unit_ctas;
-  d.early_prefetch = behind_prefix ? 1 : 0;
-  d.num_heads = a.num_heads;
-  d.num_kv_heads = a.p.num_kv_heads;
-  d.group = a.group;
-  d.n_hchunk = (a.group + 7) / 8;
-  d.head_dim = a.head_dim;
-  d.page_size = a.p.page_size;
-  d.num_pages = a.p.num_pages;
-  d.scale_log2 = a.scale_log2;
-  d.no_merge = 1;
-  return d;
 }
 
 }  // namespace
@@ -372,7 +317,7 @@ extern "C" int kvc_shared_plan_destroy(kvc_shared_plan_t* plan) {
   if (!plan) return KVC_OK;
   if (plan->t.device >= 0) {
     DeviceScope dev(plan->t.device);
-    plan->release();
+    plan->t.release();
   }
   delete plan;
   return KVC_OK;
@@ -389,7 +334,7 @@ extern "C" int kvc_plan_shared(kvc_shared_plan_t* plan, const kvc_pool_t* pool,
     if (int rc = refuse_capture(static_cast<cudaStream_t>(stream), "a shared-prefix plan")) return rc;
     if (plan->t.device >= 0 && plan->t.device != pool->device) {  // its buffers are elsewhere
       DeviceScope old(plan->t.device);
-      plan->release();
+      plan->t.release();
     }
     return shared_build(plan, pool, h_rows, h_lens, n_seqs, h_group_sizes, h_prefix_lens, n_groups,
                         num_heads, static_cast<cudaStream_t>(stream));
@@ -414,12 +359,11 @@ extern "C" int kvc_decode_shared(kvc_pool_t* pool, const kvc_shared_plan_t* plan
     if (p.n_tokens == 0) return KVC_OK;
     TreeArgs a = {};
     if (int rc = tree_args(pool, &p, layer, d_q, d_out, d_block_tables, bt_stride, scale, &a)) return rc;
-    a.joins = plan->dev_joins;
-    a.n_joins = plan->n_joins;
+    a.joins = p.dev_joins;
+    a.n_joins = p.n_joins;
     cudaError_t e = launch_tree(a, p.tile, static_cast<cudaStream_t>(stream));
-    if (e == cudaSuccess && plan->n_units > 0) {
-      // (the prefix's launch writes no KV, and lets this one begin only behind what came before)
-      const DecodeArgs own = own_args(plan, a, p.n_ctas > 0);
+    if (e == cudaSuccess && p.n_units > 0) {
+      const DecodeArgs own = unit_args(&p, a, p.n_ctas > 0);
       a.own_o = own.part_o;
       a.own_ml = own.part_ml;
       a.own_queue = own.queue;

@@ -266,6 +266,20 @@ constexpr int64_t kMaxScores = 1ll << 30;
 // Cuts whole runs (tile0 0, tile1 their tiles) into the CTAs' shares.
 void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
               std::vector<TreeSeg>* segs, std::vector<int>* cta_segs);
+// Work for the decode kernel: the positions [base[i], lens[i]) of query i in table row
+// rows[i], in pieces that its warps take one after another.
+struct UnitList {
+  std::vector<int4> recs;            // three records a unit
+  std::vector<JoinPieces> splits;    // of each query
+  int n_splits = 0;
+};
+// A query with a base is joined with something else: its splits are partial states, were it
+// but one.
+void build_units(const PoolGeom& g, int group, int sms, const std::vector<int>& rows,
+                 const std::vector<int>& base, const std::vector<int>& lens, UnitList* out);
+// Its arguments for units of `plan`, in a call whose attention takes `a`.  early: the launch
+// ahead writes no KV and began behind everything that does.
+DecodeArgs unit_args(const kvc_tree_plan* plan, const TreeArgs& a, bool early);
 // A plan's records go to its device buffer in one copy; dev[i]: where parts[i] will be.
 struct PlanPart {
   const void* data;
@@ -336,6 +350,13 @@ struct kvc_tree_plan {
   bool keep_scores = false, has_scores = false;
   int n_weighs = 0, n_recounts = 0;
   const kvc::TreeWeigh* dev_weighs = nullptr;
+  // Work on the decode kernel: unit records and their counter, and the joins of its splits
+  const int4* dev_units = nullptr;
+  unsigned int* dev_queue = nullptr;
+  const kvc::SharedJoin* dev_joins = nullptr;
+  const int* dev_score_base = nullptr;
+  int n_units = 0, n_unit_ctas = 0, n_joins = 0;
+  kvc::DevBuf d_own_o, d_own_ml;
   kvc::DevBuf d_blob, d_part_o, d_part_ml, d_scores, d_row_ml;
   kvc::DevBuf d_layer;                 // activations of kvc_forward_layer_tree
   kvc::HostBuf h_stage;
@@ -347,6 +368,8 @@ struct kvc_tree_plan {
     d_part_ml.release();
     d_scores.release();
     d_row_ml.release();
+    d_own_o.release();
+    d_own_ml.release();
     d_layer.release();
     h_stage.release();
     if (upload_done) cudaEventDestroy(upload_done);

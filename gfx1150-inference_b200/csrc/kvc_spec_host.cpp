@@ -195,6 +195,22 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
     a.weight_slots = weight_slots;
     // (the tensor cores' kernel takes the scale's sign into q)
     a.score_scale = plan->tile.tensor ? std::fabs(a.scale_log2) : a.scale_log2;
+    if (plan->n_units > 0 && !d_mask) {
+      DecodeArgs d = unit_args(plan, a, false);
+      d.scores = a.scores;
+      d.score_base = plan->dev_score_base;
+      d.row_ml = a.row_ml;
+      a.joins = plan->dev_joins;
+      a.n_joins = plan->n_joins;
+      a.own_o = d.part_o;
+      a.own_ml = d.part_ml;
+      a.own_queue = d.queue;
+      a.score_scale = 1.0f;   // (that kernel keeps them scaled)
+      cudaError_t e = launch_decode(d, a.dtype, a.p.layout, s);
+      if (e == cudaSuccess) e = launch_shared_join(a, s);
+      if (e == cudaSuccess) e = launch_weigh(a, plan->tile, s);
+      return e == cudaSuccess ? KVC_OK : cuda_error(e, "weighed decode kernels");
+    }
   }
   const cudaError_t e = launch_tree(a, plan->tile, s);
   return e == cudaSuccess ? KVC_OK : cuda_error(e, "tree attention kernel");
@@ -281,6 +297,65 @@ void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
       [&] { cta_segs->push_back(static_cast<int>(segs->size())); });
   if (cta_segs->back() < static_cast<int>(segs->size()))
     cta_segs->push_back(static_cast<int>(segs->size()));
+}
+
+void build_units(const PoolGeom& g, int group, int sms, const std::vector<int>& rows,
+                 const std::vector<int>& base, const std::vector<int>& lens, UnitList* out) {
+  const int n = static_cast<int>(lens.size()), chunks = (group + 7) / 8;
+  std::vector<int> own(n), refine(n);
+  for (int i = 0; i < n; ++i) own[i] = lens[i] - base[i];
+  const int C = split_partition_sms(g.page_size, own.data(), n, g.num_kv_heads * chunks, sms, refine.data());
+  out->splits.assign(n, JoinPieces{});
+  std::vector<int4> items;
+  for (int i = 0; i < n; ++i) {
+    if (own[i] == 0) continue;
+    out->splits[i].part = out->n_splits;
+    out->splits[i].n = emit_splits(i, own[i], C, refine[i], [&](int4 it) {
+      it.z += base[i];
+      it.w += base[i];
+      items.push_back(it);
+    });
+    out->n_splits += out->splits[i].n;
+  }
+  std::stable_sort(items.begin(), items.end(),
+                   [](const int4& x, const int4& y) { return x.w - x.z > y.w - y.z; });
+  for (const int4& it : items) {
+    const int i = it.x;
+    const int pieces = out->splits[i].n + (base[i] > 0 ? 1 : 0);   // (one: writes out itself)
+    for (int kvh = 0; kvh < g.num_kv_heads; ++kvh)
+      for (int c = 0; c < chunks; ++c) {
+        out->recs.push_back(it);
+        out->recs.push_back(make_int4(rows[i], lens[i], out->splits[i].part, pieces));
+        out->recs.push_back(make_int4(kvh, c, kvh * group + c * 8, std::min(8, group - c * 8)));
+      }
+  }
+}
+
+DecodeArgs unit_args(const kvc_tree_plan* plan, const TreeArgs& a, bool early) {
+  DecodeArgs d = {};
+  d.k_layer = a.p.k;
+  d.v_layer = a.p.v;
+  d.q = a.q;
+  d.out = a.out;
+  d.block_tables = a.p.block_tables;
+  d.bt_stride = a.p.bt_stride;
+  d.part_o = static_cast<float*>(plan->d_own_o.ptr);
+  d.part_ml = static_cast<float2*>(plan->d_own_ml.ptr);
+  d.sched_recs = plan->dev_units;
+  d.n_units = d.n_items = d.sched_cap = plan->n_units;
+  d.queue = plan->dev_queue;
+  d.n_sched_ctas = plan->n_unit_ctas;
+  d.early_prefetch = early ? 1 : 0;
+  d.num_heads = a.num_heads;
+  d.num_kv_heads = a.p.num_kv_heads;
+  d.group = a.group;
+  d.n_hchunk = (a.group + 7) / 8;
+  d.head_dim = a.head_dim;
+  d.page_size = a.p.page_size;
+  d.num_pages = a.p.num_pages;
+  d.scale_log2 = a.scale_log2;
+  d.no_merge = 1;
+  return d;
 }
 
 int upload_plan(kvc_tree_plan* p, const PlanPart* parts, int n, const uint8_t** dev, cudaStream_t s) {
@@ -395,6 +470,33 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     }
   }
   cut_runs(runs, tile, sms, &segs, &cta_segs);
+  // Single tokens whose weights are wanted: the decode kernel streams K and V faster for a
+  // token's few rows (32 x 1 at 1K-8K, fp16: 92 us, 105 with the kernel for trees) and keeps
+  // scores at less cost (95, 125).  The pieces above serve calls with a mask.
+  UnitList units;
+  std::vector<SharedJoin> joins;
+  std::vector<int> score_base;
+  if (p->keep_scores && tile.tensor && max_nodes == 1 && group <= kKeepRows) {
+    std::vector<int> unit_rows, lens;
+    for (int i = 0; i < n_seqs; ++i) {
+      if (h_nodes[i] == 0) continue;
+      unit_rows.push_back(h_rows ? h_rows[i] : i);
+      lens.push_back(h_ctx[i] + 1);
+    }
+    build_units(g, group, sms, unit_rows, std::vector<int>(lens.size(), 0), lens, &units);
+    for (size_t t = 0; t < lens.size(); ++t)
+      for (int kvh = 0; kvh < g.num_kv_heads && units.splits[t].n > 1; ++kvh) {
+        SharedJoin j = {};
+        j.prefix.rows = j.own.rows = 1;
+        j.own = units.splits[t];
+        j.token = static_cast<int>(t);
+        j.head = kvh * group;
+        j.rows = group;
+        joins.push_back(j);
+      }
+    for (const TreeWeigh& w : weighs)
+      if (w.kvh == 0 && w.slot0 == 0) score_base.push_back(w.scores);
+  }
   // runs in several pieces are joined from their partials
   size_t part_rows = 0;
   int max_merge_rows = 0;
@@ -437,6 +539,9 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
                    [](const TreeWeigh& x, const TreeWeigh& y) { return x.nodes > y.nodes; });
   weighs.insert(weighs.end(), recounts.begin(), recounts.end());
   p->has_scores = p->keep_scores;
+  p->n_joins = static_cast<int>(joins.size());
+  p->n_units = static_cast<int>(units.recs.size() / 3);
+  p->n_unit_ctas = std::min(sms * kPersistCtasPerSm, (p->n_units + kPersistWarps - 1) / kPersistWarps);
   p->pool_geom = g;
   p->device = pool->device;
   if (tokens == 0) {
@@ -451,14 +556,27 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
       ((e = p->d_scores.ensure(sizeof(float) * 16 * static_cast<size_t>(std::max(1, score0)))) ||
        (e = p->d_row_ml.ensure(sizeof(float2) * static_cast<size_t>(tokens) * num_heads))))
     return cuda_error(e, "plan buffers");
+  const size_t split_rows = std::max<size_t>(1, units.n_splits) * num_heads;
+  if (!units.recs.empty() && ((e = p->d_own_o.ensure(sizeof(float) * split_rows * g.head_dim)) ||
+                              (e = p->d_own_ml.ensure(sizeof(float2) * split_rows))))
+    return cuda_error(e, "plan buffers");
+  const unsigned int zero = 0;
   const PlanPart parts[] = {{segs.data(), sizeof(TreeSeg) * segs.size()},
                             {cta_segs.data(), sizeof(int) * cta_segs.size()},
                             {merges.data(), sizeof(TreeMerge) * merges.size()},
                             {rows.data(), sizeof(int32_t) * rows.size()},
                             {slots.data(), sizeof(int32_t) * slots.size()},
-                            {weighs.data(), sizeof(TreeWeigh) * weighs.size()}};
-  const uint8_t* d[6];
-  if (const int rc = upload_plan(p, parts, 6, d, s)) return rc;
+                            {weighs.data(), sizeof(TreeWeigh) * weighs.size()},
+                            {joins.data(), sizeof(SharedJoin) * joins.size()},
+                            {units.recs.data(), sizeof(int4) * units.recs.size()},
+                            {score_base.data(), sizeof(int) * score_base.size()},
+                            {&zero, sizeof(zero)}};
+  const uint8_t* d[10];
+  if (const int rc = upload_plan(p, parts, 10, d, s)) return rc;
+  p->dev_joins = reinterpret_cast<const SharedJoin*>(d[6]);
+  p->dev_units = reinterpret_cast<const int4*>(d[7]);
+  p->dev_score_base = reinterpret_cast<const int*>(d[8]);
+  p->dev_queue = reinterpret_cast<unsigned int*>(const_cast<uint8_t*>(d[9]));
   p->dev_segs = reinterpret_cast<const TreeSeg*>(d[0]);
   p->dev_cta_segs = reinterpret_cast<const int*>(d[1]);
   p->dev_merges = reinterpret_cast<const TreeMerge*>(d[2]);
@@ -530,7 +648,8 @@ extern "C" int kvc_tree_plan_info(const kvc_tree_plan_t* plan, int* n_tokens, in
   if (n_tokens) *n_tokens = plan->n_tokens;
   if (n_ctas) *n_ctas = plan->n_ctas;
   if (scratch_bytes)
-    *scratch_bytes = plan->d_part_o.cap + plan->d_part_ml.cap + plan->d_scores.cap + plan->d_row_ml.cap;
+    *scratch_bytes = plan->d_part_o.cap + plan->d_part_ml.cap + plan->d_scores.cap + plan->d_row_ml.cap + plan->d_own_o.cap +
+                     plan->d_own_ml.cap;
   return KVC_OK;
 }
 

@@ -530,22 +530,19 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const int row = (two ? x * 128 : 0) + r;
       const bool live = (two ? x * 128 : 0) + w4 * 32 < seg->rows;   // some row of the warp
       const bool mine = row < seg->rows;   // (rows behind the last hold whatever Q's memory does)
+      // where the row's scores go, 16 positions to 64 bytes (its pitch is a multiple of that)
+      float* keep = nullptr;
+      int keep_end = 0;
+      if constexpr (kScores) {
+        const TreeSeg sg = *seg;
+        keep_end = sg.ctx + sg.nodes;
+        if (mine && sg.scores >= 0) keep = a.scores + score_row(sg, sg.row0 + row);
+      }
       float m = kNegBig, l = 0.f;     // max in log2 units, less kLift
       // One tile of the stream: scores to probabilities, in place, and the running max and
       // sum.  Edge tiles hold positions that some rows do not see.
       auto softmax = [&](auto edge_tag, int t, const uint32_t* vis) {
         constexpr bool kEdge = decltype(edge_tag)::value;
-        // (a row's scores are 16 to a store of 64 bytes; its pitch is a multiple of that)
-        float* keep = nullptr;
-        int keep_n = 0;
-        if constexpr (kScores) {
-          const TreeSeg sg = *seg;
-          const int p0 = p00 + t * KP;
-          if (row < sg.rows && sg.scores >= 0) {
-            keep = a.scores + score_row(sg, sg.row0 + row) + p0;
-            keep_n = min(KP, sg.ctx + sg.nodes - p0);
-          }
-        }
         // One pass with the max as it was: the probabilities wait in registers, and only
         // when a row's max turns out to have grown too far is the pass made again.  The
         // first tile has no such max: it looks for one.
@@ -565,7 +562,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
             tmem_loaded<16>(s[w & 1]);
             if (w + 1 < KP / 16) tmem_ld16(t_s + 16 * (w + 1), s[(w + 1) & 1]);
             if constexpr (kScores) {
-              if (16 * w < keep_n) {
+              if (keep && (!kEdge || p00 + t * KP + 16 * w < keep_end)) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                   uint4 v = make_uint4(now[i], now[i + 1], now[i + 2], now[i + 3]);
@@ -576,7 +573,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
                     if (!(bits & 4u)) v.z = kUnseen;
                     if (!(bits & 8u)) v.w = kUnseen;
                   }
-                  *reinterpret_cast<uint4*>(keep + 16 * w + i) = v;
+                  *reinterpret_cast<uint4*>(keep + p00 + t * KP + 16 * w + i) = v;
                 }
               }
             }
@@ -1312,7 +1309,9 @@ __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const T
       join.add_splits(a, j.own.part, j.own.n, j.head + r, c);
     else
       join.add(a, j.own.part, j.own.n, j.own.rows, j.own.row + r, c);
-    join.store(a, static_cast<size_t>(j.token) * a.num_heads + j.head + r, c);
+    const size_t row = static_cast<size_t>(j.token) * a.num_heads + j.head + r;
+    join.store(a, row, c);
+    if (a.row_ml && c == 0) a.row_ml[row] = make_float2(join.mx, join.sum);
   }
 }
 

@@ -21,54 +21,52 @@ namespace kvc {
 namespace {
 
 // =====================================================================================
-// Weights per slot: weights[row, kvh, p] += sum over the tokens and the head group of
-// 2^(s scale log2(e) - max) / sum, from the kept scores and the rows' final statistics.  A
-// thread owns four slots and adds the rows in order, so the sums do not depend on the
-// schedule; slots of the call's own tokens start from zero.  The statistics of 256 rows
-// at a time wait in shared memory.
+// From kept scores.  A thread owns four slots and adds the rows in order, so the sums do not
+// depend on the schedule; slots of the call's own tokens start from zero.  Bound by latency:
+// eight rows' scores, their statistics (the same for all threads) and the sums so far are on
+// their way together.
 // =====================================================================================
-constexpr int kWeighThreads = kWeighSlots / 4, kWeighRows = 256;
+constexpr int kWeighThreads = kWeighSlots / 4, kWeighAtOnce = 8;
 
 __global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const TreeArgs a) {
-  __shared__ float2 s_ml[kWeighRows];
   const TreeWeigh w = a.weighs[blockIdx.x];
-  wait_prerequisites();
-  launch_dependents();
   const int end = w.ctx + w.nodes, rows = w.nodes * a.group, pitch = (end + 15) & ~15;
   const int p = w.slot0 + 4 * threadIdx.x;
   const float* s = a.scores + static_cast<size_t>(w.scores) * 16 + p;
-  const float sc = a.score_scale;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int r0 = 0; r0 < rows; r0 += kWeighRows) {
-    const int n = min(kWeighRows, rows - r0);
-    __syncthreads();
-    for (int r = threadIdx.x; r < n; r += kWeighThreads) {
-      const int node = (r0 + r) / a.group, head = w.kvh * a.group + r0 + r - node * a.group;
-      const float2 e = a.row_ml[static_cast<size_t>(w.tok0 + node) * a.num_heads + head];
-      s_ml[r] = make_float2(e.x, e.y > 0.f ? 1.0f / e.y : (e.y == 0.f ? 0.f : e.y));
-    }
-    __syncthreads();
-    if (p < end) {
-      auto weight = [&](float x, float2 e) {
-        return x == -INFINITY ? 0.f : fast_exp2(fmaf(x, sc, -e.x)) * e.y;
-      };
-#pragma unroll 8
-      for (int r = 0; r < n; ++r) {
-        const float4 x = __ldcs(reinterpret_cast<const float4*>(s + static_cast<size_t>(r0 + r) * pitch));
-        const float2 e = s_ml[r];
-        sum.x += weight(x.x, e);
-        sum.y += weight(x.y, e);
-        sum.z += weight(x.z, e);
-        sum.w += weight(x.w, e);
+  float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
+  const float2* ml = a.row_ml + static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group;
+  wait_prerequisites();
+  launch_dependents();
+  if (p >= end) return;
+  float old[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) old[i] = p + i < w.ctx ? out[i] : 0.f;
+  for (int r0 = 0, node = 0, rem = 0; r0 < rows; r0 += kWeighAtOnce) {
+    float4 x[kWeighAtOnce];
+    float2 e[kWeighAtOnce];
+#pragma unroll
+    for (int r = 0; r < kWeighAtOnce; ++r) {
+      const bool there = r0 + r < rows;
+      x[r] = there ? __ldcs(reinterpret_cast<const float4*>(s + static_cast<size_t>(r0 + r) * pitch))
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+      e[r] = there ? ml[static_cast<size_t>(node) * a.num_heads + rem] : make_float2(0.f, 0.f);
+      if (++rem == a.group) {
+        rem = 0;
+        ++node;
       }
     }
+#pragma unroll
+    for (int r = 0; r < kWeighAtOnce; ++r) {
+      const float inv = e[r].y > 0.f ? 1.0f / e[r].y : e[r].y;     // (0: a row without weight)
+      const float v[4] = {x[r].x, x[r].y, x[r].z, x[r].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v[i] != -INFINITY) sum[i] += fast_exp2(fmaf(v[i], a.score_scale, -e[r].x)) * inv;
+    }
   }
-  if (p >= end) return;
-  float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
-  const float add[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (p + i < end) out[i] = p + i < w.ctx ? out[i] + add[i] : add[i];
+    if (p + i < end) out[i] = old[i] + sum[i];
 }
 
 // =====================================================================================
