@@ -279,27 +279,29 @@ cudaError_t run_norm_rope_type(const NormRopeArgs& a, bool neox, int sms, cudaSt
 // =====================================================================================
 // Which slots stay.  A CTA takes one (layer, sequence, KV head): of the slots in front of
 // the last `recent` it keeps the budget - recent heaviest, found by a radix search for the
-// weight of the last of them, eight bits a pass, over keys that wait in shared memory; equal
-// weights at the border go to the lowest slots.  One ordered pass then writes the kept slots
-// and their weights, which may go to where they came from: a slot never moves up.
+// weight of the last of them, eight bits a pass, over weights that wait in shared memory;
+// equal ones at the border go to the lowest slots.  One ordered pass then writes the kept
+// slots and their weights, which may go to where they came from: a slot never moves up, and
+// all weights of a round are read before any of it is written.  Bound by latency (a few
+// barriers a pass and round), hidden by the other CTAs of an SM.
 // =====================================================================================
 constexpr int kSelectThreads = 256;
-constexpr int kSelectKeys = 8192;    // kept in shared memory; longer rows are read again
+constexpr int kSelectHeld = 8192;    // weights kept in shared memory; longer rows are read again
+constexpr int kSelectPer = 4;        // slots of a thread in a round of the ordered pass
 
 // Larger for a larger weight; what is not a number comes last.
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return 0u;
-  w += 0.0f;                          // (-0 ties with 0)
-  const uint32_t u = __float_as_uint(w);
+  const uint32_t u = __float_as_uint(w + 0.0f);   // (-0 ties with 0)
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
-  extern __shared__ uint32_t s_key[];
+  extern __shared__ float s_w[];
   __shared__ uint32_t s_hist[kSelectThreads];
   __shared__ uint32_t s_digit, s_need;
-  __shared__ int s_warp[2][kSelectThreads / 32];
   constexpr int kWarps = kSelectThreads / 32;
+  __shared__ int2 s_warp[kWarps];
   const int head = blockIdx.x, seq = blockIdx.y, layer = blockIdx.z;
   const int Hkv = a.p.num_kv_heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   wait_prerequisites();
@@ -323,87 +325,115 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     return;
   }
   const int old = n - a.recent, take = a.budget - a.recent;   // take of [0, old), all behind
-  uint32_t need = take, border = 0;                           // keys above it: take - need
-  const bool held = old <= kSelectKeys;
-  if (held)
-    for (int i = tid; i < old; i += kSelectThreads) s_key[i] = weight_key(w[i]);
-  auto key = [&](int i) { return held ? s_key[i] : weight_key(w[i]); };
-  if (take > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      s_hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < old; i += kSelectThreads) {
-        const uint32_t k = key(i);
-        if (shift == 24 || (k >> (shift + 8)) == (border >> (shift + 8)))
-          atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
-      }
-      __syncthreads();
-      // the digit of the need-th largest: thread d sums the bins above its own
-      if (warp == 0) {
-        uint32_t mine = 0;
+  const bool held = old <= kSelectHeld;
+  s_hist[tid] = 0;
+  if (held) {
+    for (int i0 = tid; i0 < old; i0 += 8 * kSelectThreads) {  // eight on their way
+      float v[8];
 #pragma unroll
-        for (int b = 0; b < 8; ++b) mine += s_hist[lane * 8 + b];
-        uint32_t above = mine;                       // of this lane's bins and those above
+      for (int k = 0; k < 8; ++k) v[k] = i0 + k * kSelectThreads < old ? w[i0 + k * kSelectThreads] : 0.f;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t v = __shfl_down_sync(0xffffffffu, above, o);
-          if (lane + o < 32) above += v;
-        }
-        uint32_t over = above - mine;
-        if (over < need && need <= above) {
-          for (int b = 7; b >= 0; --b) {
-            const uint32_t cnt = s_hist[lane * 8 + b];
-            if (need <= over + cnt) {
-              s_digit = lane * 8 + b;
-              s_need = need - over;
-              break;
-            }
-            over += cnt;
-          }
-        }
-      }
-      __syncthreads();
-      border |= s_digit << shift;
-      need = s_need;
-      __syncthreads();
+      for (int k = 0; k < 8; ++k)
+        if (i0 + k * kSelectThreads < old) s_w[i0 + k * kSelectThreads] = v[k];
     }
   }
-  __syncthreads();
-  // In order: slots above the border, and the first `need` on it.
-  int at = 0, ties = 0;                                       // written and ties so far
-  for (int i0 = 0; i0 < old && take > 0; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < old ? key(i) : 0u;
-    const bool over = i < old && k > border, tie = i < old && k == border;
-    const float wi = i < old ? w[i] : 0.f;
-    const uint32_t b_over = __ballot_sync(0xffffffffu, over), b_tie = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) {
-      s_warp[0][warp] = __popc(b_over);
-      s_warp[1][warp] = __popc(b_tie);
+  auto weight = [&](int i) { return held ? s_w[i] : w[i]; };
+  uint32_t need = take, border = 0;                           // keys above it: take - need
+  for (int shift = 24; shift >= 0 && take > 0; shift -= 8) {
+    __syncthreads();
+    for (int i = tid; i < old; i += kSelectThreads) {
+      const uint32_t k = weight_key(weight(i));
+      if (shift == 24 || (k >> (shift + 8)) == (border >> (shift + 8)))
+        atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
     }
-    __syncthreads();                                          // (w[i] is read by all, too)
-    int my_over = 0, my_tie = 0, all_over = 0, all_tie = 0;
+    __syncthreads();
+    // the digit of the need-th largest
+    if (warp == 0) {
+      uint32_t cnt[8], mine = 0;
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) {
-      if (v == warp) {
-        my_over = all_over;
-        my_tie = all_tie;
+      for (int b = 0; b < 8; ++b) {
+        cnt[b] = s_hist[lane * 8 + b];
+        s_hist[lane * 8 + b] = 0;                             // (for the next pass)
+        mine += cnt[b];
       }
-      all_over += s_warp[0][v];
-      all_tie += s_warp[1][v];
+      uint32_t above = mine;                                  // of this lane's bins and those above
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_down_sync(0xffffffffu, above, o);
+        if (lane + o < 32) above += v;
+      }
+      uint32_t over = above - mine;
+      if (over < need && need <= above) {
+        bool found = false;
+#pragma unroll
+        for (int b = 7; b >= 0; --b) {
+          if (!found && need <= over + cnt[b]) {
+            s_digit = lane * 8 + b;
+            s_need = need - over;
+            found = true;
+          }
+          over += cnt[b];
+        }
+      }
     }
-    const uint32_t below = (1u << lane) - 1u;
-    my_over += __popc(b_over & below);
-    my_tie += __popc(b_tie & below);
-    const int ties_before = min(ties + my_tie, static_cast<int>(need));
-    if (over || (tie && ties + my_tie < static_cast<int>(need))) {
-      const int j = at + my_over + ties_before - min(ties, static_cast<int>(need));
-      kept[j] = i;
-      left[j] = wi;
+    __syncthreads();
+    border |= s_digit << shift;
+    need = s_need;
+  }
+  __syncthreads();
+  // In order: slots above the border, and the first `need` on it; `at` and `ties` of them so far.
+  int at = 0, ties = 0;
+  const int limit = static_cast<int>(need);
+  for (int i0 = 0; i0 < old && take > 0; i0 += kSelectPer * kSelectThreads) {
+    const int i = i0 + kSelectPer * tid;
+    float v[kSelectPer];
+    uint32_t k[kSelectPer];
+    int2 mine = make_int2(0, 0);                              // above the border, on it
+#pragma unroll
+    for (int e = 0; e < kSelectPer; ++e) {
+      const bool there = i + e < old;
+      v[e] = there ? weight(i + e) : 0.f;
+      k[e] = weight_key(v[e]);
+      mine.x += there && k[e] > border;
+      mine.y += there && k[e] == border;
     }
-    const int ties_now = min(ties + all_tie, static_cast<int>(need));
-    at += all_over + ties_now - min(ties, static_cast<int>(need));
-    ties += all_tie;
+    int2 sum = mine;                                          // of the warp's lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
+      if (lane >= o) {
+        sum.x += x;
+        sum.y += y;
+      }
+    }
+    if (lane == 31) s_warp[warp] = sum;
+    __syncthreads();                                          // (and the round's weights are read)
+    int2 before = make_int2(sum.x - mine.x, sum.y - mine.y), all = make_int2(0, 0);
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
+      const int2 c = s_warp[x];
+      if (x < warp) {
+        before.x += c.x;
+        before.y += c.y;
+      }
+      all.x += c.x;
+      all.y += c.y;
+    }
+    const int taken = min(ties, limit);                       // ties that were kept so far
+    int over = at + before.x, tie = ties + before.y;
+#pragma unroll
+    for (int e = 0; e < kSelectPer; ++e) {
+      const bool there = i + e < old, is_over = there && k[e] > border, is_tie = there && k[e] == border;
+      if (is_over || (is_tie && tie < limit)) {
+        const int j = over + min(tie, limit) - taken;
+        kept[j] = i + e;
+        left[j] = v[e];
+      }
+      over += is_over;
+      tie += is_tie;
+    }
+    at += all.x + min(ties + all.y, limit) - taken;
+    ties += all.y;
     __syncthreads();
   }
   for (int i0 = 0; i0 < a.recent; i0 += kSelectThreads) {
@@ -414,7 +444,6 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       kept[take + i] = old + i;
       left[take + i] = wi;
     }
-    __syncthreads();
   }
 }
 
@@ -424,14 +453,18 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
 // moves up, so a later chunk's sources lie behind every place written before it: the next
 // chunk is read before this one is written, and only the reads of one chunk have to be done
 // (a barrier) before its first write.  Rows in front of the first one that leaves stay.
+//
+// Bound by memory traffic, which is more than the rows' bytes: a row's 16-byte pieces stand
+// 128 bytes apart, eight positions to a line, so of 64 bytes that memory reads at a time half
+// are another row's where every second slot stays.
 // =====================================================================================
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnits = 8;        // 16-byte units of a thread on their way
 constexpr int kMoveRows = 256;       // rows of a chunk at most
 
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a, const int parts) {
-  __shared__ size_t s_src[3][kMoveRows], s_dst[3][kMoveRows];
-  constexpr size_t kNone = ~static_cast<size_t>(0);
+  __shared__ uint2 s_place[3][kMoveRows];  // 16-byte units: where a row is and goes
+  constexpr uint32_t kNone = ~0u;
   const int seq = blockIdx.y, tid = threadIdx.x;
   const int part = blockIdx.x % parts, head = blockIdx.x / parts, kv = blockIdx.z & 1, layer = blockIdx.z >> 1;
   const int Hkv = a.p.num_kv_heads, U = a.p.row_units / parts, ps = a.p.page_size;
@@ -439,59 +472,51 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
   const int n = a.ctx[seq], m = a.budget, row = a.rows ? a.rows[seq] : seq;
   const int32_t* kept = a.kept + ((static_cast<size_t>(layer) * a.n + seq) * Hkv + head) * m;
   if (n <= m || kept[0] < 0) return;       // nothing leaves, or reported
-  int lo = 0, hi = m;                      // the first row that moves
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (kept[mid] > mid)
-      hi = mid;
-    else
-      lo = mid + 1;
+  // the first row that moves: kept[j] is j in front of it, and larger from there on
+  int lo = 0, hi = m;
+  while (hi - lo > 0) {
+    const int step = (hi - lo + kMoveThreads - 1) / kMoveThreads, j = lo + tid * step;
+    const int stay = __syncthreads_count(j < hi && kept[j] == j);   // of the tested ones
+    if (stay == 0) break;                  // (the first one moves)
+    hi = min(hi, lo + stay * step);
+    lo += (stay - 1) * step + 1;
   }
+  if (lo >= m) return;
   const bool core = a.p.layout == kLayoutCore;
   const int first = core ? lo & ~7 : lo;
-  if (lo >= m) return;
   uint8_t* base = (kv ? a.p.v : a.p.k) + static_cast<size_t>(layer) * a.layer_bytes;
   int chunk = kMoveThreads * kMoveUnits / U;                 // rows of a chunk
   chunk = chunk > kMoveRows ? kMoveRows : (chunk & ~7);
   const int chunks = (m - first + chunk - 1) / chunk;
   auto place = [&](int pos) {
     const int page = page_of(a.p, row, pos);
-    return page < 0 ? kNone : unit_at(a.p, page, head, pos % ps, part * U);
+    return page < 0 ? kNone : static_cast<uint32_t>(unit_at(a.p, page, head, pos % ps, part * U) / 16);
   };
   auto places = [&](int c) {               // where chunk c's rows are and go
     for (int r = tid; r < chunk && c < chunks; r += kMoveThreads) {
-      const int j = first + c * chunk + r;
-      size_t src = kNone, dst = kNone;
-      if (j < m && kept[j] > j) {
-        src = place(kept[j]);
-        dst = place(j);
-      }
-      s_src[c % 3][r] = src == kNone || dst == kNone ? kNone : src;
-      s_dst[c % 3][r] = dst;
+      const int j = first + c * chunk + r, from = j < m ? kept[j] : j;
+      uint2 x = make_uint2(kNone, kNone);
+      if (from > j) x = make_uint2(place(from), place(j));
+      if (x.y == kNone) x.x = kNone;
+      s_place[c % 3][r] = x;
     }
   };
-  const int step = core ? 128 : 16, units = chunk * U;
-  // unit x of a chunk in the order of memory: row and byte offset within the row
-  auto split = [&](int x, int& r, int& u) {
-    if (core) {
-      r = x & 7;
-      const int y = x >> 3;
-      u = y % U;
-      r += (y / U) << 3;
-    } else {
-      r = x / U;
-      u = x - r * U;
-    }
-  };
+  // A thread's units of a chunk, in the order of memory: row, and offset from the row's place.
+  int unit[kMoveUnits];
+#pragma unroll
+  for (int k = 0; k < kMoveUnits; ++k) {
+    const int x = tid + k * kMoveThreads, y = core ? x >> 3 : x;
+    const int q = y / U, u = y - q * U, r = core ? q * 8 + (x & 7) : q;
+    unit[k] = x < chunk * U ? (r << 16) | (core ? 8 * u : u) : -1;
+  }
   uint4 now[kMoveUnits], next[kMoveUnits];
   auto load = [&](int c, uint4* v) {
+    if (c >= chunks) return;
 #pragma unroll
     for (int k = 0; k < kMoveUnits; ++k) {
-      const int x = tid + k * kMoveThreads;
-      int r, u;
-      split(x, r, u);
-      if (x < units && c < chunks && s_src[c % 3][r] != kNone)
-        v[k] = *reinterpret_cast<const uint4*>(base + s_src[c % 3][r] + u * step);
+      if (unit[k] < 0) continue;
+      const uint32_t at = s_place[c % 3][unit[k] >> 16].x;
+      if (at != kNone) v[k] = reinterpret_cast<const uint4*>(base)[static_cast<size_t>(at) + (unit[k] & 0xffff)];
     }
   };
   places(0);
@@ -504,11 +529,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
     load(c + 1, next);
 #pragma unroll
     for (int k = 0; k < kMoveUnits; ++k) {
-      const int x = tid + k * kMoveThreads;
-      int r, u;
-      split(x, r, u);
-      if (x < units && s_src[c % 3][r] != kNone)
-        *reinterpret_cast<uint4*>(base + s_dst[c % 3][r] + u * step) = now[k];
+      if (unit[k] < 0) continue;
+      const uint2 at = s_place[c % 3][unit[k] >> 16];
+      if (at.x != kNone) reinterpret_cast<uint4*>(base)[static_cast<size_t>(at.y) + (unit[k] & 0xffff)] = now[k];
     }
 #pragma unroll
     for (int k = 0; k < kMoveUnits; ++k) now[k] = next[k];
@@ -530,11 +553,11 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a, int dtype, bool neox, int sm
 }
 
 cudaError_t launch_evict(const EvictArgs& a, int sms, cudaStream_t s) {
-  const size_t keys = sizeof(uint32_t) * std::min(kSelectKeys, a.weight_slots);
+  const size_t held = sizeof(float) * std::min(kSelectHeld, a.weight_slots);
   cudaError_t e = launch_early(evict_select_kernel,
                                dim3(static_cast<unsigned>(a.p.num_kv_heads), static_cast<unsigned>(a.n),
                                     static_cast<unsigned>(a.n_layers)),
-                               kSelectThreads, keys, s, a);
+                               kSelectThreads, held, s, a);
   if (e != cudaSuccess) return e;
   // few heads: their columns are spread over more CTAs
   const int64_t heads = 2ll * a.n_layers * a.n * a.p.num_kv_heads;

@@ -389,6 +389,8 @@ extern "C" int kvc_evict(kvc_pool_t* pool, const int32_t* d_block_tables, int bt
       return set_error(KVC_ERR_INVALID_ARG, "weights must have rows and slots.");
     if (2ll * pool->g.num_layers > 65535)
       return set_error(KVC_ERR_INVALID_ARG, "the pool has too many layers.");
+    if (pool->g.layer_bytes >= (size_t{1} << 36))   // (places are 32-bit counts of 16 bytes)
+      return set_error(KVC_ERR_INVALID_ARG, "a layer's K of 64 GB or more cannot be cut back.");
     if (n_seqs == 0) return KVC_OK;
     if (!d_ctx_lens || !d_weights || !d_weights_out || !d_kept)
       return set_error(KVC_ERR_INVALID_ARG, "contexts, weights and kept slots must not be null.");
