@@ -28,10 +28,11 @@ constexpr int kNormThreads = 256;
 constexpr int kNormBatch = 2;      // heads of a lane group on their way
 
 template <typename T, bool kNeox, int kPer, int kLanes>
-__global__ void __launch_bounds__(kNormThreads) norm_rope_kernel(const NormRopeArgs a) {
+__global__ void __launch_bounds__(kNormThreads, 4) norm_rope_kernel(const NormRopeArgs a) {
   constexpr int kTok = kNormThreads / kPer, kAtOnce = kPer / kLanes;
   constexpr int N = Unit<T>::N;
-  __shared__ float2 cs[kTok * kMaxRopePairs];
+  __shared__ float4 cs[kTok * kMaxRopePairs / 2];    // two pairs' (cos, sin)
+  __shared__ uint4 s_weight[2][2 * kLanes];
   __shared__ int s_page[kTok], s_slot[kTok];
   const int tok0 = blockIdx.x * kTok;
   const int toks = min(kTok, a.n - tok0);
@@ -68,23 +69,21 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_kernel(const NormRopeA
   Item items[kNormBatch];
 #pragma unroll
   for (int k = 0; k < kNormBatch; ++k) load(row0 + k * kAtOnce, items[k]);
-  Item wq = {}, wk = {};
-  if (works && a.q_weight) {
-    wq.x0.raw = *reinterpret_cast<const uint4*>(a.q_weight + u0 * 16);
-    wq.x1.raw = *reinterpret_cast<const uint4*>(a.q_weight + (u0 + du) * 16);
+  // (weights and angles are read where they are used: in registers they would leave an SM
+  // room for fewer CTAs)
+  for (int x = threadIdx.x; x < 2 * U; x += kNormThreads) {
+    const int k = x >= U, u = x - k * U;
+    const uint8_t* w = k ? a.k_weight : a.q_weight;
+    if (w) s_weight[k][u] = *reinterpret_cast<const uint4*>(w + u * 16);
   }
-  if (works && a.k_weight) {
-    wk.x0.raw = *reinterpret_cast<const uint4*>(a.k_weight + u0 * 16);
-    wk.x1.raw = *reinterpret_cast<const uint4*>(a.k_weight + (u0 + du) * 16);
-  }
-
   for (int x = threadIdx.x; x < toks * a.pairs; x += kNormThreads) {
     const int tk = kTok == 1 ? 0 : x / a.pairs, j = x - tk * a.pairs;
     double turn = static_cast<double>(a.rope_positions[static_cast<size_t>(tok0 + tk) * a.axes +
                                                        a.axis[j]]) * a.turns[j];
     turn -= rint(turn);
-    // (by pair of a unit pair, then unit pair: neighbouring threads read neighbouring angles)
-    float2& out = cs[tk * kMaxRopePairs + j % N * turned + j / N];
+    // (by pairs of a unit pair, then unit pair: neighbouring threads read neighbouring angles)
+    const int k = j % N;
+    float2& out = reinterpret_cast<float2*>(cs + tk * kMaxRopePairs / 2 + k / 2 * turned + j / N)[k & 1];
     sincospif(2.0f * static_cast<float>(turn), &out.y, &out.x);
   }
   if (threadIdx.x < toks) {
@@ -96,10 +95,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_kernel(const NormRopeA
   if (tok >= toks) return;                           // (a warp has one token)
   const int page = s_page[tok];
   if (page < 0) return;                              // padding, or reported
-  float2 c[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    c[k] = turns ? cs[tok * kMaxRopePairs + k * turned + i] : make_float2(1.f, 0.f);
+  const float4* angles = cs + tok * kMaxRopePairs / 2 + i;
   uint8_t* q_dst = a.q_out + t * H * row_bytes + u0 * 16;
   const size_t place = unit_at(a.p, page, 0, s_slot[tok], u0);
   const int dp = du * (a.p.layout == kLayoutCore ? 128 : 16);
@@ -113,35 +109,47 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_kernel(const NormRopeA
       Item& it = items[k];
       const bool is_q = head < H, is_k = !is_q && head < H + Hkv;
       const bool normed = is_q ? a.q_weight != nullptr : is_k && a.k_weight != nullptr;
-      float x0[N], x1[N], sum = 0.f;
+      float x0[N], x1[N], scale = 1.f;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         x0[e] = to_f32<T>(it.x0.v[e]);
         x1[e] = to_f32<T>(it.x1.v[e]);
-        sum = fmaf(x0[e], x0[e], sum);
-        sum = fmaf(x1[e], x1[e], sum);
       }
+      // (a warp's heads may differ in what they need: all lanes take part in the sum)
+      if (__any_sync(0xffffffffu, normed)) {
+        float sum = 0.f;
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int e = 0; e < N; ++e) {
+          sum = fmaf(x0[e], x0[e], sum);
+          sum = fmaf(x1[e], x1[e], sum);
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        scale = rsqrtf(fmaf(sum, inv_d, a.eps));
+      }
       if (works && head < heads) {
         if (normed) {
-          const float r = rsqrtf(fmaf(sum, inv_d, a.eps));
-          const Item& w = is_q ? wq : wk;
+          Unit<T> w0, w1;
+          w0.raw = s_weight[is_q ? 0 : 1][u0];
+          w1.raw = s_weight[is_q ? 0 : 1][u0 + du];
 #pragma unroll
           for (int e = 0; e < N; ++e) {
-            x0[e] = x0[e] * r * to_f32<T>(w.x0.v[e]);
-            x1[e] = x1[e] * r * to_f32<T>(w.x1.v[e]);
+            x0[e] = x0[e] * scale * to_f32<T>(w0.v[e]);
+            x1[e] = x1[e] * scale * to_f32<T>(w1.v[e]);
           }
         }
         if ((is_q || is_k) && turns) {
-          if constexpr (kNeox) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) turn_pair(x0[e], x1[e], c[e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < N / 2; ++e) {
-              turn_pair(x0[2 * e], x0[2 * e + 1], c[e]);
-              turn_pair(x1[2 * e], x1[2 * e + 1], c[N / 2 + e]);
+          for (int e = 0; e < N / 2; ++e) {
+            const float4 c = angles[e * turned];
+            if constexpr (kNeox) {
+              turn_pair(x0[2 * e], x1[2 * e], make_float2(c.x, c.y));
+              turn_pair(x0[2 * e + 1], x1[2 * e + 1], make_float2(c.z, c.w));
+            } else {
+              // pairs 2 e and 2 e + 1 of the two units' N
+              float* x = e < N / 4 ? x0 + 4 * e : x1 + 4 * e - N;
+              turn_pair(x[0], x[1], make_float2(c.x, c.y));
+              turn_pair(x[2], x[3], make_float2(c.z, c.w));
             }
           }
         }
@@ -278,30 +286,36 @@ cudaError_t run_norm_rope_type(const NormRopeArgs& a, bool neox, int sms, cudaSt
 
 // =====================================================================================
 // Which slots stay.  A CTA takes one (layer, sequence, KV head): of the slots in front of
-// the last `recent` it keeps the budget - recent heaviest, found by a radix search for the
-// weight of the last of them, eight bits a pass, over weights that wait in shared memory;
-// equal ones at the border go to the lowest slots.  One ordered pass then writes the kept
-// slots and their weights, which may go to where they came from: a slot never moves up, and
-// all weights of a round are read before any of it is written.  Bound by latency (a few
-// barriers a pass and round), hidden by the other CTAs of an SM.
+// the last `recent` it keeps the budget - recent heaviest, equal ones from the lowest slot on.
+//
+// The weight on the border is found in three steps over weights that wait in shared memory: a
+// histogram of their upper 11 bits (sign, exponent, two more) names the bin it is in, that
+// bin's weights are put on a list, and every thread counts how many of the list are above the
+// one that it takes.  (A list of more than kSelectList, as equal weights make it, is searched
+// seven bits at a time instead.)  One ordered pass then writes the kept slots and their weights,
+// which may go to where they came from: a slot never moves up, and all weights of a round are
+// read before any of it is written.  Bound by its instructions, some 90 a weight and thread
+// (8 x 32 x 8 heads of 900-3100 weights: 22 us; 36 with four passes of eight bits).
 // =====================================================================================
 constexpr int kSelectThreads = 256;
 constexpr int kSelectHeld = 8192;    // weights kept in shared memory; longer rows are read again
+constexpr int kSelectBins = 2048;
+constexpr int kSelectList = 256;
 constexpr int kSelectPer = 4;        // slots of a thread in a round of the ordered pass
 
 // Larger for a larger weight; what is not a number comes last.
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (w != w) return 0u;
   const uint32_t u = __float_as_uint(w + 0.0f);   // (-0 ties with 0)
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return w != w ? 0u : u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
   extern __shared__ float s_w[];
-  __shared__ uint32_t s_hist[kSelectThreads];
-  __shared__ uint32_t s_digit, s_need;
-  constexpr int kWarps = kSelectThreads / 32;
-  __shared__ int2 s_warp[kWarps];
+  __shared__ uint32_t s_hist[kSelectBins];
+  __shared__ uint32_t s_list[kSelectList];
+  __shared__ uint32_t s_digit, s_need, s_listed, s_ties;
+  constexpr int kWarps = kSelectThreads / 32, kBinsPer = kSelectBins / kSelectThreads;
+  __shared__ int s_warp[2][kWarps];
   const int head = blockIdx.x, seq = blockIdx.y, layer = blockIdx.z;
   const int Hkv = a.p.num_kv_heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   wait_prerequisites();
@@ -326,114 +340,154 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   }
   const int old = n - a.recent, take = a.budget - a.recent;   // take of [0, old), all behind
   const bool held = old <= kSelectHeld;
-  s_hist[tid] = 0;
-  if (held) {
+  auto weight = [&](int i) { return held ? s_w[i] : w[i]; };
+  // How many of the largest are still wanted of the bins [0, bins) of s_hist, and in which of
+  // them the last one is: s_need, s_digit.  All threads; the bins are zero afterwards.
+  auto find = [&](uint32_t need, int bins) {
+    uint32_t cnt[kBinsPer], mine = 0;
+#pragma unroll
+    for (int b = 0; b < kBinsPer; ++b) {
+      const int bin = tid * kBinsPer + b;
+      cnt[b] = bin < bins ? s_hist[bin] : 0u;
+      if (bin < bins) s_hist[bin] = 0;
+      mine += cnt[b];
+    }
+    uint32_t above = mine;                                    // of this lane's bins and those above
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_down_sync(0xffffffffu, above, o);
+      if (lane + o < 32) above += v;
+    }
+    if (lane == 0) s_warp[0][warp] = static_cast<int>(above);
+    __syncthreads();
+    uint32_t over = above - mine;
+    for (int x = warp + 1; x < kWarps; ++x) over += s_warp[0][x];
+    if (over < need && need <= over + mine) {
+      bool found = false;
+#pragma unroll
+      for (int b = kBinsPer - 1; b >= 0; --b) {
+        if (!found && need <= over + cnt[b]) {
+          s_digit = tid * kBinsPer + b;
+          s_need = need - over;
+          s_ties = cnt[b];
+          found = true;
+        }
+        over += cnt[b];
+      }
+    }
+    __syncthreads();
+  };
+  uint32_t border = 0, need = 0, ties_all = 0;                // kept: above border, and `need` on it
+  if (take > 0) {
+    for (int b = tid; b < kSelectBins; b += kSelectThreads) s_hist[b] = 0;
+    if (tid == 0) s_listed = 0;
+    __syncthreads();
     for (int i0 = tid; i0 < old; i0 += 8 * kSelectThreads) {  // eight on their way
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = i0 + k * kSelectThreads < old ? w[i0 + k * kSelectThreads] : 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i0 + k * kSelectThreads < old) s_w[i0 + k * kSelectThreads] = v[k];
-    }
-  }
-  auto weight = [&](int i) { return held ? s_w[i] : w[i]; };
-  uint32_t need = take, border = 0;                           // keys above it: take - need
-  for (int shift = 24; shift >= 0 && take > 0; shift -= 8) {
-    __syncthreads();
-    for (int i = tid; i < old; i += kSelectThreads) {
-      const uint32_t k = weight_key(weight(i));
-      if (shift == 24 || (k >> (shift + 8)) == (border >> (shift + 8)))
-        atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * kSelectThreads;
+        if (i >= old) break;
+        if (held) s_w[i] = v[k];
+        atomicAdd(&s_hist[weight_key(v[k]) >> 21], 1u);
+      }
     }
     __syncthreads();
-    // the digit of the need-th largest
-    if (warp == 0) {
-      uint32_t cnt[8], mine = 0;
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        cnt[b] = s_hist[lane * 8 + b];
-        s_hist[lane * 8 + b] = 0;                             // (for the next pass)
-        mine += cnt[b];
+    find(take, kSelectBins);
+    const uint32_t top = s_digit;
+    need = s_need;
+    ties_all = s_ties;
+    if (ties_all <= kSelectList) {
+      for (int i = tid; i < old; i += kSelectThreads) {
+        const uint32_t k = weight_key(weight(i));
+        if (k >> 21 == top) s_list[atomicAdd(&s_listed, 1u)] = k;
       }
-      uint32_t above = mine;                                  // of this lane's bins and those above
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_down_sync(0xffffffffu, above, o);
-        if (lane + o < 32) above += v;
-      }
-      uint32_t over = above - mine;
-      if (over < need && need <= above) {
-        bool found = false;
-#pragma unroll
-        for (int b = 7; b >= 0; --b) {
-          if (!found && need <= over + cnt[b]) {
-            s_digit = lane * 8 + b;
-            s_need = need - over;
-            found = true;
-          }
-          over += cnt[b];
+      __syncthreads();
+      if (tid < ties_all) {
+        const uint32_t k = s_list[tid];
+        uint32_t over = 0, same = 0;
+        for (uint32_t x = 0; x < ties_all; ++x) {
+          const uint32_t y = s_list[x];
+          over += y > k;
+          same += y == k;
+        }
+        if (over < need && need <= over + same) {             // (all equal ones write the same)
+          s_digit = k;
+          s_need = need - over;
+          s_ties = same;
         }
       }
-    }
-    __syncthreads();
-    border |= s_digit << shift;
-    need = s_need;
-  }
-  __syncthreads();
-  // In order: slots above the border, and the first `need` on it; `at` and `ties` of them so far.
-  int at = 0, ties = 0;
-  const int limit = static_cast<int>(need);
-  for (int i0 = 0; i0 < old && take > 0; i0 += kSelectPer * kSelectThreads) {
-    const int i = i0 + kSelectPer * tid;
-    float v[kSelectPer];
-    uint32_t k[kSelectPer];
-    int2 mine = make_int2(0, 0);                              // above the border, on it
-#pragma unroll
-    for (int e = 0; e < kSelectPer; ++e) {
-      const bool there = i + e < old;
-      v[e] = there ? weight(i + e) : 0.f;
-      k[e] = weight_key(v[e]);
-      mine.x += there && k[e] > border;
-      mine.y += there && k[e] == border;
-    }
-    int2 sum = mine;                                          // of the warp's lanes up to this one
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
-      if (lane >= o) {
-        sum.x += x;
-        sum.y += y;
+      __syncthreads();
+      border = s_digit;
+    } else {
+      border = top << 21;
+      for (int shift = 14; shift >= 0; shift -= 7) {
+        for (int i = tid; i < old; i += kSelectThreads) {
+          const uint32_t k = weight_key(weight(i));
+          if (k >> (shift + 7) == border >> (shift + 7)) atomicAdd(&s_hist[(k >> shift) & 127u], 1u);
+        }
+        __syncthreads();
+        find(need, 128);
+        border |= s_digit << shift;
+        need = s_need;
       }
     }
-    if (lane == 31) s_warp[warp] = sum;
+    need = s_need;
+    ties_all = s_ties;
+  }
+  // In order.  Where every weight on the border is kept, one comparison tells; `at` slots are
+  // kept so far, and `ties` on the border were seen.
+  const int limit = static_cast<int>(need);
+  const bool plain = need == ties_all;
+  int at = 0, ties = 0;
+  for (int i0 = 0; i0 < old && take > 0; i0 += kSelectPer * kSelectThreads) {
+    const int first = i0 + warp * kSelectPer * 32 + lane;     // a warp's slots are neighbours
+    float v[kSelectPer];
+    uint32_t over[kSelectPer], tie[kSelectPer];
+    int n_over = 0, n_tie = 0;
+#pragma unroll
+    for (int e = 0; e < kSelectPer; ++e) {
+      const int i = first + 32 * e;
+      v[e] = i < old ? weight(i) : 0.f;
+      const uint32_t k = weight_key(v[e]);
+      over[e] = __ballot_sync(0xffffffffu, i < old && (plain ? k >= border : k > border));
+      tie[e] = plain ? 0u : __ballot_sync(0xffffffffu, i < old && k == border);
+      n_over += __popc(over[e]);
+      n_tie += __popc(tie[e]);
+    }
+    if (lane == 0) {
+      s_warp[0][warp] = n_over;
+      s_warp[1][warp] = n_tie;
+    }
     __syncthreads();                                          // (and the round's weights are read)
-    int2 before = make_int2(sum.x - mine.x, sum.y - mine.y), all = make_int2(0, 0);
+    int my_over = at, my_tie = ties, all_over = 0, all_tie = 0;
 #pragma unroll
     for (int x = 0; x < kWarps; ++x) {
-      const int2 c = s_warp[x];
+      const int o = s_warp[0][x], t = s_warp[1][x];
       if (x < warp) {
-        before.x += c.x;
-        before.y += c.y;
+        my_over += o;
+        my_tie += t;
       }
-      all.x += c.x;
-      all.y += c.y;
+      all_over += o;
+      all_tie += t;
     }
     const int taken = min(ties, limit);                       // ties that were kept so far
-    int over = at + before.x, tie = ties + before.y;
+    const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
     for (int e = 0; e < kSelectPer; ++e) {
-      const bool there = i + e < old, is_over = there && k[e] > border, is_tie = there && k[e] == border;
-      if (is_over || (is_tie && tie < limit)) {
-        const int j = over + min(tie, limit) - taken;
-        kept[j] = i + e;
+      const int o = my_over + __popc(over[e] & below), t = my_tie + __popc(tie[e] & below);
+      if ((over[e] >> lane & 1u) || ((tie[e] >> lane & 1u) && t < limit)) {
+        const int j = o + (plain ? 0 : min(t, limit) - taken);
+        kept[j] = first + 32 * e;
         left[j] = v[e];
       }
-      over += is_over;
-      tie += is_tie;
+      my_over += __popc(over[e]);
+      my_tie += __popc(tie[e]);
     }
-    at += all.x + min(ties + all.y, limit) - taken;
-    ties += all.y;
+    at += all_over + (plain ? 0 : min(ties + all_tie, limit) - taken);
+    ties += all_tie;
     __syncthreads();
   }
   for (int i0 = 0; i0 < a.recent; i0 += kSelectThreads) {

@@ -137,8 +137,8 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   std::vector<int> cta_segs;
   std::vector<int> own_run(n_seqs, -1), prefix_run(n_groups, -1);   // of KV head 0, block 0
   std::vector<int> base(n_seqs, 0);
-  const int own_blocks = tile.tensor ? 1 : (group + tile.rows - 1) / tile.rows;
-  int64_t tiles = 0;
+  const int own_blocks = (group + tile.rows - 1) / tile.rows;
+  int64_t tiles = 0, own_tiles = 0;
   auto add = [&](int bt_row, int first, int end, int tok0, int n_rows) {
     for (int kvh = 0; kvh < Hkv; ++kvh)
       for (int r0 = 0; r0 < n_rows; r0 += tile.rows) {
@@ -167,14 +167,18 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   // Own positions.  Where the decode kernel runs on the tensor cores it takes them: its eight
   // warps an SM each work on a piece of their own, and a short piece (96 x 30-700 positions, 64 x
   // 128 heads: 39 us) costs it half of what it costs a CTA of the tree kernel (74 us), which
-  // is made for many rows.
+  // is made for many rows.  That is a launch more: while every tile finds a CTA of its own the
+  // tree kernel takes all (4 sequences on 512, 32 x 64 heads: 10 us, 14.7 with both).
+  for (int i = 0; i < n_seqs; ++i)
+    own_tiles += (h_lens[i] - base[i] + tile.positions - 1) / tile.positions * static_cast<int64_t>(own_blocks) * Hkv;
+  const bool decode = tile.tensor && tiles + own_tiles > static_cast<int64_t>(sms) * tile.ctas_per_sm;
   UnitList units;
-  if (tile.tensor) {
+  if (decode) {
     std::vector<int> rows(n_seqs);
     for (int i = 0; i < n_seqs; ++i) rows[i] = h_rows ? h_rows[i] : i;
     build_units(g, group, sms, rows, base, std::vector<int>(h_lens, h_lens + n_seqs), &units);
   }
-  for (int i = 0; i < n_seqs && !tile.tensor; ++i) {
+  for (int i = 0; i < n_seqs && !decode; ++i) {
     if (h_lens[i] <= base[i]) continue;
     own_run[i] = static_cast<int>(runs.size());
     add(h_rows ? h_rows[i] : i, base[i], h_lens[i], i, group);
@@ -216,7 +220,7 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
         for (int r = 0; r < group;) {
           // the rows up to the end of a block of the prefix or of the own run
           const int row = (i - i0) * group + r;     // within the group
-          int rows = tile.tensor ? group - r : std::min(group - r, tile.rows - r % tile.rows);
+          int rows = decode ? group - r : std::min(group - r, tile.rows - r % tile.rows);
           SharedJoin j = {};
           j.prefix.rows = j.own.rows = 1;
           if (prefix_run[k] >= 0) {
@@ -224,7 +228,7 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
             j.prefix = pieces[prefix_run[k] + kvh * prefix_blocks + row / tile.rows];
             j.prefix.row = row % tile.rows;
           }
-          if (tile.tensor) {
+          if (decode) {
             if (base[i] > 0 || units.splits[i].n > 1) j.own = units.splits[i];   // (else it is written already)
           } else if (own_run[i] >= 0) {
             j.own = pieces[own_run[i] + kvh * own_blocks + r / tile.rows];
@@ -256,8 +260,8 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
       (e = p->d_part_ml.ensure(sizeof(float2) * std::max<size_t>(1, part_rows))))
     return cuda_error(e, "plan buffers");
   const size_t split_rows = std::max<size_t>(1, units.n_splits) * num_heads;
-  if (tile.tensor && ((e = p->d_own_o.ensure(sizeof(float) * split_rows * g.head_dim)) ||
-                      (e = p->d_own_ml.ensure(sizeof(float2) * split_rows))))
+  if (decode && ((e = p->d_own_o.ensure(sizeof(float) * split_rows * g.head_dim)) ||
+                 (e = p->d_own_ml.ensure(sizeof(float2) * split_rows))))
     return cuda_error(e, "plan buffers");
   const unsigned int zero = 0;
   const PlanPart parts[] = {{segs.data(), sizeof(TreeSeg) * segs.size()},

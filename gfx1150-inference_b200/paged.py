@@ -284,6 +284,8 @@ class Rotation:
         self.axis = np.array(axis, dtype=np.uint8)
         self.inv_freq.setflags(write=False)
         self.axis.setflags(write=False)
+        # what a call hands to the library (looked up once: it takes as long as the launch)
+        self._args = (ffi.np_ptr(self.inv_freq), ffi.np_ptr(self.axis), half, 1 if neox else 0)
 
 
 class PagedKVCache:
@@ -561,28 +563,32 @@ class PagedKVCache:
             op = _on(q_out, "q_out", dt, n * heads * d, dev)
         if block_tables.dim() != 2:
             raise ValueError("block_tables must be (rows, pages)")
-        axes = 1 if rotation is None else rotation.axes
+        if rotation is None:
+            axes, (freq, axis, pairs, neox) = 1, (None, None, 0, 0)
+        else:
+            axes, (freq, axis, pairs, neox) = rotation.axes, rotation._args
         rp = None
         if rope_positions is not None:
             if rope_positions.shape != (n, axes) and (axes > 1 or rope_positions.shape != (n,)):
                 raise ValueError(f"rope_positions must be ({n}, {axes}), got "
                                  f"{tuple(rope_positions.shape)}")
             rp = _on(rope_positions, "rope_positions", torch.int32, n * axes, dev)
-        for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-            if w is not None and w.shape != (d,):
-                raise ValueError(f"{name} must be ({d},), got {tuple(w.shape)}")
+        qw = kw = None
+        if q_weight is not None:
+            qw = _on(q_weight, "q_weight", dt, 0, dev)
+            if q_weight.shape != (d,):
+                raise ValueError(f"q_weight must be ({d},), got {tuple(q_weight.shape)}")
+        if k_weight is not None:
+            kw = _on(k_weight, "k_weight", dt, 0, dev)
+            if k_weight.shape != (d,):
+                raise ValueError(f"k_weight must be ({d},), got {tuple(k_weight.shape)}")
         ffi.check(ffi.lib.kvc_append_norm_rope(
-            self.handle, layer, qp, qs, op, heads,
-            None if q_weight is None else _on(q_weight, "q_weight", dt, d, dev), kp, ks,
-            None if k_weight is None else _on(k_weight, "k_weight", dt, d, dev), vp, vs, eps,
+            self.handle, layer, qp, qs, op, heads, qw, kp, ks, kw, vp, vs, eps,
             _on(block_tables, "block_tables", torch.int32, 0, dev), block_tables.shape[0],
             block_tables.shape[1],
             None if rows is None else _on(rows, "rows", torch.int32, n, dev),
-            _on(positions, "positions", torch.int32, n, dev), rp, axes, n,
-            None if rotation is None else ffi.np_ptr(rotation.inv_freq),
-            None if rotation is None else ffi.np_ptr(rotation.axis),
-            0 if rotation is None else rotation.pairs,
-            1 if rotation is not None and rotation.neox else 0, _stream_on(stream, dev)))
+            _on(positions, "positions", torch.int32, 0, dev), rp, axes, n, freq, axis, pairs, neox,
+            _stream_on(stream, dev)))
         return q_out
 
     def plan_shared(self, lens: Sequence[int], group_sizes: Sequence[int],
