@@ -88,6 +88,31 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead, u
   return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
          (static_cast<uint64_t>(stride >> 4) << 32) | (1ull << 46);
 }
+// Rows of q, k-major and swizzled: 128-row blocks of kChunk elements (128 bytes where the head
+// dim is made of them, else 64) a row, whose 16-byte pieces are permuted by the row number.  A
+// copy of 16 bytes a lane then writes whole rows of a block, which takes shared memory a
+// quarter of the time that pieces 128 bytes apart do (in the pool's layout 256 rows of 128 dims
+// took an SM 6000 cycles).
+template <int D>
+struct RowBlocks {
+  static constexpr int kChunk = D % 64 == 0 ? 64 : 32;          // elements
+  static constexpr int kPieces = kChunk / 8;                    // of a row
+  static constexpr int kRowsPer = 32 / kPieces;                 // rows that a warp copies at a time
+  static constexpr int kBytes = 128 * kChunk * 2;               // of a block
+  // Byte offset of piece j of row r of a block.
+  static __device__ __forceinline__ uint32_t place(int r, int j) {
+    return r * (kChunk * 2) + ((j ^ (kChunk == 64 ? r & 7 : (r >> 1) & 3)) << 4);
+  }
+  static __device__ __forceinline__ uint64_t desc(uint32_t addr) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) |
+           (static_cast<uint64_t>(8 * kChunk * 2 >> 4) << 32) | (1ull << 46) |
+           ((kChunk == 64 ? 2ull : 4ull) << 61);
+  }
+  // What a descriptor grows by for k step k (16 elements).
+  static __host__ __device__ constexpr uint64_t step(int k) {
+    return static_cast<uint64_t>((k * 16 / kChunk * kBytes + k * 16 % kChunk * 2) >> 4);
+  }
+};
 // Instruction descriptor: A and B of one 16-bit type, fp32 accumulators.
 template <typename T>
 __host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool b_mn_major);

@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
   constexpr int U = D / 8, KP = S::kPos;
   constexpr uint32_t kSlabBytes = kSlab * D * 2;
   extern __shared__ __align__(1024) uint8_t smem[];
+  static_assert(S::kHeadBytes % 1024 == 0 && S::kQBytes % 1024 == 0, "swizzled rows start a pattern");
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
   volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(smem + 512);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + 516);
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       constexpr uint32_t kDescS = mma_desc<T>(128, KP, false);
       constexpr uint32_t kDescO = mma_desc<T>(128, D, true);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint64_t q_desc = operand_desc(smem_u32(q_mem), 128, U * 128);
+      const uint64_t q_desc = RowBlocks<D>::desc(smem_u32(q_mem));
       const uint64_t k_desc = operand_desc(smem_u32(stage_mem), 128, U * 128);
       const uint64_t v_desc = operand_desc(smem_u32(stage_mem), U * 128, 128);
       const bool leader = elect_one();
@@ -296,8 +297,8 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const uint64_t qd = q_desc + x * (S::kQBytes / 16), kd = k_desc + st * (S::kStageBytes / 16);
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)  // 16 dims: two core matrices on
-            mma_ss(tm + x * 128, qd + 16 * k, kd + 16 * k, kDescS, k > 0);
+          for (int k = 0; k < D / 16; ++k)  // 16 dims: two core matrices of K on
+            mma_ss(tm + x * 128, qd + RowBlocks<D>::step(k), kd + 16 * k, kDescS, k > 0);
           mma_commit(s_ready(x));
         }
       };
@@ -416,29 +417,31 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
         const bool two = sg.rows > 128;
         const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-        // Q in k-major core matrices, all its copies in flight together: a warp's copy covers
-        // 8 rows x 64 bytes.  Rows behind the last are zero up to a group of 8; what lies
-        // further on reaches no live row.  Streams that share their rows get a copy each.
+        // Q, all its copies in flight together.  Rows behind the last are zero up to a group of
+        // 8; what lies further on reaches no live row.  Streams that share their rows get a
+        // copy each.
         if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
         if (ok) {
-          const int rr = lane >> 2, uu = lane & 3;
+          using R = RowBlocks<D>;
+          const int rr = lane / R::kPieces, piece = lane % R::kPieces;
           const int n_rows = (sg.rows + 7) & ~7;
           // node and head of row g0 + rr, carried along (a division takes as long as the copies)
           int node = (sg.row0 + rr) / a.group, rem = sg.row0 + rr - node * a.group;
-          const int dn = 8 / a.group, dr = 8 - dn * a.group;
+          const int dn = R::kRowsPer / a.group, dr = R::kRowsPer - dn * a.group;
           const T* base = reinterpret_cast<const T*>(a.q) +
-                          (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D + uu * 8;
+                          (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D + piece * 8;
           const int row_step = a.num_heads * D;
-          const uint32_t dst0 = smem_u32(q_mem) + rr * 16 + uu * 128;
 #pragma unroll 2
-          for (int g0 = 0; g0 < n_rows; g0 += 8) {
+          for (int g0 = 0; g0 < n_rows; g0 += R::kRowsPer) {
             const bool there = g0 + rr < sg.rows;
             const T* src = there ? base + static_cast<size_t>(node) * row_step + rem * D : base;
-            const uint32_t dst = dst0 + (g0 >> 7) * S::kQBytes + ((g0 & 127) >> 3) * U * 128;
+            const int r = g0 + rr;
+            const uint32_t dst = smem_u32(q_mem) + (r >> 7) * S::kQBytes + R::place(r & 127, piece);
 #pragma unroll
-            for (int i = 0; i < U / 4; ++i) {
-              copy16_async(dst + i * 512, src + i * 32, there ? 16 : 0);
-              if (S::kStreams == 2 && !two) copy16_async(dst + S::kQBytes + i * 512, src + i * 32, there ? 16 : 0);
+            for (int i = 0; i < D / R::kChunk; ++i) {
+              copy16_async(dst + i * R::kBytes, src + i * R::kChunk, there ? 16 : 0);
+              if (S::kStreams == 2 && !two)
+                copy16_async(dst + S::kQBytes + i * R::kBytes, src + i * R::kChunk, there ? 16 : 0);
             }
             node += dn;
             rem += dr;
@@ -450,10 +453,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
           copy_async_wait();
           if (flip) {   // a negative scale turns q: what other lanes have copied, too
             __syncwarp();
-            for (int x = 0; x < S::kStreams; ++x) {
-              const int n = !two ? n_rows : x == 0 ? 128 : n_rows - 128;
-              uint32_t* words = reinterpret_cast<uint32_t*>(q_mem + x * S::kQBytes);
-              for (int i = lane; i < n * D / 2; i += 32) words[i] ^= flip;
+            for (int x = 0; x < S::kStreams * (D / R::kChunk); ++x) {
+              const int st = x / (D / R::kChunk), i = x - st * (D / R::kChunk);
+              const int n = !two ? n_rows : st == 0 ? 128 : n_rows - 128;
+              uint32_t* words = reinterpret_cast<uint32_t*>(q_mem + st * S::kQBytes + i * R::kBytes);
+              for (int k = lane; k < n * R::kChunk / 2; k += 32) words[k] ^= flip;
             }
           }
         }

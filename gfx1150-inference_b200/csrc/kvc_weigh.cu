@@ -137,21 +137,23 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
       bulk_g2s(smem_u32(k_mem) + lane * kSlabBytes, src, kSlabBytes, bar0, l2_policy_evict_first());
     }
   }
-  // Block b's rows of Q (zero behind the last), in k-major core matrices: a warp's copy covers
-  // 8 rows x 64 bytes; node and head are carried along.
+  // Block b's rows of Q, zero behind the last; node and head are carried along.
+  using R = RowBlocks<D>;
+  const int dn = 4 * R::kRowsPer / a.group, dr = 4 * R::kRowsPer - dn * a.group;
   auto copy_q = [&](int b) {
-    const int dn = 32 / a.group, dr = 32 - dn * a.group;
-    int row = b * kRecountRows + ww * 8 + (lane >> 2), node = row / a.group, rem = row - node * a.group;
+    const int rr = ww * R::kRowsPer + lane / R::kPieces, piece = lane % R::kPieces;
+    int row = b * kRecountRows + rr, node = row / a.group, rem = row - node * a.group;
     const T* base = reinterpret_cast<const T*>(a.q) +
-                    (static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group) * D + (lane & 3) * 8;
-    uint32_t dst = smem_u32(q_mem) + ww * U * 128 + (lane & 3) * 128 + (lane >> 2) * 16;
-    for (int g = 0; g < kRecountRows / 32; ++g) {
+                    (static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group) * D + piece * 8;
+#pragma unroll 2
+    for (int r = rr; r < kRecountRows; r += 4 * R::kRowsPer) {
       const bool there = row < rows;
       const T* src = there ? base + (static_cast<size_t>(node) * a.num_heads + rem) * D : base;
+      const uint32_t dst = smem_u32(q_mem) + R::place(r, piece);
 #pragma unroll
-      for (int i = 0; i < U / 4; ++i) copy16_async(dst + i * 512, src + i * 32, there ? 16 : 0);
-      dst += 4 * U * 128;
-      row += 32;
+      for (int i = 0; i < D / R::kChunk; ++i)
+        copy16_async(dst + i * R::kBytes, src + i * R::kChunk, there ? 16 : 0);
+      row += 4 * R::kRowsPer;
       node += dn;
       rem += dr;
       if (rem >= a.group) {
@@ -210,9 +212,9 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
     if (ww == 0 && elect_one()) {
       constexpr uint32_t kDesc = mma_desc<T>(128, kRecountRows, false);
       const uint64_t kd = operand_desc(smem_u32(k_mem), 128, U * 128);
-      const uint64_t qd = operand_desc(smem_u32(q_mem), 128, U * 128);
+      const uint64_t qd = R::desc(smem_u32(q_mem));
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) mma_ss(tmem, kd + 16 * k, qd + 16 * k, kDesc, k > 0);
+      for (int k = 0; k < D / 16; ++k) mma_ss(tmem, kd + 16 * k, qd + R::step(k), kDesc, k > 0);
       mma_commit(done);
     }
     __syncwarp();
