@@ -185,7 +185,7 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   }
   if (tiles > (1ll << 30))
     return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
-  cut_runs(runs, tile, sms, &segs, &cta_segs);
+  cut_runs(runs, tile, sms, true, &segs, &cta_segs);
   // Pieces of a run follow one another.  A run that is a row's only one, in one piece, writes
   // the output itself; the others write partials.
   std::vector<JoinPieces> pieces(runs.size());

@@ -263,8 +263,9 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
 
 // Floats that the scores of one plan take at most.
 constexpr int64_t kMaxScores = 1ll << 30;
-// Cuts whole runs (tile0 0, tile1 their tiles) into the CTAs' shares.
-void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
+// Cuts whole runs (tile0 0, tile1 their tiles) into the CTAs' shares; by_rows: counting what a
+// tile costs by its rows.
+void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms, bool by_rows,
               std::vector<TreeSeg>* segs, std::vector<int>* cta_segs);
 // Work for the decode kernel: the positions [base[i], lens[i]) of query i in table row
 // rows[i], in pieces that its warps take one after another.

@@ -232,12 +232,18 @@ int refuse_capture(cudaStream_t s, const char* what) {
 // The work list: the runs of position tiles are laid end to end and cut into shares of
 // equal cost, one per CTA.  A run that falls into several shares is joined from its pieces'
 // partials.
-void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
+void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms, bool by_rows,
               std::vector<TreeSeg>* segs, std::vector<int>* cta_segs) {
   segs->clear();
   cta_segs->assign(1, 0);
+  // A tile of a block that fills both streams of the tensor-core kernel costs twice one of a
+  // block whose tiles the streams share.
+  bool small = false, large = false;
+  for (const TreeSeg& r : runs) (2 * r.rows > tile.rows ? large : small) = true;
+  const int unit = by_rows && tile.tensor && tile.rows > 128 && small && large ? 2 : 1;
+  auto weight = [&](const TreeSeg& r) { return 2 * r.rows > tile.rows ? unit : 1; };
   int64_t tiles = 0;
-  for (const TreeSeg& r : runs) tiles += r.tile1;
+  for (const TreeSeg& r : runs) tiles += static_cast<int64_t>(r.tile1) * weight(r);
   const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(sms) * tile.ctas_per_sm, tiles);
   // A piece costs its tiles and `pc` for its start and end; a CTA's pieces cost at most `limit`
   // together, give or take a pc: a cut that would leave less than that on either side moves
@@ -247,13 +253,13 @@ void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
   // walk() lays the runs out for a limit, calls emit(run, tile, tiles) and close() for each
   // piece and each full share, and returns the number of shares.
   const int64_t pc = std::min<int64_t>(
-      tile.piece_cost, std::max<int64_t>(1, ctas > 0 ? tiles / (8 * ctas) : 1));
+      tile.piece_cost * unit, std::max<int64_t>(1, ctas > 0 ? tiles / (8 * ctas) : 1));
   auto walk = [&](int64_t limit, auto&& emit, auto&& close) {
     int64_t shares = 0, cost = 0;
     for (const TreeSeg& r : runs) {
-      const int run = r.tile1;
+      const int run = r.tile1, wt = weight(r);
       for (int t = 0; t < run;) {
-        const int64_t room = limit - cost - pc;
+        const int64_t room = (limit - cost - pc) / wt;
         if (cost > 0 && room < run - t && room < std::max<int64_t>(1, pc)) {
           close();
           ++shares;
@@ -264,7 +270,7 @@ void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms,
         if (run - t - take < pc) take = run - t;
         emit(r, t, take);
         t += take;
-        cost += take + pc;
+        cost += static_cast<int64_t>(take) * wt + pc;
       }
     }
     return shares + (cost > 0 ? 1 : 0);
@@ -469,7 +475,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
       }
     }
   }
-  cut_runs(runs, tile, sms, &segs, &cta_segs);
+  cut_runs(runs, tile, sms, p->keep_scores, &segs, &cta_segs);
   // Single tokens whose weights are wanted: the decode kernel streams K and V faster for a
   // token's few rows (32 x 1 at 1K-8K, fp16: 92 us, 105 with the kernel for trees) and keeps
   // scores at less cost (95, 125).  The pieces above serve calls with a mask.

@@ -12,8 +12,9 @@
 //   tree_merge_kernel   joins the pieces of rows whose positions were split over CTAs
 //   shared_join_kernel  the same for rows of a shared prefix and their own positions
 //                       (kvc_decode_shared)
-// The kScores variants also keep what kvc_weigh.cu makes the weights per slot of
-// (kvc_decode_tree_weights): every row's final max and sum, and the scores of short row lists.
+// With row_ml they also leave what kvc_weigh.cu makes the weights per slot of
+// (kvc_decode_tree_weights): every row's final max and sum, and the kScores variants the scores
+// of short row lists.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -423,33 +424,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
         if (ok) {
           using R = RowBlocks<D>;
-          const int rr = lane / R::kPieces, piece = lane % R::kPieces;
           const int n_rows = (sg.rows + 7) & ~7;
-          // node and head of row g0 + rr, carried along (a division takes as long as the copies)
-          int node = (sg.row0 + rr) / a.group, rem = sg.row0 + rr - node * a.group;
-          const int dn = R::kRowsPer / a.group, dr = R::kRowsPer - dn * a.group;
-          const T* base = reinterpret_cast<const T*>(a.q) +
-                          (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D + piece * 8;
-          const int row_step = a.num_heads * D;
-#pragma unroll 2
-          for (int g0 = 0; g0 < n_rows; g0 += R::kRowsPer) {
-            const bool there = g0 + rr < sg.rows;
-            const T* src = there ? base + static_cast<size_t>(node) * row_step + rem * D : base;
-            const int r = g0 + rr;
-            const uint32_t dst = smem_u32(q_mem) + (r >> 7) * S::kQBytes + R::place(r & 127, piece);
-#pragma unroll
-            for (int i = 0; i < D / R::kChunk; ++i) {
-              copy16_async(dst + i * R::kBytes, src + i * R::kChunk, there ? 16 : 0);
-              if (S::kStreams == 2 && !two)
-                copy16_async(dst + S::kQBytes + i * R::kBytes, src + i * R::kChunk, there ? 16 : 0);
-            }
-            node += dn;
-            rem += dr;
-            if (rem >= a.group) {
-              rem -= a.group;
-              ++node;
-            }
-          }
+          copy_rows<T, D>(smem_u32(q_mem), S::kQBytes, S::kStreams == 2 && !two,
+                          reinterpret_cast<const T*>(a.q) +
+                              (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D,
+                          sg.row0, sg.rows, n_rows, a.group, a.num_heads * D, 0, 1, lane);
           copy_async_wait();
           if (flip) {   // a negative scale turns q: what other lanes have copied, too
             __syncwarp();
@@ -729,9 +708,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const float inv = ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);
         if (live_row && sg.part >= 0 && (!joint || x == 0))
           a.part_ml[sg.part + row] = make_float2(mm, ll);
-        if constexpr (kScores) {
-          if (live_row && sg.part < 0 && (!joint || x == 0)) a.row_ml[io_row / D] = make_float2(mm, ll);
-        }
+        if (a.row_ml && live_row && sg.part < 0 && (!joint || x == 0)) a.row_ml[io_row / D] = make_float2(mm, ll);
         const bool add = joint && tiles > 1;
         auto load = [&](int c, uint32_t* o, uint32_t* q) {
           tmem_ld16(o0 + c, o);
@@ -995,7 +972,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) tree_f32_kernel(const TreeArgs
           po[c * step] = make_float4(acc[i][j].x * f, acc[i][j].y * f, acc[i][j].z * f, acc[i][j].w * f);
       }
       if (sg.part >= 0 && tx == 0) a.part_ml[sg.part + r] = make_float2(m[i], l[i]);
-      if constexpr (kScores) {
+      if (a.row_ml) {
         if (sg.part < 0 && tx == 0)
           a.row_ml[static_cast<size_t>(sg.tok0 + node) * a.num_heads + head] = make_float2(m[i], l[i]);
       }
@@ -1151,7 +1128,7 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
         T* po = reinterpret_cast<T*>(a.out) +
                 (static_cast<size_t>(sg.tok0 + node) * a.num_heads + head) * D;
         const float inv = l[i] > 0.f ? 1.0f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
-        if constexpr (kScores) {
+        if (a.row_ml) {
           if (lane == 0)
             a.row_ml[static_cast<size_t>(sg.tok0 + node) * a.num_heads + head] = make_float2(m[i], l[i]);
         }
@@ -1384,7 +1361,7 @@ template <typename T>
 cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (a.n_ctas > 0) {
-    if (a.weights)
+    if (a.weights && a.n_weighs > 0)   // (scores are kept)
       e = t.tensor ? run_mma_any<T, true>(a, s) : run_cuda_cores<T, true>(a, t, s);
     else
       e = t.tensor ? run_mma_any<T, false>(a, s) : run_cuda_cores<T, false>(a, t, s);

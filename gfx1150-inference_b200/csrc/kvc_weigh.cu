@@ -137,30 +137,14 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
       bulk_g2s(smem_u32(k_mem) + lane * kSlabBytes, src, kSlabBytes, bar0, l2_policy_evict_first());
     }
   }
-  // Block b's rows of Q, zero behind the last; node and head are carried along.
+  // Block b's rows of Q, zero behind the last.
   using R = RowBlocks<D>;
-  const int dn = 4 * R::kRowsPer / a.group, dr = 4 * R::kRowsPer - dn * a.group;
   auto copy_q = [&](int b) {
-    const int rr = ww * R::kRowsPer + lane / R::kPieces, piece = lane % R::kPieces;
-    int row = b * kRecountRows + rr, node = row / a.group, rem = row - node * a.group;
-    const T* base = reinterpret_cast<const T*>(a.q) +
-                    (static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group) * D + piece * 8;
-#pragma unroll 2
-    for (int r = rr; r < kRecountRows; r += 4 * R::kRowsPer) {
-      const bool there = row < rows;
-      const T* src = there ? base + (static_cast<size_t>(node) * a.num_heads + rem) * D : base;
-      const uint32_t dst = smem_u32(q_mem) + R::place(r, piece);
-#pragma unroll
-      for (int i = 0; i < D / R::kChunk; ++i)
-        copy16_async(dst + i * R::kBytes, src + i * R::kChunk, there ? 16 : 0);
-      row += 4 * R::kRowsPer;
-      node += dn;
-      rem += dr;
-      if (rem >= a.group) {
-        rem -= a.group;
-        ++node;
-      }
-    }
+    copy_rows<T, D>(smem_u32(q_mem), 0u, false,
+                    reinterpret_cast<const T*>(a.q) +
+                        (static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group) * D,
+                    b * kRecountRows, rows - b * kRecountRows, kRecountRows, a.group, a.num_heads * D, ww, 4,
+                    lane);
   };
   // Thread r: row r's max and sum.
   auto statistics = [&](int b) {
