@@ -112,11 +112,13 @@ struct alignas(16) SharedJoin {
 };
 // Slots of one (sequence, KV head) whose weights are added up: kWeighSlots from slot0 on from
 // kept scores, kRecountSlots where they are computed again.
-constexpr int kWeighSlots = 512, kRecountSlots = 128;
+constexpr int kWeighSlots = 1024, kRecountSlots = 128;
 struct alignas(16) TreeWeigh {
   int bt_row, ctx, nodes, tok0;
-  int kvh, slot0, scores, pad;   // scores: as in TreeSeg
+  int kvh, slot0, scores;        // scores: as in TreeSeg
+  int chain;                     // of its first row block in TreeArgs::chains
 };
+constexpr int kMergeThreads = 256;
 // (token, q-head) rows up to which a sequence keeps its scores on the tensor cores.
 constexpr int kKeepRows = 32;
 
@@ -148,6 +150,10 @@ struct TreeArgs {
   float* scores;
   const TreeWeigh* weighs;       // those with kept scores, then those without
   int n_weighs, n_recounts;
+  // The pieces that a row block's statistics are joined from (none: they are in row_ml), one
+  // for each chain_rows rows of a (sequence, KV head); with own_o: one for each token.
+  const JoinPieces* chains;
+  int chain_rows;
   int weight_slots;
   float score_scale;             // what a kept score is multiplied by, log2 units
 };
@@ -164,7 +170,12 @@ constexpr int kTreeSmall = 32;
 TreeTile tree_tile(const PoolGeom& g, int64_t small_tiles, int sms);
 cudaError_t launch_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s);
 cudaError_t launch_shared_join(const TreeArgs& a, cudaStream_t s);
-// The weights of what launch_tree has just attended to.
+// CTAs that take one of a.merges.
+inline int merge_ctas(const TreeArgs& a, size_t elem) {
+  const int per = a.max_merge_rows * static_cast<int>(a.head_dim * elem / 16);
+  return (per + kMergeThreads - 1) / kMergeThreads;
+}
+// The joins and the weights of what has just been attended to.
 cudaError_t launch_weigh(const TreeArgs& a, const TreeTile& t, cudaStream_t s);
 
 // ---- beam selection ---------------------------------------------------------------------
@@ -351,6 +362,8 @@ struct kvc_tree_plan {
   bool keep_scores = false, has_scores = false;
   int n_weighs = 0, n_recounts = 0;
   const kvc::TreeWeigh* dev_weighs = nullptr;
+  const kvc::JoinPieces* dev_chains = nullptr;   // of row blocks, then of single tokens
+  int token_weigh0 = 0;
   // Work on the decode kernel: unit records and their counter, and the joins of its splits
   const int4* dev_units = nullptr;
   unsigned int* dev_queue = nullptr;

@@ -190,6 +190,8 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
     a.row_ml = static_cast<float2*>(plan->d_row_ml.ptr);
     a.weighs = plan->dev_weighs;
     a.n_weighs = plan->n_weighs;
+    a.chains = plan->dev_chains;
+    a.chain_rows = plan->tile.rows;
     a.n_recounts = plan->n_recounts;
     a.weights = d_weights;
     a.weight_slots = weight_slots;
@@ -206,8 +208,8 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
       a.own_ml = d.part_ml;
       a.own_queue = d.queue;
       a.score_scale = 1.0f;   // (that kernel keeps them scaled)
+      a.weighs += plan->token_weigh0;
       cudaError_t e = launch_decode(d, a.dtype, a.p.layout, s);
-      if (e == cudaSuccess) e = launch_shared_join(a, s);
       if (e == cudaSuccess) e = launch_weigh(a, plan->tile, s);
       return e == cudaSuccess ? KVC_OK : cuda_error(e, "weighed decode kernels");
     }
@@ -466,7 +468,8 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
         if (keep) score0 += n_rows * ((end + 15) / 16);
         std::vector<TreeWeigh>& list = keep ? weighs : recounts;
         for (int slot = 0; slot < end; slot += keep ? kWeighSlots : kRecountSlots)
-          list.push_back(TreeWeigh{sg.bt_row, sg.ctx, sg.nodes, sg.tok0, kvh, slot, sg.scores, 0});
+          list.push_back(TreeWeigh{sg.bt_row, sg.ctx, sg.nodes, sg.tok0, kvh, slot, sg.scores,
+                                   static_cast<int>(runs.size())});
       }
       for (int r0 = 0; r0 < n_rows; r0 += tile.rows) {
         sg.row0 = r0;
@@ -504,9 +507,10 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
       if (w.kvh == 0 && w.slot0 == 0) score_base.push_back(w.scores);
   }
   // runs in several pieces are joined from their partials
-  size_t part_rows = 0;
+  std::vector<JoinPieces> chains(p->keep_scores ? runs.size() : 0);
+  size_t part_rows = 0, run = 0;
   int max_merge_rows = 0;
-  for (size_t first = 0; first < segs.size();) {
+  for (size_t first = 0; first < segs.size(); ++run) {
     size_t next = first + 1;
     while (next < segs.size() && segs[next].tile0 > 0) ++next;
     if (next - first > 1) {
@@ -520,6 +524,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
       m.rows = sg.rows;
       merges.push_back(m);
       max_merge_rows = std::max(max_merge_rows, sg.rows);
+      if (p->keep_scores) chains[run] = JoinPieces{m.part, m.n_parts, sg.rows, 0};
       for (size_t k = first; k < next; ++k) {
         segs[k].part = static_cast<int>(part_rows);
         part_rows += sg.rows;
@@ -566,6 +571,16 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   if (!units.recs.empty() && ((e = p->d_own_o.ensure(sizeof(float) * split_rows * g.head_dim)) ||
                               (e = p->d_own_ml.ensure(sizeof(float2) * split_rows))))
     return cuda_error(e, "plan buffers");
+  // (single tokens: their weighs again, with the tokens' chains, behind those of the row blocks)
+  p->token_weigh0 = static_cast<int>(weighs.size());
+  if (!units.recs.empty()) {
+    for (int i = 0; i < p->n_weighs; ++i) {
+      TreeWeigh w = weighs[i];
+      w.chain = static_cast<int>(chains.size()) + w.tok0;
+      weighs.push_back(w);
+    }
+    chains.insert(chains.end(), units.splits.begin(), units.splits.end());
+  }
   const unsigned int zero = 0;
   const PlanPart parts[] = {{segs.data(), sizeof(TreeSeg) * segs.size()},
                             {cta_segs.data(), sizeof(int) * cta_segs.size()},
@@ -576,9 +591,11 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
                             {joins.data(), sizeof(SharedJoin) * joins.size()},
                             {units.recs.data(), sizeof(int4) * units.recs.size()},
                             {score_base.data(), sizeof(int) * score_base.size()},
-                            {&zero, sizeof(zero)}};
-  const uint8_t* d[10];
-  if (const int rc = upload_plan(p, parts, 10, d, s)) return rc;
+                            {&zero, sizeof(zero)},
+                            {chains.data(), sizeof(JoinPieces) * chains.size()}};
+  const uint8_t* d[11];
+  if (const int rc = upload_plan(p, parts, 11, d, s)) return rc;
+  p->dev_chains = reinterpret_cast<const JoinPieces*>(d[10]);
   p->dev_joins = reinterpret_cast<const SharedJoin*>(d[6]);
   p->dev_units = reinterpret_cast<const int4*>(d[7]);
   p->dev_score_base = reinterpret_cast<const int*>(d[8]);

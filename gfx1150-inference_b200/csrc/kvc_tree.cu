@@ -1141,129 +1141,16 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const TreeArgs 
 }
 
 // =====================================================================================
-// Join of split rows: out = sum_k O_k 2^(m_k - m*) / sum_k l_k 2^(m_k - m*).  A piece's
-// partials are stored four dims of all its rows after one another, so that the threads
-// of a warp, which own a row each, write and read them side by side.  A thread joins 16
-// bytes of output of one row; the pieces are added in position order, so the result does
-// not depend on which CTA finished first.
+// Joins: see Join and the functions behind it.
 // =====================================================================================
-constexpr int kMergeThreads = 256;
-
-// 16 bytes of output of one row, gathered from pieces.
-template <typename T>
-struct Join {
-  static constexpr int N = 16 / sizeof(T), F = N / 4;
-  static constexpr int kAtOnce = 4;   // pieces on their way together
-  float mx = kNegBig, sum = 0.f;
-  float4 o[F];
-
-  __device__ __forceinline__ Join() {
-#pragma unroll
-    for (int i = 0; i < F; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  // n pieces from partial row `part` on, of `rows` rows each; 16 bytes c of their row r.
-  __device__ __forceinline__ void add(const TreeArgs& a, int part, int n, int rows, int r, int c) {
-    const float2* ml = a.part_ml + part + r;
-    const float4* po = reinterpret_cast<const float4*>(a.part_o + static_cast<size_t>(part) * a.head_dim) +
-                       c * F * rows + r;
-    const size_t po_step = static_cast<size_t>(rows) * a.head_dim / 4;
-    for (int k0 = 0; k0 < n; k0 += kAtOnce) {
-      float2 e[kAtOnce];
-      float4 v[kAtOnce][F];
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const bool there = k0 + k < n;
-        e[k] = there ? ml[static_cast<size_t>(k0 + k) * rows] : make_float2(kNegBig, 0.f);
-#pragma unroll
-        for (int i = 0; i < F; ++i)
-          v[k][i] = there ? po[(k0 + k) * po_step + i * rows] : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      take(e, v);
-    }
-  }
-  __device__ __forceinline__ void take(const float2 (&e)[kAtOnce], const float4 (&v)[kAtOnce][F]) {
-    float m2 = mx;
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) m2 = fmaxf(m2, e[k].x);
-    const float f = fast_exp2(mx - m2);
-    mx = m2;
-    sum *= f;
-#pragma unroll
-    for (int i = 0; i < F; ++i) {
-      o[i].x *= f;
-      o[i].y *= f;
-      o[i].z *= f;
-      o[i].w *= f;
-    }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const float w = fast_exp2(e[k].x - mx);
-      sum += e[k].y * w;
-#pragma unroll
-      for (int i = 0; i < F; ++i) {
-        o[i].x += v[k][i].x * w;
-        o[i].y += v[k][i].y * w;
-        o[i].z += v[k][i].z * w;
-        o[i].w += v[k][i].w * w;
-      }
-    }
-  }
-  // n splits from `split` on of the decode kernel, whose rows are plain; head `head`.
-  __device__ __forceinline__ void add_splits(const TreeArgs& a, int split, int n, int head, int c) {
-    for (int k0 = 0; k0 < n; k0 += kAtOnce) {
-      float2 e[kAtOnce];
-      float4 v[kAtOnce][F];
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const bool there = k0 + k < n;
-        const size_t row = static_cast<size_t>(split + k0 + k) * a.num_heads + head;
-        e[k] = there ? a.own_ml[row] : make_float2(kNegBig, 0.f);
-#pragma unroll
-        for (int i = 0; i < F; ++i)
-          v[k][i] = there ? reinterpret_cast<const float4*>(a.own_o + row * a.head_dim)[c * F + i]
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      take(e, v);
-    }
-  }
-  // into 16 bytes c of row `row` of the output, (tokens * heads) rows
-  __device__ __forceinline__ void store(const TreeArgs& a, size_t row, int c) const {
-    const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
-    T v[N];
-#pragma unroll
-    for (int i = 0; i < F; ++i) {
-      v[4 * i] = from_f32<T>(o[i].x * inv);
-      v[4 * i + 1] = from_f32<T>(o[i].y * inv);
-      v[4 * i + 2] = from_f32<T>(o[i].z * inv);
-      v[4 * i + 3] = from_f32<T>(o[i].w * inv);
-    }
-    T* out = reinterpret_cast<T*>(a.out) + row * a.head_dim + c * N;
-    *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);
-  }
-};
-
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
   const TreeMerge mg = a.merges[blockIdx.x];
   wait_prerequisites();
   launch_dependents();
-  const int x = blockIdx.y * kMergeThreads + threadIdx.x;
-  const int c = x / mg.rows, r = x - c * mg.rows;   // 16 bytes c of row r
-  if (c * Join<T>::N >= a.head_dim) return;
-  Join<T> join;
-  join.add(a, mg.part, mg.n_parts, mg.rows, r, c);
-  const int row = mg.row0 + r, node = row / a.group;
-  const int head = mg.kvh * a.group + row - node * a.group;
-  const size_t out_row = static_cast<size_t>(mg.tok0 + node) * a.num_heads + head;
-  join.store(a, out_row, c);
-  if (a.row_ml && c == 0) a.row_ml[out_row] = make_float2(join.mx, join.sum);
+  merge_rows<T>(a, mg, blockIdx.y * kMergeThreads + threadIdx.x);
 }
 
-// =====================================================================================
-// Join of a shared prefix and what follows it: a row's pieces are those of its group's
-// prefix, then those of its own positions.  A CTA joins one run of rows (a sequence's
-// q-heads of one KV head) with 16 bytes of one row a thread.
-// =====================================================================================
 constexpr int kSharedJoinThreads = 128;
 
 template <typename T>
@@ -1272,28 +1159,9 @@ __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const T
   SharedJoin j = {};
   if (mine) j = a.joins[blockIdx.x];
   wait_prerequisites();
-  if (a.own_queue && blockIdx.x == 0) {   // the decode is done: its work list for the next call
-    if (threadIdx.x == 0) {
-      *a.own_queue = 0u;
-      __threadfence();
-    }
-    __syncthreads();
-  }
+  if (blockIdx.x == 0) rearm_queue(a);
   launch_dependents();
-  if (!mine) return;
-  const int n = j.rows * (a.head_dim / Join<T>::N);
-  for (int x = threadIdx.x; x < n; x += kSharedJoinThreads) {
-    const int c = x / j.rows, r = x - c * j.rows;
-    Join<T> join;
-    join.add(a, j.prefix.part, j.prefix.n, j.prefix.rows, j.prefix.row + r, c);
-    if (a.own_o)
-      join.add_splits(a, j.own.part, j.own.n, j.head + r, c);
-    else
-      join.add(a, j.own.part, j.own.n, j.own.rows, j.own.row + r, c);
-    const size_t row = static_cast<size_t>(j.token) * a.num_heads + j.head + r;
-    join.store(a, row, c);
-    if (a.row_ml && c == 0) a.row_ml[row] = make_float2(join.mx, join.sum);
-  }
+  if (mine) join_rows<T>(a, j, kSharedJoinThreads);
 }
 
 // Every kernel here lets its successor begin right behind its own wait, so that nothing
@@ -1366,14 +1234,12 @@ cudaError_t run_tree(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
     else
       e = t.tensor ? run_mma_any<T, false>(a, s) : run_cuda_cores<T, false>(a, t, s);
   }
+  if (e == cudaSuccess && a.weights) return launch_weigh(a, t, s);   // (joins the pieces, too)
   if (e == cudaSuccess && a.n_merges > 0) {
     if ((e = prefer_shared<tree_merge_kernel<T>>()) != cudaSuccess) return e;
-    const int per = a.max_merge_rows * (a.head_dim * static_cast<int>(sizeof(T)) / 16);
-    e = launch_early(tree_merge_kernel<T>,
-                     dim3(a.n_merges, (per + kMergeThreads - 1) / kMergeThreads), kMergeThreads, 0,
-                     s, a);
+    e = launch_early(tree_merge_kernel<T>, dim3(a.n_merges, merge_ctas(a, sizeof(T))), kMergeThreads, 0, s, a);
   }
-  return e == cudaSuccess && a.weights ? launch_weigh(a, t, s) : e;
+  return e;
 }
 
 }  // namespace

@@ -5,7 +5,7 @@
 //   weights[row, kvh, p] += sum over the rows (token, q-head of kvh) of
 //                           2^(s scale log2(e) - max) / sum
 //
-//   weigh_kernel         from kept scores
+//   finish_kernel        from kept scores, and the joins of split rows
 //   recount_mma_kernel   computes the scores again on the tensor cores
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -21,52 +21,116 @@ namespace kvc {
 namespace {
 
 // =====================================================================================
-// From kept scores.  A thread owns four slots and adds the rows in order, so the sums do not
-// depend on the schedule; slots of the call's own tokens start from zero.  Bound by latency:
-// eight rows' scores, their statistics (the same for all threads) and the sums so far are on
-// their way together.
+// From kept scores, in one launch with the joins of the split rows.  A thread owns four slots
+// and adds the rows in order, so the sums do not depend on the schedule; slots of the call's
+// own tokens start from zero.  A row's final max and sum are joined here again from its
+// pieces (a few numbers a row), so that this does not wait for the rows' joins.  Bound by latency:
+// eight rows' scores, the sums so far and the pieces' statistics are on their way together.
 // =====================================================================================
-constexpr int kWeighThreads = kWeighSlots / 4, kWeighAtOnce = 8;
+constexpr int kFinishThreads = kWeighSlots / 4, kWeighAtOnce = 8;
+static_assert(kFinishThreads == kMergeThreads, "a join's CTA has as many threads");
 
-__global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const TreeArgs a) {
-  const TreeWeigh w = a.weighs[blockIdx.x];
+__device__ __forceinline__ float2 row_statistics(const TreeArgs& a, const TreeWeigh& w, int row) {
+  const int node = row / a.group, head = w.kvh * a.group + row - node * a.group;
+  const JoinPieces c = a.chains[w.chain + (a.own_o ? 0 : row / a.chain_rows)];
+  if (c.n == 0 || (a.own_o && c.n == 1))
+    return a.row_ml[static_cast<size_t>(w.tok0 + node) * a.num_heads + head];
+  const float2* ml = a.own_o ? a.own_ml + static_cast<size_t>(c.part) * a.num_heads + head
+                             : a.part_ml + c.part + row % a.chain_rows;
+  const size_t step = a.own_o ? a.num_heads : c.rows;
+  float2 all = make_float2(kNegBig, 0.f);
+  for (int k0 = 0; k0 < c.n; k0 += 8) {
+    float2 e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = k0 + k < c.n ? ml[(k0 + k) * step] : make_float2(kNegBig, 0.f);
+    float m = all.x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, e[k].x);
+    float sum = all.y * fast_exp2(all.x - m);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += e[k].y * fast_exp2(e[k].x - m);
+    all = make_float2(m, sum);
+  }
+  return all;
+}
+
+__device__ __forceinline__ void weigh(const TreeArgs& a, const TreeWeigh& w, float2* s_ml) {
   const int end = w.ctx + w.nodes, rows = w.nodes * a.group, pitch = (end + 15) & ~15;
   const int p = w.slot0 + 4 * threadIdx.x;
+  const bool mine = p < end;
   const float* s = a.scores + static_cast<size_t>(w.scores) * 16 + p;
   float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
-  const float2* ml = a.row_ml + static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group;
-  wait_prerequisites();
-  launch_dependents();
-  if (p >= end) return;
   float old[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float4 x[kWeighAtOnce];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int r = 0; r < kWeighAtOnce; ++r)
+      x[r] = mine && r0 + r < rows ? __ldcs(reinterpret_cast<const float4*>(s + static_cast<size_t>(r0 + r) * pitch))
+                                   : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  };
+  load(0);
 #pragma unroll
   for (int i = 0; i < 4; ++i) old[i] = p + i < w.ctx ? out[i] : 0.f;
-  for (int r0 = 0, node = 0, rem = 0; r0 < rows; r0 += kWeighAtOnce) {
-    float4 x[kWeighAtOnce];
-    float2 e[kWeighAtOnce];
-#pragma unroll
-    for (int r = 0; r < kWeighAtOnce; ++r) {
-      const bool there = r0 + r < rows;
-      x[r] = there ? __ldcs(reinterpret_cast<const float4*>(s + static_cast<size_t>(r0 + r) * pitch))
-                   : make_float4(0.f, 0.f, 0.f, 0.f);
-      e[r] = there ? ml[static_cast<size_t>(node) * a.num_heads + rem] : make_float2(0.f, 0.f);
-      if (++rem == a.group) {
-        rem = 0;
-        ++node;
-      }
+  for (int b = 0; b < rows; b += kFinishThreads) {
+    if (b > 0) __syncthreads();
+    if (b + threadIdx.x < rows) {
+      const float2 e = row_statistics(a, w, b + threadIdx.x);
+      s_ml[threadIdx.x] = make_float2(e.x, e.y > 0.f ? 1.0f / e.y : e.y);   // (0: no weight)
     }
+    __syncthreads();
+    const int n = min(kFinishThreads, rows - b);
+    for (int r0 = 0; r0 < n; r0 += kWeighAtOnce) {
+      if (b + r0 > 0) load(b + r0);
 #pragma unroll
-    for (int r = 0; r < kWeighAtOnce; ++r) {
-      const float inv = e[r].y > 0.f ? 1.0f / e[r].y : e[r].y;     // (0: a row without weight)
-      const float v[4] = {x[r].x, x[r].y, x[r].z, x[r].w};
+      for (int r = 0; r < kWeighAtOnce; ++r) {
+        if (r0 + r >= n) break;
+        const float2 e = s_ml[r0 + r];
+        const float v[4] = {x[r].x, x[r].y, x[r].z, x[r].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (v[i] != -INFINITY) sum[i] += fast_exp2(fmaf(v[i], a.score_scale, -e[r].x)) * inv;
+        for (int i = 0; i < 4; ++i)
+          if (v[i] != -INFINITY) sum[i] += fast_exp2(fmaf(v[i], a.score_scale, -e.x)) * e.y;
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (p + i < end) out[i] = old[i] + sum[i];
+}
+
+// CTAs of the grid: n_weighs, then those of the merges or the joins (one at least).
+template <typename T>
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const TreeArgs a, const int per_merge) {
+  __shared__ float2 s_ml[kFinishThreads];
+  const int b = blockIdx.x - a.n_weighs;
+  wait_prerequisites();
+  if (b == 0) rearm_queue(a);
+  launch_dependents();
+  if (b < 0) {
+    weigh(a, a.weighs[blockIdx.x], s_ml);
+  } else if (a.own_o) {
+    if (b < a.n_joins) join_rows<T>(a, a.joins[b], kFinishThreads);
+  } else if (b < a.n_merges * per_merge) {
+    merge_rows<T>(a, a.merges[b / per_merge], b % per_merge * kFinishThreads + threadIdx.x);
+  }
+}
+
+template <typename T>
+cudaError_t run_finish(const TreeArgs& a, cudaStream_t s) {
+  const int per_merge = merge_ctas(a, sizeof(T));
+  const int joins = a.own_o ? std::max(1, a.n_joins) : a.n_merges * per_merge;
+  if (a.n_weighs + joins == 0) return cudaSuccess;
+  const cudaError_t e = prefer_shared<finish_kernel<T>>();
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.n_weighs + joins));
+  cfg.blockDim = dim3(kFinishThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, finish_kernel<T>, a, per_merge);
 }
 
 // =====================================================================================
@@ -296,11 +360,9 @@ cudaError_t run_recount_any(const TreeArgs& a, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_weigh(const TreeArgs& a, const TreeTile& t, cudaStream_t s) {
-  cudaError_t e = cudaSuccess;
-  if (a.n_weighs > 0) {
-    if ((e = prefer_shared<weigh_kernel>()) != cudaSuccess) return e;
-    e = launch_early(weigh_kernel, dim3(a.n_weighs), kWeighThreads, 0, s, a);
-  }
+  const cudaError_t e = a.dtype == KVC_DTYPE_F16    ? run_finish<__half>(a, s)
+                        : a.dtype == KVC_DTYPE_BF16 ? run_finish<__nv_bfloat16>(a, s)
+                                                    : run_finish<float>(a, s);
   if (e != cudaSuccess || a.n_recounts == 0) return e;
   if (!t.tensor) return cudaErrorInvalidValue;
   return a.dtype == KVC_DTYPE_F16 ? run_recount_any<__half>(a, s) : run_recount_any<__nv_bfloat16>(a, s);
