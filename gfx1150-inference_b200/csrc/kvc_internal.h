@@ -155,6 +155,8 @@ struct DecodeArgs {
   // Block tables and KV pages are not written by the kernel launched just before
   // (plan flag KVC_PLAN_KV_STABLE): the decode kernel may start streaming them
   // before that kernel's results are visible.
+  // 2: and neither are q, the outputs and the partial states, which were ready before that
+  // kernel's own wait: the decode kernel runs beside it and waits for it only at its end.
   int early_prefetch;
   int l2_ahead = 0;              // slabs per warp prefetched into L2 before the wait
   // queries with more than one split (merged by merge_splits_kernel)

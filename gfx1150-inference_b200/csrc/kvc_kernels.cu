@@ -497,8 +497,15 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
   }
   __syncwarp();
 
-  const int gw = blockIdx.x * NW + warp;
-  const int W = gridDim.x * NW;
+  // Beside another kernel some CTAs start late, when that one leaves their SM: there the
+  // first unit, too, is the next one that nobody has.
+  const bool beside = a.early_prefetch == 2;
+  int gw = blockIdx.x * NW + warp;
+  if (beside) {
+    if (lane == 0) gw = static_cast<int>(atomicAdd(a.queue, 1u));
+    gw = __shfl_sync(0xffffffffu, gw, 0);
+  }
+  const int W = beside ? 0 : gridDim.x * NW;
   // A graph-stable plan keeps its counts in the plan's device header (its launches
   // are replayed as contexts grow); otherwise they come with the launch.
   const int n_units = a.plan_hdr ? a.plan_hdr[kHdrUnits] : a.n_units;
@@ -515,13 +522,15 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     page0 = page1 = -1;
     // A replayed launch of a rebuilt plan skips the host's check of the contexts
     // against the table width: an entry past the row's end counts as a bad page.
+    // (beside a running kernel nothing that was cached before may be taken for what is there)
+    auto entry = [&](int i) { return beside ? __ldcg(bt_row + i) : bt_row[i]; };
     if (lane < npages) {
-      const int v = pg0 + lane < a.bt_stride ? bt_row[pg0 + lane] : -1;
+      const int v = pg0 + lane < a.bt_stride ? entry(pg0 + lane) : -1;
       page0 = (v >= 0 && v < a.num_pages) ? v : -1;
       if (page0 < 0) report_error(1u, static_cast<uint32_t>(v));
     }
     if (lane + 32 < npages) {
-      const int v = pg0 + lane + 32 < a.bt_stride ? bt_row[pg0 + lane + 32] : -1;
+      const int v = pg0 + lane + 32 < a.bt_stride ? entry(pg0 + lane + 32) : -1;
       page1 = (v >= 0 && v < a.num_pages) ? v : -1;
       if (page1 < 0) report_error(1u, static_cast<uint32_t>(v));
     }
@@ -548,10 +557,14 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
   int pq_pos = -1;
   auto load_q = [&](const int4& r0, const int4& r2, auto& q) {
     const T* qrow = reinterpret_cast<const T*>(a.q) + (static_cast<size_t>(r0.x) * H + r2.z + gid) * D;
+    auto two = [&](int i) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(qrow + i);
+      return gid >= r2.w ? 0u : beside ? __ldcg(p) : *p;
+    };
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-      q[kc][0] = gid < r2.w ? *reinterpret_cast<const uint32_t*>(qrow + kc * 16 + 2 * tig) : 0u;
-      q[kc][1] = gid < r2.w ? *reinterpret_cast<const uint32_t*>(qrow + kc * 16 + 8 + 2 * tig) : 0u;
+      q[kc][0] = two(kc * 16 + 2 * tig);
+      q[kc][1] = two(kc * 16 + 8 + 2 * tig);
     }
   };
   // One step of the background fetch of the next unit.
@@ -575,7 +588,7 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
       n_state = 3;
     }
   };
-  bool dep_ready = false;  // the preceding kernel's results are visible (griddepcontrol.wait)
+  bool dep_ready = beside;  // the preceding kernel's results are visible (griddepcontrol.wait)
   auto start_unit = [&]() {
     p_j = p_r0.z / kSlab;
     p_end = (p_r0.w + kSlab - 1) / kSlab;
@@ -938,6 +951,8 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
   // wait gave up above).
   for (int k = waited; k < issued; ++k)
     (void)mbar_wait_bounded(smem_u32(&bars[k % NS]), static_cast<uint32_t>(k / NS) & 1u);
+  // Beside another kernel: what follows needs that one's results, too.
+  if (beside) asm volatile("griddepcontrol.wait;" ::: "memory");
   // The split merge (a programmatic dependent launch) may start being scheduled.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

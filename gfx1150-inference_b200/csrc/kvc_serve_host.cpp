@@ -85,6 +85,11 @@ int norm_rope_args(const kvc_pool* pool, int layer, const void* d_q, int q_strid
   return KVC_OK;
 }
 
+// Own positions beside prefixes: the longest piece of a warp, and what an SM reads in a us.
+constexpr int kBesideSplit = 256;
+constexpr double kBesideRate = 48e3;
+constexpr double kSharedTile = 1.6;
+
 // Every group's prefix is a set of runs of its members' rows, every sequence's own positions
 // another; a row's result is joined from its pieces of both.
 int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_rows,
@@ -171,21 +176,44 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   // tree kernel takes all (4 sequences on 512, 32 x 64 heads: 10 us, 14.7 with both).
   for (int i = 0; i < n_seqs; ++i)
     own_tiles += (h_lens[i] - base[i] + tile.positions - 1) / tile.positions * static_cast<int64_t>(own_blocks) * Hkv;
+  if (tiles + own_tiles > (1ll << 30))
+    return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
   const bool decode = tile.tensor && tiles + own_tiles > static_cast<int64_t>(sms) * tile.ctas_per_sm;
   UnitList units;
   if (decode) {
     std::vector<int> rows(n_seqs);
     for (int i = 0; i < n_seqs; ++i) rows[i] = h_rows ? h_rows[i] : i;
-    build_units(g, group, sms, rows, base, std::vector<int>(h_lens, h_lens + n_seqs), &units);
+    build_units(g, group, sms, rows, base, std::vector<int>(h_lens, h_lens + n_seqs),
+                tiles > 0 ? kBesideSplit : 0, &units);
   }
   for (int i = 0; i < n_seqs && !decode; ++i) {
     if (h_lens[i] <= base[i]) continue;
     own_run[i] = static_cast<int>(runs.size());
     add(h_rows ? h_rows[i] : i, base[i], h_lens[i], i, group);
   }
-  if (tiles > (1ll << 30))
-    return set_error(KVC_ERR_INVALID_ARG, "the batch is too large for one plan.");
-  cut_runs(runs, tile, sms, true, &segs, &cta_segs);
+  // The two kernels run side by side, the prefixes' on some SMs and the decode kernel on the
+  // others: each SM takes one or the other.  The prefixes get their share of the work, counted
+  // in what an SM was measured to need: 1.9 us for a tile of 256 rows x 128 positions x 128
+  // dims, half of that for a block whose tiles the two streams share, 4 us for a start and an
+  // end, and for K and V of own positions 60 bytes a ns.  (Decode CTAs follow on SMs that the
+  // prefixes leave, and take what is left of their list.)
+  int prefix_sms = sms;
+  if (decode && tiles > 0) {
+    double prefix_us = 0, own_bytes = 0;
+    for (const TreeSeg& r : runs)
+      prefix_us += (2 * r.rows > tile.rows ? 1.9 : kSharedTile) * r.tile1 * tile.positions / 128.0 * g.head_dim / 128.0;
+    for (int i = 0; i < n_seqs; ++i)
+      own_bytes += 2.0 * (h_lens[i] - base[i]) * Hkv * ((group + 7) / 8) * g.head_dim * g.elem_size;
+    const double own_us = own_bytes / kBesideRate;
+    // prefix_us / x + 4 = own_us / (sms - x)
+    double lo = 1, hi = sms;
+    for (int k = 0; k < 20; ++k) {
+      const double x = (lo + hi) / 2;
+      (prefix_us / x + 4.0 > own_us / std::max(0.01, sms - x) ? lo : hi) = x;
+    }
+    prefix_sms = std::max(1, std::min(sms, static_cast<int>(hi + 0.5)));
+  }
+  cut_runs(runs, tile, prefix_sms, true, &segs, &cta_segs);
   // Pieces of a run follow one another.  A run that is a row's only one, in one piece, writes
   // the output itself; the others write partials.
   std::vector<JoinPieces> pieces(runs.size());

@@ -286,12 +286,15 @@ struct UnitList {
   int n_splits = 0;
 };
 // A query with a base is joined with something else: its splits are partial states, were it
-// but one.
+// but one.  longest: positions of a piece at most (rounded to whole pages), 0: as many as
+// kvc_plan_decode takes.
 void build_units(const PoolGeom& g, int group, int sms, const std::vector<int>& rows,
-                 const std::vector<int>& base, const std::vector<int>& lens, UnitList* out);
-// Its arguments for units of `plan`, in a call whose attention takes `a`.  early: the launch
-// ahead writes no KV and began behind everything that does.
-DecodeArgs unit_args(const kvc_tree_plan* plan, const TreeArgs& a, bool early);
+                 const std::vector<int>& base, const std::vector<int>& lens, int longest,
+                 UnitList* out);
+// Its arguments for units of `plan`, in a call whose attention takes `a`.  beside: it runs
+// beside the launch ahead, an attention kernel that writes nothing that it reads, and which
+// began behind everything that does.
+DecodeArgs unit_args(const kvc_tree_plan* plan, const TreeArgs& a, bool beside);
 // A plan's records go to its device buffer in one copy; dev[i]: where parts[i] will be.
 struct PlanPart {
   const void* data;

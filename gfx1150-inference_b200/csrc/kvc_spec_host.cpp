@@ -308,11 +308,16 @@ void cut_runs(const std::vector<TreeSeg>& runs, const TreeTile& tile, int sms, b
 }
 
 void build_units(const PoolGeom& g, int group, int sms, const std::vector<int>& rows,
-                 const std::vector<int>& base, const std::vector<int>& lens, UnitList* out) {
+                 const std::vector<int>& base, const std::vector<int>& lens, int longest,
+                 UnitList* out) {
   const int n = static_cast<int>(lens.size()), chunks = (group + 7) / 8;
   std::vector<int> own(n), refine(n);
   for (int i = 0; i < n; ++i) own[i] = lens[i] - base[i];
-  const int C = split_partition_sms(g.page_size, own.data(), n, g.num_kv_heads * chunks, sms, refine.data());
+  int C = split_partition_sms(g.page_size, own.data(), n, g.num_kv_heads * chunks, sms, refine.data());
+  if (longest > 0 && C > longest) {
+    C = (longest + g.page_size - 1) / g.page_size * g.page_size;
+    std::fill(refine.begin(), refine.end(), 0);
+  }
   out->splits.assign(n, JoinPieces{});
   std::vector<int4> items;
   for (int i = 0; i < n; ++i) {
@@ -339,7 +344,7 @@ void build_units(const PoolGeom& g, int group, int sms, const std::vector<int>& 
   }
 }
 
-DecodeArgs unit_args(const kvc_tree_plan* plan, const TreeArgs& a, bool early) {
+DecodeArgs unit_args(const kvc_tree_plan* plan, const TreeArgs& a, bool beside) {
   DecodeArgs d = {};
   d.k_layer = a.p.k;
   d.v_layer = a.p.v;
@@ -353,7 +358,7 @@ DecodeArgs unit_args(const kvc_tree_plan* plan, const TreeArgs& a, bool early) {
   d.n_units = d.n_items = d.sched_cap = plan->n_units;
   d.queue = plan->dev_queue;
   d.n_sched_ctas = plan->n_unit_ctas;
-  d.early_prefetch = early ? 1 : 0;
+  d.early_prefetch = beside ? 2 : 0;
   d.num_heads = a.num_heads;
   d.num_kv_heads = a.p.num_kv_heads;
   d.group = a.group;
@@ -492,7 +497,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
       unit_rows.push_back(h_rows ? h_rows[i] : i);
       lens.push_back(h_ctx[i] + 1);
     }
-    build_units(g, group, sms, unit_rows, std::vector<int>(lens.size(), 0), lens, &units);
+    build_units(g, group, sms, unit_rows, std::vector<int>(lens.size(), 0), lens, 0, &units);
     for (size_t t = 0; t < lens.size(); ++t)
       for (int kvh = 0; kvh < g.num_kv_heads && units.splits[t].n > 1; ++kvh) {
         SharedJoin j = {};
@@ -703,8 +708,8 @@ extern "C" int kvc_decode_tree_weights(kvc_pool_t* pool, const kvc_tree_plan_t* 
   if (!pool || !plan) return set_error(KVC_ERR_INVALID_ARG, "pool and plan must not be null.");
   return guarded("kvc_decode_tree_weights", [&]() -> int {
     if (!d_weights) return set_error(KVC_ERR_INVALID_ARG, "weights must not be null.");
-    if (!aligned16(d_weights))
-      return set_error(KVC_ERR_INVALID_ARG, "weights must be 16-byte aligned.");
+    if (reinterpret_cast<uintptr_t>(d_weights) & 3u)
+      return set_error(KVC_ERR_INVALID_ARG, "weights must be 4-byte aligned.");
     DeviceScope dev(pool->device);
     if (dev.rc()) return dev.rc();
     return do_decode_tree(pool, plan, layer, d_q, d_mask, mask_words, d_out, d_block_tables,
