@@ -85,10 +85,15 @@ int norm_rope_args(const kvc_pool* pool, int layer, const void* d_q, int q_strid
   return KVC_OK;
 }
 
-// Own positions beside prefixes: the longest piece of a warp, and what an SM reads in a us.
+// Bytes that sharing saves a layer, from which on it is done.
+constexpr double kSharedSaving = 32e6;
+// Prefixes and own positions side by side.  An SM needs kFullTile us for 128 positions x 128 dims
+// of more than 128 rows, kPartTile for one of fewer rows, kPieceTime for a start and an end, and
+// reads kBesideRate bytes a us of own positions, of which a warp takes kBesideSplit at a time.
+// (Swept on 96 x 24K, 9 ragged groups and six more shapes: 128, 192 and 256 positions x 28e3 to
+// 120e3 bytes; within 5 % of the best on each.)
+constexpr double kFullTile = 1.9, kPartTile = 1.6, kPieceTime = 4.0, kBesideRate = 48e3;
 constexpr int kBesideSplit = 256;
-constexpr double kBesideRate = 48e3;
-constexpr double kSharedTile = 1.6;
 
 // Every group's prefix is a set of runs of its members' rows, every sequence's own positions
 // another; a row's result is joined from its pieces of both.
@@ -161,10 +166,19 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
         runs.push_back(sg);
       }
   };
+  // What sharing saves has to pay for a launch and the joins.  Measured over groups of 2-64
+  // members, prefixes of 128-8192 positions, 2 x 64 and 8 x 128 dims, 16 bit: below 32 MB of K
+  // and V that are not read again it costs 0-5 us (8 x 2 members on 512, 17 MB: 19.3 against
+  // 16.3 us), above that it wins (8 x 4 on 512, 50 MB: 18.9 against 21.3; 8 x 16 on 2048, 1 GB: 43
+  // against 167).  The CUDA-core kernels, whose tiles cost the same for any number of rows,
+  // gain from every tile.
+  double saved = 0;
+  for (int k = 0; k < n_groups; ++k)
+    saved += 2.0 * (h_sizes[k] - 1) * h_prefix[k] * Hkv * g.head_dim * g.elem_size;
+  const bool worth = !tile.tensor || saved >= kSharedSaving;
   for (int k = 0, i = 0; k < n_groups; i += h_sizes[k++]) {
-    // A prefix is worth a run of its own from one tile on: below that the members' own first
-    // tiles hold it anyway.
-    if (h_sizes[k] < 2 || h_prefix[k] < tile.positions) continue;
+    // (below one tile the members' own first tiles hold the prefix anyway)
+    if (!worth || h_sizes[k] < 2 || h_prefix[k] < tile.positions) continue;
     prefix_run[k] = static_cast<int>(runs.size());
     add(h_rows ? h_rows[i] : i, 0, h_prefix[k], i, h_sizes[k] * group);
     std::fill(base.begin() + i, base.begin() + i + h_sizes[k], h_prefix[k]);
@@ -192,27 +206,29 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
     add(h_rows ? h_rows[i] : i, base[i], h_lens[i], i, group);
   }
   // The two kernels run side by side, the prefixes' on some SMs and the decode kernel on the
-  // others: each SM takes one or the other.  The prefixes get their share of the work, counted
-  // in what an SM was measured to need: 1.9 us for a tile of 256 rows x 128 positions x 128
-  // dims, half of that for a block whose tiles the two streams share, 4 us for a start and an
-  // end, and for K and V of own positions 60 bytes a ns.  (Decode CTAs follow on SMs that the
-  // prefixes leave, and take what is left of their list.)
+  // others: each SM takes one or the other.  The prefixes get their share of the work.  (Decode
+  // CTAs follow on SMs that the prefixes leave, and take what is left of their list.)
   int prefix_sms = sms;
   if (decode && tiles > 0) {
     double prefix_us = 0, own_bytes = 0;
     for (const TreeSeg& r : runs)
-      prefix_us += (2 * r.rows > tile.rows ? 1.9 : kSharedTile) * r.tile1 * tile.positions / 128.0 * g.head_dim / 128.0;
+      prefix_us += (2 * r.rows > tile.rows ? kFullTile : kPartTile) * r.tile1 * tile.positions / 128.0 * g.head_dim / 128.0;
     for (int i = 0; i < n_seqs; ++i)
       own_bytes += 2.0 * (h_lens[i] - base[i]) * Hkv * ((group + 7) / 8) * g.head_dim * g.elem_size;
     const double own_us = own_bytes / kBesideRate;
-    // prefix_us / x + 4 = own_us / (sms - x)
+    // prefix_us / x + kPieceTime = own_us / (sms - x)
     double lo = 1, hi = sms;
     for (int k = 0; k < 20; ++k) {
       const double x = (lo + hi) / 2;
-      (prefix_us / x + 4.0 > own_us / std::max(0.01, sms - x) ? lo : hi) = x;
+      (prefix_us / x + kPieceTime > own_us / std::max(0.01, sms - x) ? lo : hi) = x;
     }
     prefix_sms = std::max(1, std::min(sms, static_cast<int>(hi + 0.5)));
   }
+  // A join takes about as long for four pieces as a tile: t tiles in p pieces are done after
+  // t / p + p / 4 of them, which p = 2 sqrt(t) makes least.
+  double pieces_at_most = 0;
+  for (const TreeSeg& r : runs) pieces_at_most += std::ceil(2.0 * std::sqrt(static_cast<double>(r.tile1)));
+  if (tile.tensor) prefix_sms = static_cast<int>(std::min<double>(prefix_sms, std::max(1.0, pieces_at_most)));
   cut_runs(runs, tile, prefix_sms, true, &segs, &cta_segs);
   // Pieces of a run follow one another.  A run that is a row's only one, in one piece, writes
   // the output itself; the others write partials.
