@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
 // layer's K or V and goes through the kept slots in order, a chunk at a time.  A slot never
 // moves up, so a later chunk's sources lie behind every place written before it: the next
 // chunk is read before this one is written, and only the reads of one chunk have to be done
-// (a barrier) before its first write.  Rows in front of the first one that leaves stay.
+// (a barrier) before its first write.  Rows that stay where they are are not touched.
 //
 // Bound by memory traffic, which is more than the rows' bytes: a row's 16-byte pieces stand
 // 128 bytes apart, eight positions to a line, so of 64 bytes that memory reads at a time half
@@ -525,30 +525,19 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
   wait_prerequisites();
   const int n = a.ctx[seq], m = a.budget, row = a.rows ? a.rows[seq] : seq;
   const int32_t* kept = a.kept + ((static_cast<size_t>(layer) * a.n + seq) * Hkv + head) * m;
-  if (n <= m || kept[0] < 0) return;       // nothing leaves, or reported
-  // the first row that moves: kept[j] is j in front of it, and larger from there on
-  int lo = 0, hi = m;
-  while (hi - lo > 0) {
-    const int step = (hi - lo + kMoveThreads - 1) / kMoveThreads, j = lo + tid * step;
-    const int stay = __syncthreads_count(j < hi && kept[j] == j);   // of the tested ones
-    if (stay == 0) break;                  // (the first one moves)
-    hi = min(hi, lo + stay * step);
-    lo += (stay - 1) * step + 1;
-  }
-  if (lo >= m) return;
+  if (n <= m) return;                      // nothing leaves
   const bool core = a.p.layout == kLayoutCore;
-  const int first = core ? lo & ~7 : lo;
   uint8_t* base = (kv ? a.p.v : a.p.k) + static_cast<size_t>(layer) * a.layer_bytes;
   int chunk = kMoveThreads * kMoveUnits / U;                 // rows of a chunk
   chunk = chunk > kMoveRows ? kMoveRows : (chunk & ~7);
-  const int chunks = (m - first + chunk - 1) / chunk;
+  const int chunks = (m + chunk - 1) / chunk;
   auto place = [&](int pos) {
     const int page = page_of(a.p, row, pos);
     return page < 0 ? kNone : static_cast<uint32_t>(unit_at(a.p, page, head, pos % ps, part * U) / 16);
   };
   auto places = [&](int c) {               // where chunk c's rows are and go
     for (int r = tid; r < chunk && c < chunks; r += kMoveThreads) {
-      const int j = first + c * chunk + r, from = j < m ? kept[j] : j;
+      const int j = c * chunk + r, from = j < m ? kept[j] : j;   // (-1: reported)
       uint2 x = make_uint2(kNone, kNone);
       if (from > j) x = make_uint2(place(from), place(j));
       if (x.y == kNone) x.x = kNone;
