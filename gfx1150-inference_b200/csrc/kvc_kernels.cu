@@ -468,10 +468,17 @@ constexpr int persist_stages() {
              : (196608 / (kPersistWarpsPerSm * 2 * kSlab * D * 2));
 }
 
-template <typename T, int D, int NW, int NS, bool kScores>
+// What it does beside attending.  Variants rather than branches: with them the plain decode
+// took 1.4 % longer.
+enum DecodeMode {
+  kPlainDecode,
+  kKeepScores,     // scores and final statistics are kept for kvc_decode_tree_weights
+  kBeside,         // it runs beside the kernel ahead of it (DecodeArgs::early_prefetch 2)
+};
+
+template <typename T, int D, int NW, int NS, DecodeMode kMode>
 __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     decode_persistent_kernel(const DecodeArgs a) {
-  // kScores: the scores and final statistics are kept for kvc_decode_tree_weights
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int SLAB_BYTES = kSlab * D * 2;
   constexpr int STAGE_BYTES = 2 * SLAB_BYTES;
@@ -499,9 +506,9 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
 
   // Beside another kernel some CTAs start late, when that one leaves their SM: there the
   // first unit, too, is the next one that nobody has.
-  const bool beside = a.early_prefetch == 2;
+  constexpr bool beside = kMode == kBeside;
   int gw = blockIdx.x * NW + warp;
-  if (beside) {
+  if constexpr (beside) {
     if (lane == 0) gw = static_cast<int>(atomicAdd(a.queue, 1u));
     gw = __shfl_sync(0xffffffffu, gw, 0);
   }
@@ -523,7 +530,10 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     // A replayed launch of a rebuilt plan skips the host's check of the contexts
     // against the table width: an entry past the row's end counts as a bad page.
     // (beside a running kernel nothing that was cached before may be taken for what is there)
-    auto entry = [&](int i) { return beside ? __ldcg(bt_row + i) : bt_row[i]; };
+    auto entry = [&](int i) {
+      if constexpr (beside) return __ldcg(bt_row + i);
+      return bt_row[i];
+    };
     if (lane < npages) {
       const int v = pg0 + lane < a.bt_stride ? entry(pg0 + lane) : -1;
       page0 = (v >= 0 && v < a.num_pages) ? v : -1;
@@ -559,7 +569,8 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     const T* qrow = reinterpret_cast<const T*>(a.q) + (static_cast<size_t>(r0.x) * H + r2.z + gid) * D;
     auto two = [&](int i) {
       const uint32_t* p = reinterpret_cast<const uint32_t*>(qrow + i);
-      return gid >= r2.w ? 0u : beside ? __ldcg(p) : *p;
+      if constexpr (beside) return gid < r2.w ? __ldcg(p) : 0u;
+      return gid < r2.w ? *p : 0u;
     };
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
@@ -724,7 +735,7 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     const float l_hi = __shfl_sync(0xffffffffu, l_run, (2 * tig + 1) * 4);
     const int h_lo = 2 * tig, h_hi = 2 * tig + 1;
     if (n_splits == 1 && a.xchg_peers == 0) {  // exchanged outputs all go through the merge
-      if constexpr (kScores) {
+      if constexpr (kMode == kKeepScores) {
         if (tig == 0 && gid < nh) a.row_ml[static_cast<size_t>(query) * H + hq0 + gid] = make_float2(m_run, l_run);
       }
       const float i_lo = l_lo > 0.f ? 1.0f / l_lo : 0.f;
@@ -792,7 +803,7 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
         }
       }
       if (!have_q) load_q(c_r0, c_r2, qa);
-      if constexpr (kScores)
+      if constexpr (kMode == kKeepScores)
         score_row = a.scores + static_cast<size_t>(a.score_base[c_r0.x]) * 16 +
                     static_cast<size_t>(c_r2.z + gid) * ((c_r1.y + 15) & ~15);
       m_run = kNegBig;
@@ -902,7 +913,7 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     const float x1 = (sc[0][0][1] + sc[0][1][1]) * a.scale_log2;
     const float x2 = (sc[1][0][0] + sc[1][1][0]) * a.scale_log2;
     const float x3 = (sc[1][0][1] + sc[1][1][1]) * a.scale_log2;
-    if constexpr (kScores) {
+    if constexpr (kMode == kKeepScores) {
       if (gid < c_r2.w) {   // (whole slabs: a row has room for them)
         *reinterpret_cast<float2*>(score_row + j * kSlab + t0) = make_float2(x0, x1);
         *reinterpret_cast<float2*>(score_row + j * kSlab + t0 + 8) = make_float2(x2, x3);
@@ -952,7 +963,7 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
   for (int k = waited; k < issued; ++k)
     (void)mbar_wait_bounded(smem_u32(&bars[k % NS]), static_cast<uint32_t>(k / NS) & 1u);
   // Beside another kernel: what follows needs that one's results, too.
-  if (beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if constexpr (beside) asm volatile("griddepcontrol.wait;" ::: "memory");
   // The split merge (a programmatic dependent launch) may start being scheduled.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
@@ -1373,13 +1384,13 @@ cudaError_t set_smem_once(F kern, size_t smem) {
   return e;
 }
 
-template <typename T, int D, int NW, bool kScores>
+template <typename T, int D, int NW, DecodeMode kMode>
 cudaError_t run_persistent(const DecodeArgs& a, cudaStream_t s) {
   constexpr int NS = persist_stages<D>();
   const size_t smem =
       kPersistBarBytes + kPersistMetaBytes + static_cast<size_t>(NW) * NS * 2 * kSlab * D * 2;
-  auto kern = decode_persistent_kernel<T, D, NW, NS, kScores>;
-  cudaError_t e = set_smem_once<decode_persistent_kernel<T, D, NW, NS, kScores>>(kern, smem);
+  auto kern = decode_persistent_kernel<T, D, NW, NS, kMode>;
+  cudaError_t e = set_smem_once<decode_persistent_kernel<T, D, NW, NS, kMode>>(kern, smem);
   if (e != cudaSuccess) return e;
   if (a.n_sched_ctas <= 0) return cudaSuccess;
   cudaLaunchAttribute attr[1];
@@ -1426,8 +1437,9 @@ cudaError_t run_persistent(const DecodeArgs& a, cudaStream_t s) {
 
 template <typename T, int D>
 cudaError_t run_mma(const DecodeArgs& a, cudaStream_t s) {
-  if (a.scores) return run_persistent<T, D, kPersistWarps, true>(a, s);
-  return run_persistent<T, D, kPersistWarps, false>(a, s);
+  if (a.scores) return run_persistent<T, D, kPersistWarps, kKeepScores>(a, s);
+  if (a.early_prefetch == 2) return run_persistent<T, D, kPersistWarps, kBeside>(a, s);
+  return run_persistent<T, D, kPersistWarps, kPlainDecode>(a, s);
 }
 
 template <typename T, int EPL>

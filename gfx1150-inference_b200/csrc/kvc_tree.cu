@@ -165,6 +165,11 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     *s_abort = 0;
     for (int i = 0; i < 4; ++i) s_dirty[i] = -1;
   }
+  // Rows without a token are zeros: whatever else Q's memory holds reaches no result, but it
+  // costs power in every MMA (32 ragged trees: 143 us for 132).
+  for (int i = threadIdx.x; i < S::kStreams * S::kQBytes / 16; i += S::kThreads)
+    reinterpret_cast<uint4*>(q_mem)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
   // (the plan's records are no kernel's output: they may be read before the wait)
   const int seg0 = a.cta_segs[blockIdx.x], seg1 = a.cta_segs[blockIdx.x + 1];
   wait_prerequisites();
@@ -411,6 +416,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
     } else {
       // ---- helper: each piece's Q, and the V tiles that hold drafted positions --------------
       const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+      int high0 = 0, high1 = 0;   // rows of the streams' copies that may not be zero
       uint32_t ring = 0, nf = 0, ng = 0;
       bool ok = true;
       for (int si = seg0; si < seg1; ++si) {
@@ -418,13 +424,16 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
         const int tiles = sg.tile1 - sg.tile0, end = sg.ctx + sg.nodes;
         const bool two = sg.rows > 128;
         const int ahead = S::kStreams == 2 && !two ? 2 : 1;
-        // Q, all its copies in flight together.  Rows behind the last are zero up to a group of
-        // 8; what lies further on reaches no live row.  Streams that share their rows get a
-        // copy each.
+        // Q, all its copies in flight together, and zeros as far as an earlier piece had rows.
+        // Streams that share their rows get a copy each.
         if (si > seg0) ok = ok && wait(q_free, nf++ & 1);   // the last piece's scores are done
         if (ok) {
           using R = RowBlocks<D>;
-          const int n_rows = (sg.rows + 7) & ~7;
+          int n_rows = (sg.rows + 7) & ~7;
+          const int now0 = two ? 128 : n_rows, now1 = two ? n_rows - 128 : n_rows;
+          n_rows = two ? 128 + max(now1, high1) : max(n_rows, max(high0, high1));
+          high0 = now0;
+          high1 = now1;
           copy_rows<T, D>(smem_u32(q_mem), S::kQBytes, S::kStreams == 2 && !two,
                           reinterpret_cast<const T*>(a.q) +
                               (static_cast<size_t>(sg.tok0) * a.num_heads + sg.kvh * a.group) * D,
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
       const bool joint = ahead == 2;
       const int row = (two ? x * 128 : 0) + r;
       const bool live = (two ? x * 128 : 0) + w4 * 32 < seg->rows;   // some row of the warp
-      const bool mine = row < seg->rows;   // (rows behind the last hold whatever Q's memory does)
+      const bool mine = row < seg->rows; 
       // where the row's scores go, 16 positions to 64 bytes (its pitch is a multiple of that)
       float* keep = nullptr;
       int keep_end = 0;
