@@ -23,6 +23,11 @@ namespace {
 // does), each pair with the position of its own axis.  A head belongs to kLanes lanes of one
 // warp, each of which owns two 16-byte units that hold each other's pairs, so the sum of
 // squares is a few shuffles and the head is read once.  All in 32 bits, rounded once.
+//
+// Bound by memory traffic and by how many heads are on their way: 8,626 tokens of 32 + 8 + 8
+// heads of 128 dims, fp16, three axes, 50 us for 212 MB (32 at the copy rate; append_rope_kernel
+// 45).  An SM takes four CTAs, which weights and angles in registers do not leave room for
+// (104 registers, two CTAs: 65 us; three heads a lane group on their way: 60); three CTAs 52.
 // =====================================================================================
 constexpr int kNormThreads = 256;
 constexpr int kNormBatch = 2;      // heads of a lane group on their way
@@ -294,8 +299,9 @@ cudaError_t run_norm_rope_type(const NormRopeArgs& a, bool neox, int sms, cudaSt
 // one that it takes.  (A list of more than kSelectList, as equal weights make it, is searched
 // seven bits at a time instead.)  One ordered pass then writes the kept slots and their weights,
 // which may go to where they came from: a slot never moves up, and all weights of a round are
-// read before any of it is written.  Bound by its instructions, some 90 a weight and thread
-// (8 x 32 x 8 heads of 900-3100 weights: 22 us; 36 with four passes of eight bits).
+// read before any of it is written.  Bound by latency where there are few heads (88 of 600
+// weights: 6.7 us; 8.8 with four passes of eight bits), by its instructions and barriers where
+// there are many (2,048 of 900-3,100: 38 us, issue slots 60 % busy; 36 with the passes).
 // =====================================================================================
 constexpr int kSelectThreads = 256;
 constexpr int kSelectHeld = 8192;    // weights kept in shared memory; longer rows are read again
@@ -510,7 +516,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
 //
 // Bound by memory traffic, which is more than the rows' bytes: a row's 16-byte pieces stand
 // 128 bytes apart, eight positions to a line, so of 64 bytes that memory reads at a time half
-// are another row's where every second slot stays.
+// are another row's where every second slot stays.  8 sequences of 900-3,100 cut to 1024 in 32
+// layers of 8 x 128 dims, bf16: 404 us for 1.9 GB of rows, which are 2.7 GB of traffic at 6.7
+// TB/s, the rate of a copy.  (Offsets of a thread's units kept in registers, places as 32-bit
+// units: 475 us with divisions by the unit count in every chunk.)
 // =====================================================================================
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnits = 8;        // 16-byte units of a thread on their way

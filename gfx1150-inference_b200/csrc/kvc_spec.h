@@ -119,7 +119,8 @@ struct alignas(16) TreeWeigh {
   int chain;                     // of its first row block in TreeArgs::chains
 };
 constexpr int kMergeThreads = 256;
-// (token, q-head) rows up to which a sequence keeps its scores on the tensor cores.
+// (token, q-head) rows up to which a sequence keeps its scores on the tensor cores (measured
+// beside recount_mma_kernel).
 constexpr int kKeepRows = 32;
 
 struct TreeArgs {
