@@ -700,9 +700,11 @@ KVC_API int kvc_append_norm_rope(
  * appended already.  The batch is cut into n_groups runs of consecutive queries:
  * group k has h_group_sizes[k] members whose first h_prefix_lens[k] positions (a
  * whole number of pages, none longer than a member) are the same, in the pages that
- * the first member's row names; they are read once for the whole group.  A query
- * without company is a group of one, whose prefix does not matter.  Built on the host
- * and uploaded on `stream`, which must not be capturing. */
+ * the first member's row names; they are read once for the whole group where that
+ * pays (16-bit pools: from 32 MB a layer on that the batch need not read again), and
+ * from any member's row otherwise.  A query without company is a group of one, whose
+ * prefix does not matter.  Built on the host and uploaded on `stream`, which must not
+ * be capturing. */
 KVC_API int kvc_shared_plan_create(kvc_shared_plan_t** out);
 KVC_API int kvc_shared_plan_destroy(kvc_shared_plan_t* plan);
 KVC_API int kvc_plan_shared(kvc_shared_plan_t* plan, const kvc_pool_t* pool,
@@ -754,7 +756,8 @@ KVC_API int kvc_decode_tree_weights(kvc_pool_t* pool, const kvc_tree_plan_t* pla
  * share a row or a page below their length: pages that are read by others (a shared
  * prefix) must be copied first.  A row, length or page out of range is reported
  * (KVC_DEVERR_BAD_POSITION / _BAD_PAGE); a sequence with a bad row or length is left
- * alone, and its d_kept is -1. */
+ * alone, and its d_kept is -1; a bad page leaves out the rows that come from it or go
+ * there.  A layer's K must be smaller than 64 GB. */
 KVC_API int kvc_evict(kvc_pool_t* pool, const int32_t* d_block_tables, int bt_rows,
                       int bt_stride, const int32_t* d_rows, const int32_t* d_ctx_lens, int n_seqs,
                       const float* d_weights, float* d_weights_out, int weight_rows,
