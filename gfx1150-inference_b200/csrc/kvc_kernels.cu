@@ -578,6 +578,10 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
       q[kc][1] = two(kc * 16 + 8 + 2 * tig);
     }
   };
+  auto record = [&](const int4* r) {
+    if constexpr (beside) return __ldcg(r);
+    return *r;
+  };
   // One step of the background fetch of the next unit.
   auto next_step = [&]() {
     if (n_state == 0) {
@@ -590,9 +594,9 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
         return;
       }
       const int4* rec = a.sched_recs + static_cast<size_t>(n_pos) * 3;
-      n_r0 = rec[0];
-      n_r1 = rec[1];
-      n_r2 = rec[2];
+      n_r0 = record(rec);
+      n_r1 = record(rec + 1);
+      n_r2 = record(rec + 2);
       n_state = 2;
     } else if (n_state == 2) {
       load_pages(n_r0, n_r1, n_pg0, n_page0, n_page1);
@@ -622,9 +626,9 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
   // bounds the load, the count decides whether the record is used.
   if (p_pos < a.sched_cap) {
     const int4* rec = a.sched_recs + static_cast<size_t>(p_pos) * 3;
-    p_r0 = rec[0];
-    p_r1 = rec[1];
-    p_r2 = rec[2];
+    p_r0 = record(rec);
+    p_r1 = record(rec + 1);
+    p_r2 = record(rec + 2);
   }
   auto first_unit_pages = [&]() {
     if (p_pos < n_units) {

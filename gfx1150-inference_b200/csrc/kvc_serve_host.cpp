@@ -13,74 +13,69 @@
 namespace kvc {
 namespace {
 
-int norm_rope_args(const kvc_pool* pool, int layer, const void* d_q, int q_stride, void* d_q_out,
-                   int num_heads, const void* d_q_weight, const void* d_k_new, int k_stride,
-                   const void* d_k_weight, const void* d_v_new, int v_stride, float eps,
-                   const int32_t* d_bt, int bt_rows, int bt_stride, const int32_t* d_rows,
-                   const int32_t* d_positions, const int32_t* d_rope_positions, int n_axes, int n,
-                   const double* h_inv_freq, const uint8_t* h_axes, int n_pairs, NormRopeArgs* out) {
+int norm_rope_args(const kvc_pool* pool, const kvc_norm_rope_args& in, NormRopeArgs* out) {
   const PoolGeom& g = pool->g;
-  if (layer < 0 || layer >= g.num_layers)
+  if (in.layer < 0 || in.layer >= g.num_layers)
     return set_error(KVC_ERR_OUT_OF_RANGE, "layer_idx out of range for the KV pool.");
-  if (n < 0) return set_error(KVC_ERR_INVALID_ARG, "row count must be non-negative.");
-  if (n_pairs < 0 || 2 * static_cast<int64_t>(n_pairs) > g.head_dim)
+  if (in.n < 0) return set_error(KVC_ERR_INVALID_ARG, "row count must be non-negative.");
+  if (in.n_pairs < 0 || 2 * static_cast<int64_t>(in.n_pairs) > g.head_dim)
     return set_error(KVC_ERR_INVALID_ARG, "a head has at most head_dim / 2 pairs to rotate.");
-  if (n_pairs > 0 && !h_inv_freq)
+  if (in.n_pairs > 0 && !in.h_inv_freq)
     return set_error(KVC_ERR_INVALID_ARG, "the pairs' frequencies must not be null.");
-  if (n_axes < 1 || n_axes > kMaxRopeAxes)
+  if (in.n_axes < 1 || in.n_axes > kMaxRopeAxes)
     return set_error(KVC_ERR_INVALID_ARG, "axes must be in [1, %d].", kMaxRopeAxes);
-  for (int j = 0; j < n_pairs; ++j) {
-    if (!std::isfinite(h_inv_freq[j]))
+  for (int j = 0; j < in.n_pairs; ++j) {
+    if (!std::isfinite(in.h_inv_freq[j]))
       return set_error(KVC_ERR_INVALID_ARG, "the pairs' frequencies must be finite.");
-    if (h_axes && h_axes[j] >= n_axes)
+    if (in.h_axes && in.h_axes[j] >= in.n_axes)
       return set_error(KVC_ERR_INVALID_ARG, "a pair's axis is out of range.");
   }
-  if ((d_q_weight || d_k_weight) && (!(eps > 0.0f) || !std::isfinite(eps)))
+  if ((in.d_q_weight || in.d_k_weight) && (!(in.eps > 0.0f) || !std::isfinite(in.eps)))
     return set_error(KVC_ERR_INVALID_ARG, "eps must be positive.");
-  if (n == 0) return KVC_OK;
-  if (!d_k_new || !d_v_new || !d_positions)
+  if (in.n == 0) return KVC_OK;
+  if (!in.d_k_new || !in.d_v_new || !in.d_positions)
     return set_error(KVC_ERR_INVALID_ARG, "K/V rows and positions must not be null.");
-  if (d_q && (!d_q_out || num_heads <= 0))
+  if (in.d_q && (!in.d_q_out || in.num_heads <= 0))
     return set_error(KVC_ERR_INVALID_ARG, "q needs its output and a positive head count.");
-  if (int rc = check_table(d_bt, bt_rows, bt_stride)) return rc;
-  if (!aligned16(d_q) || !aligned16(d_q_out) || !aligned16(d_k_new) || !aligned16(d_v_new) ||
-      !aligned16(d_q_weight) || !aligned16(d_k_weight))
+  if (int rc = check_table(in.d_block_tables, in.bt_rows, in.bt_stride)) return rc;
+  if (!aligned16(in.d_q) || !aligned16(in.d_q_out) || !aligned16(in.d_k_new) || !aligned16(in.d_v_new) ||
+      !aligned16(in.d_q_weight) || !aligned16(in.d_k_weight))
     return set_error(KVC_ERR_INVALID_ARG, "q, K/V rows and weights must be 16-byte aligned.");
-  const int heads = d_q ? num_heads : 0;
+  const int heads = in.d_q ? in.num_heads : 0;
   const int64_t q_row = static_cast<int64_t>(heads) * g.head_dim;
   const int64_t kv_row = static_cast<int64_t>(g.num_kv_heads) * g.head_dim;
-  const int64_t qs = q_stride ? q_stride : q_row, ks = k_stride ? k_stride : kv_row;
-  const int64_t vs = v_stride ? v_stride : kv_row;
-  if ((d_q && qs < q_row) || ks < kv_row || vs < kv_row)
+  const int64_t qs = in.q_stride ? in.q_stride : q_row, ks = in.k_stride ? in.k_stride : kv_row;
+  const int64_t vs = in.v_stride ? in.v_stride : kv_row;
+  if ((in.d_q && qs < q_row) || ks < kv_row || vs < kv_row)
     return set_error(KVC_ERR_INVALID_ARG, "a token stride is smaller than its row.");
-  if ((d_q && qs * g.elem_size % 16) || ks * g.elem_size % 16 || vs * g.elem_size % 16)
+  if ((in.d_q && qs * g.elem_size % 16) || ks * g.elem_size % 16 || vs * g.elem_size % 16)
     return set_error(KVC_ERR_INVALID_ARG, "token strides must be multiples of 16 bytes.");
-  if (d_q && d_q_out == d_q && qs != q_row)
+  if (in.d_q && in.d_q_out == in.d_q && qs != q_row)
     return set_error(KVC_ERR_INVALID_ARG, "q can be rotated in place only when it is packed.");
   NormRopeArgs& a = *out;
-  if (int rc = paged_view(pool, layer, d_bt, bt_rows, bt_stride, &a.p)) return rc;
-  a.q = static_cast<const uint8_t*>(d_q);
-  a.q_out = static_cast<uint8_t*>(d_q_out);
-  a.k_new = static_cast<const uint8_t*>(d_k_new);
-  a.v_new = static_cast<const uint8_t*>(d_v_new);
-  a.q_weight = static_cast<const uint8_t*>(d_q_weight);
-  a.k_weight = static_cast<const uint8_t*>(d_k_weight);
+  if (int rc = paged_view(pool, in.layer, in.d_block_tables, in.bt_rows, in.bt_stride, &a.p)) return rc;
+  a.q = static_cast<const uint8_t*>(in.d_q);
+  a.q_out = static_cast<uint8_t*>(in.d_q_out);
+  a.k_new = static_cast<const uint8_t*>(in.d_k_new);
+  a.v_new = static_cast<const uint8_t*>(in.d_v_new);
+  a.q_weight = static_cast<const uint8_t*>(in.d_q_weight);
+  a.k_weight = static_cast<const uint8_t*>(in.d_k_weight);
   a.q_stride = static_cast<size_t>(qs) * g.elem_size;
   a.k_stride = static_cast<size_t>(ks) * g.elem_size;
   a.v_stride = static_cast<size_t>(vs) * g.elem_size;
-  a.rows = d_rows;
-  a.positions = d_positions;
+  a.rows = in.d_rows;
+  a.positions = in.d_positions;
   // (without positions of their own all axes count the slots)
-  a.rope_positions = d_rope_positions ? d_rope_positions : d_positions;
-  a.axes = d_rope_positions ? n_axes : 1;
-  a.n = n;
+  a.rope_positions = in.d_rope_positions ? in.d_rope_positions : in.d_positions;
+  a.axes = in.d_rope_positions ? in.n_axes : 1;
+  a.n = in.n;
   a.num_heads = heads;
   a.head_dim = g.head_dim;
-  a.pairs = n_pairs;
-  a.eps = eps;
-  for (int j = 0; j < n_pairs; ++j) {
-    a.turns[j] = h_inv_freq[j] / 6.283185307179586476925286766559;
-    a.axis[j] = d_rope_positions && h_axes ? h_axes[j] : 0;
+  a.pairs = in.n_pairs;
+  a.eps = in.eps;
+  for (int j = 0; j < in.n_pairs; ++j) {
+    a.turns[j] = in.h_inv_freq[j] / 6.283185307179586476925286766559;
+    a.axis[j] = in.d_rope_positions && in.h_axes ? in.h_axes[j] : 0;
   }
   return KVC_OK;
 }
@@ -331,25 +326,15 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
 
 using namespace kvc;
 
-extern "C" int kvc_append_norm_rope(
-    kvc_pool_t* pool, int layer, const void* d_q, int q_stride, void* d_q_out, int num_heads,
-    const void* d_q_weight, const void* d_k_new, int k_stride, const void* d_k_weight,
-    const void* d_v_new, int v_stride, float eps, const int32_t* d_block_tables, int bt_rows,
-    int bt_stride, const int32_t* d_rows, const int32_t* d_positions,
-    const int32_t* d_rope_positions, int n_axes, int n, const double* h_inv_freq,
-    const uint8_t* h_axes, int n_pairs, int neox, void* stream) {
-  if (!pool) return set_error(KVC_ERR_INVALID_ARG, "pool must not be null.");
+extern "C" int kvc_append_norm_rope(kvc_pool_t* pool, const kvc_norm_rope_args_t* args, void* stream) {
+  if (!pool || !args) return set_error(KVC_ERR_INVALID_ARG, "pool and arguments must not be null.");
   return guarded("kvc_append_norm_rope", [&]() -> int {
     DeviceScope dev(pool->device);
     if (dev.rc()) return dev.rc();
     NormRopeArgs a = {};
-    if (int rc = norm_rope_args(pool, layer, d_q, q_stride, d_q_out, num_heads, d_q_weight, d_k_new,
-                                k_stride, d_k_weight, d_v_new, v_stride, eps, d_block_tables, bt_rows,
-                                bt_stride, d_rows, d_positions, d_rope_positions, n_axes, n,
-                                h_inv_freq, h_axes, n_pairs, &a))
-      return rc;
-    if (n == 0) return KVC_OK;
-    const cudaError_t e = launch_norm_rope(a, pool->g.dtype, neox != 0, sms_of(pool->device),
+    if (int rc = norm_rope_args(pool, *args, &a)) return rc;
+    if (args->n == 0) return KVC_OK;
+    const cudaError_t e = launch_norm_rope(a, pool->g.dtype, args->neox != 0, sms_of(pool->device),
                                            static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? KVC_OK : cuda_error(e, "append + norm + rope kernel");
   });

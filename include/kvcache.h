@@ -673,27 +673,45 @@ KVC_API int kvc_reorder_beams(kvc_pool_t* pool, int32_t* d_block_tables, int bt_
 
 typedef struct kvc_shared_plan kvc_shared_plan_t;
 
+/* The arguments of kvc_append_norm_rope; what is not named is 0 or NULL. */
+typedef struct kvc_norm_rope_args {
+  const void* d_q;                 /* (n, num_heads, head_dim), or NULL */
+  void* d_q_out;                   /* the same shape, packed; may be d_q when that is */
+  const void* d_q_weight;          /* (head_dim) in the pool's type, or NULL */
+  const void* d_k_new;             /* (n, num_kv_heads, head_dim) */
+  const void* d_k_weight;
+  const void* d_v_new;
+  const int32_t* d_block_tables;   /* (bt_rows, bt_stride) */
+  const int32_t* d_rows;           /* (n), or NULL: row 0 */
+  const int32_t* d_positions;      /* (n) slots; negative: padding */
+  const int32_t* d_rope_positions; /* (n, n_axes), or NULL: the slots, on every axis */
+  const double* h_inv_freq;        /* (n_pairs) host */
+  const uint8_t* h_axes;           /* (n_pairs) host, or NULL: axis 0 */
+  int layer;
+  int num_heads;
+  int q_stride, k_stride, v_stride; /* elements between tokens, 0: packed */
+  int bt_rows, bt_stride;
+  int n;
+  int n_axes;                      /* 1 ... KVC_MAX_ROPE_AXES */
+  int n_pairs;
+  int neox;
+  float eps;
+} kvc_norm_rope_args_t;
+
 /* Normalises, rotates and appends n tokens in one pass: K row = R(N(d_k_new[i])) and
- * V row = d_v_new[i] at slot d_positions[i] of block-table row d_rows[i] (NULL: row
- * 0), and, when d_q is given, d_q_out[i] = R(N(d_q[i])).
+ * V row = d_v_new[i] at slot d_positions[i] of block-table row d_rows[i], and, when
+ * d_q is given, d_q_out[i] = R(N(d_q[i])).
  * N, per head: x * w / sqrt(mean(x^2) + eps) over the head_dim values, w = d_q_weight
- * or d_k_weight, (head_dim) in the pool's type; NULL leaves that tensor as it is.
- * R, per head: pair j < n_pairs is turned by p_a * h_inv_freq[j], a = h_axes[j]
- * (NULL: 0) and p_a = d_rope_positions[i * n_axes + a]; without d_rope_positions
- * every axis counts d_positions[i].  Pair j is dims (j, j + n_pairs) if neox, else
- * (2 j, 2 j + 1); dims from 2 n_pairs on are not rotated, and n_pairs 0 rotates
- * nothing.  h_inv_freq and h_axes are host memory, read before the call returns.
+ * or d_k_weight; without it that tensor stays as it is.
+ * R, per head: pair j < n_pairs is turned by p_a * h_inv_freq[j], a = h_axes[j] and
+ * p_a = d_rope_positions[i * n_axes + a].  Pair j is dims (j, j + n_pairs) if neox,
+ * else (2 j, 2 j + 1); dims from 2 n_pairs on are not rotated, and n_pairs 0 rotates
+ * nothing.  Host memory is read before the call returns.
  * Angles are reduced in 64 bits and so exact at any position; norm and rotation are
  * in 32 bits (a head whose squares pass 3.4e38 in sum becomes zero), rounded once to
  * the pool's type.  Strides, padding, errors and alignment as in kvc_append_rope; eps
- * must be positive. */
-KVC_API int kvc_append_norm_rope(
-    kvc_pool_t* pool, int layer, const void* d_q, int q_stride, void* d_q_out, int num_heads,
-    const void* d_q_weight, const void* d_k_new, int k_stride, const void* d_k_weight,
-    const void* d_v_new, int v_stride, float eps, const int32_t* d_block_tables, int bt_rows,
-    int bt_stride, const int32_t* d_rows, const int32_t* d_positions,
-    const int32_t* d_rope_positions, int n_axes, int n, const double* h_inv_freq,
-    const uint8_t* h_axes, int n_pairs, int neox, void* stream);
+ * must be positive where a weight is given. */
+KVC_API int kvc_append_norm_rope(kvc_pool_t* pool, const kvc_norm_rope_args_t* args, void* stream);
 
 /* The work list of one decode step, used by all its layers.  Query i attends over
  * positions [0, h_lens[i]) of block-table row h_rows[i] (NULL: row i), its own row

@@ -349,11 +349,13 @@ def test_refusals():
                                     (1, 1, None, None)):
         f = None if freq is None else np.array(freq)
         x = None if axis is None else np.array(axis, dtype=np.uint8)
-        rc = ffi.lib.kvc_append_norm_rope(
-            pool.handle, 0, None, 0, None, 0, None, k.data_ptr(), 0, None, k.data_ptr(), 0, 1e-6,
-            bt.data_ptr(), 2, 2, None, pos.data_ptr(), None, axes, 3, ffi.np_ptr(f), ffi.np_ptr(x), pairs,
-            1, None)
-        assert rc == ffi.KVC_ERR_INVALID_ARG
+        args = ffi.NORM_ROPE_ARGS.pack(
+            0, 0, 0, k.data_ptr(), 0, k.data_ptr(), bt.data_ptr(), 0, pos.data_ptr(), 0,
+            ffi.np_ptr(f) or 0, ffi.np_ptr(x) or 0, 0, 0, 0, 0, 0, 2, 2, 3, axes, pairs, 1, 1e-6)
+        assert ffi.lib.kvc_append_norm_rope(pool.handle, args, None) == ffi.KVC_ERR_INVALID_ARG
+    assert ffi.lib.kvc_append_norm_rope(pool.handle, None, None) == ffi.KVC_ERR_INVALID_ARG
+    with pytest.raises(ValueError, match="32 bits"):
+        norm(layer=1 << 40)
 
     for bad in (([20, 20], [2], [8]), ([20, 20], [2], [32]), ([20, 20], [1], [16]), ([20], [1, 1], [0, 0]),
                 ([20], [0], [0]), ([20], [1], [-16]), ([-1], [1], [0]), ([20], [-1], [0])):

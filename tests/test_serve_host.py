@@ -69,9 +69,9 @@ def test_unbuilt_handles_and_null_pools():
     assert ffi.lib.kvc_decode_shared(None, None, 0, None, None, None, 1, 1.0, None) == none
     assert ffi.lib.kvc_decode_tree_weights(None, None, 0, None, None, 0, None, 1, 1, None, None, 1,
                                            1.0, None) == none
-    assert ffi.lib.kvc_append_norm_rope(None, 0, None, 0, None, 0, None, None, 0, None, None, 0, 1e-6,
-                                        None, 1, 1, None, None, None, 1, 0, None, None, 0, 0,
-                                        None) == none
+    args = ffi.NORM_ROPE_ARGS.pack(*[0] * 12, *[0] * 11, 1e-6)
+    assert len(args) == 12 * 8 + 11 * 4 + 4
+    assert ffi.lib.kvc_append_norm_rope(None, args, None) == none
     assert ffi.lib.kvc_evict(None, None, 1, 1, None, None, 1, None, None, 1, 1, 1, 0, None,
                              None) == none
     h = ctypes.c_void_p()
