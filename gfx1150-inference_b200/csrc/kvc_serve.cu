@@ -18,39 +18,35 @@ namespace {
 
 // =====================================================================================
 // Norm + rotate + append.  y = R(p) (x w / sqrt(mean(x^2) + eps)) for the heads of q and K,
-// V as it is.  kPer threads take a token: its angles are computed once and serve all its
+// V as it is.  A CTA takes a token: its angles are computed once and serve all its
 // heads (turns in 64 bits with the whole ones removed, then sincospif, as append_rope_kernel
 // does), each pair with the position of its own axis.  A head belongs to kLanes lanes of one
 // warp, each of which owns two 16-byte units that hold each other's pairs, so the sum of
 // squares is a few shuffles and the head is read once.  All in 32 bits, rounded once.
 //
 // Bound by memory traffic and by how many heads are on their way: 8,626 tokens of 32 + 8 + 8
-// heads of 128 dims, fp16, three axes, 50 us for 212 MB (32 at the copy rate; append_rope_kernel
-// 45).  An SM takes four CTAs, which weights and angles in registers do not leave room for
-// (104 registers, two CTAs: 65 us; three heads a lane group on their way: 60); three CTAs 52.
+// heads of 128 dims, fp16, three axes, 43.8 us for 212 MB (32 at the copy rate; append_rope_kernel
+// 45); two heads of a lane group on their way 47.4, four 47.3.  An SM takes 1,024 threads (768:
+// 47.4), which weights and angles in registers do not leave room for.
 // =====================================================================================
 constexpr int kNormThreads = 256;
-constexpr int kNormBatch = 2;      // heads of a lane group on their way
+constexpr int kNormBatch = 3;      // heads of a lane group on their way
 
-template <typename T, bool kNeox, int kPer, int kLanes>
-__global__ void __launch_bounds__(kNormThreads, 4) norm_rope_kernel(const NormRopeArgs a) {
-  constexpr int kTok = kNormThreads / kPer, kAtOnce = kPer / kLanes;
-  constexpr int N = Unit<T>::N;
-  __shared__ float4 cs[kTok * kMaxRopePairs / 2];    // two pairs' (cos, sin)
+template <typename T, bool kNeox, int kThreads, int kLanes>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) norm_rope_kernel(const NormRopeArgs a) {
+  constexpr int kAtOnce = kThreads / kLanes, N = Unit<T>::N;
+  __shared__ float4 cs[kMaxRopePairs / 2];    // two pairs' (cos, sin)
   __shared__ uint4 s_weight[2][2 * kLanes];
-  __shared__ int s_page[kTok], s_slot[kTok];
-  const int tok0 = blockIdx.x * kTok;
-  const int toks = min(kTok, a.n - tok0);
+  __shared__ int s_page;
   const int U = a.p.row_units, Hkv = a.p.num_kv_heads, H = a.num_heads;
   const int heads = H + 2 * Hkv;                     // q, K and V heads
-  const int tok = threadIdx.x / kPer, me = threadIdx.x % kPer;
-  const int row0 = me / kLanes, i = me % kLanes;     // first head, unit pair
-  const bool works = i < U / 2 && tok < toks;
+  const int row0 = threadIdx.x / kLanes, i = threadIdx.x % kLanes;   // first head, unit pair
+  const bool works = i < U / 2;
   const int turned = a.pairs / N;                    // unit pairs that are rotated
   const bool turns = i < turned;
   // the rotated front of a NeoX head: units i and i + turned; neighbours otherwise
   const int u0 = kNeox && turns ? i : 2 * i, du = kNeox && turns ? turned : 1;
-  const size_t t = tok0 + tok;
+  const size_t t = blockIdx.x;
   const size_t row_bytes = static_cast<size_t>(U) * 16;
   wait_prerequisites();
 
@@ -76,33 +72,27 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_rope_kernel(const NormRo
   for (int k = 0; k < kNormBatch; ++k) load(row0 + k * kAtOnce, items[k]);
   // (weights and angles are read where they are used: in registers they would leave an SM
   // room for fewer CTAs)
-  for (int x = threadIdx.x; x < 2 * U; x += kNormThreads) {
+  for (int x = threadIdx.x; x < 2 * U; x += kThreads) {
     const int k = x >= U, u = x - k * U;
     const uint8_t* w = k ? a.k_weight : a.q_weight;
     if (w) s_weight[k][u] = *reinterpret_cast<const uint4*>(w + u * 16);
   }
-  for (int x = threadIdx.x; x < toks * a.pairs; x += kNormThreads) {
-    const int tk = kTok == 1 ? 0 : x / a.pairs, j = x - tk * a.pairs;
-    double turn = static_cast<double>(a.rope_positions[static_cast<size_t>(tok0 + tk) * a.axes +
-                                                       a.axis[j]]) * a.turns[j];
+  for (int j = threadIdx.x; j < a.pairs; j += kThreads) {
+    double turn = static_cast<double>(a.rope_positions[t * a.axes + a.axis[j]]) * a.turns[j];
     turn -= rint(turn);
     // (by pairs of a unit pair, then unit pair: neighbouring threads read neighbouring angles)
     const int k = j % N;
-    float2& out = reinterpret_cast<float2*>(cs + tk * kMaxRopePairs / 2 + k / 2 * turned + j / N)[k & 1];
+    float2& out = reinterpret_cast<float2*>(cs + k / 2 * turned + j / N)[k & 1];
     sincospif(2.0f * static_cast<float>(turn), &out.y, &out.x);
   }
-  if (threadIdx.x < toks) {
-    const int pos = a.positions[tok0 + threadIdx.x];
-    s_page[threadIdx.x] = pos < 0 ? -1 : page_of(a.p, a.rows ? a.rows[tok0 + threadIdx.x] : 0, pos);
-    s_slot[threadIdx.x] = pos < 0 ? 0 : pos % a.p.page_size;
-  }
+  const int pos = a.positions[t];
+  if (threadIdx.x == 0) s_page = pos < 0 ? -1 : page_of(a.p, a.rows ? a.rows[t] : 0, pos);
   __syncthreads();
-  if (tok >= toks) return;                           // (a warp has one token)
-  const int page = s_page[tok];
+  const int page = s_page;
   if (page < 0) return;                              // padding, or reported
-  const float4* angles = cs + tok * kMaxRopePairs / 2 + i;
+  const float4* angles = cs + i;
   uint8_t* q_dst = a.q_out + t * H * row_bytes + u0 * 16;
-  const size_t place = unit_at(a.p, page, 0, s_slot[tok], u0);
+  const size_t place = unit_at(a.p, page, 0, pos % a.p.page_size, u0);
   const int dp = du * (a.p.layout == kLayoutCore ? 128 : 16);
   const float inv_d = 1.0f / a.head_dim;
   const int last = heads - 1;
@@ -264,11 +254,12 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_any_kernel(const NormR
   }
 }
 
-// Many tokens: 64 threads each, four in a CTA; few tokens: a CTA each.
+// Many tokens: 64 threads each (8,626 tokens, two heads on their way: 47.6 us; 32: 53, with
+// two or four tokens in a CTA, which wait for one another's angles, 48.3 and 49.9); few: 256.
 template <typename T, bool kNeox, int kLanes>
 cudaError_t run_norm_rope(const NormRopeArgs& a, int sms, cudaStream_t s) {
   if (a.n >= 4 * sms)
-    return launch_early(norm_rope_kernel<T, kNeox, 64, kLanes>, dim3((a.n + 3) / 4), kNormThreads, 0, s, a);
+    return launch_early(norm_rope_kernel<T, kNeox, 64, kLanes>, dim3(a.n), 64, 0, s, a);
   return launch_early(norm_rope_kernel<T, kNeox, kNormThreads, kLanes>, dim3(a.n), kNormThreads, 0, s, a);
 }
 
