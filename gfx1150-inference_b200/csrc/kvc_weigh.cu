@@ -185,7 +185,6 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);          // K, the two warpgroups' products
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + 64);
-  volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(smem + 68);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wg = warp >> 2, wt = tid & 127, ww = warp & 3;     // warpgroup; thread and warp in it
   float* s_shift = reinterpret_cast<float*>(smem + 1024) + wg * kRecountRows;
@@ -200,7 +199,6 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) mbar_init(bar0 + 8 * i, 1);
     fence_mbar_init();
-    *s_abort = 0;
   }
   wait_prerequisites();
   launch_dependents();
@@ -255,16 +253,28 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
     s_shift[wt] = e.y == 0.f ? INFINITY : e.x + log2f(e.y);     // (infinity: no weight)
     if (edge) s_vis[wt] = make_uint4(vis[0], vis[1], vis[2], vis[3]);
   };
+  bool failed = false;
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (!mbar_wait_bounded(bar, parity)) {
       report_error_at(a.p.err, KVC_DEVERR_WAIT_LIMIT, blockIdx.x);
-      *s_abort = 1;
+      failed = true;
     }
   };
-  auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory"); };
+  // A barrier of the warpgroup; true if a wait of any of its threads gave up (all get the same
+  // answer, so all leave the loop at the same barrier).
+  auto group_failed = [&]() {
+    uint32_t any;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, %2, 128, p;\n"
+        " selp.b32 %0, 1, 0, q;\n}"
+        : "=r"(any)
+        : "r"(static_cast<uint32_t>(failed)), "r"(1 + wg)
+        : "memory");
+    return any != 0;
+  };
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   const float2 sc = make_float2(a.scale_log2, a.scale_log2);   // (q as it is, whatever the sign)
-  bool issued = false;
+  int issued = 0;
   float2 next = make_float2(0.f, 0.f);
   if (wg < blocks) {
     copy_q(wg);
@@ -276,9 +286,9 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
     copy_async_wait();
     fence_proxy_async();
     tmem_fence_before();
-    group_sync();                      // the block is here, and the last one's sums are made
+    const bool stop = group_failed();  // the block is here, and the last one's sums are made
     tmem_fence_after();
-    if (*s_abort) break;
+    if (stop) break;
     if (ww == 0 && elect_one()) {
       constexpr uint32_t kDesc = mma_desc<T>(128, kRecountRows, false);
       const uint64_t kd = operand_desc(smem_u32(k_mem), 128, U * 128);
@@ -288,7 +298,7 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
       mma_commit(done);
     }
     __syncwarp();
-    issued = true;
+    ++issued;
     if (b + 2 < blocks) next = statistics(b + 2);
     wait(done, n & 1);
     tmem_fence_after();
@@ -333,24 +343,23 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
       }
     }
     tmem_fence_before();
-    group_sync();                      // the shifts have been read by all
-    if (*s_abort) break;
+    if (group_failed()) break;         // the shifts have been read by all
   }
   copy_async_wait();
   float* s_sum = reinterpret_cast<float*>(smem + 1024) + kRecountRows;   // (the second group's shifts)
   const float add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
   if (wg == 1) s_sum[wt] = add;
   tmem_fence_before();
-  __syncthreads();
+  const bool stopped = __syncthreads_or(failed);
   const int p = p0 + wt;
-  if (wg == 0 && p < end && !*s_abort) {
+  if (wg == 0 && p < end && !stopped) {
     float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
     const float total = add + s_sum[wt];
     *out = p < w.ctx ? *out + total : total;
   }
-  if (*s_abort && wt == 0) {           // what is in flight lands before the memory goes
+  if (stopped && wt == 0) {            // what is in flight lands before the memory goes
     mbar_wait_bounded(bar0, 0);
-    if (issued) mbar_wait_bounded(done, 0);
+    if (issued > 0) mbar_wait_bounded(done, (issued - 1) & 1);
   }
   __syncthreads();
   tmem_fence_after();
