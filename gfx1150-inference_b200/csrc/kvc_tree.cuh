@@ -49,12 +49,12 @@ __device__ __forceinline__ uint32_t mask_word(const TreeArgs& a, const TreeSeg& 
 }
 
 // Copies (token, q-head) rows of one KV head into RowBlocks: rows row0 ... row0 + live - 1 of
-// the list to places 0 ..., then zeros up to place n (a multiple of 8).  Places from 128 on go
-// `second` bytes further; with `twin` every row goes there, too.  Warp w of `warps` takes its
-// eighths of rows; q is that of the list's first token and the KV head's first q-head.  What a
-// row needs is carried along: with a division, or a handful of instructions more, one warp's
-// copies of 256 rows take 3 us.
-template <typename T, int D>
+// the list to places 0 ..., then zeros (kRepeat: the list's first row) up to place n (a
+// multiple of 8).  Places from 128 on go `second` bytes further; with `twin` every row goes
+// there, too.  Warp w of `warps` takes its eighths of rows; q is that of the list's first token
+// and the KV head's first q-head.  What a row needs is carried along: with a division, or a
+// handful of instructions more, one warp's copies of 256 rows take 3 us.
+template <typename T, int D, bool kRepeat = false>
 __device__ __forceinline__ void copy_rows(uint32_t dst, uint32_t second, bool twin, const T* q, int row0,
                                           int live, int n, int group, int row_step, int w, int warps,
                                           int lane) {
@@ -78,8 +78,9 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, uint32_t second, bool tw
     const uint32_t at = (g0 & 127) * (R::kChunk * 2) + (g0 >= 128 ? second : 0u);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const uint32_t bytes = g0 + s * R::kRowsPer + rr < live ? 16 : 0;
-      const T* from = bytes ? src[s] : q;
+      const bool here = g0 + s * R::kRowsPer + rr < live;
+      const uint32_t bytes = here || kRepeat ? 16 : 0;
+      const T* from = here ? src[s] : kRepeat ? q + piece * 8 : q;
 #pragma unroll
       for (int i = 0; i < D / R::kChunk; ++i) {
         copy16_async(off[s] + at + i * R::kBytes, from + i * R::kChunk, bytes);

@@ -221,10 +221,11 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
       bulk_g2s(smem_u32(k_mem) + lane * kSlabBytes, src, kSlabBytes, bar0, l2_policy_evict_first());
     }
   }
-  // Block b's rows of Q, zero behind the last.
+  // Block b's rows of Q, and the first one again behind the last (its scores are taken back by
+  // the shift; with zeros there, an infinite key would leave what is not a number).
   using R = RowBlocks<D>;
   auto copy_q = [&](int b) {
-    copy_rows<T, D>(smem_u32(q_mem), 0u, false,
+    copy_rows<T, D, true>(smem_u32(q_mem), 0u, false,
                     reinterpret_cast<const T*>(a.q) +
                         (static_cast<size_t>(w.tok0) * a.num_heads + w.kvh * a.group) * D,
                     b * kRecountRows, rows - b * kRecountRows, kRecountRows, a.group, a.num_heads * D, ww, 4,

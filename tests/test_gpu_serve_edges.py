@@ -21,7 +21,7 @@ if HAS_GPU:
     import paged
 
 from test_gpu_serve_ops import attend64, check, evict_case, keep64, norm_case, shared_case, weigh_case
-from test_gpu_spec_ops import BF16, F16, F32, dev, make_pool, no_error, raw
+from test_gpu_spec_ops import BF16, F16, F32, dev, make_pool, no_error, raw, tables
 
 # -- prefixes that are shared (more than 32 MB a layer saved) -------------------------------------
 LARGE = [
@@ -317,6 +317,40 @@ def test_odd_slots_and_layer_slices_of_weights(dtype):
         total = w.double().sum(-1)                       # every row's weights add up to one
         assert float((total - 2 * nodes).abs().max()) <= 2 * nodes * 2.0 ** -14
         assert torch.all(w[..., 600 + nodes:] == 0)
+
+
+@pytest.mark.parametrize("nodes", [1, 20, 45])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_an_infinite_key_has_no_weight(dtype, nodes):
+    """A key whose scores are all minus infinity gets the weight zero, and the others what they
+    have without it (tokens of 4 q-heads: 4, 80 and 180 rows)."""
+    ctx, d, h, hkv, ps, at = 300, 64, 8, 2, 16, 5
+    n = ctx + nodes
+    g = torch.Generator(device="cuda")
+    g.manual_seed(nodes)
+    dt = getattr(torch, dtype)
+    bt, total = tables([-(-n // ps)], 1)
+    pool = make_pool(1, total, ps, hkv, d, dtype)
+    k, v = (torch.randn(n, hkv, d, generator=g, device="cuda").to(dt) for _ in range(2))
+    q = torch.randn(nodes, h, d, generator=g, device="cuda").to(dt)
+    q[:, :, 0] = 1.0
+    vis = torch.ones(nodes, n, dtype=torch.bool, device="cuda").tril(ctx)
+    vis[:, at] = False
+    ref, tol, wt, rel = attend64(q, k, v, 1.0 / math.sqrt(d), dtype, vis)
+    want = wt.view(nodes, hkv, -1, n).sum((0, 2))
+    wtol = (wt * rel).view(nodes, hkv, -1, n).sum((0, 2)) + \
+        (nodes * h // hkv + 4) * 2.0 ** -24 * want + 1e-30
+    k[at, :, 0] = -math.inf
+    pool.append(0, k, v, bt, torch.arange(n, dtype=torch.int32, device="cuda"),
+                torch.zeros(n, dtype=torch.int32, device="cuda"))
+    weights = torch.zeros(1, hkv, n, device="cuda")
+    out = torch.zeros_like(q)
+    pool.decode_tree_weights(pool.plan_tree([ctx], [nodes], h, weights=True), 0, q, None, weights, out, bt,
+                             1.0 / math.sqrt(d))
+    no_error()
+    assert torch.all(weights[0, :, at] == 0.0)
+    check(weights[0], want, wtol)
+    check(out, ref, tol)
 
 
 # -- refusals ---------------------------------------------------------------------------------------------
