@@ -486,7 +486,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
   cut_runs(runs, tile, sms, p->keep_scores, &segs, &cta_segs);
   // Single tokens whose weights are wanted: the decode kernel streams K and V faster for a
   // token's few rows (32 x 1 at 1K-8K, fp16: 92 us, 105 with the kernel for trees) and keeps
-  // scores at less cost (95, 125).  The pieces above serve calls with a mask.
+  // scores at less cost (98, 125).  The pieces above serve calls with a mask.
   UnitList units;
   std::vector<SharedJoin> joins;
   std::vector<int> score_base;
