@@ -252,7 +252,13 @@ class Rotation:
       ``freq_base^(-i / pairs of the axis)`` for its i-th pair.
 
     ``inv_freq`` (rotary_dim / 2 numbers) replaces the frequencies, for stretched or scaled
-    ones.  ``neox``: pair j is dims j and j + rotary_dim / 2, else 2j and 2j + 1."""
+    ones.  ``neox``: pair j is dims j and j + rotary_dim / 2, else 2j and 2j + 1.
+
+    A rotation does not change: calls hand the addresses of its tables to the library, so
+    its attributes cannot be set, and a copy (or a pickle) has tables of its own."""
+
+    _TABLES = ("rotary_dim", "pairs", "axes", "neox", "inv_freq", "axis", "_args")
+    __slots__ = _TABLES + ("__dict__", "__weakref__")
 
     def __init__(self, rotary_dim: int, freq_base: float = 10000.0,
                  sections: Optional[Sequence[int]] = None, order: str = "blocks",
@@ -283,13 +289,38 @@ class Rotation:
             inv = np.asarray(inv_freq, dtype=np.float64)
             if inv.shape != (half,) or not np.all(np.isfinite(inv)):
                 raise ValueError(f"inv_freq must be {half} finite numbers")
-        self.rotary_dim, self.pairs, self.axes, self.neox = rotary_dim, half, len(sec), bool(neox)
-        self.inv_freq = np.array(inv, dtype=np.float64)
-        self.axis = np.array(axis, dtype=np.uint8)
-        self.inv_freq.setflags(write=False)
-        self.axis.setflags(write=False)
-        # what a call hands to the library (looked up once: it takes as long as the launch)
-        self._args = (ffi.np_ptr(self.inv_freq), ffi.np_ptr(self.axis), half, 1 if neox else 0)
+        self._hold(inv, axis, len(sec), neox)
+
+    def _hold(self, inv_freq, axis, axes: int, neox: bool):
+        inv_freq, axis = np.array(inv_freq, dtype=np.float64), np.array(axis, dtype=np.uint8)
+        inv_freq.setflags(write=False)
+        axis.setflags(write=False)
+        pairs = inv_freq.size
+        for name, value in (
+                ("rotary_dim", 2 * pairs), ("pairs", pairs), ("axes", axes), ("neox", bool(neox)),
+                ("inv_freq", inv_freq), ("axis", axis),
+                # what a call hands to the library (looked up once: it takes as long as the launch)
+                ("_args", (ffi.np_ptr(inv_freq), ffi.np_ptr(axis), pairs, 1 if neox else 0))):
+            object.__setattr__(self, name, value)
+        return self
+
+    def __setattr__(self, name, value):
+        if name in self._TABLES:
+            raise AttributeError(f"{name} of a Rotation does not change: make another one.")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        if name in self._TABLES:
+            raise AttributeError(f"{name} of a Rotation does not change: make another one.")
+        object.__delattr__(self, name)
+
+    def __reduce__(self):      # copies and pickles; addresses are of this object's tables only
+        return (_held, (type(self), self.inv_freq, self.axis, self.axes, self.neox),
+                self.__dict__ or None)
+
+
+def _held(cls, *tables) -> Rotation:
+    return cls.__new__(cls)._hold(*tables)
 
 
 class PagedKVCache:
