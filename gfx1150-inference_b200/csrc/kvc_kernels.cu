@@ -901,7 +901,17 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
       if (lane == 0) fence_proxy_async();
       p_issue();
     }
+    const int t0 = 2 * tig;
     if (!have) {
+      if constexpr (kMode == kKeepScores) {
+        // A page out of range: its positions take no part, and get no weight.  (What an earlier
+        // call kept in their place would be added to the sums.)
+        if (gid < c_r2.w) {
+          const float2 none = make_float2(-INFINITY, -INFINITY);
+          *reinterpret_cast<float2*>(score_row + j * kSlab + t0) = none;
+          *reinterpret_cast<float2*>(score_row + j * kSlab + t0 + 8) = none;
+        }
+      }
       if constexpr (!kAllFragsFirst) {
         __syncwarp();
         ++consumed;
@@ -911,7 +921,6 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
       continue;
     }
 
-    const int t0 = 2 * tig;
     const bool v0 = t0 < valid, v1 = t0 + 1 < valid, v2 = t0 + 8 < valid, v3 = t0 + 9 < valid;
     const float x0 = (sc[0][0][0] + sc[0][1][0]) * a.scale_log2;
     const float x1 = (sc[0][0][1] + sc[0][1][1]) * a.scale_log2;

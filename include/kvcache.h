@@ -752,7 +752,10 @@ KVC_API int kvc_tree_plan_set_weights(kvc_tree_plan_t* plan, int on);
  * tokens, [ctx, ctx + nodes), are set to that sum instead.  Other slots and rows stay
  * as they were.  The weights are in 32 bits, not rounded to the pool's type, and the
  * rows are added in order, so a call repeats bit by bit.  The plan needs
- * kvc_tree_plan_set_weights before its build; its score buffer, too, is its own. */
+ * kvc_tree_plan_set_weights before its build; its score buffer, too, is its own.
+ * A page out of range is reported (KVC_DEVERR_BAD_PAGE) and harms no other sequence:
+ * where a sequence has a single token, 16-bit pools without a mask leave its positions
+ * out, without weight; the other forms read page 0 in its place. */
 KVC_API int kvc_decode_tree_weights(kvc_pool_t* pool, const kvc_tree_plan_t* plan, int layer,
                                     const void* d_q, const int32_t* d_mask, int mask_words,
                                     float* d_weights, int weight_rows, int weight_slots,
