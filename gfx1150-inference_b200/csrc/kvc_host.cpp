@@ -87,7 +87,7 @@ int wait_event(cudaEvent_t ev, const char* what) {
 
 // ---- host-side fault injection (kvc_test_inject_failure) ----------------------
 namespace {
-constexpr int kFaultSites = 5;
+constexpr int kFaultSites = 6;
 std::mutex g_fault_mu;
 int g_fault_skip[kFaultSites] = {};
 int g_fault_count[kFaultSites] = {};

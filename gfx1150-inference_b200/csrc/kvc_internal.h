@@ -205,6 +205,7 @@ struct DecodeArgs {
   float* scores = nullptr;
   const int* score_base = nullptr;
   float2* row_ml = nullptr;
+  unsigned int* gave_up = nullptr;   // set where a wait gave up: the scores are not all there
 };
 // Slots of the plan's device header (int32).
 constexpr int kHdrUnits = 0;

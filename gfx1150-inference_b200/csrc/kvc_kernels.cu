@@ -784,6 +784,9 @@ __global__ void __launch_bounds__(NW * 32, kPersistCtasPerSm)
     const bool ok = mbar_wait_bounded(smem_u32(&bars[s]), static_cast<uint32_t>(consumed / NS) & 1u);
     if (__any_sync(0xffffffffu, !ok)) {
       if (lane == 0) report_error(2u /*KVC_DEVERR_WAIT_LIMIT*/, static_cast<uint32_t>(consumed));
+      if constexpr (kMode == kKeepScores) {
+        if (lane == 0) atomicExch(a.gave_up, 1u);
+      }
       dead = true;
       break;
     }

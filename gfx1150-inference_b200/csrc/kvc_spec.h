@@ -147,6 +147,7 @@ struct TreeArgs {
   // Attention that adds its weights up (null otherwise): where the sums go, (table rows, KV
   // heads, weight_slots), every row's final (max, sum), and kept raw scores.
   float* weights;
+  unsigned int* gave_up;         // set where a wait gave up: no weights until the plan is built again
   float2* row_ml;                // (tokens, H)
   float* scores;
   const TreeWeigh* weighs;       // those with kept scores, then those without
@@ -371,6 +372,7 @@ struct kvc_tree_plan {
   // Work on the decode kernel: unit records and their counter, and the joins of its splits
   const int4* dev_units = nullptr;
   unsigned int* dev_queue = nullptr;
+  unsigned int* dev_gave_up = nullptr;   // TreeArgs::gave_up
   const kvc::SharedJoin* dev_joins = nullptr;
   const int* dev_score_base = nullptr;
   int n_units = 0, n_unit_ctas = 0, n_joins = 0;

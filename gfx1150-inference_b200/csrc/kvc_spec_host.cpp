@@ -194,6 +194,7 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
     a.chain_rows = plan->tile.rows;
     a.n_recounts = plan->n_recounts;
     a.weights = d_weights;
+    a.gave_up = plan->dev_gave_up;
     a.weight_slots = weight_slots;
     // (the tensor cores' kernel takes the scale's sign into q)
     a.score_scale = plan->tile.tensor ? std::fabs(a.scale_log2) : a.scale_log2;
@@ -202,6 +203,7 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
       d.scores = a.scores;
       d.score_base = plan->dev_score_base;
       d.row_ml = a.row_ml;
+      d.gave_up = a.gave_up;
       a.joins = plan->dev_joins;
       a.n_joins = plan->n_joins;
       a.own_o = d.part_o;
@@ -586,7 +588,7 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
     }
     chains.insert(chains.end(), units.splits.begin(), units.splits.end());
   }
-  const unsigned int zero = 0;
+  const unsigned int zero = 0, gave_up = injected_failure(KVC_FAULT_KERNEL_WAIT);
   const PlanPart parts[] = {{segs.data(), sizeof(TreeSeg) * segs.size()},
                             {cta_segs.data(), sizeof(int) * cta_segs.size()},
                             {merges.data(), sizeof(TreeMerge) * merges.size()},
@@ -597,9 +599,11 @@ int tree_build(kvc_tree_plan* p, const kvc_pool* pool, const int32_t* h_rows,
                             {units.recs.data(), sizeof(int4) * units.recs.size()},
                             {score_base.data(), sizeof(int) * score_base.size()},
                             {&zero, sizeof(zero)},
-                            {chains.data(), sizeof(JoinPieces) * chains.size()}};
-  const uint8_t* d[11];
-  if (const int rc = upload_plan(p, parts, 11, d, s)) return rc;
+                            {chains.data(), sizeof(JoinPieces) * chains.size()},
+                            {&gave_up, sizeof(gave_up)}};
+  const uint8_t* d[12];
+  if (const int rc = upload_plan(p, parts, 12, d, s)) return rc;
+  p->dev_gave_up = reinterpret_cast<unsigned int*>(const_cast<uint8_t*>(d[11]));
   p->dev_chains = reinterpret_cast<const JoinPieces*>(d[10]);
   p->dev_joins = reinterpret_cast<const SharedJoin*>(d[6]);
   p->dev_units = reinterpret_cast<const int4*>(d[7]);

@@ -60,12 +60,22 @@ __device__ __forceinline__ float2 row_statistics(const TreeArgs& a, const TreeWe
   return all;
 }
 
+// Where a wait of the attention gave up, in this call or an earlier one of the plan, what rows and
+// scores hold is an older call's: the sums stay as they are.  (The mark is read with the first
+// loads and looked at in front of the stores.)
+__device__ __forceinline__ bool attention_gave_up(const TreeArgs& a, unsigned int mark) {
+  if (mark == 0u) return false;
+  if (threadIdx.x == 0) report_error_at(a.p.err, KVC_DEVERR_WAIT_LIMIT, blockIdx.x);
+  return true;
+}
+
 // chain: that of row threadIdx.x.
 __device__ __forceinline__ void weigh(const TreeArgs& a, const TreeWeigh& w, JoinPieces chain,
                                       float2* s_ml) {
   const int end = w.ctx + w.nodes, rows = w.nodes * a.group, pitch = (end + 15) & ~15;
   const int p = w.slot0 + 4 * threadIdx.x;
   const bool mine = p < end;
+  const unsigned int mark = __ldcg(a.gave_up);
   const float* s = a.scores + static_cast<size_t>(w.scores) * 16 + p;
   float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
   float old[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -101,6 +111,7 @@ __device__ __forceinline__ void weigh(const TreeArgs& a, const TreeWeigh& w, Joi
       }
     }
   }
+  if (attention_gave_up(a, mark)) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (p + i < end) out[i] = old[i] + sum[i];
@@ -255,6 +266,7 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
     if (edge) s_vis[wt] = make_uint4(vis[0], vis[1], vis[2], vis[3]);
   };
   bool failed = false;
+  const unsigned int mark = __ldcg(a.gave_up);
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (!mbar_wait_bounded(bar, parity)) {
       report_error_at(a.p.err, KVC_DEVERR_WAIT_LIMIT, blockIdx.x);
@@ -353,7 +365,7 @@ __global__ void __launch_bounds__(kRecountThreads, D <= 128 ? 2 : 1)
   tmem_fence_before();
   const bool stopped = __syncthreads_or(failed);
   const int p = p0 + wt;
-  if (wg == 0 && p < end && !stopped) {
+  if (wg == 0 && !stopped && !attention_gave_up(a, mark) && p < end) {
     float* out = a.weights + (static_cast<size_t>(w.bt_row) * a.p.num_kv_heads + w.kvh) * a.weight_slots + p;
     const float total = add + s_sum[wt];
     *out = p < w.ctx ? *out + total : total;

@@ -48,6 +48,7 @@ FAULT_DEVICE_ALLOC = 1
 FAULT_HOST_ALLOC = 2
 FAULT_HOST_REGISTER = 3
 FAULT_WAIT = 4
+FAULT_KERNEL_WAIT = 5
 
 _NP_DTYPE = {DTYPE_F16: np.dtype(np.float16), DTYPE_F32: np.dtype(np.float32)}
 

@@ -93,11 +93,13 @@ KVC_API int kvc_set_host_wait_limit(double seconds);
  * `skip` further calls at `site` succeed, the next `count` fail the way the CUDA
  * call would (device / page-locked allocations: cudaErrorMemoryAllocation;
  * page-locking caller memory: cudaErrorNotPermitted; a host wait: its limit runs
- * out at once).  Nothing reaches the GPU.  count 0 disarms the site. */
+ * out at once; a kernel's wait: the plan carries the mark that it would leave).  No
+ * failure reaches the GPU.  count 0 disarms the site. */
 #define KVC_FAULT_DEVICE_ALLOC 1   /* cudaMalloc of pools, scratch, staging */
 #define KVC_FAULT_HOST_ALLOC 2     /* cudaHostAlloc of page-locked staging */
 #define KVC_FAULT_HOST_REGISTER 3  /* cudaHostRegister of caller memory (offload) */
 #define KVC_FAULT_WAIT 4           /* bounded host waits */
+#define KVC_FAULT_KERNEL_WAIT 5    /* a tree plan's build: as if a wait of its attention had given up */
 KVC_API int kvc_test_inject_failure(int site, int skip, int count);
 
 /* ==== 1. Reference-compatible process-wide pool ============================ */
@@ -755,7 +757,9 @@ KVC_API int kvc_tree_plan_set_weights(kvc_tree_plan_t* plan, int on);
  * kvc_tree_plan_set_weights before its build; its score buffer, too, is its own.
  * A page out of range is reported (KVC_DEVERR_BAD_PAGE) and harms no other sequence:
  * where a sequence has a single token, 16-bit pools without a mask leave its positions
- * out, without weight; the other forms read page 0 in its place. */
+ * out, without weight; the other forms read page 0 in its place.  Once a wait of the
+ * attention has given up (KVC_DEVERR_WAIT_LIMIT), calls of the plan add nothing, and
+ * report it again, until the plan is built anew. */
 KVC_API int kvc_decode_tree_weights(kvc_pool_t* pool, const kvc_tree_plan_t* plan, int layer,
                                     const void* d_q, const int32_t* d_mask, int mask_words,
                                     float* d_weights, int weight_rows, int weight_slots,

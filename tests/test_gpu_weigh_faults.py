@@ -21,6 +21,7 @@ if HAS_GPU:
 from test_gpu_serve_ops import BAD_PAGE, attend64, check
 from test_gpu_spec_ops import BF16, F16, F32, dev, make_pool, no_error
 
+WAIT_LIMIT = 2           # KVC_DEVERR_*
 BAD = 1 << 20            # no pool here has as many pages
 
 
@@ -115,3 +116,43 @@ def test_pages_out_of_range_stay_with_their_sequence(dtype, nodes):
         assert torch.all(torch.isfinite(weights)) and torch.all(torch.isfinite(out))
         got.append((weights[1], out[nodes:]))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("nodes,mask", [(1, None), (1, "any"), (3, None), (60, None)])
+def test_an_attention_that_gave_up_adds_nothing(dtype, nodes, mask):
+    """A wait that gives up leaves scores and statistics of an older call behind.  The plan carries
+    the mark that such a wait sets: its calls leave the sums alone, bit by bit, and say so, until it
+    is built again; another plan's calls are not concerned."""
+    ctx, d, h, hkv, ps = [900, 333], 64, 8, 2, 16
+    dt = getattr(torch, dtype)
+    pool = make_pool(1, 2 * 64, ps, hkv, d, dtype, fill=0.0)
+    pool.fill_normal(seed=4)
+    table = dev(np.random.default_rng(2).permutation(128).reshape(2, 64))
+    q = torch.randn(2 * nodes, h, d, device="cuda").to(dt)
+    bits = None if mask is None else dev(np.full((2 * nodes, 2), -1, np.int32))
+    weights, out = torch.rand(2, hkv, 1000, device="cuda"), torch.zeros_like(q)
+    want, start = weights.clone(), weights.clone()
+    args = (0, q, bits)
+    fresh = pool.plan_tree(ctx, [nodes] * 2, h, weights=True)
+    pool.decode_tree_weights(fresh, *args, want, out, table, 0.125)
+    no_error()
+    ffi.inject_failure(ffi.FAULT_KERNEL_WAIT)
+    try:
+        plan = pool.plan_tree(ctx, [nodes] * 2, h, weights=True)
+    finally:
+        ffi.inject_failure(ffi.FAULT_KERNEL_WAIT, 0)
+    for _ in range(2):
+        pool.decode_tree_weights(plan, *args, weights, out, table, 0.125)
+        torch.cuda.synchronize()
+        assert ffi.device_error(0)[0] == WAIT_LIMIT
+        assert torch.equal(weights, start)
+    pool.decode_tree(plan, *args, out, table, 0.125)      # (adds nothing anyway)
+    no_error()
+    pool.decode_tree_weights(fresh, *args, start, out, table, 0.125)
+    no_error()
+    assert torch.equal(start, want)
+    pool.plan_tree(ctx, [nodes] * 2, h, plan=plan, weights=True)
+    pool.decode_tree_weights(plan, *args, weights, out, table, 0.125)
+    no_error()
+    assert torch.equal(weights, want)
