@@ -114,14 +114,18 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
     max_end = std::max(max_end, h_lens[i]);
     max_row = std::max(max_row, h_rows ? h_rows[i] : i);
   }
+  std::vector<int> prefix(std::max(0, n_groups));   // shared by the members of group k
   for (int k = 0; k < n_groups; ++k) {
     if (h_sizes[k] <= 0) return set_error(KVC_ERR_INVALID_ARG, "a group has at least one member.");
-    if (h_prefix[k] < 0 || h_prefix[k] % g.page_size != 0)
-      return set_error(KVC_ERR_INVALID_ARG, "a shared prefix is a whole number of pages.");
+    if (h_prefix[k] < 0)
+      return set_error(KVC_ERR_INVALID_ARG, "a prefix has a non-negative length.");
     if (members + h_sizes[k] > n_seqs)
       return set_error(KVC_ERR_INVALID_ARG, "the groups have more members than the batch.");
+    prefix[k] = h_sizes[k] > 1 ? h_prefix[k] : 0;   // (without company it does not matter)
+    if (prefix[k] % g.page_size != 0)
+      return set_error(KVC_ERR_INVALID_ARG, "a shared prefix is a whole number of pages.");
     for (int64_t i = members; i < members + h_sizes[k]; ++i)
-      if (h_lens[i] < h_prefix[k])
+      if (h_lens[i] < prefix[k])
         return set_error(KVC_ERR_INVALID_ARG, "a sequence is shorter than its group's prefix.");
     members += h_sizes[k];
   }
@@ -133,9 +137,9 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   // tiles of the small fp32 kernel, which are what decides between the two
   for (int k = 0, i = 0; k < n_groups; i += h_sizes[k++]) {
     auto blocks = [&](int64_t rows) { return (rows * group + kTreeSmall - 1) / kTreeSmall * Hkv; };
-    small += blocks(h_sizes[k]) * (h_prefix[k] / kTreeSmall);
+    small += blocks(h_sizes[k]) * (prefix[k] / kTreeSmall);
     for (int j = i; j < i + h_sizes[k]; ++j)
-      small += blocks(1) * ((h_lens[j] - h_prefix[k] + kTreeSmall - 1) / kTreeSmall);
+      small += blocks(1) * ((h_lens[j] - prefix[k] + kTreeSmall - 1) / kTreeSmall);
   }
   const TreeTile tile = tree_tile(g, small, sms);
   std::vector<TreeSeg> runs, segs;
@@ -169,14 +173,14 @@ int shared_build(kvc_shared_plan* sp, const kvc_pool* pool, const int32_t* h_row
   // gain from every tile.
   double saved = 0;
   for (int k = 0; k < n_groups; ++k)
-    saved += 2.0 * (h_sizes[k] - 1) * h_prefix[k] * Hkv * g.head_dim * g.elem_size;
+    saved += 2.0 * (h_sizes[k] - 1) * prefix[k] * Hkv * g.head_dim * g.elem_size;
   const bool worth = !tile.tensor || saved >= kSharedSaving;
   for (int k = 0, i = 0; k < n_groups; i += h_sizes[k++]) {
     // (below one tile the members' own first tiles hold the prefix anyway)
-    if (!worth || h_sizes[k] < 2 || h_prefix[k] < tile.positions) continue;
+    if (!worth || h_sizes[k] < 2 || prefix[k] < tile.positions) continue;
     prefix_run[k] = static_cast<int>(runs.size());
-    add(h_rows ? h_rows[i] : i, 0, h_prefix[k], i, h_sizes[k] * group);
-    std::fill(base.begin() + i, base.begin() + i + h_sizes[k], h_prefix[k]);
+    add(h_rows ? h_rows[i] : i, 0, prefix[k], i, h_sizes[k] * group);
+    std::fill(base.begin() + i, base.begin() + i + h_sizes[k], prefix[k]);
   }
   // Own positions.  Where the decode kernel runs on the tensor cores it takes them: its eight
   // warps an SM each work on a piece of their own, and a short piece (96 x 30-700 positions, 64 x

@@ -723,7 +723,7 @@ KVC_API int kvc_append_norm_rope(kvc_pool_t* pool, const kvc_norm_rope_args_t* a
  * the first member's row names; they are read once for the whole group where that
  * pays (16-bit pools: from 32 MB a layer on that the batch need not read again), and
  * from any member's row otherwise.  A query without company is a group of one, whose
- * prefix does not matter.  Built on the host and uploaded on `stream`, which must not
+ * prefix (any length from 0 on) does not matter.  Built on the host and uploaded on `stream`, which must not
  * be capturing. */
 KVC_API int kvc_shared_plan_create(kvc_shared_plan_t** out);
 KVC_API int kvc_shared_plan_destroy(kvc_shared_plan_t* plan);
