@@ -186,6 +186,11 @@ int do_decode_tree(kvc_pool* pool, const kvc_tree_plan* plan, int layer, const v
       return set_error(KVC_ERR_OUT_OF_RANGE, "a sequence's row is outside the weights.");
     if (plan->max_end > weight_slots)
       return set_error(KVC_ERR_OUT_OF_RANGE, "a sequence exceeds the weights' slots.");
+    const size_t q_bytes = static_cast<size_t>(plan->n_tokens) * plan->num_heads * a.head_dim * pool->g.elem_size;
+    const uintptr_t q0 = reinterpret_cast<uintptr_t>(d_q), o0 = reinterpret_cast<uintptr_t>(d_out);
+    if (plan->n_recounts > 0 && q0 < o0 + q_bytes && o0 < q0 + q_bytes)
+      return set_error(KVC_ERR_INVALID_ARG,
+                       "out must not overlap q where rows are counted again from it.");
     a.scores = static_cast<float*>(plan->d_scores.ptr);
     a.row_ml = static_cast<float2*>(plan->d_row_ml.ptr);
     a.weighs = plan->dev_weighs;

@@ -742,9 +742,11 @@ KVC_API int kvc_decode_shared(kvc_pool_t* pool, const kvc_shared_plan_t* plan, i
                               const void* d_q, void* d_out, const int32_t* d_block_tables,
                               int bt_stride, float scale, void* stream);
 
-/* Builds of the plan from now on (do not) make room for kvc_decode_tree_weights: 4
- * bytes for each token, q-head and position it may see, at most 2^30 of them.  Such a
- * plan's sequences must be in different block-table rows. */
+/* Builds of the plan from now on (do not) make room for kvc_decode_tree_weights.  The
+ * scores of a sequence are kept, 4 bytes for each token, q-head and position it may see,
+ * in CUDA-core pools (fp32, head dims other than 32, 64, 96, 128, 160, 192 and 256) and
+ * for at most 32 (token, q-head) rows of a KV head; other sequences take no room.  A plan
+ * holds 2^30 kept scores at most.  Its sequences must be in different block-table rows. */
 KVC_API int kvc_tree_plan_set_weights(kvc_tree_plan_t* plan, int on);
 
 /* kvc_decode_tree that also adds its softmax weights up: d_weights is (weight_rows,
@@ -755,9 +757,12 @@ KVC_API int kvc_tree_plan_set_weights(kvc_tree_plan_t* plan, int on);
  * as they were.  The weights are in 32 bits, not rounded to the pool's type, and the
  * rows are added in order, so a call repeats bit by bit.  The plan needs
  * kvc_tree_plan_set_weights before its build; its score buffer, too, is its own.
+ * Where the scores of a sequence are not kept (see there) they are computed again behind
+ * the attention: d_out must not overlap d_q then.
  * A page out of range is reported (KVC_DEVERR_BAD_PAGE) and harms no other sequence:
- * where a sequence has a single token, 16-bit pools without a mask leave its positions
- * out, without weight; the other forms read page 0 in its place.  Once a wait of the
+ * calls of single tokens that keep their scores on the tensor cores (no mask, one token
+ * a sequence at most) leave its positions out, without weight; others read page 0 in
+ * its place.  Once a wait of the
  * attention has given up (KVC_DEVERR_WAIT_LIMIT), calls of the plan add nothing, and
  * report it again, until the plan is built anew. */
 KVC_API int kvc_decode_tree_weights(kvc_pool_t* pool, const kvc_tree_plan_t* plan, int layer,

@@ -102,3 +102,36 @@ def test_the_prefix_of_a_group_of_one_does_not_matter(dtype, large):
     for bad in ([-1, 0, 0], [0, 0, -ps]):
         with pytest.raises(ValueError):
             pool.plan_shared(lens, sizes, [pre] + bad, h)
+
+
+# -- outputs over their own queries --------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nodes", [1, 4, 50])
+def test_weights_with_the_output_over_its_queries(dtype, nodes):
+    """Rows that are counted again are read again behind the attention: there the call is refused,
+    with nothing written; elsewhere an output in place of q is what it is in a tensor of its own."""
+    ctx, d, h, hkv, ps = [500, 90], 64, 8, 2, 16
+    dt = getattr(torch, dtype)
+    pool = make_pool(1, 80, ps, hkv, d, dtype, fill=0.0)
+    pool.fill_normal(seed=6)
+    bt = dev(np.random.default_rng(3).permutation(80).reshape(2, 40))
+    tokens = 2 * nodes
+    buf = torch.randn(2 * tokens, h, d, device="cuda").to(dt)
+    was, q = buf.clone(), buf[:tokens]
+    plan = pool.plan_tree(ctx, [nodes] * 2, h, weights=True)
+    want, out = torch.zeros(2, hkv, 640, device="cuda"), torch.zeros_like(q)
+    pool.decode_tree_weights(plan, 0, q, None, want, out, bt, 0.125)
+    no_error()
+    weights = torch.zeros_like(want)
+    if dtype != F32 and nodes == 50:
+        for over in (q, buf[tokens - 1:2 * tokens - 1], buf[1:tokens + 1]):
+            with pytest.raises(ValueError, match="overlap"):
+                pool.decode_tree_weights(plan, 0, q, None, weights, over, bt, 0.125)
+        assert torch.equal(buf, was) and torch.all(weights == 0)
+        pool.decode_tree_weights(plan, 0, q, None, weights, buf[tokens:], bt, 0.125)
+        assert torch.equal(buf[tokens:], out)
+    else:
+        pool.decode_tree_weights(plan, 0, q, None, weights, q, bt, 0.125)
+        assert torch.equal(q, out)
+    no_error()
+    assert torch.equal(weights, want)
