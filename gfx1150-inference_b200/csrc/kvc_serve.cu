@@ -24,10 +24,12 @@ namespace {
 // warp, each of which owns two 16-byte units that hold each other's pairs, so the sum of
 // squares is a few shuffles and the head is read once.  All in 32 bits, rounded once.
 //
-// Bound by memory traffic and by how many heads are on their way: 8,626 tokens of 32 + 8 + 8
+// Bound by the chain of a CTA (its first heads and page, the angles, the stores) and by how many
+// heads an SM has on their way; DRAM is at 43 % of its nominal rate.  8,634 tokens of 32 + 8 + 8
 // heads of 128 dims, fp16, three axes, 43.8 us for 212 MB (32 at the copy rate; append_rope_kernel
-// 45); two heads of a lane group on their way 47.4, four 47.3.  An SM takes 1,024 threads (768:
-// 47.4), which weights and angles in registers do not leave room for.
+// 45); two heads of a lane group on their way 47.4, four 47.3; fp32, with twice the bytes in the
+// same chain, 70.9 (65).  An SM takes 1,024 threads (768: 47.4), which weights and angles in
+// registers do not leave room for.
 // =====================================================================================
 constexpr int kNormThreads = 256;
 constexpr int kNormBatch = 3;      // heads of a lane group on their way
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_any_kernel(const NormR
   }
 }
 
-// Many tokens: 64 threads each (8,626 tokens, two heads on their way: 47.6 us; 32: 53, with
+// Many tokens: 64 threads each (8,634 tokens, two heads on their way: 47.6 us; 32: 53, with
 // two or four tokens in a CTA, which wait for one another's angles, 48.3 and 49.9); few: 256.
 template <typename T, bool kNeox, int kLanes>
 cudaError_t run_norm_rope(const NormRopeArgs& a, int sms, cudaStream_t s) {

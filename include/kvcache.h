@@ -731,7 +731,8 @@ KVC_API int kvc_plan_shared(kvc_shared_plan_t* plan, const kvc_pool_t* pool,
                             const int32_t* h_rows, const int32_t* h_lens, int n_seqs,
                             const int32_t* h_group_sizes, const int32_t* h_prefix_lens,
                             int n_groups, int num_heads, void* stream);
-/* Of the last build: queries, CTAs of the attention kernel, bytes of partials. */
+/* Of the last build: queries, CTAs of the tree kernel (prefixes that are shared, small
+ * batches; 0 where the decode kernel takes everything), bytes of partials. */
 KVC_API int kvc_shared_plan_info(const kvc_shared_plan_t* plan, int* n_queries, int* n_ctas,
                                  size_t* scratch_bytes);
 
