@@ -773,8 +773,10 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 1) tree_mma_kernel(con
   }
   __syncthreads();
   // (here, not in the wait, where it costs the loops 4 %)
-  if (threadIdx.x == 0 && *s_abort && a.gave_up) atomicExch(a.gave_up, 1u);
-  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+  if (warp == 1) {
+    if (*s_abort && a.gave_up) atomicExch(a.gave_up, 1u);
+    tmem_dealloc(tmem, kTmemCols);
+  }
 }
 
 // =====================================================================================
